@@ -7,7 +7,7 @@ GEMM API over torch device tensors, and the INT4 packing/quantisation helpers.
 """
 from ._lib import (  # noqa: F401
     CloveError, CLOVE_ERR_SCRATCH_LIMIT, CLOVE_ERR_WORKSPACE, CLOVE_INT4_GROUPWISE,
-    CLOVE_INT4_REFERENCE_LITERAL, CLOVE_INT8_EXACT, CLOVE_INT8_REFERENCE_LITERAL, CLOVE_NOALLOC_SCRATCH_BYTES,
+    CLOVE_INT4_REFERENCE_LITERAL, CLOVE_INT8_EXACT, CLOVE_INT8_REFERENCE_LITERAL, CLOVE_MAX_HEAD_DIM, CLOVE_NOALLOC_SCRATCH_BYTES,
     CLOVE_WORKSPACE_MIN_BYTES,
 )
 from .gemm import (  # noqa: F401
@@ -29,5 +29,12 @@ from .gemm import (  # noqa: F401
     w4a16_swiglu,
     workspace_bind,
     workspace_query,
+)
+from .decode import (  # noqa: F401
+    KVCache,
+    cache_evict,
+    paged_attention,
+    penalize_logits,
+    qk_norm_rope,
 )
 from . import quant  # noqa: F401

@@ -30,10 +30,25 @@ CLOVE_INT4_REFERENCE_LITERAL = 1
 CLOVE_INT8_EXACT = 0
 CLOVE_INT8_REFERENCE_LITERAL = 1
 
+CLOVE_DTYPE_FP16 = 0
+CLOVE_DTYPE_BF16 = 1
+CLOVE_DTYPE_FP32 = 2
+CLOVE_MAX_HEAD_DIM = 1024
+
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
 I8 = ctypes.c_int8
+L = ctypes.c_int64
+
+
+class KVCacheDesc(ctypes.Structure):
+    """clove_kv_cache_t"""
+    _fields_ = [("k", P), ("v", P), ("page_stride", L), ("num_pages", I), ("page_size", I), ("kv_heads", I),
+                ("head_dim", I), ("dtype", I)]
+
+
+KV = ctypes.POINTER(KVCacheDesc)
 
 # name -> argtypes (every entry point declared in include/clove/gemm_c.h)
 SIGNATURES = {
@@ -53,6 +68,10 @@ SIGNATURES = {
     "clove_swiglu": ([P, P, P, I, P], I),
     "clove_swiglu_fused": ([P, P, P, P, I, I, I, P], I),
     "clove_w4a16_swiglu": ([P, P, P, P, P, I, I, I, P], I),
+    "clove_qk_norm_rope": ([P, L, P, P, F, P, P, I, P, P, L, P, L, KV, P, I, I, I, I, I, I, I, P], I),
+    "clove_paged_attention": ([P, L, KV, P, L, P, P, L, P, L, I, I, I, F, F, I, P], I),
+    "clove_cache_evict": ([KV, P, L, P, P, L, P, L, P, L, P, L, P, I, I, I, I, I, P], I),
+    "clove_penalize_logits": ([P, L, I, P, L, I, I, I, P, L, P, P, P, P, P, P, P, L, P, P, L, P], I),
     "clove_workspace_bind": ([P, ctypes.c_size_t], I),
     "clove_workspace_query_begin": ([], I),
     "clove_workspace_query_end": ([], ctypes.c_size_t),
@@ -75,12 +94,12 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError(
                 f"{LIB_PATH} is missing: build the HIP library first "
                 "(python -c 'import __graft_entry__ as g; g.build()')")
-        L = ctypes.CDLL(LIB_PATH)
+        loaded = ctypes.CDLL(LIB_PATH)
         for name, (args, res) in SIGNATURES.items():
-            fn = getattr(L, name)
+            fn = getattr(loaded, name)
             fn.argtypes = args
             fn.restype = res
-        _lib = L
+        _lib = loaded
     return _lib
 
 

@@ -11,6 +11,7 @@
 
 #include "clove/gemm_c.h"
 #include "common.hpp"
+#include "decode.hpp"
 #include "dispatch.hpp"
 
 namespace clove {
@@ -81,6 +82,25 @@ bool overlaps(const void* a, size_t abytes, const void* b, size_t bbytes) {
     if (!a || !b || abytes == 0 || bbytes == 0) return false;
     const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
     return a0 < b0 + bbytes && b0 < a0 + abytes;
+}
+
+// Rows of one tensor: `rows` of `width` bytes, `stride` bytes apart.
+struct Rows {
+    const void* p;
+    int64_t stride, width, rows;
+};
+
+// Whether two such tensors share a byte.  Rows of the same stride may lie
+// between each other's (parts of one wider tensor); otherwise their whole
+// extents must be apart.
+bool overlaps(const Rows& a, const Rows& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    if (!overlaps(a.p, (size_t)((a.rows - 1) * a.stride + a.width), b.p, (size_t)((b.rows - 1) * b.stride + b.width)))
+        return false;
+    if (a.stride != b.stride || a.width > a.stride || b.width > a.stride) return true;
+    const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));
+    const int64_t off = ((d % a.stride) + a.stride) % a.stride;  // of b's rows within a's stride
+    return off < a.width || a.stride - off < b.width;
 }
 
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
@@ -583,6 +603,257 @@ clove_status_t clove_w4a16_swiglu(const void* X, const uint8_t* W_q, const void*
     a.Y = static_cast<uint16_t*>(H);
     a.T = T; a.O = I; a.K = K;
     return launch_w4a16_swiglu(a, s);
+}
+
+// The descriptor of a cache checked and laid out for kernels.
+static clove_status_t read_cache(const clove_kv_cache_t* c, PagedCache* out) {
+    if (c->dtype != CLOVE_DTYPE_FP16 && c->dtype != CLOVE_DTYPE_BF16) return CLOVE_ERR_INVALID_ARG;
+    if (c->num_pages < 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_dim <= 0 || c->head_dim > CLOVE_MAX_HEAD_DIM)
+        return CLOVE_ERR_INVALID_DIM;
+    const int64_t rows = (int64_t)c->kv_heads * c->page_size;
+    if (rows > ((int64_t)1 << 40) / c->head_dim) return CLOVE_ERR_INVALID_DIM;
+    const int64_t dense = rows * c->head_dim;
+    if (c->page_stride != 0 && c->page_stride < dense) return CLOVE_ERR_INVALID_ARG;
+    if (c->num_pages > 0 && (!c->k || !c->v)) return CLOVE_ERR_NULL_POINTER;
+    if (!aligned2(c->k) || !aligned2(c->v)) return CLOVE_ERR_INVALID_ARG;
+    out->k = static_cast<uint16_t*>(c->k);
+    out->v = static_cast<uint16_t*>(c->v);
+    out->page_stride = c->page_stride ? c->page_stride : dense;
+    out->num_pages = c->num_pages;
+    out->page_size = c->page_size;
+    out->kv_heads = c->kv_heads;
+    out->head_dim = c->head_dim;
+    out->dtype = c->dtype;
+    return CLOVE_OK;
+}
+
+static Rows cache_rows(const PagedCache& c, const void* p) {
+    return Rows{p, c.page_stride * 2, (int64_t)c.kv_heads * c.page_size * c.head_dim * 2, c.num_pages};
+}
+
+clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight,
+                                  float eps, const float* rope_cos, const float* rope_sin, int max_position,
+                                  const int32_t* positions, void* q_out, int64_t q_out_stride, void* k_out,
+                                  int64_t k_out_stride, const clove_kv_cache_t* cache, const int32_t* slots, int T,
+                                  int q_heads, int kv_heads, int head_dim, int rot_dim, int interleaved, int dtype,
+                                  void* stream) {
+    CallScope scope;
+    if (dtype != CLOVE_DTYPE_FP16 && dtype != CLOVE_DTYPE_BF16) return CLOVE_ERR_INVALID_ARG;
+    if (T < 0 || q_heads < 0 || kv_heads < 0 || head_dim < 1 || head_dim > CLOVE_MAX_HEAD_DIM || rot_dim < 0 ||
+        max_position < 0 || q_heads > 0x10000 || kv_heads > 0x10000)
+        return CLOVE_ERR_INVALID_DIM;
+    if (rot_dim > head_dim || rot_dim % 2 != 0) return CLOVE_ERR_INVALID_ARG;
+    const int64_t qw = (int64_t)q_heads * head_dim, kw = (int64_t)kv_heads * head_dim;
+    if (T == 0 || q_heads + kv_heads == 0) return CLOVE_OK;
+    if (!qkv || (q_heads > 0 && !q_out)) return CLOVE_ERR_NULL_POINTER;
+    if (rot_dim > 0 && (!positions || (max_position > 0 && (!rope_cos || !rope_sin)))) return CLOVE_ERR_NULL_POINTER;
+    if (qkv_stride < qw + 2 * kw || (q_heads > 0 && q_out_stride < qw) || (k_out && k_out_stride < kw))
+        return CLOVE_ERR_INVALID_ARG;
+    if (!aligned2(qkv) || !aligned2(q_weight) || !aligned2(k_weight) || !aligned2(q_out) || !aligned2(k_out) ||
+        !aligned4(rope_cos) || !aligned4(rope_sin) || !aligned4(positions) || !aligned4(slots))
+        return CLOVE_ERR_INVALID_ARG;
+    RopeArgs a;
+    if (cache) {
+        const clove_status_t st = read_cache(cache, &a.cache);
+        if (st != CLOVE_OK) return st;
+        if (cache->dtype != dtype || cache->kv_heads != kv_heads || cache->head_dim != head_dim) return CLOVE_ERR_INVALID_ARG;
+        if (!slots) return CLOVE_ERR_NULL_POINTER;
+        if (cache->num_pages == 0) a.cache.k = a.cache.v = nullptr;
+    }
+    // outputs against inputs: the queries / keys of qkv may be their own output
+    const char* x = static_cast<const char*>(qkv);
+    const Rows in[] = {{x, qkv_stride * 2, qw * 2, T}, {x + qw * 2, qkv_stride * 2, kw * 2, T},
+                       {x + (qw + kw) * 2, qkv_stride * 2, kw * 2, T}};
+    const Rows outs[] = {{q_heads > 0 ? q_out : nullptr, q_out_stride * 2, qw * 2, T}, {k_out, k_out_stride * 2, kw * 2, T},
+                         cache_rows(a.cache, a.cache.k), cache_rows(a.cache, a.cache.v)};
+    const int64_t half = rot_dim / 2;
+    const Rows small[] = {{q_weight, 0, head_dim * 2, 1}, {k_weight, 0, head_dim * 2, 1},
+                          {rope_cos, 0, max_position * half * 4, 1}, {rope_sin, 0, max_position * half * 4, 1},
+                          {positions, 0, (int64_t)T * 4, 1}, {slots, 0, (int64_t)T * 4, 1}};
+    for (int o = 0; o < 4; ++o) {
+        for (int i = 0; i < 3; ++i) {
+            const bool own = o == i && outs[o].p == in[i].p && outs[o].stride == in[i].stride;
+            if (!own && overlaps(outs[o], in[i])) return CLOVE_ERR_ALIASING;
+        }
+        for (const Rows& r : small)
+            if (overlaps(outs[o], r)) return CLOVE_ERR_ALIASING;
+        for (int i = 0; i < o; ++i)
+            if (overlaps(outs[o], outs[i])) return CLOVE_ERR_ALIASING;
+    }
+    a.qkv = static_cast<const uint16_t*>(qkv);
+    a.qkv_stride = qkv_stride;
+    a.q_weight = static_cast<const uint16_t*>(q_weight);
+    a.k_weight = static_cast<const uint16_t*>(k_weight);
+    a.eps = eps;
+    a.cos = rope_cos;
+    a.sin = rope_sin;
+    a.max_position = max_position;
+    a.positions = positions;
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.q_out_stride = q_out_stride;
+    a.k_out = static_cast<uint16_t*>(k_out);
+    a.k_out_stride = k_out_stride;
+    a.slots = slots;
+    a.T = T; a.q_heads = q_heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.rot_dim = rot_dim;
+    a.interleaved = interleaved != 0;
+    a.dtype = dtype;
+    return launch_qk_norm_rope(a, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clove_kv_cache_t* cache,
+                                     const int32_t* block_table, int64_t table_stride, const int32_t* context_lens,
+                                     void* out, int64_t out_stride, float* weights, int64_t weights_stride, int batch,
+                                     int q_heads, int max_context, float scale, float softcap, int window,
+                                     void* stream) {
+    CallScope scope;
+    if (!cache) return CLOVE_ERR_NULL_POINTER;
+    PagedAttentionArgs a;
+    const clove_status_t st = read_cache(cache, &a.cache);
+    if (st != CLOVE_OK) return st;
+    if (batch < 0 || q_heads < 0 || max_context < 0 || window < 0 || table_stride < 0) return CLOVE_ERR_INVALID_DIM;
+    if (q_heads % a.cache.kv_heads != 0 || !(softcap >= 0.0f)) return CLOVE_ERR_INVALID_ARG;
+    if (batch == 0 || q_heads == 0) return CLOVE_OK;
+    if (!q || !out || !context_lens || (max_context > 0 && !block_table)) return CLOVE_ERR_NULL_POINTER;
+    const int64_t width = (int64_t)q_heads * a.cache.head_dim;
+    if (q_stride < width || out_stride < width || (weights && weights_stride < max_context) ||
+        (int64_t)max_context > table_stride * a.cache.page_size)
+        return CLOVE_ERR_INVALID_ARG;
+    if ((int64_t)batch * q_heads > 0x1000000 || (int64_t)batch * q_heads * hw::cdiv64(max_context, 16) > 0x3fffffffff)
+        return CLOVE_ERR_INVALID_DIM;
+    if (!aligned2(q) || !aligned2(out) || !aligned4(block_table) || !aligned4(context_lens) || !aligned4(weights))
+        return CLOVE_ERR_INVALID_ARG;
+    const Rows in[] = {{q, q_stride * 2, width * 2, batch}, cache_rows(a.cache, a.cache.k), cache_rows(a.cache, a.cache.v),
+                       {block_table, table_stride * 4, table_stride * 4, batch}, {context_lens, 0, (int64_t)batch * 4, 1}};
+    const Rows outs[] = {{out, out_stride * 2, width * 2, batch}, {weights, weights_stride * 4, (int64_t)max_context * 4, batch}};
+    for (const Rows& o : outs)
+        for (const Rows& i : in)
+            if (overlaps(o, i)) return CLOVE_ERR_ALIASING;
+    if (overlaps(outs[0], outs[1])) return CLOVE_ERR_ALIASING;
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_stride = q_stride;
+    a.block_table = block_table;
+    a.table_stride = table_stride;
+    a.context_lens = context_lens;
+    a.out = static_cast<uint16_t*>(out);
+    a.out_stride = out_stride;
+    a.weights = weights;
+    a.weights_stride = weights_stride;
+    a.batch = batch; a.q_heads = q_heads; a.max_context = max_context;
+    a.scale = scale;
+    a.softcap = softcap;
+    a.window = window;
+    return launch_paged_attention(a, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* block_table, int64_t table_stride,
+                                 const int32_t* context_lens, const float* weights, int64_t weights_stride,
+                                 const int32_t* positions, int64_t positions_stride, float* weights_out,
+                                 int64_t weights_out_stride, int32_t* positions_out, int64_t positions_out_stride,
+                                 int32_t* lens_out, int batch, int max_context, int budget, int sinks, int recent,
+                                 void* stream) {
+    CallScope scope;
+    if (!cache) return CLOVE_ERR_NULL_POINTER;
+    EvictArgs a;
+    const clove_status_t st = read_cache(cache, &a.cache);
+    if (st != CLOVE_OK) return st;
+    if (batch < 0 || batch > 0x10000 || max_context < 0 || budget < 0 || sinks < 0 || recent < 0 || table_stride < 0)
+        return CLOVE_ERR_INVALID_DIM;
+    if (batch == 0) return CLOVE_OK;
+    if (!context_lens || !lens_out) return CLOVE_ERR_NULL_POINTER;
+    if (max_context > 0 && (!block_table || !weights || !positions || !weights_out || !positions_out))
+        return CLOVE_ERR_NULL_POINTER;
+    if ((int64_t)max_context > table_stride * a.cache.page_size || weights_stride < max_context ||
+        positions_stride < max_context || weights_out_stride < max_context || positions_out_stride < max_context)
+        return CLOVE_ERR_INVALID_ARG;
+    if (!aligned4(block_table) || !aligned4(context_lens) || !aligned4(weights) || !aligned4(positions) ||
+        !aligned4(weights_out) || !aligned4(positions_out) || !aligned4(lens_out))
+        return CLOVE_ERR_INVALID_ARG;
+    const int64_t row = (int64_t)max_context * 4, ints = (int64_t)batch * 4;
+    const Rows in[] = {{weights, weights_stride * 4, row, batch}, {positions, positions_stride * 4, row, batch},
+                       {context_lens, 0, ints, 1}, {block_table, table_stride * 4, table_stride * 4, batch}};
+    const Rows outs[] = {{weights_out, weights_out_stride * 4, row, batch},
+                         {positions_out, positions_out_stride * 4, row, batch},
+                         {lens_out, 0, ints, 1},
+                         cache_rows(a.cache, a.cache.k),
+                         cache_rows(a.cache, a.cache.v)};
+    for (int o = 0; o < 5; ++o) {
+        for (int i = 0; i < 4; ++i) {
+            const bool own = o == i && outs[o].p == in[i].p && outs[o].stride == in[i].stride;
+            if (!own && overlaps(outs[o], in[i])) return CLOVE_ERR_ALIASING;
+        }
+        for (int i = 0; i < o; ++i)
+            if (overlaps(outs[o], outs[i])) return CLOVE_ERR_ALIASING;
+    }
+    a.block_table = block_table;
+    a.table_stride = table_stride;
+    a.context_lens = context_lens;
+    a.weights = weights;
+    a.weights_stride = weights_stride;
+    a.positions = positions;
+    a.positions_stride = positions_stride;
+    a.weights_out = weights_out;
+    a.weights_out_stride = weights_out_stride;
+    a.positions_out = positions_out;
+    a.positions_out_stride = positions_out_stride;
+    a.lens_out = lens_out;
+    a.batch = batch; a.max_context = max_context; a.budget = budget; a.sinks = sinks; a.recent = recent;
+    return launch_cache_evict(a, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, int dtype, void* out,
+                                     int64_t out_stride, int out_dtype, int batch, int vocab, const int32_t* history,
+                                     int64_t history_stride, const int32_t* history_lens, const int32_t* prompt_lens,
+                                     const float* repetition, const float* presence, const float* frequency,
+                                     const int32_t* bias_ids, const float* bias_values, int64_t bias_stride,
+                                     const int32_t* bias_counts, const uint32_t* allowed, int64_t allowed_stride,
+                                     void* stream) {
+    CallScope scope;
+    if (dtype < CLOVE_DTYPE_FP16 || dtype > CLOVE_DTYPE_FP32 || (out_dtype != dtype && out_dtype != CLOVE_DTYPE_FP32))
+        return CLOVE_ERR_INVALID_ARG;
+    if (batch < 0 || vocab < 0 || (history && history_stride < 0) || (bias_ids && bias_stride < 0)) return CLOVE_ERR_INVALID_DIM;
+    if ((history && history_stride > 0x7fffffff) || (bias_ids && bias_stride > 0x7fffffff)) return CLOVE_ERR_INVALID_DIM;
+    if (batch == 0 || vocab == 0) return CLOVE_OK;
+    if (!logits || !out || (history && !history_lens) || (bias_ids && !bias_values)) return CLOVE_ERR_NULL_POINTER;
+    const int64_t words = hw::cdiv64(vocab, 32);
+    if (logits_stride < vocab || out_stride < vocab || (allowed && allowed_stride < words)) return CLOVE_ERR_INVALID_ARG;
+    const int64_t is = dtype == CLOVE_DTYPE_FP32 ? 4 : 2, os = out_dtype == CLOVE_DTYPE_FP32 ? 4 : 2;
+    if (!(is == 4 ? aligned4(logits) : aligned2(logits)) || !(os == 4 ? aligned4(out) : aligned2(out)) ||
+        !aligned4(history) || !aligned4(history_lens) || !aligned4(prompt_lens) || !aligned4(repetition) ||
+        !aligned4(presence) || !aligned4(frequency) || !aligned4(bias_ids) || !aligned4(bias_values) ||
+        !aligned4(bias_counts) || !aligned4(allowed))
+        return CLOVE_ERR_INVALID_ARG;
+    const int64_t per = (int64_t)batch * 4;
+    const Rows o{out, out_stride * os, (int64_t)vocab * os, batch}, x{logits, logits_stride * is, (int64_t)vocab * is, batch};
+    const bool own = out == logits && os == is && out_stride == logits_stride;
+    if (!own && overlaps(o, x)) return CLOVE_ERR_ALIASING;
+    const Rows in[] = {{history, history_stride * 4, history_stride * 4, batch}, {history_lens, 0, per, 1},
+                       {prompt_lens, 0, per, 1}, {repetition, 0, per, 1}, {presence, 0, per, 1}, {frequency, 0, per, 1},
+                       {bias_ids, bias_stride * 4, bias_stride * 4, batch}, {bias_values, bias_stride * 4, bias_stride * 4, batch},
+                       {bias_counts, 0, per, 1}, {allowed, allowed_stride * 4, words * 4, batch}};
+    for (const Rows& i : in)
+        if (overlaps(o, i)) return CLOVE_ERR_ALIASING;
+    LogitsArgs a;
+    a.logits = logits;
+    a.logits_stride = logits_stride;
+    a.dtype = dtype;
+    a.out = out;
+    a.out_stride = out_stride;
+    a.out_dtype = out_dtype;
+    a.batch = batch; a.vocab = vocab;
+    a.history = history;
+    a.history_stride = history_stride;
+    a.history_lens = history_lens;
+    a.prompt_lens = prompt_lens;
+    a.repetition = repetition;
+    a.presence = presence;
+    a.frequency = frequency;
+    a.bias_ids = bias_ids;
+    a.bias_values = bias_values;
+    a.bias_stride = bias_stride;
+    a.bias_counts = bias_counts;
+    a.allowed = allowed;
+    a.allowed_stride = allowed_stride;
+    return launch_penalize_logits(a, static_cast<hipStream_t>(stream));
 }
 
 clove_status_t clove_workspace_bind(void* ptr, size_t bytes) {

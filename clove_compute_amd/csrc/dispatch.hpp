@@ -148,6 +148,7 @@ clove_status_t launch_swiglu_fused_fp16(const uint16_t* X, const uint16_t* W_gat
 // workspace as acquire_scratch; slot 0 is reserved for the split-K scratch.
 clove_status_t acquire_buffer(hipStream_t stream, int slot, size_t bytes, void** out);
 constexpr int kBufSwiglu = 1;  // gate / up intermediates of the unfused SwiGLU paths
+constexpr int kBufDecode = 2;  // lists, partial results and scores of the decode-step operators
 
 // FP16 with up to four rows of A: the skinny MFMA kernel rather than the GEMV.
 // Large weights first (cold, us per call: 11008 x 4096 at M = 2 / 3 / 4 21.1 /

@@ -244,6 +244,147 @@ clove_status_t clove_w4a16_swiglu(const void* X, const uint8_t* W_q, const void*
                                   const void* W_zero, void* H, int T, int I, int K,
                                   void* stream);
 
+/* ------------------------------------------------------------------------
+ * The decode step around the linear layers.  No reference counterpart is
+ * replaced (the reference declares a paged_attention in include/clove/kernels/
+ * attention.cuh:85-100 and never defines it).  Element type `dtype`: see
+ * clove_dtype_t; every sum, norm and softmax statistic is fp32 and a result is
+ * rounded once.  Row strides count elements.  All of these take their scratch
+ * as the GEMMs do (library buffers, a bound workspace, or a size query).
+ * ------------------------------------------------------------------------ */
+typedef enum clove_dtype {
+    CLOVE_DTYPE_FP16 = 0,
+    CLOVE_DTYPE_BF16 = 1,
+    CLOVE_DTYPE_FP32 = 2 /* logits only */
+} clove_dtype_t;
+
+/* Largest head_dim of these operators. */
+#define CLOVE_MAX_HEAD_DIM 1024
+
+/* The key-value cache of one layer, in pages.  Key (page, head, row) starts at
+ * element page * page_stride + (head * page_size + row) * head_dim of `k`, its
+ * value at the same element of `v`; page_stride 0 means dense pages
+ * (kv_heads * page_size * head_dim).  Slot s is row s % page_size of page
+ * s / page_size.  dtype is FP16 or BF16. */
+typedef struct clove_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride;
+    int num_pages;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+    int dtype;
+} clove_kv_cache_t;
+
+/*
+ * Norms of queries and keys for each head, the position rotation, and the
+ * write into the cache, in one pass over the fused QKV projection's output:
+ *   qkv row t (qkv_stride elements apart): q_heads queries, kv_heads keys, then
+ *   kv_heads values of head_dim elements each
+ *   x = a query or key;  y = x / sqrt(mean(x^2) + eps) * weight, where its
+ *   weight (q_weight, k_weight [head_dim], `dtype`) is not NULL, else y = x
+ *   first rot_dim elements rotated by c, s = rope_cos/rope_sin[positions[t], i]
+ *   (fp32 [max_position, rot_dim / 2]): (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)
+ *   with (a, b) = (i, i + rot_dim / 2), or (2i, 2i + 1) where `interleaved`
+ * Queries go to q_out [T, q_heads, head_dim] (rows q_out_stride apart); keys to
+ * k_out likewise (NULL: not wanted); keys and values to slot slots[t] of
+ * `cache` (NULL: not wanted).  A slot outside the cache (a negative one marks a
+ * padding token) is not written; two tokens of one call must not name the same
+ * slot.  A position outside [0, max_position) makes that token's q and k NaN
+ * (rot_dim > 0).  q_out / k_out may be the queries / keys of qkv themselves
+ * (same rows, same stride), else outputs must not overlap inputs.  rot_dim is
+ * even and at most head_dim; with rot_dim 0 the tables and positions are not
+ * read.  T == 0 is a no-op.
+ */
+clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const void* q_weight,
+                                  const void* k_weight, float eps, const float* rope_cos,
+                                  const float* rope_sin, int max_position, const int32_t* positions,
+                                  void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                                  const clove_kv_cache_t* cache, const int32_t* slots, int T,
+                                  int q_heads, int kv_heads, int head_dim, int rot_dim,
+                                  int interleaved, int dtype, void* stream);
+
+/*
+ * Attention of one new token per sequence over the paged cache.  Query head h
+ * of sequence b reads KV head h / (q_heads / kv_heads).  Key j of sequence b is
+ * row j % page_size of page block_table[b * table_stride + j / page_size];
+ * with n = context_lens[b] (taken as at most max_context, at least 0) it sees
+ * the keys j in [window > 0 ? max(0, n - window) : 0, n) whose page lies in
+ * [0, num_pages), a page outside it being absent:
+ *   s_j = scale * q . k_j   (softcap > 0: softcap * tanh(s_j / softcap))
+ *   p = softmax(s),  out = sum_j p_j v_j      (a query that sees no key: 0)
+ * and, where `weights` (fp32, rows weights_stride apart) is not NULL,
+ *   weights[b, j] += sum over the heads of p_j      for every key it sees.
+ * q, out [batch, q_heads, head_dim] (rows q_stride / out_stride apart) are the
+ * cache's dtype.  Cache rows and table entries that no key names are not read.
+ * max_context bounds the lengths on the host: it sizes the launch, and is at
+ * most table_stride * page_size (and weights_stride).  Sums run in a fixed
+ * order: a call gives the same bits every time.
+ */
+clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clove_kv_cache_t* cache,
+                                     const int32_t* block_table, int64_t table_stride,
+                                     const int32_t* context_lens, void* out, int64_t out_stride,
+                                     float* weights, int64_t weights_stride, int batch, int q_heads,
+                                     int max_context, float scale, float softcap, int window,
+                                     void* stream);
+
+/*
+ * Eviction from the cache by accumulated attention weight: cuts every sequence
+ * longer than `budget` down to it, in place.  Of the n = context_lens[b] tokens
+ * (at most max_context) those are kept first whose position (positions[b, i],
+ * of the token in slot i) is < sinks or > newest - recent (newest: the largest
+ * of them), then those of the largest weights[b, i]; at equal weight (-0 equals
+ * 0, NaN is below everything) the lower slot stays.  Kept tokens below slot
+ * `budget` do not move; the j-th kept one past it moves into the j-th slot
+ * below it that is free: its K and V rows of every head, its weight and its
+ * position.  Keys hold their rotation, so attention without a window does not
+ * depend on their order.
+ *   lens_out[b]            min(n, budget)
+ *   weights_out[b, i], positions_out[b, i]   of the slots as they are then; 0
+ *                          and -1 for lens_out[b] <= i < max_context
+ * Each output may be its input (same address and stride).  A row whose page
+ * lies outside the cache is not copied.  Sequences must not share pages, or
+ * have a page twice.  A second call with the same inputs moves the same rows
+ * again and changes nothing.
+ */
+clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* block_table,
+                                 int64_t table_stride, const int32_t* context_lens,
+                                 const float* weights, int64_t weights_stride,
+                                 const int32_t* positions, int64_t positions_stride,
+                                 float* weights_out, int64_t weights_out_stride,
+                                 int32_t* positions_out, int64_t positions_out_stride,
+                                 int32_t* lens_out, int batch, int max_context, int budget,
+                                 int sinks, int recent, void* stream);
+
+/*
+ * Penalties for repeated tokens, biases and a grammar mask on logits, fp32:
+ *   x = logits[b, v]
+ *   v anywhere in history[b, 0 : history_lens[b]]:  x = x > 0 ? x / r : x * r
+ *   c = how often v is in history[b, prompt_lens[b] : history_lens[b]]
+ *   x -= frequency[b] * c;  c > 0: x -= presence[b]
+ *   v in bias_ids[b, 0 : bias_counts[b]]:  x += its bias_values (the last entry
+ *   for v counts)
+ *   bit v % 32 of allowed[b, v / 32] clear:  x = -infinity
+ *   out[b, v] = x
+ * r = repetition[b].  Any of repetition, presence, frequency [batch], history,
+ * bias_ids and allowed may be NULL: that part is left out (prompt_lens NULL: no
+ * prompt, everything was generated; bias_counts NULL: all bias_stride entries).
+ * Lengths are taken as at least 0 and at most the row's stride; ids outside
+ * [0, vocab) are ignored.  logits are `dtype` (FP16, BF16 or FP32), out is
+ * `out_dtype` (the same, or FP32), rows logits_stride / out_stride elements
+ * apart; out may be logits itself where dtype and stride agree.
+ */
+clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, int dtype, void* out,
+                                     int64_t out_stride, int out_dtype, int batch, int vocab,
+                                     const int32_t* history, int64_t history_stride,
+                                     const int32_t* history_lens, const int32_t* prompt_lens,
+                                     const float* repetition, const float* presence,
+                                     const float* frequency, const int32_t* bias_ids,
+                                     const float* bias_values, int64_t bias_stride,
+                                     const int32_t* bias_counts, const uint32_t* allowed,
+                                     int64_t allowed_stride, void* stream);
+
 /* Caller-owned workspace (no reference counterpart: the reference allocates no
  * scratch).  Per host thread, three modes:
  *
