@@ -43,8 +43,10 @@ CFLAGS = [
 
 # per-source additions: the INT4-weight GEMMs keep their per-group MFMA sums in
 # VGPRs (the group fold reads every one of them; in AGPRs each read would be a
-# separate v_accvgpr_read)
-EXTRA = {"i4w_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+# separate v_accvgpr_read), as the attention kernel does its output sums, which
+# a new maximum rescales
+EXTRA = {"paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "i4w_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "i4i4_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

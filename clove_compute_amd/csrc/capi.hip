@@ -718,7 +718,8 @@ clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clov
     if (q_stride < width || out_stride < width || (weights && weights_stride < max_context) ||
         (int64_t)max_context > table_stride * a.cache.page_size)
         return CLOVE_ERR_INVALID_ARG;
-    if ((int64_t)batch * q_heads > 0x1000000 || (int64_t)batch * q_heads * hw::cdiv64(max_context, 16) > 0x3fffffffff)
+    if (max_context > CLOVE_MAX_CONTEXT || (int64_t)batch * q_heads > 0x1000000 ||
+        (weights && batch * hw::cdiv64(max_context, 256) > 0x7fffffff))
         return CLOVE_ERR_INVALID_DIM;
     if (!aligned2(q) || !aligned2(out) || !aligned4(block_table) || !aligned4(context_lens) || !aligned4(weights))
         return CLOVE_ERR_INVALID_ARG;
@@ -756,7 +757,7 @@ clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* b
     EvictArgs a;
     const clove_status_t st = read_cache(cache, &a.cache);
     if (st != CLOVE_OK) return st;
-    if (batch < 0 || batch > 0x10000 || max_context < 0 || budget < 0 || sinks < 0 || recent < 0 || table_stride < 0)
+    if (batch < 0 || batch > 0x10000 || max_context < 0 || max_context > CLOVE_MAX_CONTEXT || budget < 0 || sinks < 0 || recent < 0 || table_stride < 0)
         return CLOVE_ERR_INVALID_DIM;
     if (batch == 0) return CLOVE_OK;
     if (!context_lens || !lens_out) return CLOVE_ERR_NULL_POINTER;

@@ -36,6 +36,22 @@ struct Elem<CLOVE_DTYPE_FP32> {
 
 }  // namespace hw
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and
+// m = ceil(2^(31+s) / d), m d - 2^(31+s) < d <= 2^s, so that n times it stays
+// below 2^(31+s) and floor(n m / 2^(31+s)) is the quotient.
+struct FastDiv {
+    unsigned m = 1u << 31;
+    int shift = 31, d = 1;
+    FastDiv() = default;
+    explicit FastDiv(int by) : d(by) {
+        int s = 0;
+        while (((int64_t)1 << s) < by) ++s;
+        shift = 31 + s;
+        m = (unsigned)((((uint64_t)1 << shift) + (uint64_t)by - 1) / (uint64_t)by);
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(unsigned)n * m) >> shift); }
+};
+
 // The paged cache of one layer as kernels take it: element (page, head, row, d)
 // of k and v lies at page * page_stride + (head * page_size + row) * head_dim + d.
 struct PagedCache {

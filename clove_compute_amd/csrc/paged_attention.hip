@@ -22,9 +22,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
     PagedAttentionArgs a;
-    int group;      // query heads per KV head
-    float* scores;  // [batch, q_heads, max_context] base 2, -inf where unseen; null: not wanted
-    float2* stats;  // [batch, q_heads] (m, l)
+    FastDiv page;        // by the page size
+    int group;           // query heads per KV head
+    int tiles;           // tiles of 16 query heads per KV head (MFMA kernel)
+    int chunk, splits;   // keys per workgroup (a multiple of 32), workgroups per (sequence, KV head, tile) at most
+    float* partials;     // [sequence, KV head, tile, split] slabs of `slab` floats; null: one split
+    unsigned* counters;  // [sequence, KV head, tile]
+    int slab;
+    float* scores;       // [batch, q_heads] rows of score_stride, base 2, -inf where unseen; null: not wanted
+    int64_t score_stride;
+    float2* stats;       // [batch, q_heads] (m, l)
 };
 
 // score in base 2 of the scaled dot product
@@ -38,9 +45,10 @@ __device__ __forceinline__ int context(const PagedAttentionArgs& a, int b) {
 }
 
 // Element offset of key j's row (of KV head `kh`), or -1 where its page is absent.
-__device__ __forceinline__ int64_t row_at(const PagedAttentionArgs& a, int b, int kh, int j) {
+__device__ __forceinline__ int64_t row_at(const Params& p, int b, int kh, int j) {
+    const PagedAttentionArgs& a = p.a;
     const PagedCache& c = a.cache;
-    const int page = j / c.page_size, row = j - page * c.page_size;
+    const int page = p.page.div(j), row = j - page * c.page_size;
     const int id = a.block_table[b * a.table_stride + page];
     if ((unsigned)id >= (unsigned)c.num_pages) return -1;
     return (int64_t)id * c.page_stride + ((int64_t)kh * c.page_size + row) * c.head_dim;
@@ -66,9 +74,9 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
         q[e] = lane + 64 * e < D ? T::load(qr[lane + 64 * e]) : 0.0f;
         o[e] = 0.0f;
     }
-    float* scores = p.scores ? p.scores + ((int64_t)b * a.q_heads + h) * a.max_context : nullptr;
+    float* scores = p.scores ? p.scores + ((int64_t)b * a.q_heads + h) * p.score_stride : nullptr;
     for (int j = first + wave; j < n; j += 4) {
-        const int64_t at = row_at(a, b, kh, j);
+        const int64_t at = row_at(p, b, kh, j);
         if (at < 0) {
             if (scores && lane == 0) scores[j] = -__builtin_inff();
             continue;
@@ -120,11 +128,11 @@ __global__ void __launch_bounds__(256) add_weights(const Params p, int blocks) {
     const int b = blockIdx.x / blocks, j = (blockIdx.x - b * blocks) * 256 + threadIdx.x;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0;
     if (j < first || j >= n) return;
-    const float* s = p.scores + (int64_t)b * a.q_heads * a.max_context + j;
+    const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + j;
     const float2* st = p.stats + (int64_t)b * a.q_heads;
     float sum = 0.0f;
     for (int h = 0; h < a.q_heads; ++h) {
-        const float w = exp2f(s[(int64_t)h * a.max_context] - st[h].x) / st[h].y;
+        const float w = exp2f(s[(int64_t)h * p.score_stride] - st[h].x) / st[h].y;
         if (st[h].y != 0.0f) sum += w;
     }
     a.weights[b * a.weights_stride + j] += sum;
@@ -137,21 +145,426 @@ void launch_any(const Params& p, hipStream_t stream) {
     CLOVE_LAUNCH(kernel, dim3((unsigned)(p.a.batch * p.a.q_heads)), dim3(256), 0, stream, p);
 }
 
+// ---------------------------------------------------------------------------
+// head_dim 8 .. 256: MFMA
+//
+// A workgroup of four waves takes `chunk` keys of one (sequence, KV head, tile
+// of up to 16 query heads); a wave takes every fourth 32 of them.  With keys as
+// rows and query heads as columns of v_mfma_f32_16x16x32,
+//   S [16 keys x 16 heads] = K [keys x d] Q^T [d x heads]       (two of them)
+//   O^T [d x heads] += V^T [d x 32 keys] P^T [32 keys x heads]
+// K's operand is K's row in memory (lane l: key l % 16, 8 elements from 8 (l / 16)
+// of each 32), and a lane gets four scores of its head (l % 16) per 16 keys: the
+// P^T operand of the second product, if its 8 k-slots of lane group g name the
+// keys 4 g .. 4 g + 3 of either 16.  So softmax needs no exchange but the
+// maximum over the four lane groups, and only V passes through LDS, private to
+// the wave, where ds_read_b64_tr_b16 turns its rows.  P is used as the sum of two
+// 16-bit numbers (16 bits in bf16, 22 in fp16), so that what a result loses is its
+// own rounding alone; the second product's MFMAs hide under the loads.
+//
+// Registers of K are loaded for the wave's next 32 keys as soon as the first
+// product has read them, those of V as soon as they are in LDS: 8 to 16 KB (at
+// head_dim 128) are in flight per wave nearly all the time.
+//
+// Workgroups of one (sequence, KV head, tile) publish (O, m, l) past the L2s; the
+// last to arrive joins them in the order of the splits.
+// ---------------------------------------------------------------------------
+template <int DT>
+struct Mfma;
+template <>
+struct Mfma<CLOVE_DTYPE_FP16> {
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<f16x8>(a), bitcast<f16x8>(b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mfma<CLOVE_DTYPE_BF16> {
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<bf16x8>(a), bitcast<bf16x8>(b), c, 0, 0, 0);
+    }
+};
+
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float groups_max(float x) {
+    const auto s = __builtin_amdgcn_permlane16_swap(bitcast<unsigned>(x), bitcast<unsigned>(x), false, false);
+    const float y = fmaxf(bitcast<float>(s[0]), bitcast<float>(s[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(bitcast<unsigned>(y), bitcast<unsigned>(y), false, false);
+    return fmaxf(bitcast<float>(t[0]), bitcast<float>(t[1]));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+    const float y = swap_sum16(x, x);
+    return swap_sum32(y, y);
+}
+
+constexpr int kW = 4;  // waves of a workgroup
+
+template <int NC>
+constexpr int row_bytes() { return NC * 64 + 32; }  // a V row in LDS: 8 banks further each row
+template <int NC>
+constexpr int wave_lds() { return 32 * row_bytes<NC>(); }
+// after the keys the same LDS holds the waves' O [16 heads][32 NC + 4] and (m, l) [16]
+template <int NC>
+constexpr int o_stride() { return 32 * NC + 4; }
+static_assert(16 * o_stride<1>() * 4 + 128 <= wave_lds<1>() && 16 * o_stride<8>() * 4 + 128 <= wave_lds<8>(), "O fits where V was");
+
+// Sixteen bytes of a row from element d: the first D - d elements of it where
+// there are fewer than 8 (TAIL: rows at any alignment, head_dim any number).
+template <bool TAIL>
+__device__ __forceinline__ u32x4 load_row(const uint16_t* row, int d, int D) {
+    if constexpr (!TAIL) return *reinterpret_cast<const u32x4*>(row + d);
+    const int back = max(d + 8 - D, 0);  // the last 8 elements of the row, moved down
+    const u32x4 x = load_any16(reinterpret_cast<const unsigned char*>(row + d - back));
+    return back ? shift_bytes(x, 2 * back) : x;
+}
+
+typedef short i16x4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4v lds_i16x4v;
+__device__ __forceinline__ u32x2 lds_turned(const char* p) {
+    return bitcast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4v*)p));
+}
+
+template <int DT>
+__device__ __forceinline__ unsigned pack2(float lo, float hi) {
+    return (unsigned)Elem<DT>::store(lo) | ((unsigned)Elem<DT>::store(hi) << 16);
+}
+
+// Four outputs of one row from element d.
+template <int DT>
+__device__ __forceinline__ void store4(uint16_t* row, int d, int D, bool vec, const f32x4& x) {
+    if (vec && d + 4 <= D) {
+        *reinterpret_cast<u32x2*>(row + d) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (d + i < D) row[d + i] = Elem<DT>::store(x[i]);
+}
+
+// Running (m, l, o) of disjoint keys merged: both maxima may be -infinity.
+__device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, float l2, const f32x4& o2) {
+    const float top = fmaxf(m, m2), sub = finite_max(top);
+    const float f = exp2f(m - sub), f2 = exp2f(m2 - sub);
+    m = top;
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * f + o2[i] * f2;
+}
+
+template <int DT, int NC, bool TAIL>
+__global__ void __launch_bounds__(64 * kW) attend(const Params p) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ int last;
+    const PagedAttentionArgs& a = p.a;
+    const PagedCache& cache = a.cache;
+    const int split = blockIdx.x % p.splits, pair = blockIdx.x / p.splits;
+    const int tile = pair % p.tiles, bk = pair / p.tiles, b = bk / cache.kv_heads, kh = bk - b * cache.kv_heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+    const int D = cache.head_dim, G = min(16, p.group - 16 * tile), h0 = kh * p.group + 16 * tile;
+    const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0, base = first & ~31;
+    const int total = max(1, cdiv(n - base, p.chunk));  // workgroups that have keys (one of them where there are none)
+    if (split >= total) return;
+    const int begin = base + split * p.chunk, end = min(n, begin + p.chunk);
+    const bool vec = !TAIL;
+
+    u32x4 q[NC];
+    const uint16_t* qr = a.q + b * a.q_stride + (int64_t)(h0 + min(row, G - 1)) * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = 32 * c + 8 * g;
+        q[c] = row < G && d < D ? load_row<TAIL>(qr, d, D) : u32x4{0u, 0u, 0u, 0u};
+    }
+
+    // the pages of this lane's two keys (16 apart) of the wave's 32 from key j
+    const int32_t* table = a.block_table + b * a.table_stride;
+    auto page_of = [&](int j) { return j >= first && j < end ? table[p.page.div(j)] : -1; };
+    auto offset_of = [&](int j, int id, bool& ok) {
+        ok = (unsigned)id < (unsigned)cache.num_pages;
+        const int in_page = j - p.page.div(j) * cache.page_size;
+        return ok ? (int64_t)id * cache.page_stride + ((int64_t)kh * cache.page_size + in_page) * D : (int64_t)0;
+    };
+    u32x4 k[2][NC], v[2][NC];
+    int64_t off[2];
+    unsigned seen = 0, seen_next = 0;  // bit i: key i of the 32 is there
+    int id[2];
+    auto look_up = [&](int j) {
+        id[0] = page_of(j + row);
+        id[1] = page_of(j + 16 + row);
+    };
+    auto resolve = [&](int j) {
+        bool ok0, ok1;
+        off[0] = offset_of(j + row, id[0], ok0);
+        off[1] = offset_of(j + 16 + row, id[1], ok1);
+        seen_next = (unsigned)(__ballot(ok0) & 0xffffu) | ((unsigned)(__ballot(ok1) & 0xffffu) << 16);
+    };
+    // (an absent key's loads go to the first row of the cache and are dropped;
+    // where none of the 32 is there, nothing is loaded)
+    auto load = [&](u32x4(&x)[2][NC], const uint16_t* from) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = 32 * c + 8 * g;
+                x[r][c] = load_row<TAIL>(from + off[r], d < D ? d : 0, D);
+            }
+    };
+    // lanes past the end of the row hold zeros there
+    auto clip = [&](u32x4(&x)[2][NC]) {
+        if (32 * (NC - 1) + 8 * g >= D) x[0][NC - 1] = x[1][NC - 1] = u32x4{0u, 0u, 0u, 0u};
+    };
+
+    float m = -__builtin_inff(), l = 0.0f;
+    f32x4 o[2 * NC];
+#pragma unroll
+    for (int c = 0; c < 2 * NC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    char* const vs = lds + wave * wave_lds<NC>();
+    const char* const turned = vs + (4 * g + (row >> 2)) * row_bytes<NC>() + 8 * (row & 3);
+    float* score_row = p.scores && row < G ? p.scores + ((int64_t)b * a.q_heads + h0 + row) * p.score_stride : nullptr;
+
+    int j = begin + 32 * wave;
+    look_up(j);
+    resolve(j);
+    if (seen_next) {
+        load(k, cache.k);
+        load(v, cache.v);
+    }
+    look_up(j + 32 * kW);
+    for (; j < end; j += 32 * kW) {
+        seen = seen_next;
+        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        if (seen) {
+            clip(k);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s[0] = Mfma<DT>::mul(k[0][c], q[c], s[0]);
+                s[1] = Mfma<DT>::mul(k[1][c], q[c], s[1]);
+            }
+        }
+        resolve(j + 32 * kW);
+        if (seen_next) load(k, cache.k);
+        look_up(j + 64 * kW);
+        if (seen) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[r][i] = base2(a, s[r][i]);
+            if (seen != 0xffffffffu) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!((seen >> (16 * r + 4 * g + i)) & 1u)) s[r][i] = -__builtin_inff();
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    if (!((seen >> (16 * r + row)) & 1u))
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) v[r][c] = u32x4{0u, 0u, 0u, 0u};
+            }
+            clip(v);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    *reinterpret_cast<u32x4*>(vs + (16 * r + row) * row_bytes<NC>() + 64 * c + 16 * g) = v[r][c];
+        } else {
+            s[0] = s[1] = f32x4{-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+        }
+        if (score_row) {  // rows are long enough for whole 32 keys
+            *reinterpret_cast<f32x4*>(score_row + j + 4 * g) = s[0];
+            *reinterpret_cast<f32x4*>(score_row + j + 16 + 4 * g) = s[1];
+        }
+        if (seen_next) load(v, cache.v);
+        if (!seen) continue;
+
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+        top = groups_max(top);
+        const float sub = finite_max(top);
+        if (__any(top != m)) {
+            const float f = exp2f(m - sub);
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < 2 * NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][i] *= f;
+            m = top;
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float x = exp2f(s[r][i] - sub), y = exp2f(s[r][i + 1] - sub);
+                l += x + y;
+                const unsigned h = pack2<DT>(x, y);
+                hi[2 * r + i / 2] = h;
+                lo[2 * r + i / 2] = pack2<DT>(x - Elem<DT>::load((uint16_t)(h & 0xffffu)), y - Elem<DT>::load((uint16_t)(h >> 16)));
+            }
+#pragma unroll
+        for (int c = 0; c < 2 * NC; ++c) {
+            const u32x2 x = lds_turned(turned + 32 * c), y = lds_turned(turned + 16 * row_bytes<NC>() + 32 * c);
+            const u32x4 vt{x[0], x[1], y[0], y[1]};
+            o[c] = Mfma<DT>::mul(vt, hi, o[c]);
+            o[c] = Mfma<DT>::mul(vt, lo, o[c]);
+        }
+    }
+    l = groups_sum(l);
+
+    // the four waves, merged in their order
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(lds + wave * wave_lds<NC>());
+    if (row < G) {
+#pragma unroll
+        for (int c = 0; c < 2 * NC; ++c) *reinterpret_cast<f32x4*>(mine + row * o_stride<NC>() + 16 * c + 4 * g) = o[c];
+        if (g == 0) *reinterpret_cast<float2*>(mine + 16 * o_stride<NC>() + 2 * row) = float2{m, l};
+    }
+    __syncthreads();
+    const int quads = cdiv(D, 4), items = G * quads;
+    float* const slabs = p.partials + (int64_t)pair * p.splits * p.slab;
+    auto finish = [&](int h, int quad, float M, float L, const f32x4& O) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = L == 0.0f ? 0.0f : O[i] / L;
+        store4<DT>(a.out + b * a.out_stride + (int64_t)(h0 + h) * D, 4 * quad, D, vec, x);
+        if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L};
+    };
+    const __amdgpu_buffer_rsrc_t slab_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        slabs + (int64_t)split * p.slab, (short)0, total > 1 ? p.slab * 4 : 0, 0x00020000);
+    for (int i = threadIdx.x; i < items; i += 64 * kW) {
+        const int h = i / quads, quad = i - h * quads;
+        float M = -__builtin_inff(), L = 0.0f;
+        f32x4 O{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kW; ++w) {
+            const float* x = reinterpret_cast<const float*>(lds + w * wave_lds<NC>());
+            const float2 ml = *reinterpret_cast<const float2*>(x + 16 * o_stride<NC>() + 2 * h);
+            merge(M, L, O, ml.x, ml.y, *reinterpret_cast<const f32x4*>(x + h * o_stride<NC>() + 4 * quad));
+        }
+        if (total == 1) {
+            finish(h, quad, M, L, O);
+        } else {
+            __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(O), slab_rsrc, (h * quads + quad) * 16, 0, kCpolSc1);
+            if (quad == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{bitcast<unsigned>(M), bitcast<unsigned>(L)}, slab_rsrc,
+                                                      16 * 16 * quads + 8 * h, 0, kCpolSc1);
+        }
+    }
+    if (total == 1 || !splitk_arrive_is_last(p.counters + pair, total, &last)) return;
+
+    // the last workgroup joins the splits: teams of `items` threads take runs of
+    // them, then team 0 merges the teams
+    const int teams = max(1, min(64 * kW / items, total)), run = cdiv(total, teams);
+    f32x4* const team_o = reinterpret_cast<f32x4*>(lds);
+    float2* const team_ml = reinterpret_cast<float2*>(lds + 64 * kW * 16);
+    for (int i0 = 0; i0 < items; i0 += 64 * kW) {
+        const int i = i0 + (int)threadIdx.x, team = teams > 1 ? i / items : 0, item = teams > 1 ? i - team * items : i;
+        const bool on = team < teams && item < items;
+        const int h = on ? item / quads : 0, quad = on ? item - h * quads : 0;
+        float M = -__builtin_inff(), L = 0.0f;
+        f32x4 O{0.f, 0.f, 0.f, 0.f};
+        if (on) {
+            constexpr int U = 8;
+            const int s1 = min(total, (team + 1) * run);
+            for (int s0 = team * run; s0 < s1; s0 += U) {
+                u32x4 x[U];
+                u32x2 ml[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (s0 + u >= s1) break;
+                    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(slabs + (int64_t)(s0 + u) * p.slab, (short)0,
+                                                                                       p.slab * 4, 0x00020000);
+                    x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (h * quads + quad) * 16, 0, kCpolSc1);
+                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, 16 * 16 * quads + 8 * h, 0, kCpolSc1);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (s0 + u >= s1) break;
+                    merge(M, L, O, bitcast<float>(ml[u][0]), bitcast<float>(ml[u][1]), bitcast<f32x4>(x[u]));
+                }
+            }
+        }
+        if (teams > 1) {  // (then items < 64 kW: one round)
+            __syncthreads();
+            team_o[threadIdx.x] = O;
+            team_ml[threadIdx.x] = float2{M, L};
+            __syncthreads();
+            if (team == 0)
+                for (int t = 1; t < teams; ++t) {
+                    const float2 ml = team_ml[t * items + item];
+                    merge(M, L, O, ml.x, ml.y, team_o[t * items + item]);
+                }
+        }
+        if (on && team == 0) finish(h, quad, M, L, O);
+    }
+}
+
+template <int DT, bool TAIL>
+clove_status_t launch_mfma(const Params& p, hipStream_t stream) {
+    typedef void (*Kernel)(const Params);
+    static const Kernel kernels[8] = {attend<DT, 1, TAIL>, attend<DT, 2, TAIL>, attend<DT, 3, TAIL>, attend<DT, 4, TAIL>,
+                                      attend<DT, 5, TAIL>, attend<DT, 6, TAIL>, attend<DT, 7, TAIL>, attend<DT, 8, TAIL>};
+    static const int bytes[8] = {wave_lds<1>(), wave_lds<2>(), wave_lds<3>(), wave_lds<4>(),
+                                 wave_lds<5>(), wave_lds<6>(), wave_lds<7>(), wave_lds<8>()};
+    const int nc = cdiv(p.a.cache.head_dim, 32) - 1;
+    const int64_t grid = (int64_t)p.a.batch * p.a.cache.kv_heads * p.tiles * p.splits;
+    const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(kernels[nc]), kW * bytes[nc]);
+    if (st != CLOVE_OK) return st;
+    CLOVE_LAUNCH(kernels[nc], dim3((unsigned)grid), dim3(64 * kW), (size_t)kW * bytes[nc], stream, p);
+    return CLOVE_OK;
+}
+
 }  // namespace paged
 
 clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream) {
-    clove_status_t st;
-    paged::Params p{a, a.q_heads / a.cache.kv_heads, nullptr, nullptr};
+    DeviceInfo dev;
+    clove_status_t st = current_device_info(&dev);
+    if (st != CLOVE_OK) return st;
+    const PagedCache& c = a.cache;
+    paged::Params p{};
+    p.a = a;
+    p.page = FastDiv(c.page_size);
+    p.group = a.q_heads / c.kv_heads;
+    p.score_stride = (int64_t)hw::cdiv(a.max_context, 32) * 32;
     if (a.weights && a.max_context > 0) {
         const size_t heads = (size_t)a.batch * a.q_heads;
         void* buf = nullptr;
-        if ((st = acquire_buffer(stream, kBufDecode, heads * (a.max_context * sizeof(float) + sizeof(float2)), &buf)) != CLOVE_OK)
+        if ((st = acquire_buffer(stream, kBufDecode, heads * (p.score_stride * sizeof(float) + sizeof(float2)) + 16, &buf)) != CLOVE_OK)
             return st;
-        p.stats = static_cast<float2*>(buf);
-        p.scores = reinterpret_cast<float*>(p.stats + heads);
+        p.scores = static_cast<float*>(buf);
+        p.stats = reinterpret_cast<float2*>(p.scores + heads * p.score_stride);
     }
-    if (a.cache.dtype == CLOVE_DTYPE_FP16) paged::launch_any<CLOVE_DTYPE_FP16>(p, stream);
-    else paged::launch_any<CLOVE_DTYPE_BF16>(p, stream);
+    if (c.head_dim < 8 || c.head_dim > 256) {
+        if (c.dtype == CLOVE_DTYPE_FP16) paged::launch_any<CLOVE_DTYPE_FP16>(p, stream);
+        else paged::launch_any<CLOVE_DTYPE_BF16>(p, stream);
+    } else {
+        p.tiles = hw::cdiv(p.group, 16);
+        const int64_t pairs = (int64_t)a.batch * c.kv_heads * p.tiles;
+        // a window need not start at a whole 32 keys
+        const int span = std::max(1, a.window > 0 ? (int)std::min<int64_t>(a.max_context, (int64_t)a.window + 31) : a.max_context);
+        int64_t chunk = hw::cdiv64((int64_t)span * pairs, 3 * dev.num_cus);
+        chunk = std::max<int64_t>(chunk, 128);
+        chunk = std::max<int64_t>(std::min<int64_t>(chunk, 1024), (int64_t)span * pairs >> 28);
+        p.chunk = (int)(hw::cdiv64(chunk, 128) * 128);
+        p.splits = hw::cdiv(span, p.chunk);
+        if (pairs > 16384 || p.splits == 1) {
+            p.splits = 1;
+            p.chunk = (int)std::min<int64_t>(hw::cdiv64(span, 128) * 128, 0x7fffff80);
+        } else {
+            p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
+            Scratch scratch;
+            if ((st = acquire_scratch(stream, (size_t)pairs * p.splits * p.slab * 4, (size_t)pairs, &scratch)) != CLOVE_OK) return st;
+            p.partials = scratch.partials;
+            p.counters = scratch.counters;
+        }
+        const bool whole = c.head_dim % 8 == 0 && c.page_stride % 8 == 0 && a.q_stride % 8 == 0 && a.out_stride % 4 == 0 &&
+                           aligned16(a.q) && aligned16(c.k) && aligned16(c.v) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
+        if (c.dtype == CLOVE_DTYPE_FP16)
+            st = whole ? paged::launch_mfma<CLOVE_DTYPE_FP16, false>(p, stream) : paged::launch_mfma<CLOVE_DTYPE_FP16, true>(p, stream);
+        else
+            st = whole ? paged::launch_mfma<CLOVE_DTYPE_BF16, false>(p, stream) : paged::launch_mfma<CLOVE_DTYPE_BF16, true>(p, stream);
+        if (st != CLOVE_OK) return st;
+    }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;
     const int blocks = hw::cdiv(a.max_context, 256);
     CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(256), 0, stream, p, blocks);

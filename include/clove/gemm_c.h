@@ -258,8 +258,9 @@ typedef enum clove_dtype {
     CLOVE_DTYPE_FP32 = 2 /* logits only */
 } clove_dtype_t;
 
-/* Largest head_dim of these operators. */
+/* Largest head_dim and max_context of these operators. */
 #define CLOVE_MAX_HEAD_DIM 1024
+#define CLOVE_MAX_CONTEXT (1 << 30)
 
 /* The key-value cache of one layer, in pages.  Key (page, head, row) starts at
  * element page * page_stride + (head * page_size + row) * head_dim of `k`, its
