@@ -13,51 +13,62 @@ elements of a row are adjacent.
 from __future__ import annotations
 
 import ctypes
-import math
 
 from . import _lib
 from .gemm import _stream
 
-_CODES = {}  # torch dtype -> clove_dtype_t
+class _Bound:
+    """What every call needs, looked up on the first: the library's functions and
+    torch's element types (importing torch and resolving a function by name cost
+    a microsecond a call, a third of what the smallest kernels take)."""
+
+    def __getattr__(self, name):
+        import torch
+        lib = _lib.lib()
+        self.f16, self.f32, self.i32 = torch.float16, torch.float32, torch.int32
+        self.codes = {torch.float16: _lib.CLOVE_DTYPE_FP16, torch.bfloat16: _lib.CLOVE_DTYPE_BF16,
+                      torch.float32: _lib.CLOVE_DTYPE_FP32}
+        self.rope, self.attend = lib.clove_qk_norm_rope, lib.clove_paged_attention
+        self.evict, self.penalize = lib.clove_cache_evict, lib.clove_penalize_logits
+        return self.__dict__[name]
 
 
-def _codes():
-    import torch
-    _CODES.update({torch.float16: _lib.CLOVE_DTYPE_FP16, torch.bfloat16: _lib.CLOVE_DTYPE_BF16,
-                   torch.float32: _lib.CLOVE_DTYPE_FP32})
-    return _CODES
+_b = _Bound()
 
 
-def _code(x) -> int:
-    c = _CODES.get(x.dtype)
+def _code(dtype) -> int:
+    c = _b.codes.get(dtype)
     if c is None:
-        c = _codes().get(x.dtype)
-        if c is None:
-            raise ValueError(f"element type {x.dtype} is not fp16, bf16 or fp32")
+        raise ValueError(f"element type {dtype} is not fp16, bf16 or fp32")
     return c
 
 
-def _rows(x, name, rows, width, dtype=None):
-    """(address, row stride) of a tensor read as `rows` rows of `width` elements;
-    its first dimension is the row where it has more than one."""
-    if not x.is_cuda:
-        raise ValueError(f"{name} must live on the GPU")
-    if dtype is not None and x.dtype != dtype:
-        raise ValueError(f"{name} is {x.dtype}, not {dtype}")
-    if x.dim() < 2:
-        if x.dim() == 1 and x.numel() >= rows * width and (x.numel() < 2 or x.stride(0) == 1):
-            return x.data_ptr(), width
+def _rows(x, name, rows, width, dtype):
+    """(address, row stride) of a tensor read as `rows` rows of `width` adjacent
+    elements; its first dimension is the row where it has more than one."""
+    if x.dtype is not dtype or not x.is_cuda:
+        raise ValueError(f"{name} must be {dtype} on the GPU, not {x.dtype} on {x.device}")
+    if x.numel() == rows * width and x.is_contiguous():
+        return x.data_ptr(), width
+    shape, strides = x.shape, x.stride()
+    n, inner = shape[0] if shape else 1, 1
+    if len(shape) < 2:
+        n, shape, strides = 1, (1, *shape), (n, *strides)
+    for size, stride in zip(shape[:0:-1], strides[:0:-1]):
+        if size != 1 and stride != inner:
+            inner = -1
+            break
+        inner *= size
+    if n < rows or inner < width:
         raise ValueError(f"{name} holds {tuple(x.shape)} elements, {rows} rows of {width} adjacent ones are wanted")
-    if x.shape[0] < rows or x.numel() < x.shape[0] * width or (rows and x.numel() and not x[0].is_contiguous()):
-        raise ValueError(f"{name} holds {tuple(x.shape)} elements, {rows} rows of {width} adjacent ones are wanted")
-    return x.data_ptr(), (x.stride(0) if rows > 1 else max(width, x.stride(0)))
+    return x.data_ptr(), strides[0] if rows > 1 else max(width, strides[0])
 
 
 def _flat(x, name, n, dtype):
     """Address of at least `n` adjacent elements (None stays None)."""
     if x is None:
         return None
-    if not x.is_cuda or x.dtype != dtype or x.numel() < n or not x.is_contiguous():
+    if x.dtype is not dtype or not x.is_cuda or x.numel() < n or not x.is_contiguous():
         raise ValueError(f"{name} must be {n} adjacent {dtype} elements on the GPU, not {tuple(x.shape)} {x.dtype}")
     return x.data_ptr()
 
@@ -80,7 +91,7 @@ class KVCache:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype = k.dtype
         self._c = _lib.KVCacheDesc(k.data_ptr(), v.data_ptr(), k.stride(0) if k.shape[0] > 1 else 0, self.num_pages,
-                                   self.page_size, self.kv_heads, self.head_dim, _code(k))
+                                   self.page_size, self.kv_heads, self.head_dim, _code(k.dtype))
         self._ref = ctypes.byref(self._c)
 
 
@@ -91,24 +102,22 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, positions, q_out, T: int, q_
     ``rot_dim`` (default: all) elements by ``cos`` / ``sin`` [max_position, rot_dim / 2] at
     ``positions`` [T], and the write of keys and values into ``slots`` [T] of ``cache``: one pass
     over the fused projection's rows ``qkv`` [T, (q_heads + 2 kv_heads) head_dim]."""
-    import torch
     R = head_dim if rot_dim is None else rot_dim
-    dt, half = qkv.dtype, R // 2
-    x, xs = _rows(qkv, "qkv", T, (q_heads + 2 * kv_heads) * head_dim)
+    dt, i, half, most = qkv.dtype, _b.i32, R // 2, 0
+    x, xs = _rows(qkv, "qkv", T, (q_heads + 2 * kv_heads) * head_dim, dt)
     q, qs = _rows(q_out, "q_out", T, q_heads * head_dim, dt)
     k, ks = _rows(k_out, "k_out", T, kv_heads * head_dim, dt) if k_out is not None else (None, 0)
-    most = 0
+    c = s = None
     if R:
         most = cos.shape[0]
-        if cos.dim() != 2 or cos.shape[1] != half or sin.shape != cos.shape:
+        c, s = _flat(cos, "cos", most * half, _b.f32), _flat(sin, "sin", most * half, _b.f32)
+        if cos.numel() != most * half or sin.shape != cos.shape:
             raise ValueError(f"cos and sin are [max_position, {half}], not {tuple(cos.shape)} and {tuple(sin.shape)}")
-    _lib.check(_lib.lib().clove_qk_norm_rope(
-        x, xs, _flat(q_weight, "q_weight", head_dim, dt), _flat(k_weight, "k_weight", head_dim, dt), eps,
-        _flat(cos, "cos", most * half, torch.float32) if R else None,
-        _flat(sin, "sin", most * half, torch.float32) if R else None, most,
-        _flat(positions, "positions", T, torch.int32) if R else None, q, qs, k, ks,
-        cache._ref if cache is not None else None, _flat(slots, "slots", T, torch.int32), T, q_heads, kv_heads, head_dim,
-        R, 1 if interleaved else 0, _code(qkv), _stream(stream)), "qk_norm_rope")
+    st = _b.rope(x, xs, _flat(q_weight, "q_weight", head_dim, dt), _flat(k_weight, "k_weight", head_dim, dt), eps, c, s, most,
+                 _flat(positions, "positions", T, i) if R else None, q, qs, k, ks, None if cache is None else cache._ref,
+                 _flat(slots, "slots", T, i), T, q_heads, kv_heads, head_dim, R, interleaved, _code(dt), _stream(stream))
+    if st:
+        _lib.check(st, "qk_norm_rope")
 
 
 def paged_attention(q, cache: KVCache, block_table, context_lens, out, batch: int, q_heads: int, max_context: int,
@@ -118,16 +127,15 @@ def paged_attention(q, cache: KVCache, block_table, context_lens, out, batch: in
     ``scale`` defaults to head_dim ** -0.5; ``window`` > 0 sees the last keys only; ``softcap`` > 0
     bounds the scores; ``weights`` [batch, max_context] fp32 gains each key's softmax weight,
     summed over the heads."""
-    import torch
-    D, dt = cache.head_dim, cache.dtype
+    D, dt, i = cache.head_dim, cache.dtype, _b.i32
     x, xs = _rows(q, "q", batch, q_heads * D, dt)
     o, os_ = _rows(out, "out", batch, q_heads * D, dt)
-    t, ts = _rows(block_table, "block_table", batch, -(-max_context // cache.page_size), torch.int32)
-    w, ws = _rows(weights, "weights", batch, max_context, torch.float32) if weights is not None else (None, 0)
-    _lib.check(_lib.lib().clove_paged_attention(
-        x, xs, cache._ref, t, ts, _flat(context_lens, "context_lens", batch, torch.int32), o, os_, w, ws, batch, q_heads,
-        max_context, 1.0 / math.sqrt(D) if scale is None else scale, softcap, window, _stream(stream)),
-        "paged_attention")
+    t, ts = _rows(block_table, "block_table", batch, -(-max_context // cache.page_size), i)
+    w, ws = _rows(weights, "weights", batch, max_context, _b.f32) if weights is not None else (None, 0)
+    st = _b.attend(x, xs, cache._ref, t, ts, _flat(context_lens, "context_lens", batch, i), o, os_, w, ws, batch, q_heads,
+                   max_context, D ** -0.5 if scale is None else scale, softcap, window, _stream(stream))
+    if st:
+        _lib.check(st, "paged_attention")
 
 
 def cache_evict(cache: KVCache, block_table, context_lens, weights, positions, weights_out, positions_out, lens_out,
@@ -136,16 +144,16 @@ def cache_evict(cache: KVCache, block_table, context_lens, weights, positions, w
     ``sinks`` and the newest ``recent`` positions stay, then those of the largest ``weights``
     [batch, max_context]; kept tokens past the budget move into the holes below it.  Outputs hold the
     new weights, positions and lengths, and may be the inputs."""
-    import torch
-    f, i = torch.float32, torch.int32
+    f, i = _b.f32, _b.i32
     t, ts = _rows(block_table, "block_table", batch, -(-max_context // cache.page_size), i)
     w, ws = _rows(weights, "weights", batch, max_context, f)
     p, ps = _rows(positions, "positions", batch, max_context, i)
     wo, wos = _rows(weights_out, "weights_out", batch, max_context, f)
     po, pos = _rows(positions_out, "positions_out", batch, max_context, i)
-    _lib.check(_lib.lib().clove_cache_evict(
-        cache._ref, t, ts, _flat(context_lens, "context_lens", batch, i), w, ws, p, ps, wo, wos, po, pos,
-        _flat(lens_out, "lens_out", batch, i), batch, max_context, budget, sinks, recent, _stream(stream)), "cache_evict")
+    st = _b.evict(cache._ref, t, ts, _flat(context_lens, "context_lens", batch, i), w, ws, p, ps, wo, wos, po, pos,
+                  _flat(lens_out, "lens_out", batch, i), batch, max_context, budget, sinks, recent, _stream(stream))
+    if st:
+        _lib.check(st, "cache_evict")
 
 
 def penalize_logits(logits, out, batch: int, vocab: int, history=None, history_lens=None, prompt_lens=None,
@@ -156,22 +164,25 @@ def penalize_logits(logits, out, batch: int, vocab: int, history=None, history_l
     past ``prompt_lens``, the biases of ``bias_ids`` / ``bias_values`` (the last entry for a token
     counts) and the mask ``allowed`` [batch, ceil(vocab / 32)] (int32 words, token v is bit v % 32;
     a clear bit gives -inf).  fp32 inside; ``out`` is fp32 or of the logits' type."""
-    import torch
-    f, i = torch.float32, torch.int32
-    x, xs = _rows(logits, "logits", batch, vocab)
-    o, os_ = _rows(out, "out", batch, vocab)
-    h, hs = (_rows(history, "history", batch, history.shape[-1], i)) if history is not None else (None, 0)
-    b, bs = (_rows(bias_ids, "bias_ids", batch, bias_ids.shape[-1], i)) if bias_ids is not None else (None, 0)
-    if b is not None:
-        bv, bvs = _rows(bias_values, "bias_values", batch, bias_ids.shape[-1], f)
-        if bvs != bs:
+    f, i = _b.f32, _b.i32
+    x, xs = _rows(logits, "logits", batch, vocab, logits.dtype)
+    o, os_ = _rows(out, "out", batch, vocab, out.dtype)
+    h = b = bv = m = None
+    hs = bs = ms = 0
+    if history is not None:
+        h, hs = _rows(history, "history", batch, history.shape[-1], i)
+    if bias_ids is not None:
+        n = bias_ids.shape[-1]
+        b, bs = _rows(bias_ids, "bias_ids", batch, n, i)
+        bv, ms = _rows(bias_values, "bias_values", batch, n, f)
+        if ms != bs:
             raise ValueError("the rows of bias_ids and bias_values must be equally far apart")
-    else:
-        bv = None
-    m, ms = _rows(allowed, "allowed", batch, -(-vocab // 32), i) if allowed is not None else (None, 0)
-    _lib.check(_lib.lib().clove_penalize_logits(
-        x, xs, _code(logits), o, os_, _code(out), batch, vocab, h, hs,
-        _flat(history_lens, "history_lens", batch, i), _flat(prompt_lens, "prompt_lens", batch, i),
-        _flat(repetition, "repetition", batch, f), _flat(presence, "presence", batch, f),
-        _flat(frequency, "frequency", batch, f), b, bv, bs, _flat(bias_counts, "bias_counts", batch, i), m, ms,
-        _stream(stream)), "penalize_logits")
+    if allowed is not None:
+        m, ms = _rows(allowed, "allowed", batch, -(-vocab // 32), i)
+    st = _b.penalize(x, xs, _code(logits.dtype), o, os_, _code(out.dtype), batch, vocab, h, hs,
+                     _flat(history_lens, "history_lens", batch, i), _flat(prompt_lens, "prompt_lens", batch, i),
+                     _flat(repetition, "repetition", batch, f), _flat(presence, "presence", batch, f),
+                     _flat(frequency, "frequency", batch, f), b, bv, bs, _flat(bias_counts, "bias_counts", batch, i), m, ms,
+                     _stream(stream))
+    if st:
+        _lib.check(st, "penalize_logits")
