@@ -3,10 +3,14 @@
 //   x = logits[v];  seen: x > 0 ? x / r : x * r;  x -= f c + p [c > 0];
 //   x += bias[v];  disallowed: -inf                          (fp32 throughout)
 //
-// A workgroup owns a slice of one row's vocabulary.  How often each token of
-// the slice was produced comes from the row's history, counted in LDS (whole
-// numbers: atomics give the same counts in any order), so nothing of the
-// vocabulary's size is written to memory but the result.
+// A workgroup owns a slice of one row's vocabulary, 16 tokens a thread.  How
+// often each token of the slice was produced comes from the row's history,
+// counted in LDS (whole numbers: atomics give the same counts in any order), so
+// nothing of the vocabulary's size is written to memory but the result.  Bound
+// by HBM for large batches: the slice's logits are loaded before the history is
+// read, which every slice of a row reads anew (from L2), so slices are as long
+// as a batch leaves room for: 256 rows of 128000 logits with 8000 tokens of
+// history each take 252 us with slices of 4096 one element at a time.
 #include <algorithm>
 
 #include "decode.hpp"
@@ -16,81 +20,165 @@ namespace logits {
 
 using namespace hw;
 
-constexpr int kThreads = 256;
+constexpr int kGroups = 2, kPer = 8 * kGroups;  // tokens of a thread: groups of 8 adjacent ones
 
-// LDS words of a token: count of the generated part, with the top bit for "in
-// the history at all"; and, with biases, 1 + the last list entry that names it.
-constexpr unsigned kSeen = 0x80000000u;
+// A token's word in LDS.  PACKED: 15 bits of how often it was generated, bit 15
+// for "in the prompt", and above them 1 + the last bias entry that names it,
+// which holds for histories and lists of fewer than 32768 entries.  Otherwise
+// the count has 31 bits under bit 31, and the entry a word of its own.
+template <bool PACKED>
+constexpr unsigned prompt_bit() { return PACKED ? 0x8000u : 0x80000000u; }
 
-template <int DI, int DO>
-__global__ void __launch_bounds__(kThreads) penalize(const LogitsArgs a, int slice, int slices) {
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// 8 adjacent elements at any alignment of their type
+template <int DT>
+struct Eight {
+    u32x4 x;
+    __device__ __forceinline__ void load(const uint16_t* p) { x = load_any16(reinterpret_cast<const unsigned char*>(p)); }
+    __device__ __forceinline__ float get(int i) const { return Elem<DT>::load((uint16_t)(x[i / 2] >> (16 * (i & 1)))); }
+};
+template <>
+struct Eight<CLOVE_DTYPE_FP32> {
+    f32x4 x, y;
+    __device__ __forceinline__ void load(const float* p) {
+        x = *reinterpret_cast<const f32x4u*>(p);
+        y = *reinterpret_cast<const f32x4u*>(p + 4);
+    }
+    __device__ __forceinline__ float get(int i) const { return i < 4 ? x[i] : y[i - 4]; }
+};
+template <int DT>
+__device__ __forceinline__ void store_eight(typename Elem<DT>::raw* p, const float (&v)[8]) {
+    if constexpr (DT == CLOVE_DTYPE_FP32) {
+        *reinterpret_cast<f32x4u*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4u*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+        u32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (unsigned)Elem<DT>::store(v[2 * i]) | ((unsigned)Elem<DT>::store(v[2 * i + 1]) << 16);
+        *reinterpret_cast<u32x4u*>(p) = x;
+    }
+}
+
+template <int DI, int DO, bool PACKED>
+__global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv slices) {
     using EI = Elem<DI>;
     using EO = Elem<DO>;
-    extern __shared__ unsigned lds[];
-    const int b = blockIdx.x / slices, v0 = (blockIdx.x - b * slices) * slice;
+    constexpr unsigned kPrompt = prompt_bit<PACKED>(), kCount = kPrompt - 1;
+    extern __shared__ __align__(16) unsigned words[];
+    const int threads = blockDim.x, tid = threadIdx.x, slice = threads * kPer;
+    const int b = slices.div(blockIdx.x), v0 = (blockIdx.x - b * slices.d) * slice;
     const int n = min(slice, a.vocab - v0);
-    unsigned* const count = lds;
-    unsigned* const last = lds + slice;
-    const bool biased = a.bias_ids != nullptr;
-    const int words = biased ? 2 * slice : slice;
-    for (int i = threadIdx.x; i < words; i += kThreads) lds[i] = 0u;
-    __syncthreads();
-    if (a.history) {
-        const int len = (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride);
-        const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-        const int32_t* ids = a.history + b * a.history_stride;
-        for (int i = threadIdx.x; i < len; i += kThreads) {
-            const unsigned at = (unsigned)ids[i] - (unsigned)v0;
-            if (at < (unsigned)n && ids[i] >= 0) {
-                atomicOr(&count[at], kSeen);
-                if (i >= prompt) atomicAdd(&count[at], 1u);
-            }
-        }
+    const typename EI::raw* in = static_cast<const typename EI::raw*>(a.logits) + b * a.logits_stride + v0;
+    typename EO::raw* out = static_cast<typename EO::raw*>(a.out) + b * a.out_stride + v0;
+    Eight<DI> x[kGroups];
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const int at = (k * threads + tid) * 8;
+        if (at + 8 <= n) x[k].load(in + at);
+    }
+    unsigned* const entry = words + slice;  // PACKED: not there
+    const bool biased = a.bias_ids != nullptr, counted = a.history != nullptr || biased;
+    if (counted) {
+        u32x4* const w = reinterpret_cast<u32x4*>(words);
+        for (int i = tid; i < slice * (PACKED ? 1 : 2) / 4; i += threads) w[i] = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
     }
     if (biased) {
         const int m = (int)(a.bias_counts ? min((int64_t)max(a.bias_counts[b], 0), a.bias_stride) : a.bias_stride);
         const int32_t* ids = a.bias_ids + b * a.bias_stride;
-        for (int i = threadIdx.x; i < m; i += kThreads) {
-            const unsigned at = (unsigned)ids[i] - (unsigned)v0;
-            if (at < (unsigned)n && ids[i] >= 0) atomicMax(&last[at], (unsigned)i + 1u);
+        for (int i = tid; i < m; i += threads) {
+            const unsigned at = (unsigned)ids[i] - (unsigned)v0;  // (an id below 0 is past every slice)
+            if (at < (unsigned)n) PACKED ? atomicMax(&words[at], ((unsigned)i + 1u) << 16) : atomicMax(&entry[at], (unsigned)i + 1u);
         }
+        if constexpr (PACKED) __syncthreads();  // the counts go below
     }
-    __syncthreads();
+    if (a.history) {
+        const int len = (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride);
+        const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
+        const int32_t* ids = a.history + b * a.history_stride;
+        auto count = [&](int id, int i) {
+            const unsigned at = (unsigned)id - (unsigned)v0;
+            if (at < (unsigned)n) i < prompt ? atomicOr(&words[at], kPrompt) : atomicAdd(&words[at], 1u);
+        };
+        int i = tid * 4;
+        for (; i + 4 <= len; i += threads * 4) {
+            const i32x4 id = *reinterpret_cast<const i32x4u*>(ids + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) count(id[e], i + e);
+        }
+        for (; i < len; ++i) count(ids[i], i);  // (the one thread that the last, shorter four fall to)
+    }
+    if (counted) __syncthreads();
     const float r = a.repetition ? a.repetition[b] : 1.0f;
     const float f = a.frequency ? a.frequency[b] : 0.0f, p = a.presence ? a.presence[b] : 0.0f;
-    const typename EI::raw* in = static_cast<const typename EI::raw*>(a.logits) + b * a.logits_stride + v0;
-    typename EO::raw* out = static_cast<typename EO::raw*>(a.out) + b * a.out_stride + v0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        float x = EI::load(in[i]);
-        const unsigned seen = count[i], c = seen & ~kSeen;
-        if (seen) {
-            if (a.repetition) x = x > 0.0f ? x / r : x * r;
-            if (c) x = x - f * (float)c - p;
+    const float* bias = a.bias_values + b * a.bias_stride;
+    const uint32_t* allowed = a.allowed ? a.allowed + b * a.allowed_stride : nullptr;
+    auto result = [&](float l, int at, unsigned word, unsigned e, unsigned open) {
+        if constexpr (PACKED) e = word >> 16;
+        if (word & (kPrompt | kCount)) {
+            const unsigned c = word & kCount;
+            if (a.repetition) l = l > 0.0f ? l / r : l * r;
+            if (c) l = l - f * (float)c - p;
         }
-        if (biased && last[i]) x += a.bias_values[b * a.bias_stride + (last[i] - 1u)];
-        if (a.allowed && !((a.allowed[b * a.allowed_stride + ((v0 + i) >> 5)] >> ((v0 + i) & 31)) & 1u))
-            x = -__builtin_inff();
-        out[i] = EO::store(x);
+        if (e) l += bias[e - 1u];
+        return open ? l : -__builtin_inff();
+    };
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const int at = (k * threads + tid) * 8;
+        if (at >= n) break;
+        const unsigned open = allowed ? allowed[(v0 + at) >> 5] >> ((v0 + at) & 31) : 0xffu;
+        u32x4 w[2] = {}, e[2] = {};
+        if (counted) {
+            w[0] = *reinterpret_cast<const u32x4*>(words + at);
+            w[1] = *reinterpret_cast<const u32x4*>(words + at + 4);
+            if (!PACKED && biased) {
+                e[0] = *reinterpret_cast<const u32x4*>(entry + at);
+                e[1] = *reinterpret_cast<const u32x4*>(entry + at + 4);
+            }
+        }
+        if (at + 8 <= n) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = result(x[k].get(i), at + i, w[i / 4][i % 4], e[i / 4][i % 4], (open >> i) & 1u);
+            store_eight<DO>(out + at, y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (at + i < n) out[at + i] = EO::store(result(EI::load(in[at + i]), at + i, w[i / 4][i % 4], e[i / 4][i % 4], (open >> i) & 1u));
+        }
     }
 }
 
-typedef void (*Kernel)(const LogitsArgs, int, int);
+typedef void (*Kernel)(const LogitsArgs, FastDiv);
 template <int DI>
-Kernel pick(int out) {
-    return out == CLOVE_DTYPE_FP32 ? (Kernel)penalize<DI, CLOVE_DTYPE_FP32> : (Kernel)penalize<DI, DI>;
+Kernel pick(int out, bool packed) {
+    if (out == CLOVE_DTYPE_FP32)
+        return packed ? (Kernel)penalize<DI, CLOVE_DTYPE_FP32, true> : (Kernel)penalize<DI, CLOVE_DTYPE_FP32, false>;
+    return packed ? (Kernel)penalize<DI, DI, true> : (Kernel)penalize<DI, DI, false>;
 }
 
 }  // namespace logits
 
 clove_status_t launch_penalize_logits(const LogitsArgs& a, hipStream_t stream) {
-    const int slice = 4096;
-    const int slices = hw::cdiv(a.vocab, slice);
+    DeviceInfo dev;
+    clove_status_t st = current_device_info(&dev);
+    if (st != CLOVE_OK) return st;
+    const bool counted = a.history || a.bias_ids;
+    const bool packed = !(a.history && a.history_stride >= 32768) && !(a.bias_ids && a.bias_stride >= 32768);
+    // the longest slices that still give two workgroups per CU
+    int threads = packed ? 1024 : 512;
+    while (threads > 256 && (int64_t)a.batch * hw::cdiv(a.vocab, threads * logits::kPer) < 2 * dev.num_cus) threads /= 2;
+    const int slice = threads * logits::kPer, slices = hw::cdiv(a.vocab, slice);
     if ((int64_t)a.batch * slices > 0x7fffffff) return CLOVE_ERR_INVALID_DIM;
-    const logits::Kernel kernel = a.dtype == CLOVE_DTYPE_FP16   ? logits::pick<CLOVE_DTYPE_FP16>(a.out_dtype)
-                                  : a.dtype == CLOVE_DTYPE_BF16 ? logits::pick<CLOVE_DTYPE_BF16>(a.out_dtype)
-                                                                : logits::pick<CLOVE_DTYPE_FP32>(a.out_dtype);
-    CLOVE_LAUNCH(kernel, dim3((unsigned)(a.batch * slices)), dim3(logits::kThreads),
-                 (a.bias_ids ? 2 : 1) * slice * sizeof(unsigned), stream, a, slice, slices);
+    const logits::Kernel kernel = a.dtype == CLOVE_DTYPE_FP16   ? logits::pick<CLOVE_DTYPE_FP16>(a.out_dtype, packed)
+                                  : a.dtype == CLOVE_DTYPE_BF16 ? logits::pick<CLOVE_DTYPE_BF16>(a.out_dtype, packed)
+                                                                : logits::pick<CLOVE_DTYPE_FP32>(a.out_dtype, packed);
+    const int lds = counted ? slice * (packed ? 4 : 8) : 0;
+    if ((st = ensure_lds(reinterpret_cast<const void*>(kernel), lds)) != CLOVE_OK) return st;
+    CLOVE_LAUNCH(kernel, dim3((unsigned)(a.batch * slices)), dim3(threads), lds, stream, a, FastDiv(slices));
     return check_launch();
 }
 
