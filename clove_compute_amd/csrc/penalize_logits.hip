@@ -20,7 +20,7 @@ namespace logits {
 
 using namespace hw;
 
-constexpr int kGroups = 2, kPer = 8 * kGroups;  // tokens of a thread: groups of 8 adjacent ones
+constexpr int kPer = 16;  // tokens of a thread, in groups of adjacent ones
 
 // A token's word in LDS.  PACKED: 15 bits of how often it was generated, bit 15
 // for "in the prompt", and above them 1 + the last bias entry that names it,
@@ -32,32 +32,32 @@ constexpr unsigned prompt_bit() { return PACKED ? 0x8000u : 0x80000000u; }
 typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// 8 adjacent elements at any alignment of their type
+// Adjacent elements in one 16-byte access at any alignment of their type
 template <int DT>
-struct Eight {
+struct Group {
+    static constexpr int E = 8;
     u32x4 x;
     __device__ __forceinline__ void load(const uint16_t* p) { x = load_any16(reinterpret_cast<const unsigned char*>(p)); }
     __device__ __forceinline__ float get(int i) const { return Elem<DT>::load((uint16_t)(x[i / 2] >> (16 * (i & 1)))); }
 };
 template <>
-struct Eight<CLOVE_DTYPE_FP32> {
-    f32x4 x, y;
-    __device__ __forceinline__ void load(const float* p) {
-        x = *reinterpret_cast<const f32x4u*>(p);
-        y = *reinterpret_cast<const f32x4u*>(p + 4);
-    }
-    __device__ __forceinline__ float get(int i) const { return i < 4 ? x[i] : y[i - 4]; }
+struct Group<CLOVE_DTYPE_FP32> {
+    static constexpr int E = 4;
+    f32x4 x;
+    __device__ __forceinline__ void load(const float* p) { x = *reinterpret_cast<const f32x4u*>(p); }
+    __device__ __forceinline__ float get(int i) const { return x[i]; }
 };
-template <int DT>
-__device__ __forceinline__ void store_eight(typename Elem<DT>::raw* p, const float (&v)[8]) {
+template <int DT, int E>
+__device__ __forceinline__ void store_group(typename Elem<DT>::raw* p, const float (&v)[E]) {
     if constexpr (DT == CLOVE_DTYPE_FP32) {
-        *reinterpret_cast<f32x4u*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4u*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+            __builtin_nontemporal_store(f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]}, reinterpret_cast<f32x4u*>(p + i));
     } else {
         u32x4 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = (unsigned)Elem<DT>::store(v[2 * i]) | ((unsigned)Elem<DT>::store(v[2 * i + 1]) << 16);
-        *reinterpret_cast<u32x4u*>(p) = x;
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4u*>(p));
     }
 }
 
@@ -72,12 +72,25 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     const int n = min(slice, a.vocab - v0);
     const typename EI::raw* in = static_cast<const typename EI::raw*>(a.logits) + b * a.logits_stride + v0;
     typename EO::raw* out = static_cast<typename EO::raw*>(a.out) + b * a.out_stride + v0;
-    Eight<DI> x[kGroups];
+    constexpr int E = Group<DI>::E, kGroups = kPer / E;
+    Group<DI> x[kGroups];
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
-        const int at = (k * threads + tid) * 8;
-        if (at + 8 <= n) x[k].load(in + at);
+        const int at = (k * threads + tid) * E;
+        if (at + E <= n) x[k].load(in + at);
     }
+    // what else is known in advance: the mask of the thread's tokens, and the first
+    // ids of the history, whatever its length is
+    unsigned open[kGroups];
+    const uint32_t* allowed = a.allowed ? a.allowed + b * a.allowed_stride : nullptr;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const int at = (k * threads + tid) * E;
+        open[k] = allowed && at < n ? allowed[(v0 + at) >> 5] >> ((v0 + at) & 31) : 0xffu;
+    }
+    const int32_t* told = a.history + b * a.history_stride;
+    i32x4 first = {};
+    if (a.history && tid * 4 + 4 <= a.history_stride) first = *reinterpret_cast<const i32x4u*>(told + tid * 4);
     unsigned* const entry = words + slice;  // PACKED: not there
     const bool biased = a.bias_ids != nullptr, counted = a.history != nullptr || biased;
     if (counted) {
@@ -97,25 +110,23 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     if (a.history) {
         const int len = (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride);
         const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
-        const int32_t* ids = a.history + b * a.history_stride;
         auto count = [&](int id, int i) {
             const unsigned at = (unsigned)id - (unsigned)v0;
             if (at < (unsigned)n) i < prompt ? atomicOr(&words[at], kPrompt) : atomicAdd(&words[at], 1u);
         };
         int i = tid * 4;
         for (; i + 4 <= len; i += threads * 4) {
-            const i32x4 id = *reinterpret_cast<const i32x4u*>(ids + i);
+            const i32x4 id = i == tid * 4 ? first : *reinterpret_cast<const i32x4u*>(told + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) count(id[e], i + e);
         }
-        for (; i < len; ++i) count(ids[i], i);  // (the one thread that the last, shorter four fall to)
+        for (; i < len; ++i) count(told[i], i);  // (the one thread that the last, shorter four fall to)
     }
     if (counted) __syncthreads();
     const float r = a.repetition ? a.repetition[b] : 1.0f;
     const float f = a.frequency ? a.frequency[b] : 0.0f, p = a.presence ? a.presence[b] : 0.0f;
     const float* bias = a.bias_values + b * a.bias_stride;
-    const uint32_t* allowed = a.allowed ? a.allowed + b * a.allowed_stride : nullptr;
-    auto result = [&](float l, int at, unsigned word, unsigned e, unsigned open) {
+    auto result = [&](float l, unsigned word, unsigned e, unsigned open) {
         if constexpr (PACKED) e = word >> 16;
         if (word & (kPrompt | kCount)) {
             const unsigned c = word & kCount;
@@ -127,27 +138,25 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     };
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
-        const int at = (k * threads + tid) * 8;
+        const int at = (k * threads + tid) * E;
         if (at >= n) break;
-        const unsigned open = allowed ? allowed[(v0 + at) >> 5] >> ((v0 + at) & 31) : 0xffu;
-        u32x4 w[2] = {}, e[2] = {};
+        u32x4 w[E / 4] = {}, e[E / 4] = {};
         if (counted) {
-            w[0] = *reinterpret_cast<const u32x4*>(words + at);
-            w[1] = *reinterpret_cast<const u32x4*>(words + at + 4);
-            if (!PACKED && biased) {
-                e[0] = *reinterpret_cast<const u32x4*>(entry + at);
-                e[1] = *reinterpret_cast<const u32x4*>(entry + at + 4);
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) {
+                w[i] = *reinterpret_cast<const u32x4*>(words + at + 4 * i);
+                if (!PACKED && biased) e[i] = *reinterpret_cast<const u32x4*>(entry + at + 4 * i);
             }
         }
-        if (at + 8 <= n) {
-            float y[8];
+        if (at + E <= n) {
+            float y[E];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = result(x[k].get(i), at + i, w[i / 4][i % 4], e[i / 4][i % 4], (open >> i) & 1u);
-            store_eight<DO>(out + at, y);
+            for (int i = 0; i < E; ++i) y[i] = result(x[k].get(i), w[i / 4][i % 4], e[i / 4][i % 4], (open[k] >> i) & 1u);
+            store_group<DO, E>(out + at, y);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + i < n) out[at + i] = EO::store(result(EI::load(in[at + i]), at + i, w[i / 4][i % 4], e[i / 4][i % 4], (open >> i) & 1u));
+            for (int i = 0; i < E; ++i)
+                if (at + i < n) out[at + i] = EO::store(result(EI::load(in[at + i]), w[i / 4][i % 4], e[i / 4][i % 4], (open[k] >> i) & 1u));
         }
     }
 }
