@@ -29,7 +29,7 @@ using namespace hw;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kLdsKeys = 32768;  // 128 KB of the CU's 160
-constexpr int kCopies = 16;      // of the digit histogram, by lane: same-address atomics serialise
+constexpr int kCopies = 8;       // of the digit histogram, by lane: same-address atomics serialise
 constexpr unsigned kStays = 0xffffffffu, kGoes = 0u;
 
 // Ordered bits of a weight: a larger weight has the larger key; -0 as 0; NaN
@@ -94,228 +94,278 @@ __device__ __forceinline__ void move_rows(const Params& p, const int32_t* table,
 }
 
 struct Lds {
-    unsigned hist[256 * kCopies];
-    unsigned total[256];
-    int part[kWaves][3];
-    int pick[2];
+    unsigned hist[3][kCopies][256];
+    int part[kWaves][2];
 };
 
-// One value per wave summed or maximised over the workgroup; two barriers.
-template <bool MAX>
-__device__ __forceinline__ int block_reduce(int v, Lds& s) {
-    v = MAX ? wave_max(v) : wave_sum(v);
-    if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6][0] = v;
-    __syncthreads();
-    int r = s.part[0][0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) r = MAX ? max(r, s.part[w][0]) : r + s.part[w][0];
-    __syncthreads();
-    return r;
+// Inclusive prefix sum over the wave: DPP row_shr 1, 2, 4, 8 inside the rows of
+// 16, then the last lane of a row added to the rows after it.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
+    return v;
 }
 
-constexpr int kBatch = 8;  // global loads of a thread in flight
+constexpr int kHeld = 16;  // tokens of a thread that stay in registers from the first load on
 
 template <bool IN_LDS>
 __global__ void __launch_bounds__(kThreads) select(const Params p) {
     extern __shared__ __align__(16) unsigned lds_keys[];
-    __shared__ Lds s;
+    __shared__ __align__(16) Lds s;
     const EvictArgs& a = p.a;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = min(max(a.context_lens[b], 0), a.max_context);
-    const int keep = min(n, a.budget);
     const float* weights = a.weights + b * a.weights_stride;
     const int32_t* positions = a.positions + b * a.positions_stride;
     float* weights_out = a.weights_out + b * a.weights_out_stride;
     int32_t* positions_out = a.positions_out + b * a.positions_out_stride;
+    const int n = min(max(a.context_lens[b], 0), a.max_context);
+    const int keep = min(n, a.budget);
+    // rows hold max_context tokens whatever the length is, which is not awaited
+    int32_t held_pos[kHeld];
+    float held_w[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        const int i = tid + u * kThreads;
+        held_pos[u] = i < a.max_context ? positions[i] : 0;
+        held_w[u] = i < a.max_context ? weights[i] : 0.0f;
+    }
+    // f(slot, position, weight) for every slot of the row that this thread has
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (tid + u * kThreads < a.max_context) f(tid + u * kThreads, held_pos[u], held_w[u]);
+        for (int i0 = tid + kHeld * kThreads; i0 < a.max_context; i0 += kHeld * kThreads) {
+            int32_t v[kHeld];
+            float w[kHeld];
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) {
+                const int i = i0 + u * kThreads;
+                v[u] = i < a.max_context ? positions[i] : 0;
+                w[u] = i < a.max_context ? weights[i] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u)
+                if (i0 + u * kThreads < a.max_context) f(i0 + u * kThreads, v[u], w[u]);
+        }
+    };
+    const bool apart = weights_out != weights && positions_out != positions;
     int* const src = p.lists + (int64_t)b * 2 * p.moves;
     int* const dst = src + p.moves;
     int moving = 0;
-    if (n > keep && keep > 0) {
+    if (n <= keep || keep == 0) {  // nothing to choose
+        if (apart)
+            each([&](int i, int32_t pos, float w) {
+                weights_out[i] = i < keep ? w : 0.0f;
+                positions_out[i] = i < keep ? pos : -1;
+            });
+    } else {
         unsigned* const keys = IN_LDS ? lds_keys : p.keys + b * p.key_stride;
         const int padded = cdiv(n, 4) * 4;  // keys are read by fours; past n they are kGoes
         int newest = INT32_MIN;
-        for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
-            int v[kBatch];
+        each([&](int i, int32_t pos, float) { newest = i < n ? max(newest, pos) : newest; });
+        newest = wave_max(newest);
+        if (lane == 0) s.part[wave][0] = newest;
+        reinterpret_cast<u32x2*>(&s.hist[0][0][0])[tid] = u32x2{0u, 0u};
+        static_assert(kCopies * 256 == 2 * kThreads, "one access a thread");
+        __syncthreads();
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) v[u] = i0 + u * kThreads < n ? positions[i0 + u * kThreads] : INT32_MIN;
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) newest = max(newest, v[u]);
-        }
-        newest = block_reduce<true>(newest, s);
+        for (int w = 0; w < kWaves; ++w) newest = max(newest, s.part[w][0]);
         const int64_t from = (int64_t)newest - a.recent;
-        auto safe_at = [&](int pos) { return pos < a.sinks || (int64_t)pos > from; };
+        auto safe_at = [&](int32_t pos) { return pos < a.sinks || (int64_t)pos > from; };
         int safes = 0;
-        for (int i0 = tid; i0 < padded; i0 += kBatch * kThreads) {
-            int v[kBatch];
-            float w[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int i = i0 + u * kThreads;
-                v[u] = i < n ? positions[i] : INT32_MAX;
-                w[u] = i < n ? weights[i] : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int i = i0 + u * kThreads;
-                if (i >= padded) continue;
-                const bool safe = i < n && safe_at(v[u]);
+        each([&](int i, int32_t pos, float w) {
+            if (i < n) {
+                const bool safe = safe_at(pos);
+                const unsigned k = safe ? kStays : order_key(w);
                 safes += safe ? 1 : 0;
-                keys[i] = i >= n ? kGoes : safe ? kStays : order_key(w[u]);
+                keys[i] = k;
+                atomicAdd(&s.hist[0][lane & (kCopies - 1)][k >> 24], 1u);
+            } else if (i < padded) {
+                keys[i] = kGoes;
             }
+            if (apart) {  // the moved ones are written over below
+                weights_out[i] = i < keep ? w : 0.0f;
+                positions_out[i] = i < keep ? pos : -1;
+            }
+        });
+        if (tid < padded - n && a.max_context < padded) keys[n + tid] = kGoes;  // a row shorter than its keys
+        safes = wave_sum(safes);
+        if (lane == 0) s.part[wave][1] = safes;
+        reinterpret_cast<u32x2*>(&s.hist[1][0][0])[tid] = u32x2{0u, 0u};
+        __syncthreads();
+        safes = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) safes += s.part[w][1];
+        if (safes >= keep) {  // the protected compete among themselves: keys and first digits anew
+            reinterpret_cast<u32x2*>(&s.hist[0][0][0])[tid] = u32x2{0u, 0u};
+            __syncthreads();
+            each([&](int i, int32_t pos, float w) {
+                if (i >= n) return;
+                const unsigned k = safe_at(pos) ? order_key(w) : kGoes;
+                keys[i] = k;
+                atomicAdd(&s.hist[0][lane & (kCopies - 1)][k >> 24], 1u);
+            });
+            __syncthreads();
         }
-        safes = block_reduce<false>(safes, s);
-        if (safes >= keep) {  // the protected compete among themselves
-            for (int i = tid; i < n; i += kThreads) keys[i] = safe_at(positions[i]) ? order_key(weights[i]) : kGoes;
-            __syncthreads();
-        }
-        // the keep-th largest key, digit by digit: `prefix` its bits so far,
-        // `need` how many of the keys with that prefix are kept
-        unsigned prefix = 0, mask = 0;
-        int need = keep;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            *reinterpret_cast<u32x4*>(s.hist + 4 * tid) = u32x4{0u, 0u, 0u, 0u};
-            static_assert(4 * kThreads == 256 * kCopies, "one access a thread");
-            __syncthreads();
-            for (int i = 4 * tid; i < padded; i += 4 * kThreads) {
-                const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+        // the keep-th largest key, digit by digit: `prefix` its bits so far, `need`
+        // how many of the `equal` keys with that prefix are kept.  Every wave reads
+        // the counts for itself, so a digit costs one barrier; of three histograms
+        // one is read, one counted and one cleared.
+        unsigned prefix = 0;
+        int need = keep, equal = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if ((k[e] & mask) == prefix) atomicAdd(&s.hist[((k[e] >> shift) & 255u) * kCopies + (lane & (kCopies - 1))], 1u);
-            }
-            __syncthreads();
-            {  // the copies of a digit: four lanes of four
-                const u32x4 c = *reinterpret_cast<const u32x4*>(s.hist + 4 * tid);
-                int v = (int)(c[0] + c[1] + c[2] + c[3]);
-                v += __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, false);
-                v += __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, false);
-                if ((tid & 3) == 0) s.total[255 - tid / 4] = (unsigned)v;  // from the top
-            }
-            __syncthreads();
-            if (wave == 0) {  // lane l: digits 255 - 4 l .. 252 - 4 l
-                const u32x4 c = *reinterpret_cast<const u32x4*>(s.total + 4 * lane);
-                const int sum = (int)(c[0] + c[1] + c[2] + c[3]);
-                int above = sum;  // keys of this lane's digits and all higher ones
+        for (int digit = 0; digit < 4; ++digit) {
+            const int shift = 24 - 8 * digit;
+            if (digit) {
+                const unsigned mask = 0xffffffffu << (shift + 8);
+                if (digit < 3) reinterpret_cast<u32x2*>(&s.hist[(digit + 1) % 3][0][0])[tid] = u32x2{0u, 0u};
+                for (int i = 4 * tid; i < padded; i += 4 * kThreads) {
+                    const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
 #pragma unroll
-                for (int m = 1; m < 64; m <<= 1) {
-                    const int o = __shfl_up(above, m);
-                    if (lane >= m) above += o;
+                    for (int e = 0; e < 4; ++e)
+                        if ((k[e] & mask) == prefix) atomicAdd(&s.hist[digit % 3][lane & (kCopies - 1)][(k[e] >> shift) & 255u], 1u);
                 }
-                above -= sum;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (above < need && above + (int)c[j] >= need) {
-                        s.pick[0] = 255 - 4 * lane - j;
-                        s.pick[1] = need - above;
-                    }
-                    above += (int)c[j];
-                }
+                __syncthreads();
             }
-            __syncthreads();
-            prefix |= (unsigned)s.pick[0] << shift;
-            mask |= 255u << shift;
-            need = s.pick[1];
+            // lane l: digits 4 l .. 4 l + 3 and how many keys have a higher one
+            u32x4 c = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int r = 0; r < kCopies; ++r) c += *reinterpret_cast<const u32x4*>(&s.hist[digit % 3][r][4 * lane]);
+            const int sum = (int)(c[0] + c[1] + c[2] + c[3]), upto = wave_scan(sum);
+            int above = __builtin_amdgcn_readlane(upto, 63) - upto, mine = -1, rest = 0, same = 0;
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                if (above < need && above + (int)c[j] >= need) {
+                    mine = 4 * lane + j;
+                    rest = need - above;
+                    same = (int)c[j];
+                }
+                above += (int)c[j];
+            }
+            const int who = __ffsll((long long)__ballot(mine >= 0)) - 1;  // one lane has it
+            prefix |= (unsigned)__builtin_amdgcn_readlane(mine, who) << shift;
+            need = __builtin_amdgcn_readlane(rest, who);
+            equal = __builtin_amdgcn_readlane(same, who);
         }
         // in slot order from here: wave w has slots [w seg, (w + 1) seg), 256 at a
         // time, four adjacent ones a lane
         const int seg = cdiv(cdiv(n, kWaves), 256) * 256;
         const int i0 = min(wave * seg, padded), i1 = min(i0 + seg, padded);
-        const unsigned long long below = (1ull << lane) - 1ull;
-        int equal = 0;
-        for (int i = i0 + 4 * lane; i < i1; i += 256) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+        if (need < equal) {  // of the equal keys the lowest slots stay, the others drop below them
+            int count = 0;
+            for (int i = i0 + 4 * lane; i < i1; i += 256) {
+                const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) equal += k[e] == prefix ? 1 : 0;
-        }
-        equal = wave_sum(equal);
-        if (lane == 0) s.part[wave][0] = equal;
-        __syncthreads();
-        int before = 0;  // equal keys of lower slots
-        for (int w = 0; w < wave; ++w) before += s.part[w][0];
-        // the lists of slots that move and of holes: counted, then written
-        int at_src = 0, at_dst = 0;
-        for (int pass = 0; pass < 2; ++pass) {
-            int ties = before;
+                for (int e = 0; e < 4; ++e) count += k[e] == prefix ? 1 : 0;
+            }
+            count = wave_sum(count);
+            if (lane == 0) s.part[wave][0] = count;
+            __syncthreads();
+            int ties = 0;
+            for (int w = 0; w < wave; ++w) ties += s.part[w][0];
             for (int i = i0; i < i1; i += 256) {
                 const int at = i + 4 * lane;
                 const u32x4 k = at < i1 ? *reinterpret_cast<const u32x4*>(keys + at) : u32x4{kGoes, kGoes, kGoes, kGoes};
-                int rank = ties, n_eq = 0;  // of this lane's first slot among the equal keys
+                int own = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) own += k[e] == prefix ? 1 : 0;
+                const int upto = wave_scan(own);
+                int rank = ties + upto - own;
+                ties += __builtin_amdgcn_readlane(upto, 63);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const unsigned long long eq = __ballot(k[e] == prefix);
-                    rank += __popcll(eq & below);
-                    n_eq += __popcll(eq);
-                }
-                ties += n_eq;
-                unsigned out = 0, hole = 0;  // this lane's four
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool kept = k[e] > prefix || (k[e] == prefix && rank < need);
-                    rank += k[e] == prefix ? 1 : 0;
-                    out |= (kept && at + e >= keep ? 1u : 0u) << e;
-                    hole |= (!kept && at + e < keep ? 1u : 0u) << e;
-                }
-                int my_src = at_src, my_dst = at_dst;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned long long x = __ballot((out >> e) & 1u), y = __ballot((hole >> e) & 1u);
-                    my_src += __popcll(x & below);
-                    my_dst += __popcll(y & below);
-                    at_src += __popcll(x);
-                    at_dst += __popcll(y);
-                }
-                if (pass) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if ((out >> e) & 1u) src[my_src++] = at + e;
-                        if ((hole >> e) & 1u) dst[my_dst++] = at + e;
-                    }
+                    if (k[e] != prefix) continue;
+                    if (rank >= need) keys[at + e] = prefix - 1u;
+                    ++rank;
                 }
             }
-            if (!pass) {
-                if (lane == 0) {
-                    s.part[wave][1] = at_src;
-                    s.part[wave][2] = at_dst;
-                }
-                __syncthreads();
-                at_src = at_dst = 0;
-                for (int w = 0; w < kWaves; ++w) {
-                    if (w < wave) {
-                        at_src += s.part[w][1];
-                        at_dst += s.part[w][2];
-                    }
-                    moving += s.part[w][1];
-                }
+            __syncthreads();
+        }
+        // the lists of slots that move and of holes: counted, then written
+        int n_src = 0, n_dst = 0;
+        for (int i = i0 + 4 * lane; i < i1; i += 256) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                n_src += k[e] >= prefix && i + e >= keep ? 1 : 0;
+                n_dst += k[e] < prefix && i + e < keep ? 1 : 0;
             }
+        }
+        n_src = wave_sum(n_src);
+        n_dst = wave_sum(n_dst);
+        __syncthreads();  // (s.part may still be read as the counts of ties)
+        if (lane == 0) {
+            s.part[wave][0] = n_src;
+            s.part[wave][1] = n_dst;
         }
         __syncthreads();
-    }
-    // the slots as they are now; the moved ones are read past `keep` and
-    // written below it, so in-place outputs need only the barrier before the
-    // rest of the row is cleared
-    auto copy = [&](const auto* from, auto* to) {
-        if (to == from) return;
-        for (int i0 = tid; i0 < keep; i0 += 4 * kThreads) {
-            std::remove_reference_t<decltype(*to)> v[4];
+        int at_src = 0, at_dst = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i0 + u * kThreads < keep) v[u] = from[i0 + u * kThreads];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i0 + u * kThreads < keep) to[i0 + u * kThreads] = v[u];
+        for (int w = 0; w < kWaves; ++w) {
+            at_src += w < wave ? s.part[w][0] : 0;
+            at_dst += w < wave ? s.part[w][1] : 0;
+            moving += s.part[w][0];
         }
-    };
-    copy(weights, weights_out);
-    copy(positions, positions_out);
-    __syncthreads();
-    for (int j = tid; j < moving; j += kThreads) {
-        const int from = src[j], to = dst[j];
-        weights_out[to] = weights[from];
-        positions_out[to] = positions[from];
+        for (int i = i0; i < i1; i += 256) {
+            const int at = i + 4 * lane;
+            const u32x4 k = at < i1 ? *reinterpret_cast<const u32x4*>(keys + at) : u32x4{kStays, kStays, kStays, kStays};
+            unsigned out = 0, hole = 0;  // this lane's four
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                out |= (k[e] >= prefix && at + e >= keep && at < i1 ? 1u : 0u) << e;
+                hole |= (k[e] < prefix && at + e < keep ? 1u : 0u) << e;
+            }
+            const int own = __popc(out) | __popc(hole) << 16, upto = wave_scan(own), all = __builtin_amdgcn_readlane(upto, 63);
+            int my_src = at_src + ((upto - own) & 0xffff), my_dst = at_dst + ((upto - own) >> 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if ((out >> e) & 1u) src[my_src++] = at + e;
+                if ((hole >> e) & 1u) dst[my_dst++] = at + e;
+            }
+            at_src += all & 0xffff;
+            at_dst += all >> 16;
+        }
     }
     __syncthreads();
-    for (int i = keep + tid; i < a.max_context; i += kThreads) {
-        weights_out[i] = 0.0f;
-        positions_out[i] = -1;
+    // Moved slots are read at or past `keep` and written below it.  Where an output
+    // is its input, they are moved before the rest of its row is cleared.
+    if (!apart && weights_out != weights)
+        for (int i = tid; i < keep; i += kThreads) weights_out[i] = weights[i];
+    if (!apart && positions_out != positions)
+        for (int i = tid; i < keep; i += kThreads) positions_out[i] = positions[i];
+    if (!apart) __syncthreads();
+    for (int j0 = tid; j0 < moving; j0 += 4 * kThreads) {
+        int from[4], to[4];
+        float w[4];
+        int32_t pos[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = min(j0 + u * kThreads, moving - 1);
+            from[u] = src[j];
+            to[u] = dst[j];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            w[u] = weights[from[u]];
+            pos[u] = positions[from[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (j0 + u * kThreads >= moving) break;
+            weights_out[to[u]] = w[u];
+            positions_out[to[u]] = pos[u];
+        }
+    }
+    if (!apart) {
+        __syncthreads();
+        for (int i = keep + tid; i < a.max_context; i += kThreads) {
+            weights_out[i] = 0.0f;
+            positions_out[i] = -1;
+        }
     }
     if (tid == 0) {
         a.lens_out[b] = keep;

@@ -587,3 +587,41 @@ def test_python_checks():
         cg.penalize_logits(st["logits"].double(), st["y"], B, 5000)
     with pytest.raises(cg.CloveError):
         cg.paged_attention(st["q"], st["cache"], st["table"], st["lens"], st["q"], B, 8, L)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("lens,budget,sinks,recent,kind", [
+    ([17000, 16384, 16390], 4096, 4, 300, "free"), ([33000, 20000], 12000, 0, 1, "ties"), ([18001], 18000, 4, 100, "free"),
+    ([18001], 3, 4, 100, "free"), ([16385, 1], 16384, 0, 0, "equal"), ([20000], 9000, 12000, 0, "ties"), ([33001], 9000, 12000, 0, "ties")])
+def test_evict_long(in_place, lens, budget, sinks, recent, kind):
+    import torch
+    cg = _cg()
+    g = rng("evict-long", tuple(lens), budget)
+    B, L, P = len(lens), max(lens), 128
+    k, v, k64, v64, table = _paged(g, "fp16", lens, 1, 8, P, nan_rest=False)
+    w = np.exp(1.5 * g.standard_normal((B, L))).astype(np.float32)
+    w = {"free": w, "ties": np.round(w), "equal": np.full_like(w, 2.0)}[kind]
+    pos = np.stack([g.permutation(L) for _ in range(B)]).astype(np.int32)
+    want = ref.evict(k64, v64, table, lens, w, pos, L, budget, sinks, recent)
+    dw, dp, dl = _dev(w), _dev(pos), _dev(np.array(lens, np.int32))
+    wo, po, lo = (dw, torch.full_like(dp, 9), dl) if in_place else (torch.full_like(dw, 9), torch.full_like(dp, 9), torch.full_like(dl, 9))
+    cg.cache_evict(cg.KVCache(k, v), _dev(table), dl, dw, dp, wo, po, lo, B, L, budget, sinks=sinks, recent=recent)
+    for got, exact in zip((k, v, wo, po, lo), want):
+        assert np.array_equal(_f64(got), exact.astype(np.float64))
+
+
+def test_logits_histories_and_lists_past_15_bits():
+    """40000 ids of a few tokens (counts past 2^15), and a bias list as long."""
+    import torch
+    cg = _cg()
+    g = rng("logits-long")
+    B, V, H = 2, 9000, 40000
+    for bias in (40000, 5):
+        x, x64, opts = _logits_case(g, B, V, H, bias, True, "fp32")
+        opts["history"][1] = 8995
+        opts["history_lens"] = np.array([H, H], np.int32)
+        opts["prompt_lens"] = np.array([100, 0], np.int32)
+        want = ref.penalties(x64, **opts)
+        y = torch.empty_like(x)
+        cg.penalize_logits(x, y, B, V, **{n: _dev(a) for n, a in opts.items()})
+        _close(y, want, "fp32", _logit_slack(x64, opts) + 4 * 2.0 ** -24 * np.abs(want[np.isfinite(want)]).max())
