@@ -15,8 +15,11 @@
 //    at about 47 GB/s, and each of its dozen passes waits for the one before, so
 //    loads and LDS reads of a pass are issued together (8 of each per thread; one
 //    by one, 24576 tokens took 68 us).
-//  * move: the rows of K and V, 16 bytes per lane; few rows are moved by select
-//    itself, which saves the second launch.
+//  * move: the rows of K and V, 16 bytes per lane where rows are multiples of
+//    that; few rows are moved by select itself, which saves the second launch.
+//    HBM-bound; the stores pass the L2
+//    by, as nothing reads the rows soon: 24576 tokens to 4096 in 12 mixed
+//    sequences 71.5 us with ordinary stores, 61.5 so, loads past it too 64.4.
 #include <algorithm>
 #include <type_traits>
 
@@ -63,40 +66,126 @@ struct Params {
     unsigned* keys; // [batch][key_stride] where they do not fit LDS
     int64_t key_stride;
     FastDiv per;    // by the accesses of a row
-    FastDiv heads;  // by the KV heads
-    bool vec;       // 8 elements an access, else 1
+    int team;       // lanes of a move: a power of two up to 64
+    int vec;        // elements of an access: the most of 8, 4, 2, 1 that rows and addresses are multiples of
     bool fused;     // select moves the rows
 };
 
-// Accesses first, first + step, .. of a sequence's moves: (move, head, access of the row).
+// Moves first, first + step, .. of a sequence, a team of p.team lanes (`at` of it)
+// each: its accesses are those of the row of every head, four of K and V in flight.
 template <int V>
-__device__ __forceinline__ void move_rows(const Params& p, const int32_t* table, const int* src, const int* dst, int count, int64_t first,
-                                          int64_t step) {
+__device__ __forceinline__ void move_rows(const Params& p, const int32_t* table, const int* src, const int* dst, int count, int first,
+                                          int step, int at) {
+    typedef std::conditional_t<V == 8, u32x4, std::conditional_t<V == 4, u32x2, std::conditional_t<V == 2, unsigned, uint16_t>>> Word;
     const PagedCache& c = p.a.cache;
-    const int64_t head = (int64_t)c.page_size * c.head_dim, total = (int64_t)count * c.kv_heads * p.per.d;
-    for (int64_t i = first; i < total; i += step) {
-        int64_t row = total <= INT32_MAX ? p.per.div((int)i) : i / p.per.d;
-        const int at = (int)(i - row * p.per.d), j = total <= INT32_MAX ? p.heads.div((int)row) : (int)(row / c.kv_heads);
-        const int h = (int)(row - (int64_t)j * c.kv_heads);
+    const int head = c.page_size * c.head_dim, items = c.kv_heads * p.per.d;
+    for (int64_t j = first; j < count; j += step) {
         const int64_t from = row_at(c, p.page, table, src[j]), to = row_at(c, p.page, table, dst[j]);
         if (from < 0 || to < 0) continue;
-        const int64_t in_row = h * head + (int64_t)at * V;
-        if constexpr (V == 8) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(c.k + from + in_row);
-            const u32x4 v = *reinterpret_cast<const u32x4*>(c.v + from + in_row);
-            *reinterpret_cast<u32x4*>(c.k + to + in_row) = k;
-            *reinterpret_cast<u32x4*>(c.v + to + in_row) = v;
-        } else {
-            c.k[to + in_row] = c.k[from + in_row];
-            c.v[to + in_row] = c.v[from + in_row];
+        for (int i0 = at; i0 < items; i0 += 4 * p.team) {
+            Word k[4], v[4];
+            int64_t in_row[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * p.team, h = p.per.div(i);
+                in_row[u] = (int64_t)h * head + (int64_t)(i - h * p.per.d) * V;
+                if (i < items) {
+                    k[u] = *reinterpret_cast<const Word*>(c.k + from + in_row[u]);
+                    v[u] = *reinterpret_cast<const Word*>(c.v + from + in_row[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * p.team < items) {
+                    __builtin_nontemporal_store(k[u], reinterpret_cast<Word*>(c.k + to + in_row[u]));
+                    __builtin_nontemporal_store(v[u], reinterpret_cast<Word*>(c.v + to + in_row[u]));
+                }
         }
     }
 }
+
+// The end of a selection, after a barrier: the lists hold `moving` slots each.
+__device__ __forceinline__ void finish(const Params& p, int b, int keep, int moving, const int* src, const int* dst, bool apart) {
+    const EvictArgs& a = p.a;
+    const int tid = threadIdx.x;
+    const float* weights = a.weights + b * a.weights_stride;
+    const int32_t* positions = a.positions + b * a.positions_stride;
+    float* weights_out = a.weights_out + b * a.weights_out_stride;
+    int32_t* positions_out = a.positions_out + b * a.positions_out_stride;
+    // Moved slots are read at or past `keep` and written below it.  Where an output
+    // is its input, they are moved before the rest of its row is cleared.
+    if (!apart && weights_out != weights)
+        for (int i = tid; i < keep; i += kThreads) weights_out[i] = weights[i];
+    if (!apart && positions_out != positions)
+        for (int i = tid; i < keep; i += kThreads) positions_out[i] = positions[i];
+    if (!apart) __syncthreads();
+    for (int j0 = tid; j0 < moving; j0 += 4 * kThreads) {
+        int from[4], to[4];
+        float w[4];
+        int32_t pos[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = min(j0 + u * kThreads, moving - 1);
+            from[u] = src[j];
+            to[u] = dst[j];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            w[u] = weights[from[u]];
+            pos[u] = positions[from[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (j0 + u * kThreads >= moving) break;
+            weights_out[to[u]] = w[u];
+            positions_out[to[u]] = pos[u];
+        }
+    }
+    if (!apart && p.fused) {
+        __syncthreads();
+        for (int i = keep + tid; i < a.max_context; i += kThreads) {
+            weights_out[i] = 0.0f;
+            positions_out[i] = -1;
+        }
+    }
+    if (tid == 0) {
+        a.lens_out[b] = keep;
+        if (p.moves && !p.fused) p.counts[b] = moving;
+    }
+    if (p.fused && moving) {
+        const int32_t* table = a.block_table + b * a.table_stride;
+        const int first = tid / p.team, step = kThreads / p.team, at = tid & (p.team - 1);
+        if (p.vec == 8) move_rows<8>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 4) move_rows<4>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 2) move_rows<2>(p, table, src, dst, moving, first, step, at);
+        else move_rows<1>(p, table, src, dst, moving, first, step, at);
+    }
+}
+
+// Up to this many tokens past the budget are found one by one, each as the
+// smallest (protected, key, slot from the end) above the last: a step of a full
+// cache, one token over, takes one reduction where the digits, ties and lists
+// take seven barriers (48 x 2049 tokens 12.0 -> 8.2 us).
+constexpr int kFew = 4;
 
 struct Lds {
     unsigned hist[3][kCopies][256];
     int part[kWaves][2];
 };
+
+// The smallest value of the wave, in every lane: the order of wave_sum.
+__device__ __forceinline__ unsigned wave_min(unsigned v) {
+    v = min(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
+    v = min(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, false));  // row_ror:4
+    v = min(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));   // quad_perm 2301
+    v = min(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));   // quad_perm 1032
+    return min(min((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+               min((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+}
+__device__ __forceinline__ uint64_t wave_min(uint64_t v) {
+    const unsigned hi = wave_min((unsigned)(v >> 32));
+    return ((uint64_t)hi << 32) | wave_min((unsigned)(v >> 32) == hi ? (unsigned)v : 0xffffffffu);
+}
 
 // Inclusive prefix sum over the wave: DPP row_shr 1, 2, 4, 8 inside the rows of
 // 16, then the last lane of a row added to the rows after it.
@@ -153,15 +242,19 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
         }
     };
     const bool apart = weights_out != weights && positions_out != positions;
+    // outputs apart from their inputs, before the moved tokens are written over
+    // them; slots past `keep` are cleared by the second kernel where there is one
+    const int written = p.fused ? a.max_context : keep;
+    auto pass_on = [&](int i, int32_t pos, float w) {
+        if (!apart || i >= written) return;
+        weights_out[i] = i < keep ? w : 0.0f;
+        positions_out[i] = i < keep ? pos : -1;
+    };
     int* const src = p.lists + (int64_t)b * 2 * p.moves;
     int* const dst = src + p.moves;
     int moving = 0;
     if (n <= keep || keep == 0) {  // nothing to choose
-        if (apart)
-            each([&](int i, int32_t pos, float w) {
-                weights_out[i] = i < keep ? w : 0.0f;
-                positions_out[i] = i < keep ? pos : -1;
-            });
+        if (apart) each(pass_on);
     } else {
         unsigned* const keys = IN_LDS ? lds_keys : p.keys + b * p.key_stride;
         const int padded = cdiv(n, 4) * 4;  // keys are read by fours; past n they are kGoes
@@ -187,10 +280,7 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
             } else if (i < padded) {
                 keys[i] = kGoes;
             }
-            if (apart) {  // the moved ones are written over below
-                weights_out[i] = i < keep ? w : 0.0f;
-                positions_out[i] = i < keep ? pos : -1;
-            }
+            pass_on(i, pos, w);
         });
         if (tid < padded - n && a.max_context < padded) keys[n + tid] = kGoes;  // a row shorter than its keys
         safes = wave_sum(safes);
@@ -331,58 +421,126 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
         }
     }
     __syncthreads();
-    // Moved slots are read at or past `keep` and written below it.  Where an output
-    // is its input, they are moved before the rest of its row is cleared.
-    if (!apart && weights_out != weights)
-        for (int i = tid; i < keep; i += kThreads) weights_out[i] = weights[i];
-    if (!apart && positions_out != positions)
-        for (int i = tid; i < keep; i += kThreads) positions_out[i] = positions[i];
-    if (!apart) __syncthreads();
-    for (int j0 = tid; j0 < moving; j0 += 4 * kThreads) {
-        int from[4], to[4];
-        float w[4];
-        int32_t pos[4];
+    finish(p, b, keep, moving, src, dst, apart);
+}
+
+// Rows of at most budget + kFew tokens.
+__global__ void __launch_bounds__(kThreads) select_few(const Params p) {
+    __shared__ uint64_t least_of[2][kWaves];
+    __shared__ int newest_of[kWaves];
+    const EvictArgs& a = p.a;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* weights = a.weights + b * a.weights_stride;
+    const int32_t* positions = a.positions + b * a.positions_stride;
+    float* weights_out = a.weights_out + b * a.weights_out_stride;
+    int32_t* positions_out = a.positions_out + b * a.positions_out_stride;
+    const int n = min(max(a.context_lens[b], 0), a.max_context);
+    const int keep = min(n, a.budget);
+    const bool apart = weights_out != weights && positions_out != positions;
+    const int written = p.fused ? a.max_context : keep;
+    // rows hold max_context tokens whatever the length is, which is not awaited
+    constexpr int kBatch = 8;
+    int32_t pos[kBatch];
+    float w[kBatch];
+    auto load = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = min(j0 + u * kThreads, moving - 1);
-            from[u] = src[j];
-            to[u] = dst[j];
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * kThreads;
+            pos[u] = i < a.max_context ? positions[i] : 0;
+            w[u] = i < a.max_context ? weights[i] : 0.0f;
         }
+    };
+    load(tid);
+    int newest = INT32_MIN;
+    for (int i0 = tid; i0 < a.max_context; i0 += kBatch * kThreads) {
+        if (i0 != tid) load(i0);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            w[u] = weights[from[u]];
-            pos[u] = positions[from[u]];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (j0 + u * kThreads >= moving) break;
-            weights_out[to[u]] = w[u];
-            positions_out[to[u]] = pos[u];
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = i0 + u * kThreads;
+            if (i < n) newest = max(newest, pos[u]);
+            if (apart && i < written) {
+                weights_out[i] = i < keep ? w[u] : 0.0f;
+                positions_out[i] = i < keep ? pos[u] : -1;
+            }
         }
     }
-    if (!apart) {
+    int* const src = p.lists + (int64_t)b * 2 * p.moves;
+    int* const dst = src + p.moves;
+    int moving = 0;
+    if (n > keep && keep > 0) {
+        newest = wave_max(newest);
+        if (lane == 0) newest_of[wave] = newest;
         __syncthreads();
-        for (int i = keep + tid; i < a.max_context; i += kThreads) {
-            weights_out[i] = 0.0f;
-            positions_out[i] = -1;
+#pragma unroll
+        for (int x = 0; x < kWaves; ++x) newest = max(newest, newest_of[x]);
+        const int64_t from = (int64_t)newest - a.recent;
+        const bool held = a.max_context <= kBatch * kThreads;  // the registers still have every token
+        uint64_t last = 0;
+        int gone[kFew];
+#pragma unroll
+        for (int d = 0; d < kFew; ++d) {
+            gone[d] = INT32_MAX;
+            if (d >= n - keep) continue;
+            uint64_t least = ~(uint64_t)0;
+#pragma unroll 1
+            for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
+                if (!held) load(i0);
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    const int i = i0 + u * kThreads;
+                    const bool safe = pos[u] < a.sinks || (int64_t)pos[u] > from;
+                    const uint64_t c = ((uint64_t)safe << 63) | ((uint64_t)order_key(w[u]) << 31) | (unsigned)(INT32_MAX - i);
+                    if (i < n && c > last) least = min(least, c);
+                }
+            }
+            least = wave_min(least);
+            if (lane == 0) least_of[d & 1][wave] = least;
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < kWaves; ++x) least = min(least, least_of[d & 1][x]);
+            last = least;
+            gone[d] = INT32_MAX - (int)(least & INT32_MAX);
+        }
+        // in slot order: those gone below `keep` are holes, those past it that are not gone move
+#pragma unroll
+        for (int x = 0; x < kFew; ++x)
+#pragma unroll
+            for (int y = x + 1; y < kFew; ++y) {
+                const int lo = min(gone[x], gone[y]), hi = max(gone[x], gone[y]);
+                gone[x] = lo;
+                gone[y] = hi;
+            }
+        int holes = 0;
+#pragma unroll
+        for (int d = 0; d < kFew; ++d) {
+            if (gone[d] < keep) {
+                if (tid == 0) dst[holes] = gone[d];
+                ++holes;
+            }
+            const int i = keep + d;
+            bool moves = i < n;
+#pragma unroll
+            for (int e = 0; e < kFew; ++e) moves = moves && gone[e] != i;
+            if (moves) {
+                if (tid == 0) src[moving] = i;
+                ++moving;
+            }
         }
     }
-    if (tid == 0) {
-        a.lens_out[b] = keep;
-        if (p.moves && !p.fused) p.counts[b] = moving;
-    }
-    if (p.fused && moving) {
-        const int32_t* table = a.block_table + b * a.table_stride;
-        p.vec ? move_rows<8>(p, table, src, dst, moving, tid, kThreads) : move_rows<1>(p, table, src, dst, moving, tid, kThreads);
-    }
+    __syncthreads();
+    finish(p, b, keep, moving, src, dst, apart);
 }
 
 template <int V>
 __global__ void __launch_bounds__(256) move(const Params p, FastDiv blocks) {
     const int b = blocks.div(blockIdx.x);
     const int* src = p.lists + (int64_t)b * 2 * p.moves;
+    for (int64_t i = p.a.lens_out[b] + (int64_t)(blockIdx.x - b * blocks.d) * 256 + threadIdx.x; i < p.a.max_context; i += (int64_t)blocks.d * 256) {
+        p.a.weights_out[b * p.a.weights_out_stride + i] = 0.0f;
+        p.a.positions_out[b * p.a.positions_out_stride + i] = -1;
+    }
     move_rows<V>(p, p.a.block_table + b * p.a.table_stride, src, src + p.moves, p.counts[b],
-                 (int64_t)(blockIdx.x - b * blocks.d) * 256 + threadIdx.x, (int64_t)blocks.d * 256);
+                 ((blockIdx.x - b * blocks.d) * 256 + threadIdx.x) / p.team, blocks.d * 256 / p.team, threadIdx.x & (p.team - 1));
 }
 
 }  // namespace evict
@@ -396,13 +554,15 @@ clove_status_t launch_cache_evict(const EvictArgs& a, hipStream_t stream) {
     p.page = FastDiv(a.cache.page_size);
     // no sequence can move more slots than lie past the budget, or than it keeps
     p.moves = std::max(0, std::min(a.budget, a.max_context - a.budget));
-    p.vec = a.cache.head_dim % 8 == 0 && a.cache.page_stride % 8 == 0 && aligned16(a.cache.k) && aligned16(a.cache.v);
-    p.per = FastDiv(p.vec ? a.cache.head_dim / 8 : a.cache.head_dim);
-    p.heads = FastDiv(a.cache.kv_heads);
-    const int64_t most = (int64_t)p.moves * a.cache.kv_heads * p.per.d;  // accesses of a sequence's moves
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.cache.k) | reinterpret_cast<uintptr_t>(a.cache.v);
+    for (p.vec = 8; a.cache.head_dim % p.vec || a.cache.page_stride % p.vec || at % (2 * p.vec); p.vec /= 2) {}
+    p.per = FastDiv(a.cache.head_dim / p.vec);
+    const int64_t items = (int64_t)a.cache.kv_heads * p.per.d, most = p.moves * items;  // accesses of one move, of a sequence's
+    p.team = 1;
+    while (p.team < 64 && p.team < items) p.team *= 2;
     p.fused = most <= 4 * evict::kThreads;
-    const bool cuts = a.max_context > a.budget;
-    const bool in_lds = !cuts || a.max_context <= evict::kLdsKeys;
+    const bool few = a.max_context - a.budget <= evict::kFew;  // (or no row can be cut at all)
+    const bool in_lds = few || a.max_context <= evict::kLdsKeys;
     p.key_stride = (int64_t)hw::cdiv(a.max_context, 4) * 4;
     const size_t ints = ((size_t)a.batch * (1 + 2 * (size_t)p.moves) + 3) / 4 * 4, keys = in_lds ? 0 : (size_t)(a.batch * p.key_stride);
     if (p.moves) {
@@ -412,13 +572,15 @@ clove_status_t launch_cache_evict(const EvictArgs& a, hipStream_t stream) {
         p.lists = p.counts + a.batch;
         p.keys = reinterpret_cast<unsigned*>(p.counts + ints);
     }
-    const int lds = in_lds && cuts ? (int)p.key_stride * 4 : 0;
-    const auto kernel = in_lds ? evict::select<true> : evict::select<false>;
+    const int lds = in_lds && !few ? (int)p.key_stride * 4 : 0;
+    const auto kernel = few ? evict::select_few : in_lds ? evict::select<true> : evict::select<false>;
     if ((st = ensure_lds(reinterpret_cast<const void*>(kernel), lds)) != CLOVE_OK) return st;
     CLOVE_LAUNCH(kernel, dim3((unsigned)a.batch), dim3(evict::kThreads), lds, stream, p);
     if ((st = check_launch()) != CLOVE_OK || p.fused) return st;
-    const int64_t x = std::min<int64_t>(hw::cdiv64(most, 256), std::max<int64_t>(1, hw::cdiv64(16 * dev.num_cus, a.batch)));
-    CLOVE_LAUNCH(p.vec ? evict::move<8> : evict::move<1>, dim3((unsigned)(x * a.batch)), dim3(256), 0, stream, p, FastDiv((int)x));
+    // a move a team, at most 32 workgroups per CU
+    const int64_t x = std::min<int64_t>(hw::cdiv64((int64_t)p.moves * p.team, 256), std::max<int64_t>(1, hw::cdiv64(32 * dev.num_cus, a.batch)));
+    const auto move = p.vec == 8 ? evict::move<8> : p.vec == 4 ? evict::move<4> : p.vec == 2 ? evict::move<2> : evict::move<1>;
+    CLOVE_LAUNCH(move, dim3((unsigned)(x * a.batch)), dim3(256), 0, stream, p, FastDiv((int)x));
     return check_launch();
 }
 

@@ -625,3 +625,37 @@ def test_logits_histories_and_lists_past_15_bits():
         y = torch.empty_like(x)
         cg.penalize_logits(x, y, B, V, **{n: _dev(a) for n, a in opts.items()})
         _close(y, want, "fp32", _logit_slack(x64, opts) + 4 * 2.0 ** -24 * np.abs(want[np.isfinite(want)]).max())
+
+
+@pytest.mark.parametrize("over", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("kind", ["free", "ties", "equal", "odd", "safe"])
+def test_evict_a_few_tokens(over, kind):
+    """As many tokens over the budget as a step or a few bring, in lengths of one call that differ."""
+    import torch
+    cg = _cg()
+    g = rng("evict-few", over, kind)
+    budget, P = 700, 16
+    L = budget + over
+    lens = [L, L - 1, budget, 5, L]
+    B = len(lens)
+    k, v, k64, v64, table = _paged(g, "fp16", lens, 2, 64, P, nan_rest=False)
+    w = np.exp(1.5 * g.standard_normal((B, L))).astype(np.float32)
+    if kind == "ties":
+        w = np.round(w)
+    elif kind == "equal":
+        w[:] = 0.5
+    elif kind == "odd":
+        for x in (np.inf, -np.inf, np.nan, 0.0, -0.0, -1.0):
+            w[:, g.permutation(L)[:3]] = x
+    if over > 1:
+        w[0, -2:] = 0.0  # the newest slots go, and the slots past the budget with them
+    pos = np.stack([g.permutation(L) for _ in range(B)]).astype(np.int32)
+    recent = L if kind == "safe" else 20
+    want = ref.evict(k64, v64, table, lens, w, pos, L, budget, 4, recent)
+    for in_place in (False, True):
+        dk, dv = k.clone(), v.clone()
+        dw, dp, dl = _dev(w), _dev(pos), _dev(np.array(lens, np.int32))
+        wo, po, lo = (dw, dp, dl) if in_place else (torch.full_like(dw, 9), torch.full_like(dp, 9), torch.full_like(dl, 9))
+        cg.cache_evict(cg.KVCache(dk, dv), _dev(table), dl, dw, dp, wo, po, lo, B, L, budget, sinks=4, recent=recent)
+        for got, exact in zip((dk, dv, wo, po, lo), want):
+            assert np.array_equal(_f64(got), exact.astype(np.float64), equal_nan=True)
