@@ -17,9 +17,11 @@
 //    by one, 24576 tokens took 68 us).
 //  * move: the rows of K and V, 16 bytes per lane where rows are multiples of
 //    that; few rows are moved by select itself, which saves the second launch.
-//    HBM-bound; the stores pass the L2
-//    by, as nothing reads the rows soon: 24576 tokens to 4096 in 12 mixed
-//    sequences 71.5 us with ordinary stores, 61.5 so, loads past it too 64.4.
+//    HBM-bound.  Where rows are whole
+//    64-byte parts of lines the stores pass the L2 by, as nothing reads the rows
+//    soon: 32 x 8192 tokens to 2048 of 8 heads with 32, 64, 96, 160 elements take
+//    44, 56, 94, 136 us so and 55, 62, 104, 150 with ordinary stores, which other
+//    rows are better with (72 elements 109 against 120).
 #include <algorithm>
 #include <type_traits>
 
@@ -66,6 +68,7 @@ struct Params {
     unsigned* keys; // [batch][key_stride] where they do not fit LDS
     int64_t key_stride;
     FastDiv per;    // by the accesses of a row
+    bool whole;     // rows are whole 64-byte parts of lines
     int team;       // lanes of a move: a power of two up to 64
     int vec;        // elements of an access: the most of 8, 4, 2, 1 that rows and addresses are multiples of
     bool fused;     // select moves the rows
@@ -73,7 +76,7 @@ struct Params {
 
 // Moves first, first + step, .. of a sequence, a team of p.team lanes (`at` of it)
 // each: its accesses are those of the row of every head, four of K and V in flight.
-template <int V>
+template <int V, bool WHOLE = false>
 __device__ __forceinline__ void move_rows(const Params& p, const int32_t* table, const int* src, const int* dst, int count, int first,
                                           int step, int at) {
     typedef std::conditional_t<V == 8, u32x4, std::conditional_t<V == 4, u32x2, std::conditional_t<V == 2, unsigned, uint16_t>>> Word;
@@ -97,8 +100,13 @@ __device__ __forceinline__ void move_rows(const Params& p, const int32_t* table,
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (i0 + u * p.team < items) {
-                    __builtin_nontemporal_store(k[u], reinterpret_cast<Word*>(c.k + to + in_row[u]));
-                    __builtin_nontemporal_store(v[u], reinterpret_cast<Word*>(c.v + to + in_row[u]));
+                    if constexpr (WHOLE) {
+                        __builtin_nontemporal_store(k[u], reinterpret_cast<Word*>(c.k + to + in_row[u]));
+                        __builtin_nontemporal_store(v[u], reinterpret_cast<Word*>(c.v + to + in_row[u]));
+                    } else {
+                        *reinterpret_cast<Word*>(c.k + to + in_row[u]) = k[u];
+                        *reinterpret_cast<Word*>(c.v + to + in_row[u]) = v[u];
+                    }
                 }
         }
     }
@@ -155,7 +163,8 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
     if (p.fused && moving) {
         const int32_t* table = a.block_table + b * a.table_stride;
         const int first = tid / p.team, step = kThreads / p.team, at = tid & (p.team - 1);
-        if (p.vec == 8) move_rows<8>(p, table, src, dst, moving, first, step, at);
+        if (p.whole) move_rows<8, true>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 8) move_rows<8>(p, table, src, dst, moving, first, step, at);
         else if (p.vec == 4) move_rows<4>(p, table, src, dst, moving, first, step, at);
         else if (p.vec == 2) move_rows<2>(p, table, src, dst, moving, first, step, at);
         else move_rows<1>(p, table, src, dst, moving, first, step, at);
@@ -531,7 +540,7 @@ __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
     finish(p, b, keep, moving, src, dst, apart);
 }
 
-template <int V>
+template <int V, bool WHOLE>
 __global__ void __launch_bounds__(256) move(const Params p, FastDiv blocks) {
     const int b = blocks.div(blockIdx.x);
     const int* src = p.lists + (int64_t)b * 2 * p.moves;
@@ -539,7 +548,7 @@ __global__ void __launch_bounds__(256) move(const Params p, FastDiv blocks) {
         p.a.weights_out[b * p.a.weights_out_stride + i] = 0.0f;
         p.a.positions_out[b * p.a.positions_out_stride + i] = -1;
     }
-    move_rows<V>(p, p.a.block_table + b * p.a.table_stride, src, src + p.moves, p.counts[b],
+    move_rows<V, WHOLE>(p, p.a.block_table + b * p.a.table_stride, src, src + p.moves, p.counts[b],
                  ((blockIdx.x - b * blocks.d) * 256 + threadIdx.x) / p.team, blocks.d * 256 / p.team, threadIdx.x & (p.team - 1));
 }
 
@@ -556,6 +565,7 @@ clove_status_t launch_cache_evict(const EvictArgs& a, hipStream_t stream) {
     p.moves = std::max(0, std::min(a.budget, a.max_context - a.budget));
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.cache.k) | reinterpret_cast<uintptr_t>(a.cache.v);
     for (p.vec = 8; a.cache.head_dim % p.vec || a.cache.page_stride % p.vec || at % (2 * p.vec); p.vec /= 2) {}
+    p.whole = a.cache.head_dim % 32 == 0 && a.cache.page_stride % 32 == 0 && at % 64 == 0;
     p.per = FastDiv(a.cache.head_dim / p.vec);
     const int64_t items = (int64_t)a.cache.kv_heads * p.per.d, most = p.moves * items;  // accesses of one move, of a sequence's
     p.team = 1;
@@ -579,7 +589,11 @@ clove_status_t launch_cache_evict(const EvictArgs& a, hipStream_t stream) {
     if ((st = check_launch()) != CLOVE_OK || p.fused) return st;
     // a move a team, at most 32 workgroups per CU
     const int64_t x = std::min<int64_t>(hw::cdiv64((int64_t)p.moves * p.team, 256), std::max<int64_t>(1, hw::cdiv64(32 * dev.num_cus, a.batch)));
-    const auto move = p.vec == 8 ? evict::move<8> : p.vec == 4 ? evict::move<4> : p.vec == 2 ? evict::move<2> : evict::move<1>;
+    const auto move = p.whole      ? evict::move<8, true>
+                      : p.vec == 8 ? evict::move<8, false>
+                      : p.vec == 4 ? evict::move<4, false>
+                      : p.vec == 2 ? evict::move<2, false>
+                                   : evict::move<1, false>;
     CLOVE_LAUNCH(move, dim3((unsigned)(x * a.batch)), dim3(256), 0, stream, p, FastDiv((int)x));
     return check_launch();
 }
