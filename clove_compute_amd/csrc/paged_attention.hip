@@ -26,9 +26,10 @@ struct Params {
     int group;           // query heads per KV head
     int tiles;           // tiles of 16 query heads per KV head (MFMA kernel)
     int chunk, splits;   // keys per workgroup (a multiple of 32), workgroups per (sequence, KV head, tile) at most
-    float* partials;     // [sequence, KV head, tile, split] slabs of `slab` floats; null: one split
-    unsigned* counters;  // [sequence, KV head, tile]
-    int slab;
+    int heads, units;    // batch * kv_heads, and that times splits
+    float* partials;     // [sequence, KV head, tile] `slabs` slabs of `slab` floats: the splits', then the joined ones'
+    unsigned* counters;  // [sequence, KV head, tile][1 + groups of `fan` splits, where there are several]
+    int slab, slabs, counters_per, fan;  // splits that one workgroup joins at most
     float* scores;       // [batch, q_heads] rows of score_stride, base 2, -inf where unseen; null: not wanted
     int64_t score_stride;
     float2* stats;       // [batch, q_heads] (m, l)
@@ -122,20 +123,32 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
     if (p.stats && lane == 0) p.stats[(int64_t)b * a.q_heads + h] = float2{sub, sum};
 }
 
-// weights[b, j] += sum over the heads, in their order
+// weights[b, j] += sum over the heads, in their order: eight heads' scores in
+// flight, their (m, 1 / l) from LDS
 __global__ void __launch_bounds__(256) add_weights(const Params p, int blocks) {
+    extern __shared__ float2 ml[];
     const PagedAttentionArgs& a = p.a;
     const int b = blockIdx.x / blocks, j = (blockIdx.x - b * blocks) * 256 + threadIdx.x;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0;
+    if (j - (int)threadIdx.x >= n) return;
+    const float2* st = p.stats + (int64_t)b * a.q_heads;
+    for (int h = threadIdx.x; h < a.q_heads; h += 256) ml[h] = float2{st[h].x, st[h].y == 0.0f ? 0.0f : 1.0f / st[h].y};
+    __syncthreads();
     if (j < first || j >= n) return;
     const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + j;
-    const float2* st = p.stats + (int64_t)b * a.q_heads;
+    const float before = a.weights[b * a.weights_stride + j];
     float sum = 0.0f;
-    for (int h = 0; h < a.q_heads; ++h) {
-        const float w = exp2f(s[(int64_t)h * p.score_stride] - st[h].x) / st[h].y;
-        if (st[h].y != 0.0f) sum += w;
+    for (int h0 = 0; h0 < a.q_heads; h0 += 8) {
+        float t[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) t[u] = h0 + u < a.q_heads ? s[(int64_t)(h0 + u) * p.score_stride] : -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float2 x = ml[min(h0 + u, a.q_heads - 1)];
+            sum += x.y == 0.0f ? 0.0f : exp2f(t[u] - x.x) * x.y;
+        }
     }
-    a.weights[b * a.weights_stride + j] += sum;
+    a.weights[b * a.weights_stride + j] = before + sum;
 }
 
 template <int DT>
@@ -166,8 +179,10 @@ void launch_any(const Params& p, hipStream_t stream) {
 // product has read them, those of V as soon as they are in LDS: 8 to 16 KB (at
 // head_dim 128) are in flight per wave nearly all the time.
 //
-// Workgroups of one (sequence, KV head, tile) publish (O, m, l) past the L2s; the
-// last to arrive joins them in the order of the splits.
+// Workgroups of one (sequence, KV head, tile) publish (O, m, l) past the L2s and
+// the last to arrive joins them, or, where they are much to read for one, the
+// last of each group its group's, and the last of those the joined ones.  The
+// order of a sum is that of the splits whoever does it.
 // ---------------------------------------------------------------------------
 template <int DT>
 struct Mfma;
@@ -251,14 +266,91 @@ __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, fl
     for (int i = 0; i < 4; ++i) o[i] = o[i] * f + o2[i] * f2;
 }
 
+// A slab: O [16 heads][quads] of four, then (m, l) [16].
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slab_of(const Params& p, int pair, int i) {
+    return __builtin_amdgcn_make_buffer_rsrc(p.partials + ((int64_t)pair * p.slabs + i) * p.slab, (short)0, p.slab * 4, 0x00020000);
+}
+__device__ __forceinline__ void publish(const __amdgpu_buffer_rsrc_t& r, int h, int quad, int quads, float M, float L, const f32x4& O) {
+    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(O), r, (h * quads + quad) * 16, 0, kCpolSc1);
+    if (quad == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{bitcast<unsigned>(M), bitcast<unsigned>(L)}, r, 256 * quads + 8 * h, 0, kCpolSc1);
+}
+// `count` slabs from slab `first`, joined in their order
+__device__ __forceinline__ void join(const Params& p, int pair, int first, int count, int h, int quad, int quads, float& M, float& L, f32x4& O) {
+    constexpr int U = 16;  // in flight
+    M = -__builtin_inff();
+    L = 0.0f;
+    O = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < count; s0 += U) {
+        u32x4 x[U];
+        u32x2 ml[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const __amdgpu_buffer_rsrc_t r = slab_of(p, pair, first + min(s0 + u, count - 1));
+            ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, 256 * quads + 8 * h, 0, kCpolSc1);
+            x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (h * quads + quad) * 16, 0, kCpolSc1);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < count) merge(M, L, O, bitcast<float>(ml[u][0]), bitcast<float>(ml[u][1]), bitcast<f32x4>(x[u]));
+    }
+}
+
+// The same by the whole workgroup, done(head, quad, M, L, O) for each of its
+// heads' quads: teams of as many threads as there are quads take runs of the
+// slabs, and the first merges theirs in their order.
+template <typename F>
+__device__ __forceinline__ void join_all(const Params& p, char* lds, int pair, int first, int count, int quads, int items, F done) {
+    const int teams = max(1, min(64 * kW / items, count / 8)), run = cdiv(count, teams), tid = threadIdx.x;
+    if (teams == 1) {
+        for (int i = tid; i < items; i += 64 * kW) {
+            const int h = i / quads, quad = i - h * quads;
+            float M, L;
+            f32x4 O;
+            join(p, pair, first, count, h, quad, quads, M, L, O);
+            done(h, quad, M, L, O);
+        }
+        return;
+    }
+    f32x4* const team_o = reinterpret_cast<f32x4*>(lds);
+    float2* const team_ml = reinterpret_cast<float2*>(lds + 64 * kW * 16);
+    const int team = tid / items, item = tid - team * items, h = item / quads, quad = item - h * quads;
+    const int mine = min(run, count - team * run);  // none for a thread past the teams
+    float M = -__builtin_inff(), L = 0.0f;
+    f32x4 O{0.f, 0.f, 0.f, 0.f};
+    if (team < teams && mine > 0) join(p, pair, first + team * run, mine, h, quad, quads, M, L, O);
+    team_o[tid] = O;
+    team_ml[tid] = float2{M, L};
+    __syncthreads();
+    if (team == 0) {
+        for (int t = 1; t < teams; ++t) {
+            const float2 ml = team_ml[t * items + item];
+            merge(M, L, O, ml.x, ml.y, team_o[t * items + item]);
+        }
+        done(h, quad, M, L, O);
+    }
+}
+
 template <int DT, int NC, bool TAIL>
 __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
     extern __shared__ __align__(16) char lds[];
     __shared__ int last;
     const PagedAttentionArgs& a = p.a;
     const PagedCache& cache = a.cache;
-    const int split = blockIdx.x % p.splits, pair = blockIdx.x / p.splits;
-    const int tile = pair % p.tiles, bk = pair / p.tiles, b = bk / cache.kv_heads, kh = bk - b * cache.kv_heads;
+    // Workgroups go to the XCDs in turn: the splits of a sequence, of which a short
+    // one has fewer, are the slowest index, so that each XCD has its share of
+    // the work (as the fastest, 48 mixed sequences in 8 splits took 70 us, each
+    // split on an XCD of its own).  Tiles of the same keys lie eight
+    // workgroups apart: on one XCD, whose L2 the first of them fills.
+    int unit = blockIdx.x, tile = 0;
+    if (p.tiles > 1) {
+        const int run = unit / (8 * p.tiles), in_run = unit - run * 8 * p.tiles;
+        tile = in_run >> 3;
+        unit = 8 * run + (in_run & 7);
+        if (unit >= p.units) return;
+    }
+    const int split = unit / p.heads, bk = unit - split * p.heads, b = bk / cache.kv_heads, kh = bk - b * cache.kv_heads;
+    const int pair = bk * p.tiles + tile;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
     const int D = cache.head_dim, G = min(16, p.group - 16 * tile), h0 = kh * p.group + 16 * tile;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0, base = first & ~31;
@@ -277,9 +369,10 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
 
     // the pages of this lane's two keys (16 apart) of the wave's 32 from key j
     const int32_t* table = a.block_table + b * a.table_stride;
-    auto page_of = [&](int j) { return j >= first && j < end ? table[p.page.div(j)] : -1; };
+    // (read by the bound of the lengths and judged by the length, which the first look-up so need not await)
+    auto page_of = [&](int j) { return j < a.max_context ? table[p.page.div(j)] : -1; };
     auto offset_of = [&](int j, int id, bool& ok) {
-        ok = (unsigned)id < (unsigned)cache.num_pages;
+        ok = j >= first && j < end && (unsigned)id < (unsigned)cache.num_pages;
         const int in_page = j - p.page.div(j) * cache.page_size;
         return ok ? (int64_t)id * cache.page_stride + ((int64_t)kh * cache.page_size + in_page) * D : (int64_t)0;
     };
@@ -421,7 +514,6 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
     }
     __syncthreads();
     const int quads = cdiv(D, 4), items = G * quads;
-    float* const slabs = p.partials + (int64_t)pair * p.splits * p.slab;
     auto finish = [&](int h, int quad, float M, float L, const f32x4& O) {
         f32x4 x;
 #pragma unroll
@@ -429,8 +521,6 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         store4<DT>(a.out + b * a.out_stride + (int64_t)(h0 + h) * D, 4 * quad, D, vec, x);
         if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L};
     };
-    const __amdgpu_buffer_rsrc_t slab_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        slabs + (int64_t)split * p.slab, (short)0, total > 1 ? p.slab * 4 : 0, 0x00020000);
     for (int i = threadIdx.x; i < items; i += 64 * kW) {
         const int h = i / quads, quad = i - h * quads;
         float M = -__builtin_inff(), L = 0.0f;
@@ -441,63 +531,29 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
             const float2 ml = *reinterpret_cast<const float2*>(x + 16 * o_stride<NC>() + 2 * h);
             merge(M, L, O, ml.x, ml.y, *reinterpret_cast<const f32x4*>(x + h * o_stride<NC>() + 4 * quad));
         }
-        if (total == 1) {
-            finish(h, quad, M, L, O);
-        } else {
-            __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(O), slab_rsrc, (h * quads + quad) * 16, 0, kCpolSc1);
-            if (quad == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u32x2{bitcast<unsigned>(M), bitcast<unsigned>(L)}, slab_rsrc,
-                                                      16 * 16 * quads + 8 * h, 0, kCpolSc1);
-        }
+        if (total == 1) finish(h, quad, M, L, O);
+        else publish(slab_of(p, pair, split), h, quad, quads, M, L, O);
     }
-    if (total == 1 || !splitk_arrive_is_last(p.counters + pair, total, &last)) return;
-
-    // the last workgroup joins the splits: teams of `items` threads take runs of
-    // them, then team 0 merges the teams
-    const int teams = max(1, min(64 * kW / items, total)), run = cdiv(total, teams);
-    f32x4* const team_o = reinterpret_cast<f32x4*>(lds);
-    float2* const team_ml = reinterpret_cast<float2*>(lds + 64 * kW * 16);
-    for (int i0 = 0; i0 < items; i0 += 64 * kW) {
-        const int i = i0 + (int)threadIdx.x, team = teams > 1 ? i / items : 0, item = teams > 1 ? i - team * items : i;
-        const bool on = team < teams && item < items;
-        const int h = on ? item / quads : 0, quad = on ? item - h * quads : 0;
-        float M = -__builtin_inff(), L = 0.0f;
-        f32x4 O{0.f, 0.f, 0.f, 0.f};
-        if (on) {
-            constexpr int U = 8;
-            const int s1 = min(total, (team + 1) * run);
-            for (int s0 = team * run; s0 < s1; s0 += U) {
-                u32x4 x[U];
-                u32x2 ml[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (s0 + u >= s1) break;
-                    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(slabs + (int64_t)(s0 + u) * p.slab, (short)0,
-                                                                                       p.slab * 4, 0x00020000);
-                    x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (h * quads + quad) * 16, 0, kCpolSc1);
-                    ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, 16 * 16 * quads + 8 * h, 0, kCpolSc1);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (s0 + u >= s1) break;
-                    merge(M, L, O, bitcast<float>(ml[u][0]), bitcast<float>(ml[u][1]), bitcast<f32x4>(x[u]));
-                }
-            }
-        }
-        if (teams > 1) {  // (then items < 64 kW: one round)
-            __syncthreads();
-            team_o[threadIdx.x] = O;
-            team_ml[threadIdx.x] = float2{M, L};
-            __syncthreads();
-            if (team == 0)
-                for (int t = 1; t < teams; ++t) {
-                    const float2 ml = team_ml[t * items + item];
-                    merge(M, L, O, ml.x, ml.y, team_o[t * items + item]);
-                }
-        }
-        if (on && team == 0) finish(h, quad, M, L, O);
+    if (total == 1) return;
+    unsigned* const counters = p.counters + (int64_t)pair * p.counters_per;
+    int from = 0, count = total;
+    if (total > p.fan) {
+        const int group = split / p.fan, members = min(p.fan, total - group * p.fan);
+        if (!splitk_arrive_is_last(counters + 1 + group, members, &last)) return;
+        join_all(p, lds, pair, group * p.fan, members, quads, items, [&](int h, int quad, float M, float L, const f32x4& O) {
+            publish(slab_of(p, pair, p.splits + group), h, quad, quads, M, L, O);
+        });
+        from = p.splits;
+        count = cdiv(total, p.fan);
     }
+    if (!splitk_arrive_is_last(counters, count, &last)) return;
+    join_all(p, lds, pair, from, count, quads, items, finish);
 }
+
+// Workgroups of the MFMA kernel that a CU holds at once, by head_dim / 32: what
+// its registers leave (a workgroup has one wave on each SIMD; rows at any
+// alignment hold one fewer at 3 and 6)
+constexpr int kResident[8] = {5, 4, 3, 2, 2, 2, 1, 1};
 
 template <int DT, bool TAIL>
 clove_status_t launch_mfma(const Params& p, hipStream_t stream) {
@@ -507,7 +563,7 @@ clove_status_t launch_mfma(const Params& p, hipStream_t stream) {
     static const int bytes[8] = {wave_lds<1>(), wave_lds<2>(), wave_lds<3>(), wave_lds<4>(),
                                  wave_lds<5>(), wave_lds<6>(), wave_lds<7>(), wave_lds<8>()};
     const int nc = cdiv(p.a.cache.head_dim, 32) - 1;
-    const int64_t grid = (int64_t)p.a.batch * p.a.cache.kv_heads * p.tiles * p.splits;
+    const int64_t grid = p.tiles > 1 ? (int64_t)cdiv(p.units, 8) * 8 * p.tiles : p.units;
     const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(kernels[nc]), kW * bytes[nc]);
     if (st != CLOVE_OK) return st;
     CLOVE_LAUNCH(kernels[nc], dim3((unsigned)grid), dim3(64 * kW), (size_t)kW * bytes[nc], stream, p);
@@ -542,21 +598,32 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         const int64_t pairs = (int64_t)a.batch * c.kv_heads * p.tiles;
         // a window need not start at a whole 32 keys
         const int span = std::max(1, a.window > 0 ? (int)std::min<int64_t>(a.max_context, (int64_t)a.window + 31) : a.max_context);
-        int64_t chunk = hw::cdiv64((int64_t)span * pairs, 3 * dev.num_cus);
-        chunk = std::max<int64_t>(chunk, 128);
-        chunk = std::max<int64_t>(std::min<int64_t>(chunk, 1024), (int64_t)span * pairs >> 28);
-        p.chunk = (int)(hw::cdiv64(chunk, 128) * 128);
+        // Splits that fill the CUs a whole number of times, of up to 1024 keys
+        const int64_t fill = (int64_t)dev.num_cus * paged::kResident[hw::cdiv(c.head_dim, 32) - 1];
+        const int64_t keys = pairs * span, rounds = hw::cdiv64(keys, fill * 1024);
+        int64_t chunk = hw::cdiv64(hw::cdiv64(keys, fill * rounds), 128) * 128;
+        chunk = std::max<int64_t>(chunk, hw::cdiv64(keys >> 28, 128) * 128);
+        p.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
         p.splits = hw::cdiv(span, p.chunk);
-        if (pairs > 16384 || p.splits == 1) {
+        // what a workgroup reads in about 3 us; another round of arrivals takes as long
+        p.fan = std::max(16, std::min(64, (128 << 10) / (std::min(p.group, 16) * c.head_dim * 4)));
+        const int groups = p.splits > p.fan ? hw::cdiv(p.splits, p.fan) : 0;
+        p.counters_per = 1 + groups;
+        if (pairs * p.counters_per > 16384 || p.splits == 1) {
             p.splits = 1;
-            p.chunk = (int)std::min<int64_t>(hw::cdiv64(span, 128) * 128, 0x7fffff80);
+            p.chunk = (int)(hw::cdiv64(span, 128) * 128);
         } else {
             p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
+            p.slabs = p.splits + groups;
             Scratch scratch;
-            if ((st = acquire_scratch(stream, (size_t)pairs * p.splits * p.slab * 4, (size_t)pairs, &scratch)) != CLOVE_OK) return st;
+            if ((st = acquire_scratch(stream, (size_t)pairs * p.slabs * p.slab * 4, (size_t)pairs * p.counters_per, &scratch)) != CLOVE_OK)
+                return st;
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
+        if ((int64_t)a.batch * c.kv_heads * p.splits * p.tiles > 0x7fffff00) return CLOVE_ERR_INVALID_DIM;
+        p.heads = a.batch * c.kv_heads;
+        p.units = p.heads * p.splits;
         const bool whole = c.head_dim % 8 == 0 && c.page_stride % 8 == 0 && a.q_stride % 8 == 0 && a.out_stride % 4 == 0 &&
                            aligned16(a.q) && aligned16(c.k) && aligned16(c.v) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
         if (c.dtype == CLOVE_DTYPE_FP16)
@@ -567,7 +634,7 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
     }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;
     const int blocks = hw::cdiv(a.max_context, 256);
-    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(256), 0, stream, p, blocks);
+    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(256), a.q_heads * sizeof(float2), stream, p, blocks);
     return check_launch();
 }
 
