@@ -196,18 +196,6 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t v) {
     return ((uint64_t)hi << 32) | wave_min((unsigned)(v >> 32) == hi ? (unsigned)v : 0xffffffffu);
 }
 
-// Inclusive prefix sum over the wave: DPP row_shr 1, 2, 4, 8 inside the rows of
-// 16, then the last lane of a row added to the rows after it.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
-    return v;
-}
-
 constexpr int kHeld = 16;  // tokens of a thread that stay in registers from the first load on
 
 template <bool IN_LDS>

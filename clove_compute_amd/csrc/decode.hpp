@@ -34,6 +34,18 @@ struct Elem<CLOVE_DTYPE_FP32> {
     static __device__ __forceinline__ raw store(float f) { return f; }
 };
 
+// Inclusive prefix sum over the wave: DPP row_shr 1, 2, 4, 8 inside the rows of
+// 16, then the last lane of a row added to the rows after it.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
+    return v;
+}
+
 }  // namespace hw
 
 // n / d for 0 <= n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and

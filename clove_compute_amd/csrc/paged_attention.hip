@@ -25,11 +25,14 @@ struct Params {
     FastDiv page;        // by the page size
     int group;           // query heads per KV head
     int tiles;           // tiles of 16 query heads per KV head (MFMA kernel)
-    int chunk, splits;   // keys per workgroup (a multiple of 32), workgroups per (sequence, KV head, tile) at most
-    int heads, units;    // batch * kv_heads, and that times splits
-    float* partials;     // [sequence, KV head, tile] `slabs` slabs of `slab` floats: the splits', then the joined ones'
-    unsigned* counters;  // [sequence, KV head, tile][1 + groups of `fan` splits, where there are several]
-    int slab, slabs, counters_per, fan;  // splits that one workgroup joins at most
+    // With more keys than one workgroup per (sequence, KV head, tile) should take,
+    // the kernel cuts each sequence by the lengths it finds (Cut)
+    bool cuts;
+    int fill;            // workgroups that the CUs hold at once
+    int slots;           // most workgroups with keys: all of them, where it does not cut
+    float* partials;     // [slots] slabs of `slab` floats, then as many for joined ones
+    unsigned* counters;  // [sequence, KV head, tile], then [slots] of groups of `fan` splits
+    int slab, fan;       // (a workgroup joins `fan` at most)
     float* scores;       // [batch, q_heads] rows of score_stride, base 2, -inf where unseen; null: not wanted
     int64_t score_stride;
     float2* stats;       // [batch, q_heads] (m, l)
@@ -266,18 +269,79 @@ __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, fl
     for (int i = 0; i < 4; ++i) o[i] = o[i] * f + o2[i] * f2;
 }
 
-// A slab: O [16 heads][quads] of four, then (m, l) [16].
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t slab_of(const Params& p, int pair, int i) {
-    return __builtin_amdgcn_make_buffer_rsrc(p.partials + ((int64_t)pair * p.slabs + i) * p.slab, (short)0, p.slab * 4, 0x00020000);
+// How the kernel shares out the keys: into `chunk`s of so many 32s of keys that
+// there are about `fill` of them (per KV head and tile), or several times that
+// where they would be longer than kLongest, a sequence's chunks of one length.
+// Every wave works it out for itself from the lengths, 64 sequences at a time.
+// (By the bound of the lengths alone, most workgroups of 48 mixed sequences had no
+// keys, and those that had some waited for them to pass: 55 us instead of WORKUS.)
+constexpr int kLongest = 32;  // x 32 keys
+
+struct Cut {
+    int b, split, total;     // this workgroup's sequence, its split and how many it has
+    int first;               // workgroup of split 0 among those of all sequences, before KV heads and tiles
+    int chunk;               // 32s of keys of each split
+};
+
+__device__ __forceinline__ int keys32(const PagedAttentionArgs& a, int n) {
+    const int first = a.window > 0 ? max(0, n - a.window) & ~31 : 0;
+    return cdiv(n - first, 32);
 }
-__device__ __forceinline__ void publish(const __amdgpu_buffer_rsrc_t& r, int h, int quad, int quads, float M, float L, const f32x4& O) {
-    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(O), r, (h * quads + quad) * 16, 0, kCpolSc1);
+
+// Sequence and split of workgroup `i` (of those before KV heads and tiles);
+// .b < 0 where there are fewer.
+__device__ __forceinline__ Cut cut(const Params& p, int i, int per) {
+    const PagedAttentionArgs& a = p.a;
+    const int lane = threadIdx.x & 63;
+    int sum = 0, t0 = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int t = b0 + lane < a.batch ? keys32(a, context(a, b0 + lane)) : 0;
+        if (b0 == 0) t0 = t;
+        sum += wave_sum(t);
+    }
+    const int64_t all = (int64_t)sum * per;
+    const int64_t rounds = max((int64_t)1, (all + (int64_t)p.fill * kLongest - 1) / ((int64_t)p.fill * kLongest));
+    const int64_t want = (all + p.fill * rounds - 1) / (p.fill * rounds);
+    const int chunk = max(kW, (int)((want + kW - 1) / kW) * kW);  // a wave takes every fourth of them
+    int before = 0;
+    Cut c{-1, 0, 0, 0, 0};
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const bool on = b0 + lane < a.batch;
+        const int t = b0 == 0 ? t0 : on ? keys32(a, context(a, b0 + lane)) : 0;
+        const int splits = on ? max(1, cdiv(t, chunk)) : 0, upto = before + wave_scan(splits);
+        const unsigned long long in = __ballot(on && i >= upto - splits && i < upto);
+        if (in) {
+            const int who = __ffsll((long long)in) - 1;
+            c.b = b0 + who;
+            c.total = __builtin_amdgcn_readlane(splits, who);
+            c.first = __builtin_amdgcn_readlane(upto, who) - c.total;
+            c.split = i - c.first;
+            const int own = cdiv(__builtin_amdgcn_readlane(t, who), c.total);
+            c.chunk = cdiv(own, kW) * kW;
+            return c;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return c;
+}
+
+// A slab: O [16 heads][quads] of four, then (m, l) [16].  All slabs are one
+// buffer: the slab is part of a lane's offset, as lanes may read different ones.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t slabs_of(const Params& p) {
+    return __builtin_amdgcn_make_buffer_rsrc(p.partials, (short)0, p.partials ? 2 * p.slots * p.slab * 4 : 0, 0x00020000);
+}
+__device__ __forceinline__ void publish(const Params& p, const __amdgpu_buffer_rsrc_t& r, int slab, int h, int quad, int quads, float M, float L,
+                                        const f32x4& O) {
+    const int at = slab * p.slab * 4;
+    __builtin_amdgcn_raw_buffer_store_b128(bitcast<u32x4>(O), r, at + (h * quads + quad) * 16, 0, kCpolSc1);
     if (quad == 0)
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{bitcast<unsigned>(M), bitcast<unsigned>(L)}, r, 256 * quads + 8 * h, 0, kCpolSc1);
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{bitcast<unsigned>(M), bitcast<unsigned>(L)}, r, at + 256 * quads + 8 * h, 0, kCpolSc1);
 }
-// `count` slabs from slab `first`, joined in their order
-__device__ __forceinline__ void join(const Params& p, int pair, int first, int count, int h, int quad, int quads, float& M, float& L, f32x4& O) {
-    constexpr int U = 16;  // in flight
+
+// `count` slabs `step` apart from slab `first`, joined in their order, U at a time in flight
+template <int U>
+__device__ __forceinline__ void join(const Params& p, const __amdgpu_buffer_rsrc_t& r, int first, int step, int count, int h, int quad, int quads,
+                                     float& M, float& L, f32x4& O) {
     M = -__builtin_inff();
     L = 0.0f;
     O = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -286,9 +350,9 @@ __device__ __forceinline__ void join(const Params& p, int pair, int first, int c
         u32x2 ml[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const __amdgpu_buffer_rsrc_t r = slab_of(p, pair, first + min(s0 + u, count - 1));
-            ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, 256 * quads + 8 * h, 0, kCpolSc1);
-            x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, (h * quads + quad) * 16, 0, kCpolSc1);
+            const int at = (first + min(s0 + u, count - 1) * step) * p.slab * 4;
+            ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, at + 256 * quads + 8 * h, 0, kCpolSc1);
+            x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (h * quads + quad) * 16, 0, kCpolSc1);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -300,14 +364,15 @@ __device__ __forceinline__ void join(const Params& p, int pair, int first, int c
 // heads' quads: teams of as many threads as there are quads take runs of the
 // slabs, and the first merges theirs in their order.
 template <typename F>
-__device__ __forceinline__ void join_all(const Params& p, char* lds, int pair, int first, int count, int quads, int items, F done) {
+__device__ __forceinline__ void join_all(const Params& p, const __amdgpu_buffer_rsrc_t& r, char* lds, int first, int step, int count, int quads, int items, F done) {
     const int teams = max(1, min(64 * kW / items, count / 8)), run = cdiv(count, teams), tid = threadIdx.x;
     if (teams == 1) {
         for (int i = tid; i < items; i += 64 * kW) {
             const int h = i / quads, quad = i - h * quads;
             float M, L;
             f32x4 O;
-            join(p, pair, first, count, h, quad, quads, M, L, O);
+            count <= 4 ? join<4>(p, r, first, step, count, h, quad, quads, M, L, O)
+                       : join<16>(p, r, first, step, count, h, quad, quads, M, L, O);
             done(h, quad, M, L, O);
         }
         return;
@@ -318,7 +383,7 @@ __device__ __forceinline__ void join_all(const Params& p, char* lds, int pair, i
     const int mine = min(run, count - team * run);  // none for a thread past the teams
     float M = -__builtin_inff(), L = 0.0f;
     f32x4 O{0.f, 0.f, 0.f, 0.f};
-    if (team < teams && mine > 0) join(p, pair, first + team * run, mine, h, quad, quads, M, L, O);
+    if (team < teams && mine > 0) join<16>(p, r, first + team * run * step, step, mine, h, quad, quads, M, L, O);
     team_o[tid] = O;
     team_ml[tid] = float2{M, L};
     __syncthreads();
@@ -337,26 +402,25 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
     __shared__ int last;
     const PagedAttentionArgs& a = p.a;
     const PagedCache& cache = a.cache;
-    // Workgroups go to the XCDs in turn: the splits of a sequence, of which a short
-    // one has fewer, are the slowest index, so that each XCD has its share of
-    // the work (as the fastest, 48 mixed sequences in 8 splits took 70 us, each
-    // split on an XCD of its own).  Tiles of the same keys lie eight
+    // Workgroups go to the XCDs in turn: KV heads are the fastest index, so that
+    // each XCD has its share of every sequence.  Tiles of the same keys lie eight
     // workgroups apart: on one XCD, whose L2 the first of them fills.
     int unit = blockIdx.x, tile = 0;
     if (p.tiles > 1) {
         const int run = unit / (8 * p.tiles), in_run = unit - run * 8 * p.tiles;
         tile = in_run >> 3;
         unit = 8 * run + (in_run & 7);
-        if (unit >= p.units) return;
     }
-    const int split = unit / p.heads, bk = unit - split * p.heads, b = bk / cache.kv_heads, kh = bk - b * cache.kv_heads;
-    const int pair = bk * p.tiles + tile;
+    const int seq = unit / cache.kv_heads, kh = unit - seq * cache.kv_heads, per = cache.kv_heads * p.tiles;
+    Cut c{seq, 0, 1, seq, 0};
+    if (p.cuts) c = cut(p, seq, per);
+    const int b = c.b, split = c.split, total = c.total;
+    if (b < 0 || b >= a.batch) return;
+    const int pair = (b * cache.kv_heads + kh) * p.tiles + tile, slab0 = (c.first * cache.kv_heads + kh) * p.tiles + tile;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
     const int D = cache.head_dim, G = min(16, p.group - 16 * tile), h0 = kh * p.group + 16 * tile;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0, base = first & ~31;
-    const int total = max(1, cdiv(n - base, p.chunk));  // workgroups that have keys (one of them where there are none)
-    if (split >= total) return;
-    const int begin = base + split * p.chunk, end = min(n, begin + p.chunk);
+    const int begin = base + split * c.chunk * 32, end = p.cuts ? min(n, begin + c.chunk * 32) : n;
     const bool vec = !TAIL;
 
     u32x4 q[NC];
@@ -521,6 +585,7 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         store4<DT>(a.out + b * a.out_stride + (int64_t)(h0 + h) * D, 4 * quad, D, vec, x);
         if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L};
     };
+    const __amdgpu_buffer_rsrc_t slabs = slabs_of(p);
     for (int i = threadIdx.x; i < items; i += 64 * kW) {
         const int h = i / quads, quad = i - h * quads;
         float M = -__builtin_inff(), L = 0.0f;
@@ -532,22 +597,22 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
             merge(M, L, O, ml.x, ml.y, *reinterpret_cast<const f32x4*>(x + h * o_stride<NC>() + 4 * quad));
         }
         if (total == 1) finish(h, quad, M, L, O);
-        else publish(slab_of(p, pair, split), h, quad, quads, M, L, O);
+        else publish(p, slabs, slab0 + split * per, h, quad, quads, M, L, O);
     }
     if (total == 1) return;
-    unsigned* const counters = p.counters + (int64_t)pair * p.counters_per;
-    int from = 0, count = total;
+    int from = slab0, step = per, count = total;
     if (total > p.fan) {
-        const int group = split / p.fan, members = min(p.fan, total - group * p.fan);
-        if (!splitk_arrive_is_last(counters + 1 + group, members, &last)) return;
-        join_all(p, lds, pair, group * p.fan, members, quads, items, [&](int h, int quad, float M, float L, const f32x4& O) {
-            publish(slab_of(p, pair, p.splits + group), h, quad, quads, M, L, O);
+        const int group = split / p.fan, members = min(p.fan, total - group * p.fan), lead = slab0 + group * p.fan * per;
+        if (!splitk_arrive_is_last(p.counters + a.batch * per + lead, members, &last)) return;
+        join_all(p, slabs, lds, lead, per, members, quads, items, [&](int h, int quad, float M, float L, const f32x4& O) {
+            publish(p, slabs, p.slots + lead, h, quad, quads, M, L, O);
         });
-        from = p.splits;
+        from += p.slots;
+        step *= p.fan;
         count = cdiv(total, p.fan);
     }
-    if (!splitk_arrive_is_last(counters, count, &last)) return;
-    join_all(p, lds, pair, from, count, quads, items, finish);
+    if (!splitk_arrive_is_last(p.counters + pair, count, &last)) return;
+    join_all(p, slabs, lds, from, step, count, quads, items, finish);
 }
 
 // Workgroups of the MFMA kernel that a CU holds at once, by head_dim / 32: what
@@ -563,7 +628,7 @@ clove_status_t launch_mfma(const Params& p, hipStream_t stream) {
     static const int bytes[8] = {wave_lds<1>(), wave_lds<2>(), wave_lds<3>(), wave_lds<4>(),
                                  wave_lds<5>(), wave_lds<6>(), wave_lds<7>(), wave_lds<8>()};
     const int nc = cdiv(p.a.cache.head_dim, 32) - 1;
-    const int64_t grid = p.tiles > 1 ? (int64_t)cdiv(p.units, 8) * 8 * p.tiles : p.units;
+    const int units = p.slots / p.tiles, grid = p.tiles > 1 ? cdiv(units, 8) * 8 * p.tiles : units;
     const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(kernels[nc]), kW * bytes[nc]);
     if (st != CLOVE_OK) return st;
     CLOVE_LAUNCH(kernels[nc], dim3((unsigned)grid), dim3(64 * kW), (size_t)kW * bytes[nc], stream, p);
@@ -595,35 +660,26 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         else paged::launch_any<CLOVE_DTYPE_BF16>(p, stream);
     } else {
         p.tiles = hw::cdiv(p.group, 16);
-        const int64_t pairs = (int64_t)a.batch * c.kv_heads * p.tiles;
+        const int per = c.kv_heads * p.tiles;
+        const int64_t pairs = (int64_t)a.batch * per;
         // a window need not start at a whole 32 keys
         const int span = std::max(1, a.window > 0 ? (int)std::min<int64_t>(a.max_context, (int64_t)a.window + 31) : a.max_context);
-        // Splits that fill the CUs a whole number of times, of up to 1024 keys
-        const int64_t fill = (int64_t)dev.num_cus * paged::kResident[hw::cdiv(c.head_dim, 32) - 1];
-        const int64_t keys = pairs * span, rounds = hw::cdiv64(keys, fill * 1024);
-        int64_t chunk = hw::cdiv64(hw::cdiv64(keys, fill * rounds), 128) * 128;
-        chunk = std::max<int64_t>(chunk, hw::cdiv64(keys >> 28, 128) * 128);
-        p.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
-        p.splits = hw::cdiv(span, p.chunk);
-        // what a workgroup reads in about 3 us; another round of arrivals takes as long
-        p.fan = std::max(16, std::min(64, (128 << 10) / (std::min(p.group, 16) * c.head_dim * 4)));
-        const int groups = p.splits > p.fan ? hw::cdiv(p.splits, p.fan) : 0;
-        p.counters_per = 1 + groups;
-        if (pairs * p.counters_per > 16384 || p.splits == 1) {
-            p.splits = 1;
-            p.chunk = (int)(hw::cdiv64(span, 128) * 128);
-        } else {
-            p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
-            p.slabs = p.splits + groups;
+        p.fill = dev.num_cus * paged::kResident[hw::cdiv(c.head_dim, 32) - 1];
+        // chunks: the CUs' fill a whole number of rounds, and a remainder of each sequence
+        const int64_t rounds = std::max<int64_t>(1, hw::cdiv64(pairs * hw::cdiv(span, 32), (int64_t)p.fill * paged::kLongest));
+        const int64_t slots = (hw::cdiv64(p.fill * rounds, per) + a.batch) * per;
+        p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
+        p.slots = (int)pairs;
+        p.cuts = span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
+        if (p.cuts) {
+            p.slots = (int)slots;
+            // what a workgroup reads in about 3 us; another round of arrivals takes as long
+            p.fan = std::max(16, std::min(64, (128 << 10) / (std::min(p.group, 16) * c.head_dim * 4)));
             Scratch scratch;
-            if ((st = acquire_scratch(stream, (size_t)pairs * p.slabs * p.slab * 4, (size_t)pairs * p.counters_per, &scratch)) != CLOVE_OK)
-                return st;
+            if ((st = acquire_scratch(stream, (size_t)2 * p.slots * p.slab * 4, (size_t)(pairs + slots), &scratch)) != CLOVE_OK) return st;
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
-        if ((int64_t)a.batch * c.kv_heads * p.splits * p.tiles > 0x7fffff00) return CLOVE_ERR_INVALID_DIM;
-        p.heads = a.batch * c.kv_heads;
-        p.units = p.heads * p.splits;
         const bool whole = c.head_dim % 8 == 0 && c.page_stride % 8 == 0 && a.q_stride % 8 == 0 && a.out_stride % 4 == 0 &&
                            aligned16(a.q) && aligned16(c.k) && aligned16(c.v) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
         if (c.dtype == CLOVE_DTYPE_FP16)
