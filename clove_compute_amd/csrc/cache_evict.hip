@@ -81,7 +81,8 @@ __device__ __forceinline__ void move_rows(const Params& p, const int32_t* table,
                                           int step, int at) {
     typedef std::conditional_t<V == 8, u32x4, std::conditional_t<V == 4, u32x2, std::conditional_t<V == 2, unsigned, uint16_t>>> Word;
     const PagedCache& c = p.a.cache;
-    const int head = c.page_size * c.head_dim, items = c.kv_heads * p.per.d;
+    const int64_t head = (int64_t)c.page_size * c.head_dim;
+    const int items = c.kv_heads * p.per.d;
     for (int64_t j = first; j < count; j += step) {
         const int64_t from = row_at(c, p.page, table, src[j]), to = row_at(c, p.page, table, dst[j]);
         if (from < 0 || to < 0) continue;
@@ -91,7 +92,7 @@ __device__ __forceinline__ void move_rows(const Params& p, const int32_t* table,
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int i = i0 + u * p.team, h = p.per.div(i);
-                in_row[u] = (int64_t)h * head + (int64_t)(i - h * p.per.d) * V;
+                in_row[u] = h * head + (int64_t)(i - h * p.per.d) * V;
                 if (i < items) {
                     k[u] = *reinterpret_cast<const Word*>(c.k + from + in_row[u]);
                     v[u] = *reinterpret_cast<const Word*>(c.v + from + in_row[u]);

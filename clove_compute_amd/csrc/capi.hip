@@ -608,7 +608,8 @@ clove_status_t clove_w4a16_swiglu(const void* X, const uint8_t* W_q, const void*
 // The descriptor of a cache checked and laid out for kernels.
 static clove_status_t read_cache(const clove_kv_cache_t* c, PagedCache* out) {
     if (c->dtype != CLOVE_DTYPE_FP16 && c->dtype != CLOVE_DTYPE_BF16) return CLOVE_ERR_INVALID_ARG;
-    if (c->num_pages < 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_dim <= 0 || c->head_dim > CLOVE_MAX_HEAD_DIM)
+    if (c->num_pages < 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->kv_heads > 0x10000 ||
+        c->head_dim <= 0 || c->head_dim > CLOVE_MAX_HEAD_DIM)
         return CLOVE_ERR_INVALID_DIM;
     const int64_t rows = (int64_t)c->kv_heads * c->page_size;
     if (rows > ((int64_t)1 << 40) / c->head_dim) return CLOVE_ERR_INVALID_DIM;

@@ -38,6 +38,10 @@ struct Params {
     float2* stats;       // [batch, q_heads] (m, l)
 };
 
+// 2^x by the hardware's instruction: within 1 unit in the last place, results
+// below 2^-126 as 0, which no sum here can tell from what they are
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // score in base 2 of the scaled dot product
 __device__ __forceinline__ float base2(const PagedAttentionArgs& a, float dot) {
     if (a.softcap > 0.0f) return a.softcap * kLog2e * tanhf(dot * a.scale / a.softcap);
@@ -92,7 +96,7 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
         const float t = base2(a, wave_sum(dot));
         if (scores && lane == 0) scores[j] = t;
         const float top = fmaxf(m, t), sub = finite_max(top);
-        const float old = exp2f(m - sub), w = exp2f(t - sub);
+        const float old = exp2_(m - sub), w = exp2_(t - sub);
         m = t != t ? t : top;  // a NaN stays
         l = l * old + w;
 #pragma unroll
@@ -114,7 +118,7 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
     for (int w = 0; w < 4; ++w) {
-        const float f = exp2f(part_m[w] - sub);
+        const float f = exp2_(part_m[w] - sub);
         sum += part_l[w] * f;
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = fmaf(part_o[w][lane + 64 * e], f, o[e]);
@@ -126,32 +130,41 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
     if (p.stats && lane == 0) p.stats[(int64_t)b * a.q_heads + h] = float2{sub, sum};
 }
 
-// weights[b, j] += sum over the heads, in their order: eight heads' scores in
-// flight, their (m, 1 / l) from LDS
+// weights[b, j] += sum over the heads, in their order: 16 heads' scores in flight
+// (32 take a fifth longer), their (m, 1 / l) from LDS
 __global__ void __launch_bounds__(256) add_weights(const Params p, int blocks) {
     extern __shared__ float2 ml[];
+    constexpr int U = 16;
     const PagedAttentionArgs& a = p.a;
     const int b = blockIdx.x / blocks, j = (blockIdx.x - b * blocks) * 256 + threadIdx.x;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0;
     if (j - (int)threadIdx.x >= n) return;
-    const float2* st = p.stats + (int64_t)b * a.q_heads;
-    for (int h = threadIdx.x; h < a.q_heads; h += 256) ml[h] = float2{st[h].x, st[h].y == 0.0f ? 0.0f : 1.0f / st[h].y};
-    __syncthreads();
-    if (j < first || j >= n) return;
+    const bool seen = j >= first && j < n;
     const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + j;
-    const float before = a.weights[b * a.weights_stride + j];
+    float t[U];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) t[u] = seen && h0 + u < a.q_heads ? s[(int64_t)(h0 + u) * p.score_stride] : -__builtin_inff();
+    };
+    load(0);
+    float* const w = a.weights + b * a.weights_stride + j;
+    const float before = seen ? *w : 0.0f;
+    const float2* st = p.stats + (int64_t)b * a.q_heads;
+    for (int h = threadIdx.x; h < a.q_heads; h += 256) {
+        const float2 x = st[h];
+        ml[h] = float2{x.x, x.y == 0.0f ? 0.0f : 1.0f / x.y};
+    }
+    __syncthreads();
     float sum = 0.0f;
-    for (int h0 = 0; h0 < a.q_heads; h0 += 8) {
-        float t[8];
+    for (int h0 = 0; h0 < a.q_heads; h0 += U) {
+        if (h0) load(h0);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) t[u] = h0 + u < a.q_heads ? s[(int64_t)(h0 + u) * p.score_stride] : -__builtin_inff();
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < U; ++u) {
             const float2 x = ml[min(h0 + u, a.q_heads - 1)];
-            sum += x.y == 0.0f ? 0.0f : exp2f(t[u] - x.x) * x.y;
+            sum += x.y == 0.0f ? 0.0f : exp2_(t[u] - x.x) * x.y;
         }
     }
-    a.weights[b * a.weights_stride + j] = before + sum;
+    if (seen) *w = before + sum;
 }
 
 template <int DT>
@@ -262,7 +275,7 @@ __device__ __forceinline__ void store4(uint16_t* row, int d, int D, bool vec, co
 // Running (m, l, o) of disjoint keys merged: both maxima may be -infinity.
 __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, float l2, const f32x4& o2) {
     const float top = fmaxf(m, m2), sub = finite_max(top);
-    const float f = exp2f(m - sub), f2 = exp2f(m2 - sub);
+    const float f = exp2_(m - sub), f2 = exp2_(m2 - sub);
     m = top;
     l = l * f + l2 * f2;
 #pragma unroll
@@ -274,8 +287,8 @@ __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, fl
 // where they would be longer than kLongest, a sequence's chunks of one length.
 // Every wave works it out for itself from the lengths, 64 sequences at a time.
 // (By the bound of the lengths alone, most workgroups of 48 mixed sequences had no
-// keys, and those that had some waited for them to pass: 55 us instead of WORKUS.)
-constexpr int kLongest = 32;  // x 32 keys
+// keys, and those that had some waited for them to pass: 55 us instead of 49.)
+constexpr int kLongest = 64;  // x 32 keys
 
 struct Cut {
     int b, split, total;     // this workgroup's sequence, its split and how many it has
@@ -354,9 +367,23 @@ __device__ __forceinline__ void join(const Params& p, const __amdgpu_buffer_rsrc
             ml[u] = __builtin_amdgcn_raw_buffer_load_b64(r, at + 256 * quads + 8 * h, 0, kCpolSc1);
             x[u] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (h * quads + quad) * 16, 0, kCpolSc1);
         }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, bitcast<float>(ml[u][0]));
+        const float sub = finite_max(top), f = exp2_(M - sub);
+        M = top;
+        L *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) O[i] *= f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (s0 + u < count) merge(M, L, O, bitcast<float>(ml[u][0]), bitcast<float>(ml[u][1]), bitcast<f32x4>(x[u]));
+            if (s0 + u < count) {
+                const float g = exp2_(bitcast<float>(ml[u][0]) - sub);
+                const f32x4 y = bitcast<f32x4>(x[u]);
+                L = fmaf(bitcast<float>(ml[u][1]), g, L);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[i] = fmaf(y[i], g, O[i]);
+            }
     }
 }
 
@@ -539,7 +566,7 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         top = groups_max(top);
         const float sub = finite_max(top);
         if (__any(top != m)) {
-            const float f = exp2f(m - sub);
+            const float f = exp2_(m - sub);
             l *= f;
 #pragma unroll
             for (int c = 0; c < 2 * NC; ++c)
@@ -552,7 +579,7 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                const float x = exp2f(s[r][i] - sub), y = exp2f(s[r][i + 1] - sub);
+                const float x = exp2_(s[r][i] - sub), y = exp2_(s[r][i + 1] - sub);
                 l += x + y;
                 const unsigned h = pack2<DT>(x, y);
                 hi[2 * r + i / 2] = h;
@@ -660,11 +687,17 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         else paged::launch_any<CLOVE_DTYPE_BF16>(p, stream);
     } else {
         p.tiles = hw::cdiv(p.group, 16);
+        const bool whole = c.head_dim % 8 == 0 && c.page_stride % 8 == 0 && a.q_stride % 8 == 0 && a.out_stride % 4 == 0 &&
+                           aligned16(a.q) && aligned16(c.k) && aligned16(c.v) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
         const int per = c.kv_heads * p.tiles;
         const int64_t pairs = (int64_t)a.batch * per;
         // a window need not start at a whole 32 keys
         const int span = std::max(1, a.window > 0 ? (int)std::min<int64_t>(a.max_context, (int64_t)a.window + 31) : a.max_context);
-        p.fill = dev.num_cus * paged::kResident[hw::cdiv(c.head_dim, 32) - 1];
+        // one sequence: its chunks are all alike, and fewer of them are fewer to join
+        // (65536 keys 58.3 -> 55.8 us, 8192 20.5 -> 17.2); of mixed sequences more
+        // fill the CUs better (48.2 against 52.9 us), as do rows at any alignment,
+        // whose loads are slower (51 against 78)
+        p.fill = dev.num_cus * (a.batch == 1 && whole ? (c.head_dim <= 64 ? 2 : 1) : paged::kResident[hw::cdiv(c.head_dim, 32) - 1]);
         // chunks: the CUs' fill a whole number of rounds, and a remainder of each sequence
         const int64_t rounds = std::max<int64_t>(1, hw::cdiv64(pairs * hw::cdiv(span, 32), (int64_t)p.fill * paged::kLongest));
         const int64_t slots = (hw::cdiv64(p.fill * rounds, per) + a.batch) * per;
@@ -680,8 +713,6 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
-        const bool whole = c.head_dim % 8 == 0 && c.page_stride % 8 == 0 && a.q_stride % 8 == 0 && a.out_stride % 4 == 0 &&
-                           aligned16(a.q) && aligned16(c.k) && aligned16(c.v) && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0;
         if (c.dtype == CLOVE_DTYPE_FP16)
             st = whole ? paged::launch_mfma<CLOVE_DTYPE_FP16, false>(p, stream) : paged::launch_mfma<CLOVE_DTYPE_FP16, true>(p, stream);
         else

@@ -6,11 +6,13 @@
 // A workgroup owns a slice of one row's vocabulary, 16 tokens a thread.  How
 // often each token of the slice was produced comes from the row's history,
 // counted in LDS (whole numbers: atomics give the same counts in any order), so
-// nothing of the vocabulary's size is written to memory but the result.  Bound
-// by HBM for large batches: the slice's logits are loaded before the history is
-// read, which every slice of a row reads anew (from L2), so slices are as long
-// as a batch leaves room for: 256 rows of 128000 logits with 8000 tokens of
-// history each take 252 us with slices of 4096 one element at a time.
+// nothing of the vocabulary's size is written to memory but the result.  HBM-bound
+// for large batches: 256 rows of 128000 fp32 logits with masks and 8000 tokens of
+// history each take 63.5 us (4.3 TB/s), 49 (5.3 TB/s, a copy's rate) without them.
+// What is known before the counts -- logits, mask, the first ids -- is loaded
+// ahead of them.  Every slice of a row reads its history anew (from L2), so slices
+// are as long as leaves two workgroups per CU (at 8192 tokens instead of 16384 the
+// above takes 66 us), and results pass the L2 by (68 us with ordinary stores).
 #include <algorithm>
 
 #include "decode.hpp"

@@ -141,4 +141,50 @@ inline void w4a16_swiglu(const half* X, const uint8_t* W_q, const half* W_scale,
     CLOVE_CHECK_STATUS(clove_w4a16_swiglu(X, W_q, W_scale, W_zero, H, T, I, K, stream));
 }
 
+// The decode step around the linear layers (see <clove/gemm_c.h> for each
+// formula; rows are dense unless a stride is given).
+inline void qk_norm_rope(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight, float eps,
+                         const float* rope_cos, const float* rope_sin, int max_position, const int32_t* positions,
+                         void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                         const clove_kv_cache_t* cache, const int32_t* slots, int T, int q_heads, int kv_heads,
+                         int head_dim, int rot_dim, bool interleaved, clove_dtype_t dtype, hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_qk_norm_rope(qkv, qkv_stride, q_weight, k_weight, eps, rope_cos, rope_sin, max_position,
+                                          positions, q_out, q_out_stride, k_out, k_out_stride, cache, slots, T, q_heads,
+                                          kv_heads, head_dim, rot_dim, interleaved ? 1 : 0, (int)dtype, stream));
+}
+
+inline void paged_attention(const void* q, int64_t q_stride, const clove_kv_cache_t& cache, const int32_t* block_table,
+                            int64_t table_stride, const int32_t* context_lens, void* out, int64_t out_stride, int batch,
+                            int q_heads, int max_context, float scale, float softcap = 0.0f, int window = 0,
+                            float* weights = nullptr, int64_t weights_stride = 0, hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_paged_attention(q, q_stride, &cache, block_table, table_stride, context_lens, out,
+                                             out_stride, weights, weights_stride, batch, q_heads, max_context, scale,
+                                             softcap, window, stream));
+}
+
+inline void cache_evict(const clove_kv_cache_t& cache, const int32_t* block_table, int64_t table_stride,
+                        const int32_t* context_lens, const float* weights, int64_t weights_stride,
+                        const int32_t* positions, int64_t positions_stride, float* weights_out,
+                        int64_t weights_out_stride, int32_t* positions_out, int64_t positions_out_stride,
+                        int32_t* lens_out, int batch, int max_context, int budget, int sinks, int recent,
+                        hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_cache_evict(&cache, block_table, table_stride, context_lens, weights, weights_stride,
+                                         positions, positions_stride, weights_out, weights_out_stride, positions_out,
+                                         positions_out_stride, lens_out, batch, max_context, budget, sinks, recent,
+                                         stream));
+}
+
+inline void penalize_logits(const void* logits, int64_t logits_stride, clove_dtype_t dtype, void* out,
+                            int64_t out_stride, clove_dtype_t out_dtype, int batch, int vocab, const int32_t* history,
+                            int64_t history_stride, const int32_t* history_lens, const int32_t* prompt_lens,
+                            const float* repetition, const float* presence, const float* frequency,
+                            const int32_t* bias_ids = nullptr, const float* bias_values = nullptr,
+                            int64_t bias_stride = 0, const int32_t* bias_counts = nullptr,
+                            const uint32_t* allowed = nullptr, int64_t allowed_stride = 0, hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_penalize_logits(logits, logits_stride, (int)dtype, out, out_stride, (int)out_dtype, batch,
+                                             vocab, history, history_stride, history_lens, prompt_lens, repetition,
+                                             presence, frequency, bias_ids, bias_values, bias_stride, bias_counts,
+                                             allowed, allowed_stride, stream));
+}
+
 }  // namespace clove

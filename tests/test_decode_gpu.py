@@ -659,3 +659,156 @@ def test_evict_a_few_tokens(over, kind):
         cg.cache_evict(cg.KVCache(dk, dv), _dev(table), dl, dw, dp, wo, po, lo, B, L, budget, sinks=4, recent=recent)
         for got, exact in zip((dk, dv, wo, po, lo), want):
             assert np.array_equal(_f64(got), exact.astype(np.float64), equal_nan=True)
+
+
+# ---- other alignments, bounds and lengths ---------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 100, 72])
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_attention_rows_at_any_alignment(dtype, D, shift):
+    """q, out and the cache `shift` elements past an aligned address."""
+    import torch
+    cg = _cg()
+    lens, Hq, Hk, P = [70, 300, 0], 8, 2, 16
+    g = rng("attend-align", D, shift)
+    k, v, k64, v64, table = _paged(g, dtype, lens, Hk, D, P, nan_rest=False)
+
+    def moved(t):
+        flat = torch.full((t.numel() + 64,), float("nan"), dtype=t.dtype, device="cuda")
+        out = flat[shift:shift + t.numel()].view(t.shape)
+        out.copy_(t)
+        return out
+
+    k, v = moved(k), moved(v)
+    wide, _ = _rounded(g, dtype, 3, Hq * D + 8)
+    q = wide[:, shift:shift + Hq * D]
+    out = torch.full((3, Hq * D + 16), 5.0, dtype=_dt(dtype), device="cuda")
+    cg.paged_attention(q, cg.KVCache(k, v), _dev(table), _dev(np.array(lens, np.int32)), out[:, shift:shift + Hq * D], 3, Hq, 300)
+    want, _ = ref.attention(_f64(q).reshape(3, Hq, D), k64, v64, table, lens, D ** -0.5)
+    _close(out[:, shift:shift + Hq * D], want.reshape(3, -1), dtype, 3e-5 * float(np.abs(v64).max()))
+    assert bool((out[:, :shift] == 5).all()) and bool((out[:, shift + Hq * D:] == 5).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 36])
+@pytest.mark.parametrize("shift", [1, 2, 4])
+def test_rope_rows_at_any_alignment(D, shift):
+    import torch
+    cg = _cg()
+    T, Hq, Hk = 5, 3, 1
+    g = rng("rope-align", D, shift)
+    width = (Hq + 2 * Hk) * D
+    wide, _ = _rounded(g, "fp16", T, width + 8)
+    x = wide[:, shift:shift + width]
+    w, w64 = _rounded(g, "fp16", D)
+    cos, sin = _tables(9, D)
+    pos = np.array([0, 8, 3, 1, 7], np.int32)
+    out = torch.full((T, Hq * D + 8), 5.0, dtype=torch.float16, device="cuda")
+    q64, _, _ = ref.qk_norm_rope(_f64(x), w64, w64, cos, sin, pos, Hq, Hk, D, D, 1e-6, False)
+    cg.qk_norm_rope(x, w, w, _dev(cos), _dev(sin), _dev(pos), out[:, shift:shift + Hq * D], T, Hq, Hk, D)
+    _close(out[:, shift:shift + Hq * D], q64.reshape(T, -1), "fp16", 2e-5)
+    assert bool((out[:, :shift] == 5).all()) and bool((out[:, shift + Hq * D:] == 5).all())
+
+
+@pytest.mark.parametrize("D", [5, 6, 12, 32])
+def test_evict_rows_of_every_width(D):
+    import torch
+    cg = _cg()
+    g = rng("evict-width", D)
+    lens, budget, P = [300, 120], 100, 16
+    k, v, k64, v64, table = _paged(g, "bf16", lens, 3, D, P, nan_rest=False)
+    w = g.uniform(0, 1, (2, 300)).astype(np.float32)
+    pos = np.stack([g.permutation(300) for _ in range(2)]).astype(np.int32)
+    want = ref.evict(k64, v64, table, lens, w, pos, 300, budget, 4, 10)
+    dw, dp, dl = _dev(w), _dev(pos), _dev(np.array(lens, np.int32))
+    cg.cache_evict(cg.KVCache(k, v), _dev(table), dl, dw, dp, torch.empty_like(dw), torch.empty_like(dp), torch.empty_like(dl), 2, 300,
+                   budget, sinks=4, recent=10)
+    assert np.array_equal(_f64(k), want[0]) and np.array_equal(_f64(v), want[1])
+
+
+def test_nothing_cached_and_empty_batches():
+    import torch
+    cg = _cg()
+    k = torch.empty(0, 2, 16, 64, dtype=torch.float16, device="cuda")
+    cache = cg.KVCache(k, k.clone())
+    q = torch.ones(2, 4, 64, dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 7)
+    lens, table = torch.tensor([3, 0], dtype=torch.int32, device="cuda"), torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    w = torch.ones(2, 16, device="cuda")
+    cg.paged_attention(q, cache, table, lens, out, 2, 4, 16, weights=w)  # pages of a cache that has none
+    assert bool((out == 0).all()) and bool((w == 1).all())
+    out.fill_(7)
+    cg.paged_attention(q, cache, table, lens, out, 2, 4, 0)  # no key may be read
+    assert bool((out == 0).all())
+    cg.paged_attention(q[:0], cache, table[:0], lens[:0], out[:0], 0, 4, 16)
+    cg.penalize_logits(w[:0], w[:0], 0, 16)
+    x = torch.ones(2, 16, dtype=torch.int32, device="cuda")
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+    cg.cache_evict(cache, table, lens, w, x, w.clone(), x.clone(), n, 2, 16, 1)
+    assert n.tolist() == [1, 0]
+
+
+@pytest.mark.parametrize("B", [70, 300])
+def test_attention_many_sequences(B):
+    """More sequences than a wave has lanes, of very different lengths, most of them short."""
+    cg = _cg()
+    g = rng("attend-many", B)
+    lens = [int(x) for x in np.exp(g.uniform(0, np.log(200), B))]
+    lens[0], lens[B // 2], lens[-1], lens[5] = 3000, 5000, 0, 4097
+    Hq, Hk, D, P = 4, 1, 64, 16
+    k, v, k64, v64, table = _paged(g, "fp16", lens, Hk, D, P)
+    q, q64 = _rounded(g, "fp16", B, Hq, D)
+    want, added = ref.attention(q64, k64, v64, table, lens, D ** -0.5)
+    w = _dev(np.zeros((B, 5000), np.float32))
+    out = _attend(cg, q, cg.KVCache(k, v), table, lens, B, Hq, 5000, weights=w)
+    _close(out, want, "fp16", 3e-5 * float(np.abs(v64).max()))
+    assert np.all(np.abs(_f64(w) - added[:, :5000]) <= 3e-5 * added[:, :5000] + 1e-9)
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 1, 128), (4, 1, 64), (3, 1, 250)])
+def test_attention_long_sequence_joined_in_groups(Hq, Hk, D):
+    """Splits enough for joins of joins, and the same lengths behind a larger bound."""
+    import torch
+    cg = _cg()
+    g = rng("attend-groups", Hq, D)
+    lens, P = [40000, 9], 64
+    k, v, k64, v64, table = _paged(g, "bf16", lens, Hk, D, P, nan_rest=False)
+    q, q64 = _rounded(g, "bf16", 2, Hq, D, scale=1.5)
+    want, _ = ref.attention(q64, k64, v64, table, lens, D ** -0.5)
+    out = _attend(cg, q, cg.KVCache(k, v), table, lens, 2, Hq, 40000)
+    _close(out, want, "bf16", 3e-5 * float(np.abs(v64).max()))
+    one = torch.full_like(q[:1], float("nan"))
+    cg.paged_attention(q[:1], cg.KVCache(k, v), _dev(table[:1]), _dev(np.array(lens[:1], np.int32)), one, 1, Hq, 40000)
+    _close(one, want[:1], "bf16", 3e-5 * float(np.abs(v64).max()))
+
+
+def test_attention_graph_follows_the_lengths():
+    """A recorded call cuts the sequences by the lengths of each replay."""
+    import torch
+    cg = _cg()
+    g = rng("attend-graph")
+    B, Hq, Hk, D, P, L = 3, 8, 2, 64, 16, 4000
+    k, v, k64, v64, table = _paged(g, "fp16", [L] * B, Hk, D, P, nan_rest=False)
+    q, q64 = _rounded(g, "fp16", B, Hq, D)
+    cache, dt, lens = cg.KVCache(k, v), _dev(table), torch.zeros(B, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    with cg.workspace_query() as need:
+        cg.paged_attention(q, cache, dt, lens, out, B, Hq, L)
+    ws = torch.zeros(need.bytes, dtype=torch.uint8, device="cuda")
+    cg.workspace_bind(ws)
+    try:
+        side = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            cg.paged_attention(q, cache, dt, lens, out, B, Hq, L)
+        for told in ([4000, 4000, 4000], [1, 0, 3999], [0, 0, 0], [200, 2500, 33], [4000, 1, 1]):
+            lens.copy_(torch.tensor(told, dtype=torch.int32))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            want, _ = ref.attention(q64, k64, v64, table, told, D ** -0.5)
+            _close(out, want, "fp16", 3e-5 * float(np.abs(v64).max()))
+    finally:
+        cg.workspace_bind()
