@@ -8,8 +8,8 @@
 //
 //  * select: one workgroup per sequence.  Each token's rank is one 32-bit key
 //    (the ordered bits of its weight; all ones for a token that stays in any
-//    case, 0 for one that cannot), in LDS up to 32768 tokens; four 8-bit digits
-//    from the top find the keep-th largest key, ties are counted in slot order,
+//    case, 0 for one that cannot), in LDS up to 32768 tokens; three digits from
+//    the top find the keep-th largest key, ties are counted in slot order,
 //    and the lists of moving slots and holes come out in order.  It also writes
 //    the weights, positions and lengths.  A CU takes 8 bytes a token from memory
 //    at about 47 GB/s, and each of its dozen passes waits for the one before, so
@@ -34,7 +34,7 @@ using namespace hw;
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kLdsKeys = 32768;  // 128 KB of the CU's 160
-constexpr int kCopies = 8;       // of the digit histogram, by lane: same-address atomics serialise
+constexpr int kBins = 2048;      // of a digit of 11 bits: the first holds sign, exponent and two bits of a weight
 constexpr unsigned kStays = 0xffffffffu, kGoes = 0u;
 
 // Ordered bits of a weight: a larger weight has the larger key; -0 as 0; NaN
@@ -121,6 +121,15 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
     const int32_t* positions = a.positions + b * a.positions_stride;
     float* weights_out = a.weights_out + b * a.weights_out_stride;
     int32_t* positions_out = a.positions_out + b * a.positions_out_stride;
+    if (p.fused && moving) {
+        const int32_t* table = a.block_table + b * a.table_stride;
+        const int first = tid / p.team, step = kThreads / p.team, at = tid & (p.team - 1);
+        if (p.whole) move_rows<8, true>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 8) move_rows<8>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 4) move_rows<4>(p, table, src, dst, moving, first, step, at);
+        else if (p.vec == 2) move_rows<2>(p, table, src, dst, moving, first, step, at);
+        else move_rows<1>(p, table, src, dst, moving, first, step, at);
+    }
     // Moved slots are read at or past `keep` and written below it.  Where an output
     // is its input, they are moved before the rest of its row is cleared.
     if (!apart && weights_out != weights)
@@ -128,7 +137,8 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
     if (!apart && positions_out != positions)
         for (int i = tid; i < keep; i += kThreads) positions_out[i] = positions[i];
     if (!apart) __syncthreads();
-    for (int j0 = tid; j0 < moving; j0 += 4 * kThreads) {
+    // (the last threads first: the first ones move rows)
+    for (int j0 = kThreads - 1 - tid; j0 < moving; j0 += 4 * kThreads) {
         int from[4], to[4];
         float w[4];
         int32_t pos[4];
@@ -150,8 +160,8 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
             positions_out[to[u]] = pos[u];
         }
     }
-    if (!apart && p.fused) {
-        __syncthreads();
+    if (p.fused) {  // (else the second kernel clears it)
+        if (!apart) __syncthreads();
         for (int i = keep + tid; i < a.max_context; i += kThreads) {
             weights_out[i] = 0.0f;
             positions_out[i] = -1;
@@ -160,15 +170,6 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
     if (tid == 0) {
         a.lens_out[b] = keep;
         if (p.moves && !p.fused) p.counts[b] = moving;
-    }
-    if (p.fused && moving) {
-        const int32_t* table = a.block_table + b * a.table_stride;
-        const int first = tid / p.team, step = kThreads / p.team, at = tid & (p.team - 1);
-        if (p.whole) move_rows<8, true>(p, table, src, dst, moving, first, step, at);
-        else if (p.vec == 8) move_rows<8>(p, table, src, dst, moving, first, step, at);
-        else if (p.vec == 4) move_rows<4>(p, table, src, dst, moving, first, step, at);
-        else if (p.vec == 2) move_rows<2>(p, table, src, dst, moving, first, step, at);
-        else move_rows<1>(p, table, src, dst, moving, first, step, at);
     }
 }
 
@@ -179,7 +180,7 @@ __device__ __forceinline__ void finish(const Params& p, int b, int keep, int mov
 constexpr int kFew = 4;
 
 struct Lds {
-    unsigned hist[3][kCopies][256];
+    unsigned hist[3][kBins];
     int part[kWaves][2];
 };
 
@@ -198,6 +199,7 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t v) {
 }
 
 constexpr int kHeld = 16;  // tokens of a thread that stay in registers from the first load on
+constexpr int kRest = 8;   // tokens of a thread loaded at once after them
 
 template <bool IN_LDS>
 __global__ void __launch_bounds__(kThreads) select(const Params p) {
@@ -220,127 +222,117 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
         held_pos[u] = i < a.max_context ? positions[i] : 0;
         held_w[u] = i < a.max_context ? weights[i] : 0.0f;
     }
-    // f(slot, position, weight) for every slot of the row that this thread has
-    auto each = [&](auto f) {
+    // f(first of the workgroup's slots, slot, position, weight) for each of the
+    // first `most` slots that this thread has
+    auto each = [&](int most, auto f) {
 #pragma unroll
         for (int u = 0; u < kHeld; ++u)
-            if (tid + u * kThreads < a.max_context) f(tid + u * kThreads, held_pos[u], held_w[u]);
-        for (int i0 = tid + kHeld * kThreads; i0 < a.max_context; i0 += kHeld * kThreads) {
-            int32_t v[kHeld];
-            float w[kHeld];
+            if (u * kThreads < most && tid + u * kThreads < most) f(u * kThreads, tid + u * kThreads, held_pos[u], held_w[u]);
+        for (int base = kHeld * kThreads; base < most; base += kRest * kThreads) {
+            int32_t v[kRest];
+            float w[kRest];
 #pragma unroll
-            for (int u = 0; u < kHeld; ++u) {
-                const int i = i0 + u * kThreads;
-                v[u] = i < a.max_context ? positions[i] : 0;
-                w[u] = i < a.max_context ? weights[i] : 0.0f;
+            for (int u = 0; u < kRest; ++u) {
+                const int i = base + tid + u * kThreads;
+                v[u] = i < most ? positions[i] : 0;
+                w[u] = i < most ? weights[i] : 0.0f;
             }
 #pragma unroll
-            for (int u = 0; u < kHeld; ++u)
-                if (i0 + u * kThreads < a.max_context) f(i0 + u * kThreads, v[u], w[u]);
+            for (int u = 0; u < kRest; ++u)
+                if (base + u * kThreads < most && base + tid + u * kThreads < most) f(base + u * kThreads, base + tid + u * kThreads, v[u], w[u]);
         }
     };
     const bool apart = weights_out != weights && positions_out != positions;
-    // outputs apart from their inputs, before the moved tokens are written over
-    // them; slots past `keep` are cleared by the second kernel where there is one
-    const int written = p.fused ? a.max_context : keep;
-    auto pass_on = [&](int i, int32_t pos, float w) {
-        if (!apart || i >= written) return;
-        weights_out[i] = i < keep ? w : 0.0f;
-        positions_out[i] = i < keep ? pos : -1;
+    // outputs apart from their inputs, before the moved tokens are written over them
+    auto pass_on = [&](int base, int i, int32_t pos, float w) {
+        if (!apart || base >= keep || i >= keep) return;
+        weights_out[i] = w;
+        positions_out[i] = pos;
     };
     int* const src = p.lists + (int64_t)b * 2 * p.moves;
     int* const dst = src + p.moves;
     int moving = 0;
     if (n <= keep || keep == 0) {  // nothing to choose
-        if (apart) each(pass_on);
+        if (apart) each(keep, pass_on);
     } else {
         unsigned* const keys = IN_LDS ? lds_keys : p.keys + b * p.key_stride;
         const int padded = cdiv(n, 4) * 4;  // keys are read by fours; past n they are kGoes
         int newest = INT32_MIN;
-        each([&](int i, int32_t pos, float) { newest = i < n ? max(newest, pos) : newest; });
+        each(n, [&](int, int, int32_t pos, float) { newest = max(newest, pos); });
         newest = wave_max(newest);
         if (lane == 0) s.part[wave][0] = newest;
-        reinterpret_cast<u32x2*>(&s.hist[0][0][0])[tid] = u32x2{0u, 0u};
-        static_assert(kCopies * 256 == 2 * kThreads, "one access a thread");
+        reinterpret_cast<u32x2*>(s.hist[0])[tid] = u32x2{0u, 0u};
+        static_assert(kBins == 2 * kThreads, "one access a thread");
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) newest = max(newest, s.part[w][0]);
         const int64_t from = (int64_t)newest - a.recent;
         auto safe_at = [&](int32_t pos) { return pos < a.sinks || (int64_t)pos > from; };
         int safes = 0;
-        each([&](int i, int32_t pos, float w) {
-            if (i < n) {
-                const bool safe = safe_at(pos);
-                const unsigned k = safe ? kStays : order_key(w);
-                safes += safe ? 1 : 0;
-                keys[i] = k;
-                atomicAdd(&s.hist[0][lane & (kCopies - 1)][k >> 24], 1u);
-            } else if (i < padded) {
-                keys[i] = kGoes;
-            }
-            pass_on(i, pos, w);
+        each(n, [&](int base, int i, int32_t pos, float w) {
+            const bool safe = safe_at(pos);
+            const unsigned k = safe ? kStays : order_key(w);
+            safes += safe ? 1 : 0;
+            keys[i] = k;
+            atomicAdd(&s.hist[0][k >> 21], 1u);
+            pass_on(base, i, pos, w);
         });
-        if (tid < padded - n && a.max_context < padded) keys[n + tid] = kGoes;  // a row shorter than its keys
+        if (tid < padded - n) keys[n + tid] = kGoes;
         safes = wave_sum(safes);
         if (lane == 0) s.part[wave][1] = safes;
-        reinterpret_cast<u32x2*>(&s.hist[1][0][0])[tid] = u32x2{0u, 0u};
+        reinterpret_cast<u32x2*>(s.hist[1])[tid] = u32x2{0u, 0u};
         __syncthreads();
         safes = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) safes += s.part[w][1];
         if (safes >= keep) {  // the protected compete among themselves: keys and first digits anew
-            reinterpret_cast<u32x2*>(&s.hist[0][0][0])[tid] = u32x2{0u, 0u};
+            reinterpret_cast<u32x2*>(s.hist[0])[tid] = u32x2{0u, 0u};
             __syncthreads();
-            each([&](int i, int32_t pos, float w) {
-                if (i >= n) return;
+            each(n, [&](int, int i, int32_t pos, float w) {
                 const unsigned k = safe_at(pos) ? order_key(w) : kGoes;
                 keys[i] = k;
-                atomicAdd(&s.hist[0][lane & (kCopies - 1)][k >> 24], 1u);
+                atomicAdd(&s.hist[0][k >> 21], 1u);
             });
             __syncthreads();
         }
-        // the keep-th largest key, digit by digit: `prefix` its bits so far, `need`
-        // how many of the `equal` keys with that prefix are kept.  Every wave reads
-        // the counts for itself, so a digit costs one barrier; of three histograms
-        // one is read, one counted and one cleared.
+        // the keep-th largest key, by digits of 11, 11 and 10 bits: `prefix` its bits so
+        // far, `need` how many of the `equal` keys with that prefix are kept.  Every
+        // wave reads the counts for itself, so a digit costs one barrier.
         unsigned prefix = 0;
         int need = keep, equal = 0;
 #pragma unroll
-        for (int digit = 0; digit < 4; ++digit) {
-            const int shift = 24 - 8 * digit;
+        for (int digit = 0; digit < 3; ++digit) {
+            constexpr int kShift[3] = {21, 10, 0};
+            const int shift = kShift[digit];
+            unsigned* const hist = s.hist[digit];
             if (digit) {
-                const unsigned mask = 0xffffffffu << (shift + 8);
-                if (digit < 3) reinterpret_cast<u32x2*>(&s.hist[(digit + 1) % 3][0][0])[tid] = u32x2{0u, 0u};
+                const int above_shift = kShift[digit - 1];
+                if (digit < 2) reinterpret_cast<u32x2*>(s.hist[digit + 1])[tid] = u32x2{0u, 0u};
                 for (int i = 4 * tid; i < padded; i += 4 * kThreads) {
                     const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if ((k[e] & mask) == prefix) atomicAdd(&s.hist[digit % 3][lane & (kCopies - 1)][(k[e] >> shift) & 255u], 1u);
+                        if (k[e] >> above_shift == prefix >> above_shift) atomicAdd(&hist[(k[e] >> shift) & (digit == 2 ? 1023u : 2047u)], 1u);
                 }
                 __syncthreads();
             }
-            // lane l: digits 4 l .. 4 l + 3 and how many keys have a higher one
+            // lane l: bins 32 l .. 32 l + 31 summed (read in an order of their own, which
+            // keeps the lanes on different banks) and how many keys lie above them
             u32x4 c = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int r = 0; r < kCopies; ++r) c += *reinterpret_cast<const u32x4*>(&s.hist[digit % 3][r][4 * lane]);
+            for (int r = 0; r < 8; ++r) c += *reinterpret_cast<const u32x4*>(hist + 32 * lane + 4 * ((r + lane) & 7));
             const int sum = (int)(c[0] + c[1] + c[2] + c[3]), upto = wave_scan(sum);
-            int above = __builtin_amdgcn_readlane(upto, 63) - upto, mine = -1, rest = 0, same = 0;
-#pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                if (above < need && above + (int)c[j] >= need) {
-                    mine = 4 * lane + j;
-                    rest = need - above;
-                    same = (int)c[j];
-                }
-                above += (int)c[j];
-            }
-            const int who = __ffsll((long long)__ballot(mine >= 0)) - 1;  // one lane has it
-            prefix |= (unsigned)__builtin_amdgcn_readlane(mine, who) << shift;
-            need = __builtin_amdgcn_readlane(rest, who);
-            equal = __builtin_amdgcn_readlane(same, who);
+            const int above = __builtin_amdgcn_readlane(upto, 63) - upto;
+            const int who = __ffsll((long long)__ballot(above < need && above + sum >= need)) - 1;  // one lane has it
+            // then its 32 bins, one a lane
+            const int bin = lane < 32 ? (int)hist[32 * who + lane] : 0, to_bin = wave_scan(bin);
+            const int higher = __builtin_amdgcn_readlane(above, who) + __builtin_amdgcn_readlane(sum, who) - to_bin;
+            const int at = __ffsll((long long)__ballot(higher < need && higher + bin >= need)) - 1;
+            prefix |= (unsigned)(32 * who + at) << shift;
+            need -= __builtin_amdgcn_readlane(higher, at);
+            equal = __builtin_amdgcn_readlane(bin, at);
         }
-        // in slot order from here: wave w has slots [w seg, (w + 1) seg), 256 at a
-        // time, four adjacent ones a lane
+        // in slot order from here: wave w has slots [w seg, (w + 1) seg), 256 at a time
         const int seg = cdiv(cdiv(n, kWaves), 256) * 256;
         const int i0 = min(wave * seg, padded), i1 = min(i0 + seg, padded);
         if (need < equal) {  // of the equal keys the lowest slots stay, the others drop below them
@@ -373,22 +365,42 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
             }
             __syncthreads();
         }
-        // the lists of slots that move and of holes: counted, then written
-        int n_src = 0, n_dst = 0;
-        for (int i = i0 + 4 * lane; i < i1; i += 256) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(keys + i);
+        // The lists of slots that move and of holes.  A wave takes its slots 64 at a
+        // time; lane c keeps the bits of the c-th 64, so that the second pass over
+        // them, with the lists' beginnings known, needs the keys again only where
+        // it has more than 64 of them.
+        const int groups = cdiv(i1 - i0, 4096);
+        uint64_t outs = 0, holes = 0;
+        auto bits = [&](int g) {
+            const int first = i0 + 4096 * g, chunks = min(64, cdiv(i1 - first, 64));
+            uint64_t kept = 0;
+            for (int c0 = 0; c0 < chunks; c0 += 4) {
+                unsigned k[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                n_src += k[e] >= prefix && i + e >= keep ? 1 : 0;
-                n_dst += k[e] < prefix && i + e < keep ? 1 : 0;
+                for (int u = 0; u < 4; ++u) k[u] = keys[min(first + 64 * (c0 + u) + lane, padded - 1)];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint64_t m = __ballot(k[u] >= prefix);
+                    kept = lane == c0 + u ? m : kept;
+                }
             }
+            const int base = first + 64 * lane;
+            auto up_to = [&](int end) { return end <= base ? 0ull : end >= base + 64 ? ~0ull : (1ull << (end - base)) - 1ull; };
+            const uint64_t low = up_to(keep), mine = lane < chunks ? up_to(min(i1, n)) : 0ull;
+            outs = kept & mine & ~low;
+            holes = ~kept & mine & low;
+        };
+        int n_src = 0, n_dst = 0;
+        for (int g = 0; g < groups; ++g) {
+            bits(g);
+            n_src += __popcll(outs);
+            n_dst += __popcll(holes);
         }
-        n_src = wave_sum(n_src);
-        n_dst = wave_sum(n_dst);
+        const int all_src = wave_sum(n_src), all_dst = wave_sum(n_dst);
         __syncthreads();  // (s.part may still be read as the counts of ties)
         if (lane == 0) {
-            s.part[wave][0] = n_src;
-            s.part[wave][1] = n_dst;
+            s.part[wave][0] = all_src;
+            s.part[wave][1] = all_dst;
         }
         __syncthreads();
         int at_src = 0, at_dst = 0;
@@ -398,24 +410,36 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
             at_dst += w < wave ? s.part[w][1] : 0;
             moving += s.part[w][0];
         }
-        for (int i = i0; i < i1; i += 256) {
-            const int at = i + 4 * lane;
-            const u32x4 k = at < i1 ? *reinterpret_cast<const u32x4*>(keys + at) : u32x4{kStays, kStays, kStays, kStays};
-            unsigned out = 0, hole = 0;  // this lane's four
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                out |= (k[e] >= prefix && at + e >= keep && at < i1 ? 1u : 0u) << e;
-                hole |= (k[e] < prefix && at + e < keep ? 1u : 0u) << e;
+        for (int g = 0; g < groups; ++g) {
+            if (groups > 1) bits(g);
+            const int first = i0 + 4096 * g, chunks = min(64, cdiv(i1 - first, 64));
+            const int own = __popcll(outs) | __popcll(holes) << 16, upto = wave_scan(own);  // at most 4096 of each
+            if (chunks > 16) {
+                // many 64s: each lane its own, bit by bit, as few of them are in a list
+                // (24576 tokens to 4096: 4 us, 6 the other way)
+                auto write = [&](uint64_t mask, int* list) {
+                    for (; mask; mask &= mask - 1ull) *list++ = first + 64 * lane + __ffsll((long long)mask) - 1;
+                };
+                write(outs, src + at_src + ((upto - own) & 0xffff));
+                write(holes, dst + at_dst + ((unsigned)(upto - own) >> 16));
+            } else {
+                // few: one after the other, a lane a slot (8192 to 4096: 2.8 us, 4.7 the other way)
+                for (int c = 0; c < chunks; ++c) {
+                    const unsigned before = (unsigned)(__builtin_amdgcn_readlane(upto, c) - __builtin_amdgcn_readlane(own, c));
+                    auto write = [&](uint64_t mask, int* list) {
+                        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)mask, c);
+                        const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(mask >> 32), c);
+                        if (!(lo | hi)) return;
+                        if (((lane < 32 ? lo : hi) >> (lane & 31)) & 1u)
+                            list[__builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u))] = first + 64 * c + lane;
+                    };
+                    write(outs, src + at_src + (int)(before & 0xffffu));
+                    write(holes, dst + at_dst + (int)(before >> 16));
+                }
             }
-            const int own = __popc(out) | __popc(hole) << 16, upto = wave_scan(own), all = __builtin_amdgcn_readlane(upto, 63);
-            int my_src = at_src + ((upto - own) & 0xffff), my_dst = at_dst + ((upto - own) >> 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if ((out >> e) & 1u) src[my_src++] = at + e;
-                if ((hole >> e) & 1u) dst[my_dst++] = at + e;
-            }
+            const int all = __builtin_amdgcn_readlane(upto, 63);
             at_src += all & 0xffff;
-            at_dst += all >> 16;
+            at_dst += (int)((unsigned)all >> 16);
         }
     }
     __syncthreads();
@@ -425,7 +449,7 @@ __global__ void __launch_bounds__(kThreads) select(const Params p) {
 // Rows of at most budget + kFew tokens.
 __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
     __shared__ uint64_t least_of[2][kWaves];
-    __shared__ int newest_of[kWaves];
+    __shared__ int newest_of[kWaves], lists[2][kFew];
     const EvictArgs& a = p.a;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* weights = a.weights + b * a.weights_stride;
@@ -435,7 +459,6 @@ __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
     const int n = min(max(a.context_lens[b], 0), a.max_context);
     const int keep = min(n, a.budget);
     const bool apart = weights_out != weights && positions_out != positions;
-    const int written = p.fused ? a.max_context : keep;
     // rows hold max_context tokens whatever the length is, which is not awaited
     constexpr int kBatch = 8;
     int32_t pos[kBatch];
@@ -456,14 +479,12 @@ __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
         for (int u = 0; u < kBatch; ++u) {
             const int i = i0 + u * kThreads;
             if (i < n) newest = max(newest, pos[u]);
-            if (apart && i < written) {
-                weights_out[i] = i < keep ? w[u] : 0.0f;
-                positions_out[i] = i < keep ? pos[u] : -1;
+            if (apart && i < keep) {
+                weights_out[i] = w[u];
+                positions_out[i] = pos[u];
             }
         }
     }
-    int* const src = p.lists + (int64_t)b * 2 * p.moves;
-    int* const dst = src + p.moves;
     int moving = 0;
     if (n > keep && keep > 0) {
         newest = wave_max(newest);
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
 #pragma unroll
         for (int d = 0; d < kFew; ++d) {
             if (gone[d] < keep) {
-                if (tid == 0) dst[holes] = gone[d];
+                if (tid == 0) lists[1][holes] = gone[d];
                 ++holes;
             }
             const int i = keep + d;
@@ -520,13 +541,18 @@ __global__ void __launch_bounds__(kThreads) select_few(const Params p) {
 #pragma unroll
             for (int e = 0; e < kFew; ++e) moves = moves && gone[e] != i;
             if (moves) {
-                if (tid == 0) src[moving] = i;
+                if (tid == 0) lists[0][moving] = i;
                 ++moving;
             }
         }
     }
     __syncthreads();
-    finish(p, b, keep, moving, src, dst, apart);
+    if (!p.fused && tid < moving) {  // the second kernel's
+        int* const src = p.lists + (int64_t)b * 2 * p.moves;
+        src[tid] = lists[0][tid];
+        src[p.moves + tid] = lists[1][tid];
+    }
+    finish(p, b, keep, moving, lists[0], lists[1], apart);
 }
 
 template <int V, bool WHOLE>

@@ -812,3 +812,25 @@ def test_attention_graph_follows_the_lengths():
             _close(out, want, "fp16", 3e-5 * float(np.abs(v64).max()))
     finally:
         cg.workspace_bind()
+
+
+@pytest.mark.parametrize("over", [1, 4])
+def test_evict_a_few_wide_tokens(over):
+    """Rows of so many heads that the few moved ones take a second kernel."""
+    import torch
+    cg = _cg()
+    g = rng("evict-wide", over)
+    budget, P, Hk, D = 20, 8, 16, 1024
+    L = budget + over
+    lens = [L, 7]
+    k, v, k64, v64, table = _paged(g, "fp16", lens, Hk, D, P, nan_rest=False)
+    w = g.uniform(1, 2, (2, L)).astype(np.float32)
+    w[0, :over] = 0.0
+    pos = np.tile(np.arange(L, dtype=np.int32), (2, 1))
+    want = ref.evict(k64, v64, table, lens, w, pos, L, budget, 0, 5)
+    for in_place in (False, True):
+        dk, dv, dw, dp, dl = k.clone(), v.clone(), _dev(w), _dev(pos), _dev(np.array(lens, np.int32))
+        wo, po, lo = (dw, dp, dl) if in_place else (torch.full_like(dw, 9), torch.full_like(dp, 9), torch.full_like(dl, 9))
+        cg.cache_evict(cg.KVCache(dk, dv), _dev(table), dl, dw, dp, wo, po, lo, 2, L, budget, recent=5)
+        for got, exact in zip((dk, dv, wo, po, lo), want):
+            assert np.array_equal(_f64(got), exact.astype(np.float64))
