@@ -720,7 +720,7 @@ clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clov
         (int64_t)max_context > table_stride * a.cache.page_size)
         return CLOVE_ERR_INVALID_ARG;
     if (max_context > CLOVE_MAX_CONTEXT || (int64_t)batch * q_heads > 0x1000000 ||
-        (weights && batch * hw::cdiv64(max_context, 256) > 0x7fffffff))
+        (weights && batch * hw::cdiv64(max_context, 64) > 0x7fffffff))
         return CLOVE_ERR_INVALID_DIM;
     if (!aligned2(q) || !aligned2(out) || !aligned4(block_table) || !aligned4(context_lens) || !aligned4(weights))
         return CLOVE_ERR_INVALID_ARG;

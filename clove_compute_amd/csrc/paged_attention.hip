@@ -130,41 +130,41 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
     if (p.stats && lane == 0) p.stats[(int64_t)b * a.q_heads + h] = float2{sub, sum};
 }
 
-// weights[b, j] += sum over the heads, in their order: 16 heads' scores in flight
-// (32 take a fifth longer), their (m, 1 / l) from LDS
-__global__ void __launch_bounds__(256) add_weights(const Params p, int blocks) {
-    extern __shared__ float2 ml[];
+// weights[b, j] += sum over the heads: 64 keys a workgroup, each by four threads
+// that sum a quarter of the heads in their order, 16 heads' scores in flight; the
+// quarters are added in theirs.
+constexpr int kAddKeys = 64;
+__global__ void __launch_bounds__(4 * kAddKeys) add_weights(const Params p, int blocks) {
     constexpr int U = 16;
+    __shared__ float part[4][kAddKeys];
     const PagedAttentionArgs& a = p.a;
-    const int b = blockIdx.x / blocks, j = (blockIdx.x - b * blocks) * 256 + threadIdx.x;
+    const int b = blockIdx.x / blocks, key = threadIdx.x % kAddKeys, quarter = threadIdx.x / kAddKeys;
+    const int j = (blockIdx.x - b * blocks) * kAddKeys + key;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0;
-    if (j - (int)threadIdx.x >= n) return;
+    if (j - key >= n || j - key + kAddKeys <= first) return;
     const bool seen = j >= first && j < n;
+    const int own = cdiv(a.q_heads, 4), h1 = min(a.q_heads, (quarter + 1) * own);
     const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + j;
-    float t[U];
-    auto load = [&](int h0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) t[u] = seen && h0 + u < a.q_heads ? s[(int64_t)(h0 + u) * p.score_stride] : -__builtin_inff();
-    };
-    load(0);
-    float* const w = a.weights + b * a.weights_stride + j;
-    const float before = seen ? *w : 0.0f;
     const float2* st = p.stats + (int64_t)b * a.q_heads;
-    for (int h = threadIdx.x; h < a.q_heads; h += 256) {
-        const float2 x = st[h];
-        ml[h] = float2{x.x, x.y == 0.0f ? 0.0f : 1.0f / x.y};
-    }
-    __syncthreads();
+    float* const w = a.weights + b * a.weights_stride + j;
+    const float before = seen && quarter == 0 ? *w : 0.0f;
     float sum = 0.0f;
-    for (int h0 = 0; h0 < a.q_heads; h0 += U) {
-        if (h0) load(h0);
+    for (int h0 = quarter * own; h0 < h1; h0 += U) {
+        float t[U];
+        float2 ml[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float2 x = ml[min(h0 + u, a.q_heads - 1)];
-            sum += x.y == 0.0f ? 0.0f : exp2_(t[u] - x.x) * x.y;
+            const int h = min(h0 + u, h1 - 1);
+            t[u] = seen ? s[(int64_t)h * p.score_stride] : -__builtin_inff();
+            ml[u] = st[h];
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (h0 + u < h1 && ml[u].y != 0.0f) sum += exp2_(t[u] - ml[u].x) / ml[u].y;
     }
-    if (seen) *w = before + sum;
+    part[quarter][key] = sum;
+    __syncthreads();
+    if (seen && quarter == 0) *w = before + (((part[0][key] + part[1][key]) + part[2][key]) + part[3][key]);
 }
 
 template <int DT>
@@ -720,8 +720,8 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         if (st != CLOVE_OK) return st;
     }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;
-    const int blocks = hw::cdiv(a.max_context, 256);
-    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(256), a.q_heads * sizeof(float2), stream, p, blocks);
+    const int blocks = hw::cdiv(a.max_context, paged::kAddKeys);
+    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(4 * paged::kAddKeys), 0, stream, p, blocks);
     return check_launch();
 }
 
