@@ -423,8 +423,8 @@ __device__ __forceinline__ void join_all(const Params& p, const __amdgpu_buffer_
     }
 }
 
-template <int DT, int NC, bool TAIL>
-__global__ void __launch_bounds__(64 * kW) attend(const Params p) {
+template <int DT, int NC, bool TAIL, int W>
+__global__ void __launch_bounds__(64 * W) attend(const Params p) {
     extern __shared__ __align__(16) char lds[];
     __shared__ int last;
     const PagedAttentionArgs& a = p.a;
@@ -440,14 +440,15 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
     }
     const int seq = unit / cache.kv_heads, kh = unit - seq * cache.kv_heads, per = cache.kv_heads * p.tiles;
     Cut c{seq, 0, 1, seq, 0};
-    if (p.cuts) c = cut(p, seq, per);
+    if constexpr (W == kW)
+        if (p.cuts) c = cut(p, seq, per);
     const int b = c.b, split = c.split, total = c.total;
     if (b < 0 || b >= a.batch) return;
     const int pair = (b * cache.kv_heads + kh) * p.tiles + tile, slab0 = (c.first * cache.kv_heads + kh) * p.tiles + tile;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
     const int D = cache.head_dim, G = min(16, p.group - 16 * tile), h0 = kh * p.group + 16 * tile;
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0, base = first & ~31;
-    const int begin = base + split * c.chunk * 32, end = p.cuts ? min(n, begin + c.chunk * 32) : n;
+    const int begin = base + split * c.chunk * 32, end = W == kW && p.cuts ? min(n, begin + c.chunk * 32) : n;
     const bool vec = !TAIL;
 
     u32x4 q[NC];
@@ -512,8 +513,8 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         load(k, cache.k);
         load(v, cache.v);
     }
-    look_up(j + 32 * kW);
-    for (; j < end; j += 32 * kW) {
+    look_up(j + 32 * W);
+    for (; j < end; j += 32 * W) {
         seen = seen_next;
         f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
         if (seen) {
@@ -524,9 +525,9 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
                 s[1] = Mfma<DT>::mul(k[1][c], q[c], s[1]);
             }
         }
-        resolve(j + 32 * kW);
+        resolve(j + 32 * W);
         if (seen_next) load(k, cache.k);
-        look_up(j + 64 * kW);
+        look_up(j + 64 * W);
         if (seen) {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
@@ -613,19 +614,20 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
         if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L};
     };
     const __amdgpu_buffer_rsrc_t slabs = slabs_of(p);
-    for (int i = threadIdx.x; i < items; i += 64 * kW) {
+    for (int i = threadIdx.x; i < items; i += 64 * W) {
         const int h = i / quads, quad = i - h * quads;
         float M = -__builtin_inff(), L = 0.0f;
         f32x4 O{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kW; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float* x = reinterpret_cast<const float*>(lds + w * wave_lds<NC>());
             const float2 ml = *reinterpret_cast<const float2*>(x + 16 * o_stride<NC>() + 2 * h);
             merge(M, L, O, ml.x, ml.y, *reinterpret_cast<const f32x4*>(x + h * o_stride<NC>() + 4 * quad));
         }
-        if (total == 1) finish(h, quad, M, L, O);
+        if (W != kW || total == 1) finish(h, quad, M, L, O);
         else publish(p, slabs, slab0 + split * per, h, quad, quads, M, L, O);
     }
+    if constexpr (W != kW) return;
     if (total == 1) return;
     int from = slab0, step = per, count = total;
     if (total > p.fan) {
@@ -647,18 +649,33 @@ __global__ void __launch_bounds__(64 * kW) attend(const Params p) {
 // alignment hold one fewer at 3 and 6)
 constexpr int kResident[8] = {5, 4, 3, 2, 2, 2, 1, 1};
 
-template <int DT, bool TAIL>
-clove_status_t launch_mfma(const Params& p, hipStream_t stream) {
-    typedef void (*Kernel)(const Params);
-    static const Kernel kernels[8] = {attend<DT, 1, TAIL>, attend<DT, 2, TAIL>, attend<DT, 3, TAIL>, attend<DT, 4, TAIL>,
-                                      attend<DT, 5, TAIL>, attend<DT, 6, TAIL>, attend<DT, 7, TAIL>, attend<DT, 8, TAIL>};
-    static const int bytes[8] = {wave_lds<1>(), wave_lds<2>(), wave_lds<3>(), wave_lds<4>(),
-                                 wave_lds<5>(), wave_lds<6>(), wave_lds<7>(), wave_lds<8>()};
-    const int nc = cdiv(p.a.cache.head_dim, 32) - 1;
+typedef void (*Kernel)(const Params);
+struct Form {
+    Kernel kernel;
+    int lds;
+};
+template <int DT, bool TAIL, int W>
+Form pick(int nc) {
+    switch (nc) {
+        case 1: return Form{attend<DT, 1, TAIL, W>, W * wave_lds<1>()};
+        case 2: return Form{attend<DT, 2, TAIL, W>, W * wave_lds<2>()};
+        case 3: return Form{attend<DT, 3, TAIL, W>, W * wave_lds<3>()};
+        case 4: return Form{attend<DT, 4, TAIL, W>, W * wave_lds<4>()};
+        case 5: return Form{attend<DT, 5, TAIL, W>, W * wave_lds<5>()};
+        case 6: return Form{attend<DT, 6, TAIL, W>, W * wave_lds<6>()};
+        case 7: return Form{attend<DT, 7, TAIL, W>, W * wave_lds<7>()};
+        default: return Form{attend<DT, 8, TAIL, W>, W * wave_lds<8>()};
+    }
+}
+
+template <int DT>
+clove_status_t launch_mfma(const Params& p, bool whole, bool alone, hipStream_t stream) {
+    const int nc = cdiv(p.a.cache.head_dim, 32);
+    const Form f = whole ? (alone ? pick<DT, false, 1>(nc) : pick<DT, false, kW>(nc)) : (alone ? pick<DT, true, 1>(nc) : pick<DT, true, kW>(nc));
     const int units = p.slots / p.tiles, grid = p.tiles > 1 ? cdiv(units, 8) * 8 * p.tiles : units;
-    const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(kernels[nc]), kW * bytes[nc]);
+    const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(f.kernel), f.lds);
     if (st != CLOVE_OK) return st;
-    CLOVE_LAUNCH(kernels[nc], dim3((unsigned)grid), dim3(64 * kW), (size_t)kW * bytes[nc], stream, p);
+    CLOVE_LAUNCH(f.kernel, dim3((unsigned)grid), dim3(alone ? 64 : 64 * kW), (size_t)f.lds, stream, p);
     return CLOVE_OK;
 }
 
@@ -698,12 +715,19 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         // fill the CUs better (48.2 against 52.9 us), as do rows at any alignment,
         // whose loads are slower (51 against 78)
         p.fill = dev.num_cus * (a.batch == 1 && whole ? (c.head_dim <= 64 ? 2 : 1) : paged::kResident[hw::cdiv(c.head_dim, 32) - 1]);
+        // One wave to a workgroup: nothing to merge where the keys are one wave's anyway
+        // and its heads' outputs few (one sequence of 20 keys, head_dim 64, 4.7 -> 4.3
+        // us; with 16 heads of 256 13.1 -> 15.4), and where there are more sequences of
+        // up to 512 keys than the CUs hold workgroups of four (200 x 8 heads of 64 with
+        // 20, 90, 250, 500 keys 9.1, 12.8, 30.4, 49.6 -> 6.2, 10.8, 21.8, 44.0 us; mixed
+        // ones of up to 1000 36.9 -> 48.7, one of them outlasting the rest)
+        const bool alone = (span <= 32 && std::min(p.group, 16) * c.head_dim <= 512) || (span <= 512 && pairs > p.fill);
         // chunks: the CUs' fill a whole number of rounds, and a remainder of each sequence
         const int64_t rounds = std::max<int64_t>(1, hw::cdiv64(pairs * hw::cdiv(span, 32), (int64_t)p.fill * paged::kLongest));
         const int64_t slots = (hw::cdiv64(p.fill * rounds, per) + a.batch) * per;
         p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
         p.slots = (int)pairs;
-        p.cuts = span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
+        p.cuts = !alone && span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
         if (p.cuts) {
             p.slots = (int)slots;
             // what a workgroup reads in about 3 us; another round of arrivals takes as long
@@ -713,10 +737,8 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
-        if (c.dtype == CLOVE_DTYPE_FP16)
-            st = whole ? paged::launch_mfma<CLOVE_DTYPE_FP16, false>(p, stream) : paged::launch_mfma<CLOVE_DTYPE_FP16, true>(p, stream);
-        else
-            st = whole ? paged::launch_mfma<CLOVE_DTYPE_BF16, false>(p, stream) : paged::launch_mfma<CLOVE_DTYPE_BF16, true>(p, stream);
+        st = c.dtype == CLOVE_DTYPE_FP16 ? paged::launch_mfma<CLOVE_DTYPE_FP16>(p, whole, alone, stream)
+                                         : paged::launch_mfma<CLOVE_DTYPE_BF16>(p, whole, alone, stream);
         if (st != CLOVE_OK) return st;
     }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;

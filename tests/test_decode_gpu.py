@@ -834,3 +834,20 @@ def test_evict_a_few_wide_tokens(over):
         cg.cache_evict(cg.KVCache(dk, dv), _dev(table), dl, dw, dp, wo, po, lo, 2, L, budget, recent=5)
         for got, exact in zip((dk, dv, wo, po, lo), want):
             assert np.array_equal(_f64(got), exact.astype(np.float64))
+
+
+@pytest.mark.parametrize("B,longest,D,dtype", [(300, 30, 64, "fp16"), (520, 300, 64, "bf16"), (260, 500, 100, "fp16"), (140, 90, 256, "bf16")])
+def test_attention_more_short_sequences_than_the_card_holds(B, longest, D, dtype):
+    """One wave to a sequence and head."""
+    cg = _cg()
+    g = rng("attend-crowd", B, D)
+    lens = [int(x) for x in g.integers(0, longest + 1, B)]
+    lens[7], lens[8], lens[9] = longest, 0, 1
+    Hq, Hk, P = 4, 4, 16
+    k, v, k64, v64, table = _paged(g, dtype, lens, Hk, D, P)
+    q, q64 = _rounded(g, dtype, B, Hq, D)
+    w = _dev(np.zeros((B, longest), np.float32))
+    want, added = ref.attention(q64, k64, v64, table, lens, D ** -0.5)
+    out = _attend(cg, q, cg.KVCache(k, v), table, lens, B, Hq, longest, weights=w)
+    _close(out, want, dtype, 3e-5 * float(np.abs(v64).max()))
+    assert np.all(np.abs(_f64(w) - added[:, :longest]) <= 3e-5 * added[:, :longest] + 1e-9)
