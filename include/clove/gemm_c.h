@@ -318,10 +318,14 @@ clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const voi
  * and, where `weights` (fp32, rows weights_stride apart) is not NULL,
  *   weights[b, j] += sum over the heads of p_j      for every key it sees.
  * q, out [batch, q_heads, head_dim] (rows q_stride / out_stride apart) are the
- * cache's dtype.  Cache rows and table entries that no key names are not read.
- * max_context bounds the lengths on the host: it sizes the launch, and is at
- * most table_stride * page_size (and weights_stride).  Sums run in a fixed
- * order: a call gives the same bits every time.
+ * cache's dtype.  Cache rows that no key names are not used, whatever they hold.
+ * max_context bounds the lengths on the host: it is at most table_stride *
+ * page_size (and weights_stride), and a row of the table has ceil(max_context /
+ * page_size) entries, of which those past the length may be anything.  The work
+ * is shared out on the device by the lengths themselves, so a recorded call may
+ * be replayed with others.  Sums run in a fixed order: a call gives the same
+ * bits every time.  With `weights` the call takes a buffer of batch * q_heads *
+ * max_context floats of scratch.
  */
 clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clove_kv_cache_t* cache,
                                      const int32_t* block_table, int64_t table_stride,
