@@ -183,8 +183,8 @@ void launch_any(const Params& p, hipStream_t stream) {
 // head_dim 8 .. 256: MFMA
 //
 // A workgroup of four waves takes a chunk of the keys (Cut) of one (sequence, KV
-// head, tile of up to 16 query heads), each wave every fourth 32 of them; a
-// workgroup of one wave (W = 1) takes all keys of a short sequence.  With keys as
+// head, tile of up to 16 query heads), each wave every fourth 32 of them;
+// workgroups of one wave or eight (W) take all keys of a short sequence.  With keys as
 // rows and query heads as columns of v_mfma_f32_16x16x32,
 //   S [16 keys x 16 heads] = K [keys x d] Q^T [d x heads]       (two of them)
 //   O^T [d x heads] += V^T [d x 32 keys] P^T [32 keys x heads]
@@ -656,33 +656,44 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
 // alignment hold one fewer at 3 and 6)
 constexpr int kResident[8] = {5, 4, 3, 2, 2, 2, 1, 1};
 
+constexpr int kWide = 8;  // waves of the wide form, for head_dim up to 128 (registers)
+
 typedef void (*Kernel)(const Params);
 struct Form {
     Kernel kernel;
     int lds;
 };
+template <int DT, int NC, bool TAIL, int W>
+Form form() { return Form{attend<DT, NC, TAIL, W>, W * wave_lds<NC>()}; }
 template <int DT, bool TAIL, int W>
 Form pick(int nc) {
     switch (nc) {
-        case 1: return Form{attend<DT, 1, TAIL, W>, W * wave_lds<1>()};
-        case 2: return Form{attend<DT, 2, TAIL, W>, W * wave_lds<2>()};
-        case 3: return Form{attend<DT, 3, TAIL, W>, W * wave_lds<3>()};
-        case 4: return Form{attend<DT, 4, TAIL, W>, W * wave_lds<4>()};
-        case 5: return Form{attend<DT, 5, TAIL, W>, W * wave_lds<5>()};
-        case 6: return Form{attend<DT, 6, TAIL, W>, W * wave_lds<6>()};
-        case 7: return Form{attend<DT, 7, TAIL, W>, W * wave_lds<7>()};
-        default: return Form{attend<DT, 8, TAIL, W>, W * wave_lds<8>()};
+        case 1: return form<DT, 1, TAIL, W>();
+        case 2: return form<DT, 2, TAIL, W>();
+        case 3: return form<DT, 3, TAIL, W>();
+        case 4: return form<DT, 4, TAIL, W>();
     }
+    if constexpr (W != kWide) {
+        switch (nc) {
+            case 5: return form<DT, 5, TAIL, W>();
+            case 6: return form<DT, 6, TAIL, W>();
+            case 7: return form<DT, 7, TAIL, W>();
+            case 8: return form<DT, 8, TAIL, W>();
+        }
+    }
+    return Form{nullptr, 0};
 }
 
 template <int DT>
-clove_status_t launch_mfma(const Params& p, bool whole, bool alone, hipStream_t stream) {
+clove_status_t launch_mfma(const Params& p, bool whole, int waves, hipStream_t stream) {
     const int nc = cdiv(p.a.cache.head_dim, 32);
-    const Form f = whole ? (alone ? pick<DT, false, 1>(nc) : pick<DT, false, kW>(nc)) : (alone ? pick<DT, true, 1>(nc) : pick<DT, true, kW>(nc));
+    const Form f = waves == kWide ? pick<DT, false, kWide>(nc)
+                   : waves == 1   ? (whole ? pick<DT, false, 1>(nc) : pick<DT, true, 1>(nc))
+                                  : (whole ? pick<DT, false, kW>(nc) : pick<DT, true, kW>(nc));
     const int units = p.slots / p.tiles, grid = p.tiles > 1 ? cdiv(units, 8) * 8 * p.tiles : units;
     const clove_status_t st = ensure_lds(reinterpret_cast<const void*>(f.kernel), f.lds);
     if (st != CLOVE_OK) return st;
-    CLOVE_LAUNCH(f.kernel, dim3((unsigned)grid), dim3(alone ? 64 : 64 * kW), (size_t)f.lds, stream, p);
+    CLOVE_LAUNCH(f.kernel, dim3((unsigned)grid), dim3(64 * waves), (size_t)f.lds, stream, p);
     return CLOVE_OK;
 }
 
@@ -729,13 +740,18 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         // 20, 90, 250, 500 keys 9.1, 12.8, 30.4, 49.6 -> 6.2, 10.8, 21.8, 44.0 us; mixed
         // ones of up to 1000 36.9 -> 48.7, one of them outlasting the rest)
         const bool alone = (span <= 32 && std::min(p.group, 16) * c.head_dim <= 512) || (span <= 512 && pairs > p.fill);
+        // Eight waves where they take a sequence's keys in one go and four would split
+        // it: 200 keys of 1 and 64 sequences, 8 heads of 64, 7.6, 12.9 -> 6.2, 9.7 us;
+        // twice as many keys are better split (7.75 against 8.2)
+        const bool wide = !alone && whole && c.head_dim <= 128 && span > 32 * paged::kW && span <= 32 * paged::kWide;
+        const int waves = alone ? 1 : wide ? paged::kWide : paged::kW;
         // chunks: the CUs' fill a whole number of rounds, and a remainder of each
         // sequence, but no more than whole sequences make of the shortest chunks
         const int64_t rounds = std::max<int64_t>(1, hw::cdiv64(pairs * hw::cdiv(span, 32), (int64_t)p.fill * paged::kLongest));
         const int64_t slots = std::min((hw::cdiv64(p.fill * rounds, per) + a.batch) * per, pairs * hw::cdiv(span, 32 * paged::kW));
         p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
         p.slots = (int)pairs;
-        p.cuts = !alone && span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
+        p.cuts = waves == paged::kW && span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
         if (p.cuts) {
             p.slots = (int)slots;
             // what a workgroup reads in about 3 us; another round of arrivals takes as long
@@ -745,8 +761,8 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
-        st = c.dtype == CLOVE_DTYPE_FP16 ? paged::launch_mfma<CLOVE_DTYPE_FP16>(p, whole, alone, stream)
-                                         : paged::launch_mfma<CLOVE_DTYPE_BF16>(p, whole, alone, stream);
+        st = c.dtype == CLOVE_DTYPE_FP16 ? paged::launch_mfma<CLOVE_DTYPE_FP16>(p, whole, waves, stream)
+                                         : paged::launch_mfma<CLOVE_DTYPE_BF16>(p, whole, waves, stream);
         if (st != CLOVE_OK) return st;
     }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;

@@ -851,3 +851,20 @@ def test_attention_more_short_sequences_than_the_card_holds(B, longest, D, dtype
     out = _attend(cg, q, cg.KVCache(k, v), table, lens, B, Hq, longest, weights=w)
     _close(out, want, dtype, 3e-5 * float(np.abs(v64).max()))
     assert np.all(np.abs(_f64(w) - added[:, :longest]) <= 3e-5 * added[:, :longest] + 1e-9)
+
+
+@pytest.mark.parametrize("dtype,D", [("fp16", 64), ("bf16", 128), ("fp16", 96), ("bf16", 40), ("fp16", 136)])
+def test_attention_lengths_around_the_forms_of_the_kernel(dtype, D):
+    """Bounds on either side of what one, four and eight waves take at once."""
+    cg = _cg()
+    g = rng("attend-forms", D)
+    Hq, Hk, P = 6, 2, 16
+    for longest in (31, 32, 33, 127, 128, 129, 255, 256, 257, 511, 513):
+        lens = [longest, 0, max(1, longest // 3), longest - 1]
+        k, v, k64, v64, table = _paged(g, dtype, lens, Hk, D, P)
+        q, q64 = _rounded(g, dtype, 4, Hq, D)
+        w = _dev(np.zeros((4, longest), np.float32))
+        want, added = ref.attention(q64, k64, v64, table, lens, D ** -0.5)
+        out = _attend(cg, q, cg.KVCache(k, v), table, lens, 4, Hq, longest, weights=w)
+        _close(out, want, dtype, 3e-5 * float(np.abs(v64).max()))
+        assert np.all(np.abs(_f64(w) - added[:, :longest]) <= 3e-5 * added[:, :longest] + 1e-9)
