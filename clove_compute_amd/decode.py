@@ -64,6 +64,16 @@ def _rows(x, name, rows, width, dtype):
     return x.data_ptr(), strides[0] if rows > 1 else max(width, strides[0])
 
 
+def _lists(x, name, rows, dtype):
+    """(address, length) of equally long lists one after another: how far apart they
+    lie tells the library how long they are, so no part of longer ones is taken."""
+    n = x.shape[-1]
+    p, apart = _rows(x, name, rows, n, dtype)
+    if rows > 1 and apart != n:
+        raise ValueError(f"the rows of {name} must follow one another, not {n} elements every {apart}")
+    return p, n
+
+
 def _flat(x, name, n, dtype):
     """Address of at least `n` adjacent elements (None stays None)."""
     if x is None:
@@ -163,20 +173,20 @@ def penalize_logits(logits, out, batch: int, vocab: int, history=None, history_l
     (divided where positive, multiplied where not), the frequency and presence penalties of its part
     past ``prompt_lens``, the biases of ``bias_ids`` / ``bias_values`` (the last entry for a token
     counts) and the mask ``allowed`` [batch, ceil(vocab / 32)] (int32 words, token v is bit v % 32;
-    a clear bit gives -inf).  fp32 inside; ``out`` is fp32 or of the logits' type."""
+    a clear bit gives -inf).  The rows of ``history`` and of the bias lists follow one another;
+    those of the others may lie apart.  fp32 inside; ``out`` is fp32 or of the logits' type."""
     f, i = _b.f32, _b.i32
     x, xs = _rows(logits, "logits", batch, vocab, logits.dtype)
     o, os_ = _rows(out, "out", batch, vocab, out.dtype)
     h = b = bv = m = None
     hs = bs = ms = 0
     if history is not None:
-        h, hs = _rows(history, "history", batch, history.shape[-1], i)
+        h, hs = _lists(history, "history", batch, i)
     if bias_ids is not None:
-        n = bias_ids.shape[-1]
-        b, bs = _rows(bias_ids, "bias_ids", batch, n, i)
-        bv, ms = _rows(bias_values, "bias_values", batch, n, f)
+        b, bs = _lists(bias_ids, "bias_ids", batch, i)
+        bv, ms = _lists(bias_values, "bias_values", batch, f)
         if ms != bs:
-            raise ValueError("the rows of bias_ids and bias_values must be equally far apart")
+            raise ValueError("bias_ids and bias_values must be equally long")
     if allowed is not None:
         m, ms = _rows(allowed, "allowed", batch, -(-vocab // 32), i)
     st = _b.penalize(x, xs, _code(logits.dtype), o, os_, _code(out.dtype), batch, vocab, h, hs,

@@ -375,10 +375,11 @@ clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* b
  * r = repetition[b].  Any of repetition, presence, frequency [batch], history,
  * bias_ids and allowed may be NULL: that part is left out (prompt_lens NULL: no
  * prompt, everything was generated; bias_counts NULL: all bias_stride entries).
- * Lengths are taken as at least 0 and at most the row's stride; ids outside
- * [0, vocab) are ignored.  logits are `dtype` (FP16, BF16 or FP32), out is
- * `out_dtype` (the same, or FP32), rows logits_stride / out_stride elements
- * apart; out may be logits itself where dtype and stride agree.
+ * Rows of history and of the bias lists are history_stride / bias_stride entries
+ * long, any of which may be read; lengths are taken as at least 0 and at most
+ * that.  Ids outside [0, vocab) are ignored.  logits are `dtype` (FP16, BF16 or
+ * FP32), out is `out_dtype` (the same, or FP32), rows logits_stride / out_stride
+ * elements apart; out may be logits itself where dtype and stride agree.
  */
 clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, int dtype, void* out,
                                      int64_t out_stride, int out_dtype, int batch, int vocab,

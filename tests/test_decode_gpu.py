@@ -589,6 +589,29 @@ def test_python_checks():
         cg.paged_attention(st["q"], st["cache"], st["table"], st["lens"], st["q"], B, 8, L)
 
 
+def test_logits_lists_are_whole():
+    """Part of a longer list per row is refused (the distance of rows is their length);
+    of a single row it is taken, and nothing past it."""
+    import torch
+    cg = _cg()
+    x = torch.ones(2, 64, device="cuda")
+    y, two = torch.empty_like(x), torch.tensor([2.0, 2.0], device="cuda")
+    ids = torch.arange(32, dtype=torch.int32, device="cuda").view(2, 16)
+    lens, values = torch.tensor([16, 16], dtype=torch.int32, device="cuda"), torch.ones(2, 16, device="cuda")
+    for part in (slice(0, 4), slice(8, 16)):
+        with pytest.raises(ValueError):
+            cg.penalize_logits(x, y, 2, 64, history=ids[:, part], history_lens=lens, repetition=two)
+        with pytest.raises(ValueError):
+            cg.penalize_logits(x, y, 2, 64, bias_ids=ids[:, part], bias_values=values[:, part])
+    with pytest.raises(ValueError):
+        cg.penalize_logits(x, y, 2, 64, bias_ids=ids, bias_values=values[:, :4].contiguous())
+    cg.penalize_logits(x, y, 1, 64, history=ids[:1, 4:8], history_lens=lens, repetition=two, bias_ids=ids[1:, :2],
+                       bias_values=values[1:, :2])
+    want = torch.ones(64)
+    want[4:8], want[16:18] = 0.5, 2.0
+    assert torch.equal(y[0].cpu(), want)
+
+
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("lens,budget,sinks,recent,kind", [
     ([17000, 16384, 16390], 4096, 4, 300, "free"), ([33000, 20000], 12000, 0, 1, "ties"), ([18001], 18000, 4, 100, "free"),
