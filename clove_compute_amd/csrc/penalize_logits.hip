@@ -8,11 +8,12 @@
 // counted in LDS (whole numbers: atomics give the same counts in any order), so
 // nothing of the vocabulary's size is written to memory but the result.  HBM-bound
 // for large batches: 256 rows of 128000 fp32 logits with masks and 8000 tokens of
-// history each take 63.5 us (4.3 TB/s), 49 (5.3 TB/s, a copy's rate) without them.
-// What is known before the counts -- logits, mask, the first ids -- is loaded
-// ahead of them.  Every slice of a row reads its history anew (from L2), so slices
-// are as long as leaves two workgroups per CU (at 8192 tokens instead of 16384 the
-// above takes 66 us), and results pass the L2 by (68 us with ordinary stores).
+// history each take 57 us (4.8 TB/s), 48 (5.5 TB/s, a copy's rate) without them;
+// bf16 logits to fp32 without a history 31 (6.3 TB/s).  What is known before the
+// counts -- logits, mask, the first ids -- is loaded ahead of them, and results
+// pass the L2 by.  Every slice of a row reads its history anew; a row's slices run
+// on one XCD, whose L2 then has it (55 us without masks, 58 where they are spread
+// over all XCDs; 38 and 44 with bf16 logits, masks and biases).
 #include <algorithm>
 
 #include "decode.hpp"
@@ -34,17 +35,16 @@ constexpr unsigned prompt_bit() { return PACKED ? 0x8000u : 0x80000000u; }
 typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// Adjacent elements in one 16-byte access at any alignment of their type
-template <int DT>
+// E adjacent elements in one access, at any alignment of their type
+template <int DT, int E>
 struct Group {
-    static constexpr int E = 8;
-    u32x4 x;
-    __device__ __forceinline__ void load(const uint16_t* p) { x = load_any16(reinterpret_cast<const unsigned char*>(p)); }
+    typedef unsigned any __attribute__((ext_vector_type(E / 2), aligned(2)));
+    any x;
+    __device__ __forceinline__ void load(const uint16_t* p) { x = *reinterpret_cast<const any*>(p); }
     __device__ __forceinline__ float get(int i) const { return Elem<DT>::load((uint16_t)(x[i / 2] >> (16 * (i & 1)))); }
 };
-template <>
-struct Group<CLOVE_DTYPE_FP32> {
-    static constexpr int E = 4;
+template <int E>
+struct Group<CLOVE_DTYPE_FP32, E> {
     f32x4 x;
     __device__ __forceinline__ void load(const float* p) { x = *reinterpret_cast<const f32x4u*>(p); }
     __device__ __forceinline__ float get(int i) const { return x[i]; }
@@ -52,9 +52,7 @@ struct Group<CLOVE_DTYPE_FP32> {
 template <int DT, int E>
 __device__ __forceinline__ void store_group(typename Elem<DT>::raw* p, const float (&v)[E]) {
     if constexpr (DT == CLOVE_DTYPE_FP32) {
-#pragma unroll
-        for (int i = 0; i < E; i += 4)
-            __builtin_nontemporal_store(f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]}, reinterpret_cast<f32x4u*>(p + i));
+        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4u*>(p));
     } else {
         u32x4 x;
 #pragma unroll
@@ -64,18 +62,23 @@ __device__ __forceinline__ void store_group(typename Elem<DT>::raw* p, const flo
 }
 
 template <int DI, int DO, bool PACKED>
-__global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv slices) {
+__global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv slices, int apart) {
     using EI = Elem<DI>;
     using EO = Elem<DO>;
     constexpr unsigned kPrompt = prompt_bit<PACKED>(), kCount = kPrompt - 1;
     extern __shared__ __align__(16) unsigned words[];
     const int threads = blockDim.x, tid = threadIdx.x, slice = threads * kPer;
-    const int b = slices.div(blockIdx.x), v0 = (blockIdx.x - b * slices.d) * slice;
+    // the slices of a row lie `apart` (8) workgroups apart: on one XCD, whose L2 has
+    // its history after the first of them
+    const int run = slices.div(blockIdx.x / apart), b = run * apart + blockIdx.x % apart, v0 = (blockIdx.x / apart - run * slices.d) * slice;
+    if (b >= a.batch) return;
     const int n = min(slice, a.vocab - v0);
     const typename EI::raw* in = static_cast<const typename EI::raw*>(a.logits) + b * a.logits_stride + v0;
     typename EO::raw* out = static_cast<typename EO::raw*>(a.out) + b * a.out_stride + v0;
-    constexpr int E = Group<DI>::E, kGroups = kPer / E;
-    Group<DI> x[kGroups];
+    // so many that a result is 16 bytes: a wave's store is whole lines (with 8 of
+    // bf16 in two stores of fp32, 256 x 128000 without a history take 49 us, not 31)
+    constexpr int E = DO == CLOVE_DTYPE_FP32 ? 4 : 8, kGroups = kPer / E;
+    Group<DI, E> x[kGroups];
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
         const int at = (k * threads + tid) * E;
@@ -88,30 +91,33 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
         const int at = (k * threads + tid) * E;
-        open[k] = allowed && at < n ? allowed[(v0 + at) >> 5] >> ((v0 + at) & 31) : 0xffu;
+        open[k] = allowed && at < n ? allowed[(v0 + at) >> 5] : 0xffffffffu;  // (shifted below: here it would be awaited)
     }
     const int32_t* told = a.history + b * a.history_stride;
     i32x4 first = {};
     if (a.history && tid * 4 + 4 <= a.history_stride) first = *reinterpret_cast<const i32x4u*>(told + tid * 4);
-    unsigned* const entry = words + slice;  // PACKED: not there
     const bool biased = a.bias_ids != nullptr, counted = a.history != nullptr || biased;
+    const int32_t* named = a.bias_ids + b * a.bias_stride;
+    const int first_named = biased && tid < a.bias_stride ? named[tid] : -1;
+    const int len = a.history ? (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride) : 0;
+    const int prompt = a.history && a.prompt_lens ? a.prompt_lens[b] : 0;
+    const int entries = !biased ? 0 : (int)(a.bias_counts ? min((int64_t)max(a.bias_counts[b], 0), a.bias_stride) : a.bias_stride);
+    const float r = a.repetition ? a.repetition[b] : 1.0f;
+    const float f = a.frequency ? a.frequency[b] : 0.0f, p = a.presence ? a.presence[b] : 0.0f;
+    unsigned* const entry = words + slice;  // PACKED: not there
     if (counted) {
         u32x4* const w = reinterpret_cast<u32x4*>(words);
         for (int i = tid; i < slice * (PACKED ? 1 : 2) / 4; i += threads) w[i] = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
     }
     if (biased) {
-        const int m = (int)(a.bias_counts ? min((int64_t)max(a.bias_counts[b], 0), a.bias_stride) : a.bias_stride);
-        const int32_t* ids = a.bias_ids + b * a.bias_stride;
-        for (int i = tid; i < m; i += threads) {
-            const unsigned at = (unsigned)ids[i] - (unsigned)v0;  // (an id below 0 is past every slice)
+        for (int i = tid; i < entries; i += threads) {
+            const unsigned at = (unsigned)(i == tid ? first_named : named[i]) - (unsigned)v0;  // (an id below 0 is past every slice)
             if (at < (unsigned)n) PACKED ? atomicMax(&words[at], ((unsigned)i + 1u) << 16) : atomicMax(&entry[at], (unsigned)i + 1u);
         }
         if constexpr (PACKED) __syncthreads();  // the counts go below
     }
     if (a.history) {
-        const int len = (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride);
-        const int prompt = a.prompt_lens ? a.prompt_lens[b] : 0;
         auto count = [&](int id, int i) {
             const unsigned at = (unsigned)id - (unsigned)v0;
             if (at < (unsigned)n) i < prompt ? atomicOr(&words[at], kPrompt) : atomicAdd(&words[at], 1u);
@@ -125,8 +131,6 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
         for (; i < len; ++i) count(told[i], i);  // (the one thread that the last, shorter four fall to)
     }
     if (counted) __syncthreads();
-    const float r = a.repetition ? a.repetition[b] : 1.0f;
-    const float f = a.frequency ? a.frequency[b] : 0.0f, p = a.presence ? a.presence[b] : 0.0f;
     const float* bias = a.bias_values + b * a.bias_stride;
     auto result = [&](float l, unsigned word, unsigned e, unsigned open) {
         if constexpr (PACKED) e = word >> 16;
@@ -142,6 +146,7 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     for (int k = 0; k < kGroups; ++k) {
         const int at = (k * threads + tid) * E;
         if (at >= n) break;
+        const unsigned bits = open[k] >> ((v0 + at) & 31);
         u32x4 w[E / 4] = {}, e[E / 4] = {};
         if (counted) {
 #pragma unroll
@@ -153,17 +158,17 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
         if (at + E <= n) {
             float y[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) y[i] = result(x[k].get(i), w[i / 4][i % 4], e[i / 4][i % 4], (open[k] >> i) & 1u);
+            for (int i = 0; i < E; ++i) y[i] = result(x[k].get(i), w[i / 4][i % 4], e[i / 4][i % 4], (bits >> i) & 1u);
             store_group<DO, E>(out + at, y);
         } else {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                if (at + i < n) out[at + i] = EO::store(result(EI::load(in[at + i]), w[i / 4][i % 4], e[i / 4][i % 4], (open[k] >> i) & 1u));
+                if (at + i < n) out[at + i] = EO::store(result(EI::load(in[at + i]), w[i / 4][i % 4], e[i / 4][i % 4], (bits >> i) & 1u));
         }
     }
 }
 
-typedef void (*Kernel)(const LogitsArgs, FastDiv);
+typedef void (*Kernel)(const LogitsArgs, FastDiv, int);
 template <int DI>
 Kernel pick(int out, bool packed) {
     if (out == CLOVE_DTYPE_FP32)
@@ -179,17 +184,21 @@ clove_status_t launch_penalize_logits(const LogitsArgs& a, hipStream_t stream) {
     if (st != CLOVE_OK) return st;
     const bool counted = a.history || a.bias_ids;
     const bool packed = !(a.history && a.history_stride >= 32768) && !(a.bias_ids && a.bias_stride >= 32768);
-    // the longest slices that still give two workgroups per CU
-    int threads = packed ? 1024 : 512;
+    // Counting, the longest slices that still give two workgroups per CU: each reads
+    // the history (256 x 128000 fp32 without masks take 55 us with slices of 16384,
+    // 58 with 8192).  Otherwise the shortest, of which more are in flight (48 and 49).
+    int threads = !counted ? 256 : packed ? 1024 : 512;
     while (threads > 256 && (int64_t)a.batch * hw::cdiv(a.vocab, threads * logits::kPer) < 2 * dev.num_cus) threads /= 2;
     const int slice = threads * logits::kPer, slices = hw::cdiv(a.vocab, slice);
-    if ((int64_t)a.batch * slices > 0x7fffffff) return CLOVE_ERR_INVALID_DIM;
+    const int apart = a.batch >= 8 ? 8 : 1;
+    const int64_t grid = (int64_t)hw::cdiv(a.batch, apart) * apart * slices;
+    if (grid > 0x7fffffff) return CLOVE_ERR_INVALID_DIM;
     const logits::Kernel kernel = a.dtype == CLOVE_DTYPE_FP16   ? logits::pick<CLOVE_DTYPE_FP16>(a.out_dtype, packed)
                                   : a.dtype == CLOVE_DTYPE_BF16 ? logits::pick<CLOVE_DTYPE_BF16>(a.out_dtype, packed)
                                                                 : logits::pick<CLOVE_DTYPE_FP32>(a.out_dtype, packed);
     const int lds = counted ? slice * (packed ? 4 : 8) : 0;
     if ((st = ensure_lds(reinterpret_cast<const void*>(kernel), lds)) != CLOVE_OK) return st;
-    CLOVE_LAUNCH(kernel, dim3((unsigned)(a.batch * slices)), dim3(threads), lds, stream, a, FastDiv(slices));
+    CLOVE_LAUNCH(kernel, dim3((unsigned)grid), dim3(threads), lds, stream, a, FastDiv(slices), apart);
     return check_launch();
 }
 
