@@ -1,4 +1,6 @@
-"""Builds the gfx950 GEMM library libclove_gemm.so in-tree with hipcc.
+"""Builds the gfx950 GEMM library libclove_gemm.so in-tree with hipcc, and with
+the host compiler the module through which Python calls the decode step's
+operators with torch tensors (lib/_decode.so, from csrc/decode_binding.cpp).
 
 Each .hip source under csrc/ is compiled to an object for gfx950 only, then
 linked into clove_compute_amd/lib/libclove_gemm.so.  Objects are rebuilt when
@@ -11,9 +13,11 @@ states a gfx9 hazard requires (hazards.py).
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -25,6 +29,9 @@ LIB = os.path.join(LIBDIR, "libclove_gemm.so")
 # diagnostics for bench.py --floor (not part of the GEMM C-ABI)
 DIAG_SRC = os.path.join(CSRC, "diag")
 DIAG_LIB = os.path.join(LIBDIR, "libclove_diag.so")
+BINDING_SRC = os.path.join(CSRC, "decode_binding.cpp")
+BINDING = os.path.join(LIBDIR, "_decode.so")
+CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
@@ -73,12 +80,32 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _build_binding(force: bool) -> None:
+    if (not force and os.path.exists(BINDING)
+            and os.path.getmtime(BINDING) >= max(os.path.getmtime(BINDING_SRC), _headers_mtime())):
+        return
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]  # (found, not imported: that takes seconds)
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           "-I", os.path.join(ROOT, "include"), "-isystem", os.path.join(torch, "include"),
+           "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+           BINDING_SRC, "-o", BINDING + ".tmp", "-L", os.path.join(torch, "lib"), "-ltorch_python", "-lc10", "-lc10_hip"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("compiling decode_binding.cpp failed")
+    os.replace(BINDING + ".tmp", BINDING)
+
+
 def build(force: bool = False, jobs: int = 8) -> str:
     os.makedirs(OBJ, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     srcs = _sources()
-    with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs)))) as ex:
+    with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + 1))) as ex:
+        binding = ex.submit(_build_binding, force)
         objs = list(ex.map(lambda s: _compile(s, force), srcs))
+        binding.result()
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB + ".tmp", *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -6,81 +6,44 @@ Buffers are torch tensors on the current HIP device, passed with their sizes as
 in ``gemm``; every call goes through the C ABI (include/clove/gemm_c.h states
 the formulas), is asynchronous on ``stream`` (default: torch's current stream)
 and raises CloveError where the library refuses it.  What the C ABI cannot see
--- device, element type, number of elements, inner strides -- is checked here
-(ValueError).  A tensor's rows may be further apart than they are long; the
+-- device, element type, number of elements, inner strides -- is checked on the
+way (ValueError), in compiled code: it is most of a small call's time.  A tensor's rows may be further apart than they are long; the
 elements of a row are adjacent.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
+import os
 
 from . import _lib
-from .gemm import _stream
+
+_CODES = {"torch.float16": _lib.CLOVE_DTYPE_FP16, "torch.bfloat16": _lib.CLOVE_DTYPE_BF16,
+          "torch.float32": _lib.CLOVE_DTYPE_FP32}
+
 
 class _Bound:
-    """What every call needs, looked up on the first: the library's functions and
-    torch's element types (importing torch and resolving a function by name cost
-    a microsecond a call, a third of what the smallest kernels take)."""
+    """The compiled entry points, looked up on the first call: importing torch and
+    loading the library take long, and resolving a name a microsecond a call."""
 
     def __getattr__(self, name):
-        import torch
-        lib = _lib.lib()
-        self.f16, self.f32, self.i32 = torch.float16, torch.float32, torch.int32
-        self.codes = {torch.float16: _lib.CLOVE_DTYPE_FP16, torch.bfloat16: _lib.CLOVE_DTYPE_BF16,
-                      torch.float32: _lib.CLOVE_DTYPE_FP32}
-        self.rope, self.attend = lib.clove_qk_norm_rope, lib.clove_paged_attention
-        self.evict, self.penalize = lib.clove_cache_evict, lib.clove_penalize_logits
+        import torch  # noqa: F401  (the module is linked to its libraries)
+        lib, path = _lib.lib(), os.path.join(os.path.dirname(__file__), "lib", "_decode.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build the HIP library first "
+                               "(python -c 'import __graft_entry__ as g; g.build()')")
+        loader = importlib.machinery.ExtensionFileLoader("_decode", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_decode", loader))
+        loader.exec_module(module)
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in
+                      (lib.clove_qk_norm_rope, lib.clove_paged_attention, lib.clove_cache_evict, lib.clove_penalize_logits)))
+        self.rope, self.attend, self.evict, self.penalize = (module.qk_norm_rope, module.paged_attention, module.cache_evict,
+                                                             module.penalize_logits)
         return self.__dict__[name]
 
 
 _b = _Bound()
-
-
-def _code(dtype) -> int:
-    c = _b.codes.get(dtype)
-    if c is None:
-        raise ValueError(f"element type {dtype} is not fp16, bf16 or fp32")
-    return c
-
-
-def _rows(x, name, rows, width, dtype):
-    """(address, row stride) of a tensor read as `rows` rows of `width` adjacent
-    elements; its first dimension is the row where it has more than one."""
-    if x.dtype is not dtype or not x.is_cuda:
-        raise ValueError(f"{name} must be {dtype} on the GPU, not {x.dtype} on {x.device}")
-    if x.numel() == rows * width and x.is_contiguous():
-        return x.data_ptr(), width
-    shape, strides = x.shape, x.stride()
-    n, inner = shape[0] if shape else 1, 1
-    if len(shape) < 2:
-        n, shape, strides = 1, (1, *shape), (n, *strides)
-    for size, stride in zip(shape[:0:-1], strides[:0:-1]):
-        if size != 1 and stride != inner:
-            inner = -1
-            break
-        inner *= size
-    if n < rows or inner < width:
-        raise ValueError(f"{name} holds {tuple(x.shape)} elements, {rows} rows of {width} adjacent ones are wanted")
-    return x.data_ptr(), strides[0] if rows > 1 else max(width, strides[0])
-
-
-def _lists(x, name, rows, dtype):
-    """(address, length) of equally long lists one after another: how far apart they
-    lie tells the library how long they are, so no part of longer ones is taken."""
-    n = x.shape[-1]
-    p, apart = _rows(x, name, rows, n, dtype)
-    if rows > 1 and apart != n:
-        raise ValueError(f"the rows of {name} must follow one another, not {n} elements every {apart}")
-    return p, n
-
-
-def _flat(x, name, n, dtype):
-    """Address of at least `n` adjacent elements (None stays None)."""
-    if x is None:
-        return None
-    if x.dtype is not dtype or not x.is_cuda or x.numel() < n or not x.is_contiguous():
-        raise ValueError(f"{name} must be {n} adjacent {dtype} elements on the GPU, not {tuple(x.shape)} {x.dtype}")
-    return x.data_ptr()
 
 
 class KVCache:
@@ -97,12 +60,14 @@ class KVCache:
             raise ValueError("the pages of k and v must be dense")
         if k.shape[0] > 1 and k.stride(0) != v.stride(0):
             raise ValueError("the pages of k and v must be equally far apart")
+        if str(k.dtype) not in _CODES:
+            raise ValueError(f"element type {k.dtype} is not fp16, bf16 or fp32")
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype = k.dtype
         self._c = _lib.KVCacheDesc(k.data_ptr(), v.data_ptr(), k.stride(0) if k.shape[0] > 1 else 0, self.num_pages,
-                                   self.page_size, self.kv_heads, self.head_dim, _code(k.dtype))
-        self._ref = ctypes.byref(self._c)
+                                   self.page_size, self.kv_heads, self.head_dim, _CODES[str(k.dtype)])
+        self._at = ctypes.addressof(self._c)
 
 
 def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, positions, q_out, T: int, q_heads: int, kv_heads: int,
@@ -112,20 +77,8 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, positions, q_out, T: int, q_
     ``rot_dim`` (default: all) elements by ``cos`` / ``sin`` [max_position, rot_dim / 2] at
     ``positions`` [T], and the write of keys and values into ``slots`` [T] of ``cache``: one pass
     over the fused projection's rows ``qkv`` [T, (q_heads + 2 kv_heads) head_dim]."""
-    R = head_dim if rot_dim is None else rot_dim
-    dt, i, half, most = qkv.dtype, _b.i32, R // 2, 0
-    x, xs = _rows(qkv, "qkv", T, (q_heads + 2 * kv_heads) * head_dim, dt)
-    q, qs = _rows(q_out, "q_out", T, q_heads * head_dim, dt)
-    k, ks = _rows(k_out, "k_out", T, kv_heads * head_dim, dt) if k_out is not None else (None, 0)
-    c = s = None
-    if R:
-        most = cos.shape[0]
-        c, s = _flat(cos, "cos", most * half, _b.f32), _flat(sin, "sin", most * half, _b.f32)
-        if cos.numel() != most * half or sin.shape != cos.shape:
-            raise ValueError(f"cos and sin are [max_position, {half}], not {tuple(cos.shape)} and {tuple(sin.shape)}")
-    st = _b.rope(x, xs, _flat(q_weight, "q_weight", head_dim, dt), _flat(k_weight, "k_weight", head_dim, dt), eps, c, s, most,
-                 _flat(positions, "positions", T, i) if R else None, q, qs, k, ks, None if cache is None else cache._ref,
-                 _flat(slots, "slots", T, i), T, q_heads, kv_heads, head_dim, R, interleaved, _code(dt), _stream(stream))
+    st = _b.rope(qkv, q_weight, k_weight, cos, sin, positions, q_out, T, q_heads, kv_heads, head_dim, rot_dim, eps,
+                 interleaved, k_out, None if cache is None else cache._at, slots, stream)
     if st:
         _lib.check(st, "qk_norm_rope")
 
@@ -137,13 +90,8 @@ def paged_attention(q, cache: KVCache, block_table, context_lens, out, batch: in
     ``scale`` defaults to head_dim ** -0.5; ``window`` > 0 sees the last keys only; ``softcap`` > 0
     bounds the scores; ``weights`` [batch, max_context] fp32 gains each key's softmax weight,
     summed over the heads."""
-    D, dt, i = cache.head_dim, cache.dtype, _b.i32
-    x, xs = _rows(q, "q", batch, q_heads * D, dt)
-    o, os_ = _rows(out, "out", batch, q_heads * D, dt)
-    t, ts = _rows(block_table, "block_table", batch, -(-max_context // cache.page_size), i)
-    w, ws = _rows(weights, "weights", batch, max_context, _b.f32) if weights is not None else (None, 0)
-    st = _b.attend(x, xs, cache._ref, t, ts, _flat(context_lens, "context_lens", batch, i), o, os_, w, ws, batch, q_heads,
-                   max_context, D ** -0.5 if scale is None else scale, softcap, window, _stream(stream))
+    st = _b.attend(q, cache._at, block_table, context_lens, out, batch, q_heads, max_context,
+                   cache.head_dim ** -0.5 if scale is None else scale, softcap, window, weights, stream)
     if st:
         _lib.check(st, "paged_attention")
 
@@ -154,14 +102,8 @@ def cache_evict(cache: KVCache, block_table, context_lens, weights, positions, w
     ``sinks`` and the newest ``recent`` positions stay, then those of the largest ``weights``
     [batch, max_context]; kept tokens past the budget move into the holes below it.  Outputs hold the
     new weights, positions and lengths, and may be the inputs."""
-    f, i = _b.f32, _b.i32
-    t, ts = _rows(block_table, "block_table", batch, -(-max_context // cache.page_size), i)
-    w, ws = _rows(weights, "weights", batch, max_context, f)
-    p, ps = _rows(positions, "positions", batch, max_context, i)
-    wo, wos = _rows(weights_out, "weights_out", batch, max_context, f)
-    po, pos = _rows(positions_out, "positions_out", batch, max_context, i)
-    st = _b.evict(cache._ref, t, ts, _flat(context_lens, "context_lens", batch, i), w, ws, p, ps, wo, wos, po, pos,
-                  _flat(lens_out, "lens_out", batch, i), batch, max_context, budget, sinks, recent, _stream(stream))
+    st = _b.evict(cache._at, block_table, context_lens, weights, positions, weights_out, positions_out, lens_out, batch,
+                  max_context, budget, sinks, recent, stream)
     if st:
         _lib.check(st, "cache_evict")
 
@@ -175,24 +117,7 @@ def penalize_logits(logits, out, batch: int, vocab: int, history=None, history_l
     counts) and the mask ``allowed`` [batch, ceil(vocab / 32)] (int32 words, token v is bit v % 32;
     a clear bit gives -inf).  The rows of ``history`` and of the bias lists follow one another;
     those of the others may lie apart.  fp32 inside; ``out`` is fp32 or of the logits' type."""
-    f, i = _b.f32, _b.i32
-    x, xs = _rows(logits, "logits", batch, vocab, logits.dtype)
-    o, os_ = _rows(out, "out", batch, vocab, out.dtype)
-    h = b = bv = m = None
-    hs = bs = ms = 0
-    if history is not None:
-        h, hs = _lists(history, "history", batch, i)
-    if bias_ids is not None:
-        b, bs = _lists(bias_ids, "bias_ids", batch, i)
-        bv, ms = _lists(bias_values, "bias_values", batch, f)
-        if ms != bs:
-            raise ValueError("bias_ids and bias_values must be equally long")
-    if allowed is not None:
-        m, ms = _rows(allowed, "allowed", batch, -(-vocab // 32), i)
-    st = _b.penalize(x, xs, _code(logits.dtype), o, os_, _code(out.dtype), batch, vocab, h, hs,
-                     _flat(history_lens, "history_lens", batch, i), _flat(prompt_lens, "prompt_lens", batch, i),
-                     _flat(repetition, "repetition", batch, f), _flat(presence, "presence", batch, f),
-                     _flat(frequency, "frequency", batch, f), b, bv, bs, _flat(bias_counts, "bias_counts", batch, i), m, ms,
-                     _stream(stream))
+    st = _b.penalize(logits, out, batch, vocab, history, history_lens, prompt_lens, repetition, presence, frequency, bias_ids,
+                     bias_values, bias_counts, allowed, stream)
     if st:
         _lib.check(st, "penalize_logits")
