@@ -5,14 +5,14 @@
 // in one pass over the keys with a running maximum m and sum l: scores are kept
 // in base 2 (t = s log2 e), p_j = 2^(t_j - m) / l.  The bytes are K and V once;
 // everything else is small, so long caches are bound by HBM: 65536 keys of one
-// sequence, 8 KV heads of 128 (268 MB), 55 us, 4.9 TB/s; 16 x 4096 keys of 32 KV
-// heads of 128 (1.07 GB) 190 us, 5.7 TB/s, where a copy reaches 5.1.  Short ones are
+// sequence, 8 KV heads of 128 (268 MB), 53 us, 5.0 TB/s; 16 x 4096 keys of 32 KV
+// heads of 128 (1.07 GB) 187 us, 5.7 TB/s, where a copy reaches 5.1.  Short ones are
 // bound by the latencies from the lengths to the page table to the rows, and of the
 // join: 411 keys 7.7 us, 20 keys 4.3.
 //
 // Accumulated weights need every head's final m and l, so the scores go to
 // scratch (fp32, one per query head and key) and a second kernel adds
-// sum_h 2^(t - m_h) / l_h to each key's weight: 8.5 of 49 us for 48 sequences of
+// sum_h 2^(t - m_h) / l_h to each key's weight: 8.5 of 48 us for 48 sequences of
 // up to 6144 keys (145 MB of cache, 9 MB of scores written and read again).
 #include <algorithm>
 

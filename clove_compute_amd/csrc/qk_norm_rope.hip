@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(256) rope_any(const Params p) {
 // for every head of the wave.  With few tokens each wave takes one round of
 // heads, so that the loads of a token are in flight together; with many, rounds
 // follow each other with the next head's elements loaded ahead.
-// 8192 tokens of 32 + 16 heads of 128 (206 MB): 236 us with rope_any.
+// 8192 tokens of 32 + 16 heads of 128 (206 MB): 44 us, 4.7 TB/s (236 with rope_any);
+// 200 tokens 4.3, one 2.6.
 template <int CH>
 struct Chunk {
     typedef unsigned words __attribute__((ext_vector_type(CH / 2)));

@@ -589,6 +589,41 @@ def test_python_checks():
         cg.paged_attention(st["q"], st["cache"], st["table"], st["lens"], st["q"], B, 8, L)
 
 
+def test_arguments_of_other_kinds_are_errors():
+    """What is no tensor, no number or too large a number raises and leaves nothing behind."""
+    import torch
+    cg = _cg()
+    x = torch.ones(2, 64, device="cuda")
+    y = torch.zeros_like(x)
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.float16, device="cuda")
+    q, lens = torch.zeros(2, 128, dtype=torch.float16, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    table = torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(TypeError):
+        cg.penalize_logits(x.cpu().numpy(), y, 2, 64)
+    with pytest.raises(TypeError):
+        cg.penalize_logits(x, y, 2, "64")
+    with pytest.raises(TypeError):
+        cg.penalize_logits(x, y, 2, 64, history=[1, 2])
+    with pytest.raises(OverflowError):
+        cg.penalize_logits(x, y, 2, 64 + 2 ** 32)
+    with pytest.raises(ValueError):
+        cg.penalize_logits(x, y, 2 ** 31 - 1, 2 ** 31 - 1)
+    with pytest.raises(AttributeError):
+        cg.paged_attention(q, None, table, lens, q.clone(), 2, 2, 16)
+    with pytest.raises((ValueError, OverflowError)):
+        cg.paged_attention(q, cg.KVCache(k, k.clone()), table, lens, q.clone(), 2, 2 ** 31 - 1, 16)
+    with pytest.raises(cg.CloveError):  # pages of no rows
+        cg.paged_attention(q, cg.KVCache(k[:, :, :0].contiguous(), k[:, :, :0].contiguous()), table, lens, q.clone(), 2, 2, 16)
+    with pytest.raises(ValueError):
+        cg.KVCache(k.double(), k.double())
+    with pytest.raises(ValueError):
+        cg.penalize_logits(x, y, 2, 64, history=torch.zeros((), dtype=torch.int32, device="cuda"), history_lens=lens)
+    assert not y.any()
+    cg.penalize_logits(x, y, 2, 64, stream=torch.cuda.current_stream().cuda_stream)
+    cg.penalize_logits(x, x, 2, 64, stream=torch.cuda.current_stream())
+    assert torch.equal(x, y)
+
+
 def test_logits_lists_are_whole():
     """Part of a longer list per row is refused (the distance of rows is their length);
     of a single row it is taken, and nothing past it."""
