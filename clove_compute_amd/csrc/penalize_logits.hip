@@ -8,12 +8,12 @@
 // counted in LDS (whole numbers: atomics give the same counts in any order), so
 // nothing of the vocabulary's size is written to memory but the result.  HBM-bound
 // for large batches: 256 rows of 128000 fp32 logits with masks and 8000 tokens of
-// history each take 57 us (4.8 TB/s), 48 (5.5 TB/s, a copy's rate) without them;
+// history each take 53 us (5.1 TB/s), 48 (5.5 TB/s, a copy's rate) without them;
 // bf16 logits to fp32 without a history 31 (6.3 TB/s).  What is known before the
 // counts -- logits, mask, the first ids -- is loaded ahead of them, and results
 // pass the L2 by.  Every slice of a row reads its history anew; a row's slices run
-// on one XCD, whose L2 then has it (55 us without masks, 58 where they are spread
-// over all XCDs; 38 and 44 with bf16 logits, masks and biases).
+// on one XCD, whose L2 then has it (39 us with bf16 logits, masks and biases to
+// fp32, 43 where they are spread over all XCDs; fp32 without masks 52 and 54).
 #include <algorithm>
 
 #include "decode.hpp"
@@ -24,6 +24,9 @@ namespace logits {
 using namespace hw;
 
 constexpr int kPer = 16;  // tokens of a thread, in groups of adjacent ones
+// loads of ids at once (32 x 32000 after 8191 tokens 9.9 us with one, 9.3 with two;
+// 256 x 128000 after 8000 54 and 52; four win no more)
+constexpr int kAhead = 2;
 
 // A token's word in LDS.  PACKED: 15 bits of how often it was generated, bit 15
 // for "in the prompt", and above them 1 + the last bias entry that names it,
@@ -62,7 +65,7 @@ __device__ __forceinline__ void store_group(typename Elem<DT>::raw* p, const flo
 }
 
 template <int DI, int DO, bool PACKED>
-__global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv slices, int apart) {
+__global__ void __launch_bounds__(512) penalize(const LogitsArgs a, FastDiv slices, int apart) {
     using EI = Elem<DI>;
     using EO = Elem<DO>;
     constexpr unsigned kPrompt = prompt_bit<PACKED>(), kCount = kPrompt - 1;
@@ -98,7 +101,8 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     if (a.history && tid * 4 + 4 <= a.history_stride) first = *reinterpret_cast<const i32x4u*>(told + tid * 4);
     const bool biased = a.bias_ids != nullptr, counted = a.history != nullptr || biased;
     const int32_t* named = a.bias_ids + b * a.bias_stride;
-    const int first_named = biased && tid < a.bias_stride ? named[tid] : -1;
+    int id[kAhead] = {};
+    if (biased && tid < a.bias_stride) id[0] = named[tid];
     const int len = a.history ? (int)min((int64_t)max(a.history_lens[b], 0), a.history_stride) : 0;
     const int prompt = a.history && a.prompt_lens ? a.prompt_lens[b] : 0;
     const int entries = !biased ? 0 : (int)(a.bias_counts ? min((int64_t)max(a.bias_counts[b], 0), a.bias_stride) : a.bias_stride);
@@ -108,28 +112,50 @@ __global__ void __launch_bounds__(1024) penalize(const LogitsArgs a, FastDiv sli
     if (counted) {
         u32x4* const w = reinterpret_cast<u32x4*>(words);
         for (int i = tid; i < slice * (PACKED ? 1 : 2) / 4; i += threads) w[i] = u32x4{0u, 0u, 0u, 0u};
-        __syncthreads();
     }
+    // the ids that follow the first ones, kAhead loads at a time, and the history's
+    // last one to three (the thread's is looked at behind its others)
+    // (unsigned: steps past the longest length, 2^31 - 1, do not turn negative)
+    const unsigned whole = len & ~3, step = 4 * threads;
+    const int last = tid < len - (int)whole ? told[whole + tid] : -1;
+    i32x4 ids[kAhead];
+    ids[0] = first;
+    auto load = [&](unsigned i0, int u0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (u >= u0 && i0 + u * step < whole) ids[u] = *reinterpret_cast<const i32x4u*>(told + i0 + u * step);
+    };
+    load(4 * tid, 1);
+    if (counted) __syncthreads();
     if (biased) {
-        for (int i = tid; i < entries; i += threads) {
-            const unsigned at = (unsigned)(i == tid ? first_named : named[i]) - (unsigned)v0;  // (an id below 0 is past every slice)
-            if (at < (unsigned)n) PACKED ? atomicMax(&words[at], ((unsigned)i + 1u) << 16) : atomicMax(&entry[at], (unsigned)i + 1u);
+        for (unsigned i0 = tid; i0 < (unsigned)entries; i0 += kAhead * threads) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if ((u > 0 || i0 > (unsigned)tid) && i0 + u * threads < (unsigned)entries) id[u] = named[i0 + u * threads];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const unsigned i = i0 + u * threads;
+                const unsigned at = (unsigned)id[u] - (unsigned)v0;  // (an id below 0 is past every slice)
+                if (i < (unsigned)entries && at < (unsigned)n) PACKED ? atomicMax(&words[at], (i + 1u) << 16) : atomicMax(&entry[at], i + 1u);
+            }
         }
         if constexpr (PACKED) __syncthreads();  // the counts go below
     }
-    if (a.history) {
-        auto count = [&](int id, int i) {
-            const unsigned at = (unsigned)id - (unsigned)v0;
-            if (at < (unsigned)n) i < prompt ? atomicOr(&words[at], kPrompt) : atomicAdd(&words[at], 1u);
-        };
-        int i = tid * 4;
-        for (; i + 4 <= len; i += threads * 4) {
-            const i32x4 id = i == tid * 4 ? first : *reinterpret_cast<const i32x4u*>(told + i);
+    auto count = [&](int id, int i) {
+        const unsigned at = (unsigned)id - (unsigned)v0;
+        if (at < (unsigned)n) i < prompt ? atomicOr(&words[at], kPrompt) : atomicAdd(&words[at], 1u);
+    };
+    for (unsigned i0 = 4 * tid; i0 < whole; i0 += kAhead * step) {
+        if (i0 > 4u * tid) load(i0, 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) count(id[e], i + e);
+        for (int u = 0; u < kAhead; ++u) {
+            if (i0 + u * step < whole) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) count(ids[u][e], (int)(i0 + u * step) + e);
+            }
         }
-        for (; i < len; ++i) count(told[i], i);  // (the one thread that the last, shorter four fall to)
     }
+    if (tid < len - (int)whole) count(last, (int)whole + tid);
     if (counted) __syncthreads();
     const float* bias = a.bias_values + b * a.bias_stride;
     auto result = [&](float l, unsigned word, unsigned e, unsigned open) {
@@ -184,11 +210,12 @@ clove_status_t launch_penalize_logits(const LogitsArgs& a, hipStream_t stream) {
     if (st != CLOVE_OK) return st;
     const bool counted = a.history || a.bias_ids;
     const bool packed = !(a.history && a.history_stride >= 32768) && !(a.bias_ids && a.bias_stride >= 32768);
-    // Counting, the longest slices that still give two workgroups per CU: each reads
-    // the history (256 x 128000 fp32 without masks take 55 us with slices of 16384,
-    // 58 with 8192).  Otherwise the shortest, of which more are in flight (48 and 49).
-    int threads = !counted ? 256 : packed ? 1024 : 512;
-    while (threads > 256 && (int64_t)a.batch * hw::cdiv(a.vocab, threads * logits::kPer) < 2 * dev.num_cus) threads /= 2;
+    // Counting, slices of 8192 tokens: each reads the row's history, but more of them
+    // fill the CUs better (256 x 128000 and 64 x 152064 after 8000 and 4000 tokens: 53
+    // and 16 us, with 16384 52 and 18, with 4096 57 and 17.5).  Otherwise, and with
+    // fewer than two workgroups per CU, of 4096 (256 x 128000 47.6 and 49 us).
+    int threads = counted ? 512 : 256;
+    if ((int64_t)a.batch * hw::cdiv(a.vocab, threads * logits::kPer) < 2 * dev.num_cus) threads = 256;
     const int slice = threads * logits::kPer, slices = hw::cdiv(a.vocab, slice);
     const int apart = a.batch >= 8 ? 8 : 1;
     const int64_t grid = (int64_t)hw::cdiv(a.batch, apart) * apart * slices;
