@@ -12,7 +12,7 @@
 //
 // Accumulated weights need every head's final m and l, so the scores go to
 // scratch (fp32, one per query head and key) and a second kernel adds
-// sum_h 2^(t - m_h) / l_h to each key's weight: 8.5 of 48 us for 48 sequences of
+// sum_h 2^(t - m_h) / l_h to each key's weight: 5 of 45 us for 48 sequences of
 // up to 6144 keys (145 MB of cache, 9 MB of scores written and read again).
 #include <algorithm>
 
@@ -135,41 +135,53 @@ __global__ void __launch_bounds__(256) attend_any(const Params p) {
     if (p.stats && lane == 0) p.stats[(int64_t)b * a.q_heads + h] = float2{sub, sum};
 }
 
-// weights[b, j] += sum over the heads: 64 keys a workgroup, each by four threads
-// that sum a quarter of the heads in their order, 16 heads' scores in flight; the
-// quarters are added in theirs.
-constexpr int kAddKeys = 64;
-__global__ void __launch_bounds__(4 * kAddKeys) add_weights(const Params p, int blocks) {
-    constexpr int U = 16;
-    __shared__ float part[4][kAddKeys];
+// weights[b, j] += sum over the heads: 256 keys a workgroup, four adjacent ones a
+// lane, each wave an eighth of the heads in their order, four heads' scores in
+// flight; the eighths are added in theirs.  (48 sequences of up to 6144 keys, 32
+// heads: 45.6 us with the attention, 49 with a key to a thread and four parts; 100
+// of up to 2000 keys, 8 heads, 16.9 and 22.9.  Sixteen waves 46.1 to 47.)
+constexpr int kAddKeys = 256, kAddWaves = 8;
+__global__ void __launch_bounds__(64 * kAddWaves) add_weights(const Params p, int blocks) {
+    constexpr int U = 4;
+    __shared__ __align__(16) float part[kAddWaves][kAddKeys];
     const PagedAttentionArgs& a = p.a;
-    const int b = blockIdx.x / blocks, key = threadIdx.x % kAddKeys, quarter = threadIdx.x / kAddKeys;
-    const int j = (blockIdx.x - b * blocks) * kAddKeys + key;
+    const int b = blockIdx.x / blocks, j0 = (blockIdx.x - b * blocks) * kAddKeys;
+    const int wave = threadIdx.x / 64, four = threadIdx.x % 64 * 4, own = cdiv(a.q_heads, kAddWaves), h1 = min(a.q_heads, (wave + 1) * own);
     const int n = context(a, b), first = a.window > 0 ? max(0, n - a.window) : 0;
-    if (j - key >= n || j - key + kAddKeys <= first) return;
-    const bool seen = j >= first && j < n;
-    const int own = cdiv(a.q_heads, 4), h1 = min(a.q_heads, (quarter + 1) * own);
-    const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + j;
-    const float2* st = p.stats + (int64_t)b * a.q_heads;
+    if (j0 >= n || j0 + kAddKeys <= first) return;
+    const int j = j0 + threadIdx.x;
     float* const w = a.weights + b * a.weights_stride + j;
-    const float before = seen && quarter == 0 ? *w : 0.0f;
-    float sum = 0.0f;
-    for (int h0 = quarter * own; h0 < h1; h0 += U) {
-        float t[U];
+    const bool seen = threadIdx.x < kAddKeys && j >= first && j < n;
+    const float before = seen ? *w : 0.0f;
+    // (rows of scores are whole 32s; what lies before the first key or past the last is not used)
+    const float* s = p.scores + (int64_t)b * a.q_heads * p.score_stride + min(j0 + four, (int)p.score_stride - 4);
+    const float2* st = p.stats + (int64_t)b * a.q_heads;
+    f32x4 sum = {};
+    for (int h0 = wave * own; h0 < h1; h0 += U) {
+        f32x4 t[U];
         float2 ml[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = min(h0 + u, h1 - 1);
-            t[u] = seen ? s[(int64_t)h * p.score_stride] : -__builtin_inff();
+            t[u] = *reinterpret_cast<const f32x4*>(s + (int64_t)h * p.score_stride);
             ml[u] = st[h];
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (h0 + u < h1 && ml[u].y != 0.0f) sum += exp2_(t[u] - ml[u].x) / ml[u].y;
+        for (int u = 0; u < U; ++u) {
+            if (h0 + u < h1 && ml[u].y != 0.0f) {
+                ml[u].y = 1.0f / ml[u].y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_(t[u][i] - ml[u].x), ml[u].y, sum[i]);
+            }
+        }
     }
-    part[quarter][key] = sum;
+    *reinterpret_cast<f32x4*>(&part[wave][four]) = sum;
     __syncthreads();
-    if (seen && quarter == 0) *w = before + (((part[0][key] + part[1][key]) + part[2][key]) + part[3][key]);
+    if (!seen) return;
+    float total = part[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < kAddWaves; ++i) total += part[i][threadIdx.x];
+    *w = before + total;
 }
 
 template <int DT>
@@ -767,7 +779,7 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
     }
     if ((st = check_launch()) != CLOVE_OK || !p.scores) return st;
     const int blocks = hw::cdiv(a.max_context, paged::kAddKeys);
-    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(4 * paged::kAddKeys), 0, stream, p, blocks);
+    CLOVE_LAUNCH(paged::add_weights, dim3((unsigned)(blocks * a.batch)), dim3(64 * paged::kAddWaves), 0, stream, p, blocks);
     return check_launch();
 }
 
