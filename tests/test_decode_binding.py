@@ -1,0 +1,47 @@
+"""The compiled entry points of the decode step's operators, without a GPU: they load
+beside the library and refuse what they can judge on the host."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def _cg():
+    import clove_compute_amd as cg
+    return cg
+
+
+def _int(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def test_tensors_on_the_host_are_refused():
+    cg = _cg()
+    x = torch.ones(2, 64)
+    with pytest.raises(ValueError, match="on the GPU"):
+        cg.penalize_logits(x, x, 2, 64)
+    h = torch.zeros(2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="on the GPU"):
+        cg.qk_norm_rope(h, None, None, x, x, _int(2), h, 2, 1, 1, 16)
+    with pytest.raises(ValueError):
+        cg.KVCache(torch.zeros(1, 1, 4, 8, dtype=torch.float16), torch.zeros(1, 1, 4, 8, dtype=torch.float16))
+
+
+def test_what_is_no_tensor_or_number_is_refused():
+    cg = _cg()
+    x = torch.ones(2, 64)
+    for bad in (None, 3, [1.0], "x"):
+        with pytest.raises(TypeError, match="logits is not a tensor"):
+            cg.penalize_logits(bad, x, 2, 64)
+    with pytest.raises(TypeError):
+        cg.penalize_logits(x, x, 2.5, 64)
+    with pytest.raises(OverflowError):
+        cg.penalize_logits(x, x, 2 ** 31, 64)
+    with pytest.raises(AttributeError):
+        cg.paged_attention(x, object(), _int(2, 1), _int(2), x, 2, 1, 4)
+
+
+def test_entry_points_take_their_number_of_arguments():
+    from clove_compute_amd import decode
+    for f in (decode._b.rope, decode._b.attend, decode._b.evict, decode._b.penalize):
+        with pytest.raises(TypeError, match="arguments are wanted"):
+            f()
