@@ -205,9 +205,10 @@ void launch_any(const Params& p, hipStream_t stream) {
 // P^T operand of the second product, if its 8 k-slots of lane group g name the
 // keys 4 g .. 4 g + 3 of either 16.  So softmax needs no exchange but the
 // maximum over the four lane groups, and only V passes through LDS, private to
-// the wave, where ds_read_b64_tr_b16 turns its rows.  P is used as the sum of two
-// 16-bit numbers (16 bits in bf16, 22 in fp16), so that what a result loses is its
-// own rounding alone; the second product's MFMAs hide under the loads.
+// the wave, where ds_read_b64_tr_b16 turns its rows.  P is used as the sum of
+// 16-bit numbers, two in fp16 (22 bits) and three in bf16 (all 24), so that what a
+// result loses is its own rounding alone; the MFMAs of the further products hide
+// under the loads.
 //
 // Registers of K are loaded for the wave's next 32 keys as soon as the first
 // product has read them, those of V as soon as they are in LDS: 8 to 16 KB (at
@@ -247,6 +248,10 @@ __device__ __forceinline__ float groups_sum(float x) {
 }
 
 constexpr int kW = 4;  // waves of a workgroup
+
+// 16-bit numbers that a softmax weight is the sum of
+template <int DT>
+constexpr int kParts = DT == CLOVE_DTYPE_BF16 ? 3 : 2;
 
 template <int NC>
 constexpr int row_bytes() { return NC * 64 + 32; }  // a V row in LDS: 8 banks further each row
@@ -594,23 +599,27 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
                 for (int i = 0; i < 4; ++i) o[c][i] *= f;
             m = top;
         }
-        u32x4 hi, lo;
+        u32x4 w[kParts<DT>];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                const float x = exp2_(s[r][i] - sub), y = exp2_(s[r][i + 1] - sub);
+                float x = exp2_(s[r][i] - sub), y = exp2_(s[r][i + 1] - sub);
                 l += x + y;
-                const unsigned h = pack2<DT>(x, y);
-                hi[2 * r + i / 2] = h;
-                lo[2 * r + i / 2] = pack2<DT>(x - Elem<DT>::load((uint16_t)(h & 0xffffu)), y - Elem<DT>::load((uint16_t)(h >> 16)));
+#pragma unroll
+                for (int k = 0; k < kParts<DT>; ++k) {  // each part what the ones before it leave, rounded
+                    const unsigned h = pack2<DT>(x, y);
+                    w[k][2 * r + i / 2] = h;
+                    x -= Elem<DT>::load((uint16_t)(h & 0xffffu));
+                    y -= Elem<DT>::load((uint16_t)(h >> 16));
+                }
             }
 #pragma unroll
         for (int c = 0; c < 2 * NC; ++c) {
             const u32x2 x = lds_turned(turned + 32 * c), y = lds_turned(turned + 16 * row_bytes<NC>() + 32 * c);
             const u32x4 vt{x[0], x[1], y[0], y[1]};
-            o[c] = Mfma<DT>::mul(vt, hi, o[c]);
-            o[c] = Mfma<DT>::mul(vt, lo, o[c]);
+#pragma unroll
+            for (int k = 0; k < kParts<DT>; ++k) o[c] = Mfma<DT>::mul(vt, w[k], o[c]);
         }
     }
     l = groups_sum(l);
