@@ -206,9 +206,9 @@ void launch_any(const Params& p, hipStream_t stream) {
 // keys 4 g .. 4 g + 3 of either 16.  So softmax needs no exchange but the
 // maximum over the four lane groups, and only V passes through LDS, private to
 // the wave, where ds_read_b64_tr_b16 turns its rows.  P is used as the sum of
-// 16-bit numbers, two in fp16 (22 bits) and three in bf16 (all 24), so that what a
-// result loses is its own rounding alone; the MFMAs of the further products hide
-// under the loads.
+// 16-bit numbers, two in fp16 (22 bits, kPScale) and three in bf16 (all 24), so
+// that what a result loses is its own rounding alone; the MFMAs of the further
+// products hide under the loads.
 //
 // Registers of K are loaded for the wave's next 32 keys as soon as the first
 // product has read them, those of V as soon as they are in LDS: 8 to 16 KB (at
@@ -252,6 +252,14 @@ constexpr int kW = 4;  // waves of a workgroup
 // 16-bit numbers that a softmax weight is the sum of
 template <int DT>
 constexpr int kParts = DT == CLOVE_DTYPE_BF16 ? 3 : 2;
+// What it is multiplied by for them, taken out of the wave's sums after the keys.
+// fp16's steps end at 2^-24: of a weight 2^(t - m) <= 1 as it is, the two parts hold
+// fewer than 22 bits from 2^-3 down and nothing below 2^-25, and many keys far below
+// one whose value is small are then lost (4096 positive ones 2^-24 below it came out
+// 3e-3 off, and more the more they cancel).  Times 2^15 they are whole down to 2^-18, and what is lost of
+// any weight is at most 2^-40 of the wave's largest.
+template <int DT>
+constexpr float kPScale = DT == CLOVE_DTYPE_FP16 ? 32768.0f : 1.0f;
 
 template <int NC>
 constexpr int row_bytes() { return NC * 64 + 32; }  // a V row in LDS: 8 banks further each row
@@ -606,6 +614,8 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
             for (int i = 0; i < 4; i += 2) {
                 float x = exp2_(s[r][i] - sub), y = exp2_(s[r][i + 1] - sub);
                 l += x + y;
+                x *= kPScale<DT>;
+                y *= kPScale<DT>;
 #pragma unroll
                 for (int k = 0; k < kParts<DT>; ++k) {  // each part what the ones before it leave, rounded
                     const unsigned h = pack2<DT>(x, y);
@@ -623,6 +633,12 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
         }
     }
     l = groups_sum(l);
+    if constexpr (kPScale<DT> != 1.0f) {
+#pragma unroll
+        for (int c = 0; c < 2 * NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[c][i] *= 1.0f / kPScale<DT>;
+    }
 
     // the waves, merged in their order
     __syncthreads();

@@ -75,3 +75,31 @@ def test_weights_keep_their_bits(dtype, half, n):
     tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
     bound = half * np.abs(want) * 1.0001 + tiny + 10.1 * 2.0 ** -24 * b * p[:, None] / (1 + p[:, None])
     assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) - bound))
+
+
+@pytest.mark.parametrize("dtype,half", [("fp16", 2.0 ** -11), ("bf16", 2.0 ** -8)])
+@pytest.mark.parametrize("n,below", [(30, 15), (200, 14), (500, 12), (500, 14), (500, 16), (500, 20), (4096, 16), (4096, 18), (4096, 24), (40000, 18),
+                                     (40000, 25)])
+def test_weights_far_below_the_largest(dtype, half, n, below):
+    """One key `below` above the others in base 2, its value 0: the output is what the
+    others' weights of about 2^-below bring, judged relative to itself.
+
+    A weight is off by 3 roundings of its score's factors (|t| < below + 1, times
+    ln 2) and one of the exponential; fp16 holds it to 2^-40 of the largest; a lane
+    or a matrix product adds at most 2048 of them one after the other, and joins of
+    up to 400 parts follow, 2^-24 each.
+    """
+    H, D = 4, 64
+    scale = float(np.float32(np.log(2.0)))
+    g = np.random.default_rng(n + below)
+    q, k = np.zeros((H, D)), np.zeros((H, n, D))
+    q[:, 0] = 1.0
+    k[:, :, 0] = -(below + g.integers(0, 8, (H, n)) / 8.0)
+    v = g.uniform(2.0, 6.0, (H, n, D))
+    at = n // 3
+    k[:, at, 0], v[:, at] = 0.0, 0.0
+    got, q64, (k64, v64), table = _run(dtype, q, k, v, n, scale)
+    want = ref.attention(q64, k64, v64, table, [n], scale)[0][0]
+    slack = (3 * (below + 1) * 0.694 + 2 + min(n, 2048) + 400) * 2.0 ** -24 + (2.0 ** (below + 1 - 40) if dtype == "fp16" else 0.0)
+    bound = (half * 1.0001 + slack) * np.abs(want) + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    assert np.all(np.abs(got - want) <= bound), float(np.max(np.abs(got - want) / np.abs(want)))
