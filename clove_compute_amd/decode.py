@@ -54,12 +54,16 @@ class KVCache:
     Keeps the tensors; a program makes one per layer and keeps it."""
 
     def __init__(self, k, v):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not (k.is_cuda and v.is_cuda):
-            raise ValueError("k and v are GPU tensors [num_pages, kv_heads, page_size, head_dim] of one shape and type")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v are tensors [num_pages, kv_heads, page_size, head_dim] of one shape and type")
         if k.shape[0] and not (k[0].is_contiguous() and v[0].is_contiguous()):
             raise ValueError("the pages of k and v must be dense")
         if k.shape[0] > 1 and k.stride(0) != v.stride(0):
             raise ValueError("the pages of k and v must be equally far apart")
+        if k.shape[0] > 1 and k.stride(0) < k[0].numel():  # (the library takes 0 for dense pages)
+            raise ValueError("the pages of k and v must lie apart: an expanded tensor has one page only")
+        if not (k.is_cuda and v.is_cuda):
+            raise ValueError("k and v must be on the GPU")
         if str(k.dtype) not in _CODES:
             raise ValueError(f"element type {k.dtype} is not fp16, bf16 or fp32")
         self.k, self.v = k, v

@@ -45,3 +45,18 @@ def test_entry_points_take_their_number_of_arguments():
     for f in (decode._b.rope, decode._b.attend, decode._b.evict, decode._b.penalize):
         with pytest.raises(TypeError, match="arguments are wanted"):
             f()
+
+
+def test_caches_of_pages_that_lie_on_each_other_are_refused():
+    """An expanded tensor's pages are all one: the library would take its distance, 0,
+    for that of dense pages and go past its end."""
+    cg = _cg()
+    page = torch.zeros(1, 2, 4, 8, dtype=torch.float16)
+    with pytest.raises(ValueError, match="lie apart"):
+        cg.KVCache(page.expand(5, -1, -1, -1), page.expand(5, -1, -1, -1))
+    near = torch.zeros(200, dtype=torch.float16).as_strided((3, 2, 4, 8), (63, 32, 8, 1))
+    with pytest.raises(ValueError, match="lie apart"):
+        cg.KVCache(near, near)
+    for fine in (page.expand(1, -1, -1, -1), torch.zeros(3, 2, 4, 8, dtype=torch.float16), torch.zeros(3, 2, 2, 4, 8, dtype=torch.float16)[:, 1]):
+        with pytest.raises(ValueError, match="on the GPU"):  # (nothing else is wrong with it)
+            cg.KVCache(fine, fine)
