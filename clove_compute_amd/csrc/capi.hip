@@ -43,6 +43,25 @@ struct BufferEntry {
 };
 std::map<std::tuple<int, void*, int>, BufferEntry> g_buffers;  // guarded by g_scratch_mu
 
+// A call whose launches hand each other data through these buffers (a selection
+// and its moves, scores and the weights added up from them, a repacked operand
+// and its GEMM) has the stream's to itself from the first acquisition to its end:
+// another host thread's launches on the stream would come between its own and
+// write what they are still to read.  The locks stay for good.
+std::map<std::pair<int, void*>, std::mutex> g_stream_mu;  // the map guarded by g_scratch_mu
+thread_local std::unique_lock<std::mutex> t_stream;       // of the current call; let go by CallScope
+
+// (never taken inside g_scratch_mu, which is taken inside it)
+void hold_stream(int dev, hipStream_t stream) {
+    if (t_stream.owns_lock()) return;
+    std::mutex* mu;
+    {
+        std::lock_guard<std::mutex> lk(g_scratch_mu);
+        mu = &g_stream_mu[{dev, reinterpret_cast<void*>(stream)}];
+    }
+    t_stream = std::unique_lock<std::mutex>(*mu);
+}
+
 // Buffers replaced by larger ones, per device, freed by clove_release_scratch
 // (after a device synchronize).  A replaced buffer is not freed on the spot: a
 // call on another host thread may have taken it and not yet launched the
@@ -157,10 +176,12 @@ clove_status_t ws_carve(size_t bytes, char** out) {
 }
 
 // One per C entry point that dispatches: starts the call's carving after the
-// counters and, in a query, records what the call took.
+// counters and, in a query, records what the call took; at its end, when all of
+// the call is queued, the stream's library buffers are other threads' again.
 struct CallScope {
     CallScope() { t_ws.used = kWsCounterBytes; }
     ~CallScope() {
+        if (t_stream.owns_lock()) t_stream.unlock();
         if (t_ws.mode == WsMode::kQuery && t_ws.used > kWsCounterBytes && t_ws.used > t_ws.need)
             t_ws.need = t_ws.used;
     }
@@ -232,6 +253,7 @@ clove_status_t acquire_scratch(hipStream_t stream, size_t partial_bytes, size_t 
     }
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return CLOVE_ERR_NO_DEVICE;
+    hold_stream(dev, stream);
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     ScratchEntry& e = g_scratch[{dev, reinterpret_cast<void*>(stream)}];
     if (e.base && e.view.partial_bytes >= partial_bytes && e.view.num_counters >= num_counters) {
@@ -277,6 +299,7 @@ clove_status_t acquire_buffer(hipStream_t stream, int slot, size_t bytes, void**
     }
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return CLOVE_ERR_NO_DEVICE;
+    hold_stream(dev, stream);
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     BufferEntry& e = g_buffers[std::make_tuple(dev, reinterpret_cast<void*>(stream), slot)];
     if (e.base && e.bytes >= bytes) {

@@ -18,7 +18,10 @@
  * needs more scratch than the stream holds allocates a larger buffer (twice
  * the size or more) and keeps the old one until clove_release_scratch(), so
  * that calls of other host threads on the same stream that already took it
- * stay valid; no call synchronises a stream.
+ * stay valid; no call synchronises a stream.  Host threads may issue calls on
+ * one stream at once: those that use the library's scratch queue all of their
+ * launches before another thread's begins.  (A bound workspace is the caller's:
+ * one for each thread and stream.)
  */
 #ifndef CLOVE_GEMM_C_H
 #define CLOVE_GEMM_C_H
