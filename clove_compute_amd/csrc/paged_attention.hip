@@ -256,8 +256,8 @@ constexpr int kParts = DT == CLOVE_DTYPE_BF16 ? 3 : 2;
 // fp16's steps end at 2^-24: of a weight 2^(t - m) <= 1 as it is, the two parts hold
 // fewer than 22 bits from 2^-3 down and nothing below 2^-25, and many keys far below
 // one whose value is small are then lost (4096 positive ones 2^-24 below it came out
-// 3e-3 off, and more the more they cancel).  Times 2^15 they are whole down to 2^-18, and what is lost of
-// any weight is at most 2^-40 of the wave's largest.
+// 3e-3 off, and more the more they cancel).  Times 2^15 they are whole down to
+// 2^-18, and what is lost of any weight is at most 2^-40 of the wave's largest.
 template <int DT>
 constexpr float kPScale = DT == CLOVE_DTYPE_FP16 ? 32768.0f : 1.0f;
 
@@ -289,6 +289,13 @@ __device__ __forceinline__ u32x2 lds_turned(const char* p) {
 template <int DT>
 __device__ __forceinline__ unsigned pack2(float lo, float hi) {
     return (unsigned)Elem<DT>::store(lo) | ((unsigned)Elem<DT>::store(hi) << 16);
+}
+
+// All bits of those of two elements that are infinite or NaN.
+template <int DT>
+__device__ __forceinline__ unsigned nonfinite2(unsigned x) {
+    constexpr unsigned exponent = DT == CLOVE_DTYPE_FP16 ? 0x7c007c00u : 0x7f807f80u, one = DT == CLOVE_DTYPE_FP16 ? 0x04000400u : 0x00800080u;
+    return ((((x & exponent) + one) >> 15) & 0x00010001u) * 0xffffu;
 }
 
 // Four outputs of one row from element d.
@@ -454,8 +461,15 @@ __device__ __forceinline__ void join_all(const Params& p, const __amdgpu_buffer_
     }
 }
 
+// Workgroups of four waves that a CU holds at once, by head_dim / 32: what the
+// registers leave, which are bounded to it (a workgroup has one wave on each SIMD;
+// rows at any alignment hold one fewer at 6)
+constexpr int kResident[8] = {5, 4, 3, 2, 2, 2, 1, 1};
+template <int NC, bool TAIL, int W>
+constexpr int resident() { return W == kW ? kResident[NC - 1] - (TAIL && NC == 6 ? 1 : 0) : 1; }
+
 template <int DT, int NC, bool TAIL, int W>
-__global__ void __launch_bounds__(64 * W) attend(const Params p) {
+__global__ void __launch_bounds__(64 * W, (resident<NC, TAIL, W>())) attend(const Params p) {
     extern __shared__ __align__(16) char lds[];
     __shared__ int last;
     const PagedAttentionArgs& a = p.a;
@@ -632,6 +646,71 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
             for (int k = 0; k < kParts<DT>; ++k) o[c] = Mfma<DT>::mul(vt, w[k], o[c]);
         }
     }
+    // An infinite value times a weight is infinite, but not times a weight's parts, some
+    // of which are 0 or negative.  So where a sum comes out infinite or NaN, which is
+    // seldom, the wave goes over its keys again for such values alone: times 1 for a
+    // weight above 0, times the weight where that is 0 or NaN.
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 2 * NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = fmaf(o[c][i], 0.0f, z[i]);
+    const float any = (z[0] + z[1]) + (z[2] + z[3]);
+    if (__builtin_expect(__any(any != any), 0)) {
+        f32x4 special[2 * NC];
+#pragma unroll
+        for (int c = 0; c < 2 * NC; ++c) special[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float sub = finite_max(m);
+#pragma unroll 1
+        for (j = begin + 32 * wave; j < end; j += 32 * W) {
+            look_up(j);
+            resolve(j);
+            if (!seen_next) continue;
+            load(k, cache.k);
+            clip(k);
+            f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s[0] = Mfma<DT>::mul(k[0][c], q[c], s[0]);
+                s[1] = Mfma<DT>::mul(k[1][c], q[c], s[1]);
+            }
+            u32x4 there;
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    float x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool in = (seen_next >> (16 * r + 4 * g + i + e)) & 1u;
+                        x[e] = in ? exp2_(base2(a, s[r][i + e]) - sub) : 0.0f;
+                        x[e] = x[e] > 0.0f ? 1.0f : x[e];
+                    }
+                    there[2 * r + i / 2] = pack2<DT>(x[0], x[1]);
+                }
+            load(v, cache.v);
+            clip(v);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const bool in = (seen_next >> (16 * r + row)) & 1u;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[r][c][i] &= in ? nonfinite2<DT>(v[r][c][i]) : 0u;
+                    *reinterpret_cast<u32x4*>(vs + (16 * r + row) * row_bytes<NC>() + 64 * c + 16 * g) = v[r][c];
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NC; ++c) {
+                const u32x2 x = lds_turned(turned + 32 * c), y = lds_turned(turned + 16 * row_bytes<NC>() + 32 * c);
+                special[c] = Mfma<DT>::mul(u32x4{x[0], x[1], y[0], y[1]}, there, special[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[c][i] = special[c][i] != 0.0f ? special[c][i] : o[c][i];
+    }
     l = groups_sum(l);
     if constexpr (kPScale<DT> != 1.0f) {
 #pragma unroll
@@ -687,11 +766,6 @@ __global__ void __launch_bounds__(64 * W) attend(const Params p) {
     if (!splitk_arrive_is_last(p.counters + pair, count, &last)) return;
     join_all(p, slabs, lds, from, step, count, quads, items, finish);
 }
-
-// Workgroups of the MFMA kernel that a CU holds at once, by head_dim / 32: what
-// its registers leave (a workgroup has one wave on each SIMD; rows at any
-// alignment hold one fewer at 3 and 6)
-constexpr int kResident[8] = {5, 4, 3, 2, 2, 2, 1, 1};
 
 constexpr int kWide = 8;  // waves of the wide form, for head_dim up to 128 (registers)
 

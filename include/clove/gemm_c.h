@@ -322,6 +322,10 @@ clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const voi
  *   weights[b, j] += sum over the heads of p_j      for every key it sees.
  * q, out [batch, q_heads, head_dim] (rows q_stride / out_stride apart) are the
  * cache's dtype.  Cache rows that no key names are not used, whatever they hold.
+ * An infinite value makes its element of the result infinite (values of both
+ * signs, or a weight of 0, make it NaN).  The weights enter the sum over the
+ * values with 24 bits from a BF16 cache and 22 from an FP16 one, whose weights
+ * are held to 2^-40 of the largest; below 2^-126 of it they are 0.
  * max_context bounds the lengths on the host: it is at most table_stride *
  * page_size (and weights_stride), and a row of the table has ceil(max_context /
  * page_size) entries, of which those past the length may be anything.  The work
