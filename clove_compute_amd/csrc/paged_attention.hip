@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "decode.hpp"
+#include "paged_plan.hpp"
 
 namespace clove {
 namespace paged {
@@ -247,8 +248,6 @@ __device__ __forceinline__ float groups_sum(float x) {
     return swap_sum32(y, y);
 }
 
-constexpr int kW = 4;  // waves of a workgroup
-
 // 16-bit numbers that a softmax weight is the sum of
 template <int DT>
 constexpr int kParts = DT == CLOVE_DTYPE_BF16 ? 3 : 2;
@@ -321,13 +320,10 @@ __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, fl
 }
 
 // How the kernel shares out the keys: into `chunk`s of so many 32s of keys that
-// there are about `fill` of them (per KV head and tile), or several times that
-// where they would be longer than kLongest, a sequence's chunks of one length.
+// there are about `fill` of them (with KV heads and tiles), a sequence's of one length.
 // Every wave works it out for itself from the lengths, 64 sequences at a time.
 // (By the bound of the lengths alone, most workgroups of 48 mixed sequences had no
 // keys, and those that had some waited for them to pass: 55 us instead of 49.)
-constexpr int kLongest = 64;  // x 32 keys
-
 struct Cut {
     int b, split, total;     // this workgroup's sequence, its split and how many it has
     int first;               // workgroup of split 0 among those of all sequences, before KV heads and tiles
@@ -350,16 +346,13 @@ __device__ __forceinline__ Cut cut(const Params& p, int i, int per) {
         if (b0 == 0) t0 = t;
         sum += wave_sum(t);
     }
-    const int64_t all = (int64_t)sum * per;
-    const int64_t rounds = max((int64_t)1, (all + (int64_t)p.fill * kLongest - 1) / ((int64_t)p.fill * kLongest));
-    const int64_t want = (all + p.fill * rounds - 1) / (p.fill * rounds);
-    const int chunk = max(kW, (int)((want + kW - 1) / kW) * kW);  // a wave takes every fourth of them
+    const int chunk = chunk_of(sum, per, p.fill);
     int before = 0;
     Cut c{-1, 0, 0, 0, 0};
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const bool on = b0 + lane < a.batch;
         const int t = b0 == 0 ? t0 : on ? keys32(a, context(a, b0 + lane)) : 0;
-        const int splits = on ? max(1, cdiv(t, chunk)) : 0, upto = before + wave_scan(splits);
+        const int splits = on ? splits_of(t, chunk) : 0, upto = before + wave_scan(splits);
         const unsigned long long in = __ballot(on && i >= upto - splits && i < upto);
         if (in) {
             const int who = __ffsll((long long)in) - 1;
@@ -367,8 +360,7 @@ __device__ __forceinline__ Cut cut(const Params& p, int i, int per) {
             c.total = __builtin_amdgcn_readlane(splits, who);
             c.first = __builtin_amdgcn_readlane(upto, who) - c.total;
             c.split = i - c.first;
-            const int own = cdiv(__builtin_amdgcn_readlane(t, who), c.total);
-            c.chunk = cdiv(own, kW) * kW;
+            c.chunk = own_chunk(__builtin_amdgcn_readlane(t, who), c.total);
             return c;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
@@ -856,19 +848,16 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         // twice as many keys are better split (7.75 against 8.2)
         const bool wide = !alone && whole && c.head_dim <= 128 && span > 32 * paged::kW && span <= 32 * paged::kWide;
         const int waves = alone ? 1 : wide ? paged::kWide : paged::kW;
-        // chunks: the CUs' fill a whole number of rounds, and a remainder of each
-        // sequence, but no more than whole sequences make of the shortest chunks
-        const int64_t rounds = std::max<int64_t>(1, hw::cdiv64(pairs * hw::cdiv(span, 32), (int64_t)p.fill * paged::kLongest));
-        const int64_t slots = std::min((hw::cdiv64(p.fill * rounds, per) + a.batch) * per, pairs * hw::cdiv(span, 32 * paged::kW));
         p.slab = 16 * hw::cdiv(c.head_dim, 4) * 4 + 32;
         p.slots = (int)pairs;
-        p.cuts = waves == paged::kW && span > 32 * paged::kW && pairs + slots <= 16384 && 2 * slots * p.slab * 4 < (1 << 30);
+        const paged::Plan plan = paged::plan(a.batch, per, span, p.fill);
+        p.cuts = waves == paged::kW && plan.cuts;
         if (p.cuts) {
-            p.slots = (int)slots;
+            p.slots = (int)plan.slots;
             // what a workgroup reads in about 3 us; another round of arrivals takes as long
             p.fan = std::max(16, std::min(64, (128 << 10) / (std::min(p.group, 16) * c.head_dim * 4)));
             Scratch scratch;
-            if ((st = acquire_scratch(stream, (size_t)2 * p.slots * p.slab * 4, (size_t)(pairs + slots), &scratch)) != CLOVE_OK) return st;
+            if ((st = acquire_scratch(stream, (size_t)2 * p.slots * p.slab * 4, (size_t)(pairs + p.slots), &scratch)) != CLOVE_OK) return st;
             p.partials = scratch.partials;
             p.counters = scratch.counters;
         }
