@@ -831,11 +831,16 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         const int64_t pairs = (int64_t)a.batch * per;
         // a window need not start at a whole 32 keys
         const int span = std::max(1, a.window > 0 ? (int)std::min<int64_t>(a.max_context, (int64_t)a.window + 31) : a.max_context);
-        // one sequence: its chunks are all alike, and fewer of them are fewer to join
-        // (65536 keys 58.3 -> 55.8 us, 8192 20.5 -> 17.2); of mixed sequences more
-        // fill the CUs better (48.2 against 52.9 us), as do rows at any alignment,
-        // whose loads are slower (51 against 78)
-        p.fill = dev.num_cus * (a.batch == 1 && whole ? (c.head_dim <= 64 ? 2 : 1) : paged::kResident[hw::cdiv(c.head_dim, 32) - 1]);
+        // Few sequences: fewer chunks are fewer to join.  One of 65536 keys 58.3 -> 55.8
+        // us, of 8192 20.5 -> 17.2.  Up to eight at head_dim 64, two of four workgroups a
+        // CU: 4 x 2048, 8192, 32768 keys 12.3, 24.6, 51.0 -> 12.4, 18.9, 46.1, lengths of
+        // 32768 down by halves 30.2 -> 26.7; past that mixed sequences want them all (48
+        // with weights 45.6 against 49.6, though 48 x 32768 564 -> 543).  Of longer rows
+        // one instead of two is for one sequence only: 4 x 32768 keys of 128 103.8 -> 97.6,
+        // but the halves 47.9 -> 62.8.  Rows at any alignment, whose loads are slower, want
+        // all too (51 against 78).
+        const bool fewer = whole && a.batch <= (c.head_dim <= 64 ? 8 : 1);
+        p.fill = dev.num_cus * (fewer ? (c.head_dim <= 64 ? 2 : 1) : paged::kResident[hw::cdiv(c.head_dim, 32) - 1]);
         // One wave to a workgroup: nothing to merge where the keys are one wave's anyway
         // and its heads' outputs few (one sequence of 20 keys, head_dim 64, 4.7 -> 4.3
         // us; with 16 heads of 256 13.1 -> 15.4), and where there are more sequences of
