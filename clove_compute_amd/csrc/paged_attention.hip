@@ -337,14 +337,16 @@ __device__ __forceinline__ int keys32(const PagedAttentionArgs& a, int n) {
 
 // Sequence and split of workgroup `i` (of those before KV heads and tiles);
 // .b < 0 where there are fewer.
+static_assert(CLOVE_MAX_CONTEXT / 32 <= 0xffffffff / 64, "a wave's sum of lengths has 32 bits");
 __device__ __forceinline__ Cut cut(const Params& p, int i, int per) {
     const PagedAttentionArgs& a = p.a;
     const int lane = threadIdx.x & 63;
-    int sum = 0, t0 = 0;
+    int64_t sum = 0;
+    int t0 = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int t = b0 + lane < a.batch ? keys32(a, context(a, b0 + lane)) : 0;
         if (b0 == 0) t0 = t;
-        sum += wave_sum(t);
+        sum += wave_sum((unsigned)t);  // (64 of at most 2^25)
     }
     const int chunk = chunk_of(sum, per, p.fill);
     int before = 0;

@@ -89,3 +89,14 @@ def test_no_more_workgroups_than_planned_and_every_key(L):
             total += s
         assert total * per <= slots, (B, per, longest, D, kind)
     assert seen == {True, False}
+
+
+def test_more_keys_than_32_bits_count(L):
+    """64 sequences of the longest context: 2^31 32s of keys."""
+    t = (1 << 30) // 32
+    c = L.chunk(64 * t, 1, FILL[128])
+    assert c == -(-64 * t // FILL[128] // 4) * 4 and 64 * L.splits(t, c) <= plan(L, 64, 1, 1 << 30, 128)[1]
+    # in the kernel as well: a wave's sum is unsigned, and added up in 64 bits
+    with open(os.path.join(CSRC, "paged_attention.hip")) as f:
+        code = f.read()
+    assert "int64_t sum = 0;" in code and "sum += wave_sum((unsigned)t);" in code
