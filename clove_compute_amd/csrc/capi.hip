@@ -122,6 +122,10 @@ bool overlaps(const Rows& a, const Rows& b) {
     return off < a.width || a.stride - off < b.width;
 }
 
+// Whether an output is its input: the same rows.  (How far apart a single row would
+// have its next one does not matter.)
+bool same_rows(const Rows& a, const Rows& b) { return a.p == b.p && (a.stride == b.stride || (a.rows <= 1 && b.rows <= 1)); }
+
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -696,7 +700,7 @@ clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const voi
                           {positions, 0, (int64_t)T * 4, 1}, {slots, 0, (int64_t)T * 4, 1}};
     for (int o = 0; o < 4; ++o) {
         for (int i = 0; i < 3; ++i) {
-            const bool own = o == i && outs[o].p == in[i].p && outs[o].stride == in[i].stride;
+            const bool own = o == i && same_rows(outs[o], in[i]);
             if (!own && overlaps(outs[o], in[i])) return CLOVE_ERR_ALIASING;
         }
         for (const Rows& r : small)
@@ -803,7 +807,7 @@ clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* b
                          cache_rows(a.cache, a.cache.v)};
     for (int o = 0; o < 5; ++o) {
         for (int i = 0; i < 4; ++i) {
-            const bool own = o == i && outs[o].p == in[i].p && outs[o].stride == in[i].stride;
+            const bool own = o == i && same_rows(outs[o], in[i]);
             if (!own && overlaps(outs[o], in[i])) return CLOVE_ERR_ALIASING;
         }
         for (int i = 0; i < o; ++i)
@@ -849,7 +853,7 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
         return CLOVE_ERR_INVALID_ARG;
     const int64_t per = (int64_t)batch * 4;
     const Rows o{out, out_stride * os, (int64_t)vocab * os, batch}, x{logits, logits_stride * is, (int64_t)vocab * is, batch};
-    const bool own = out == logits && os == is && out_stride == logits_stride;
+    const bool own = os == is && same_rows(o, x);
     if (!own && overlaps(o, x)) return CLOVE_ERR_ALIASING;
     const Rows in[] = {{history, history_stride * 4, history_stride * 4, batch}, {history_lens, 0, per, 1},
                        {prompt_lens, 0, per, 1}, {repetition, 0, per, 1}, {presence, 0, per, 1}, {frequency, 0, per, 1},

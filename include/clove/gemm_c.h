@@ -297,9 +297,9 @@ typedef struct clove_kv_cache {
  * padding token) is not written; two tokens of one call must not name the same
  * slot.  A position outside [0, max_position) makes that token's q and k NaN
  * (rot_dim > 0).  q_out / k_out may be the queries / keys of qkv themselves
- * (same rows, same stride), else outputs must not overlap inputs.  rot_dim is
- * even and at most head_dim; with rot_dim 0 the tables and positions are not
- * read.  T == 0 is a no-op.
+ * (same rows; of several the same stride), else outputs must not overlap inputs.
+ * rot_dim is even and at most head_dim; with rot_dim 0 the tables and positions
+ * are not read.  T == 0 is a no-op.
  */
 clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const void* q_weight,
                                   const void* k_weight, float eps, const float* rope_cos,
@@ -355,10 +355,10 @@ clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clov
  *   lens_out[b]            min(n, budget)
  *   weights_out[b, i], positions_out[b, i]   of the slots as they are then; 0
  *                          and -1 for lens_out[b] <= i < max_context
- * Each output may be its input (same address and stride).  A row whose page
- * lies outside the cache is not copied.  Sequences must not share pages, or
- * have a page twice.  A second call with the same inputs moves the same rows
- * again and changes nothing.
+ * Each output may be its input (same rows; of several the same stride).  A row
+ * whose page lies outside the cache is not copied.  Sequences must not share
+ * pages, or have a page twice.  A second call with the same inputs moves the same
+ * rows again and changes nothing.
  */
 clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* block_table,
                                  int64_t table_stride, const int32_t* context_lens,
@@ -386,7 +386,8 @@ clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* b
  * long, any of which may be read; lengths are taken as at least 0 and at most
  * that.  Ids outside [0, vocab) are ignored.  logits are `dtype` (FP16, BF16 or
  * FP32), out is `out_dtype` (the same, or FP32), rows logits_stride / out_stride
- * elements apart; out may be logits itself where dtype and stride agree.
+ * elements apart; out may be logits itself where dtype and (of several rows)
+ * stride agree.
  */
 clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, int dtype, void* out,
                                      int64_t out_stride, int out_dtype, int batch, int vocab,

@@ -107,3 +107,29 @@ def test_logits_refusals(L):
         assert call(f, LOGITS, **bad) == status, bad
     assert call(f, LOGITS, batch=0, logits=None) == OK
     assert call(f, LOGITS, vocab=0, out=None) == OK
+
+
+def _planned(L, f, args, **kw):
+    """The status of a call that is only planned: nothing is launched, so that the fake
+    addresses are safe where there is a GPU too."""
+    assert L.clove_workspace_query_begin() == OK
+    try:
+        return call(f, args, **kw)
+    finally:
+        L.clove_workspace_query_end()
+
+
+TAKEN = (OK, _lib.CLOVE_ERR_NO_DEVICE)  # (planning asks for the device, last)
+
+
+def test_a_single_row_is_its_own_output_whatever_its_stride(L):
+    one = dict(qkv=X, q_out=X, k_out=X + 512)
+    for strides in [dict(), dict(q_out_stride=512, k_out_stride=512), dict(q_out_stride=300, k_out_stride=128, qkv_stride=700)]:
+        assert _planned(L, L.clove_qk_norm_rope, ROPE, T=1, **one, **strides) in TAKEN, strides
+    assert _planned(L, L.clove_qk_norm_rope, ROPE, T=1, q_out=X + 2) == ALIASING
+    assert _planned(L, L.clove_qk_norm_rope, ROPE, T=2, **one) == ALIASING
+    own = dict(cache=cache(), weights_out=W, positions_out=X, weights_out_stride=100, positions_out_stride=101)
+    assert _planned(L, L.clove_cache_evict, EVICT, batch=1, **own) in TAKEN
+    assert _planned(L, L.clove_cache_evict, EVICT, batch=2, **own) == ALIASING
+    assert _planned(L, L.clove_penalize_logits, LOGITS, batch=1, out=X, out_stride=1001) in TAKEN
+    assert _planned(L, L.clove_penalize_logits, LOGITS, batch=1, out=X, out_dtype=2) == ALIASING

@@ -926,3 +926,20 @@ def test_attention_lengths_around_the_forms_of_the_kernel(dtype, D):
         out = _attend(cg, q, cg.KVCache(k, v), table, lens, 4, Hq, longest, weights=w)
         _close(out, want, dtype, 3e-5 * float(np.abs(v64).max()))
         assert np.all(np.abs(_f64(w) - added[:, :longest]) <= 3e-5 * added[:, :longest] + 1e-9)
+
+
+@pytest.mark.parametrize("dtype,D", [("fp16", 64), ("bf16", 36)])
+def test_rope_in_place_of_one_token(dtype, D):
+    """Queries and keys of a single row rotated where they are."""
+    cg = _cg()
+    Hq, Hk = 4, 2
+    g = rng("rope-one", D)
+    x, x64 = _rounded(g, dtype, 1, (Hq + 2 * Hk) * D)
+    w, w64 = _rounded(g, dtype, D)
+    cos, sin = _tables(20, D)
+    pos = np.array([7], np.int32)
+    q64, k64, v64 = ref.qk_norm_rope(x64, w64, w64, cos, sin, pos, Hq, Hk, D, D, 1e-6, False)
+    cg.qk_norm_rope(x, w, w, _dev(cos), _dev(sin), _dev(pos), x[:, :Hq * D], 1, Hq, Hk, D, k_out=x[:, Hq * D:(Hq + Hk) * D])
+    _close(x[:, :Hq * D], q64.reshape(1, -1), dtype, 1e-5)
+    _close(x[:, Hq * D:(Hq + Hk) * D], k64.reshape(1, -1), dtype, 1e-5)
+    assert np.array_equal(_f64(x)[:, (Hq + Hk) * D:], v64.reshape(1, -1))
