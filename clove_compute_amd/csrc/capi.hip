@@ -659,6 +659,9 @@ static Rows cache_rows(const PagedCache& c, const void* p) {
     return Rows{p, c.page_stride * 2, (int64_t)c.kv_heads * c.page_size * c.head_dim * 2, c.num_pages};
 }
 
+// The entries of a table's row, which may be part of a wider one
+static int64_t table_bytes(int max_context, const PagedCache& c) { return hw::cdiv64(max_context, c.page_size) * 4; }
+
 clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const void* q_weight, const void* k_weight,
                                   float eps, const float* rope_cos, const float* rope_sin, int max_position,
                                   const int32_t* positions, void* q_out, int64_t q_out_stride, void* k_out,
@@ -752,7 +755,7 @@ clove_status_t clove_paged_attention(const void* q, int64_t q_stride, const clov
     if (!aligned2(q) || !aligned2(out) || !aligned4(block_table) || !aligned4(context_lens) || !aligned4(weights))
         return CLOVE_ERR_INVALID_ARG;
     const Rows in[] = {{q, q_stride * 2, width * 2, batch}, cache_rows(a.cache, a.cache.k), cache_rows(a.cache, a.cache.v),
-                       {block_table, table_stride * 4, table_stride * 4, batch}, {context_lens, 0, (int64_t)batch * 4, 1}};
+                       {block_table, table_stride * 4, table_bytes(max_context, a.cache), batch}, {context_lens, 0, (int64_t)batch * 4, 1}};
     const Rows outs[] = {{out, out_stride * 2, width * 2, batch}, {weights, weights_stride * 4, (int64_t)max_context * 4, batch}};
     for (const Rows& o : outs)
         for (const Rows& i : in)
@@ -799,7 +802,7 @@ clove_status_t clove_cache_evict(const clove_kv_cache_t* cache, const int32_t* b
         return CLOVE_ERR_INVALID_ARG;
     const int64_t row = (int64_t)max_context * 4, ints = (int64_t)batch * 4;
     const Rows in[] = {{weights, weights_stride * 4, row, batch}, {positions, positions_stride * 4, row, batch},
-                       {context_lens, 0, ints, 1}, {block_table, table_stride * 4, table_stride * 4, batch}};
+                       {context_lens, 0, ints, 1}, {block_table, table_stride * 4, table_bytes(max_context, a.cache), batch}};
     const Rows outs[] = {{weights_out, weights_out_stride * 4, row, batch},
                          {positions_out, positions_out_stride * 4, row, batch},
                          {lens_out, 0, ints, 1},

@@ -133,3 +133,14 @@ def test_a_single_row_is_its_own_output_whatever_its_stride(L):
     assert _planned(L, L.clove_cache_evict, EVICT, batch=2, **own) == ALIASING
     assert _planned(L, L.clove_penalize_logits, LOGITS, batch=1, out=X, out_stride=1001) in TAKEN
     assert _planned(L, L.clove_penalize_logits, LOGITS, batch=1, out=X, out_dtype=2) == ALIASING
+
+
+def test_a_table_ends_with_its_entries(L):
+    """Rows of a table inside wider ones: what follows its ceil(100 / 16) = 7 entries may be an output."""
+    wide = dict(cache=cache(), table_stride=200)
+    evict = dict(wide, weights_stride=100, positions=X, positions_stride=100)
+    for after, status in [(28, TAKEN), (24, (ALIASING,))]:
+        assert _planned(L, L.clove_paged_attention, ATTEND, **wide, weights=T + after, weights_stride=200) in status, after
+        assert _planned(L, L.clove_cache_evict, EVICT, **evict, weights_out=T + after, weights_out_stride=200) in status, after
+    assert _planned(L, L.clove_paged_attention, ATTEND, **wide, out=T + 3 * 800 + 28) in TAKEN  # behind the last row's
+    assert _planned(L, L.clove_paged_attention, ATTEND, **wide, out=T + 3 * 800 + 24) == ALIASING
