@@ -9,6 +9,7 @@
 // that ctypes has loaded is the one called.
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
@@ -33,8 +34,22 @@ decltype(&clove_penalize_logits) g_penalize;
 
 constexpr auto kInt = at::kInt, kFloat = at::kFloat;
 
+// What decode.py's KVCache holds: the description and the device of its tensors
+struct CacheAt {
+    clove_kv_cache_t c;
+    int device;
+};
+
 struct Args {
     PyObject* const* at;
+    mutable int device = -1;  // of the tensors so far
+    // One device for all of a call's tensors, whose stream the call goes to
+    void on(int index, const char* name) const {
+        if (device < 0) device = index;
+        if (index == device) return;
+        PyErr_Format(PyExc_ValueError, "%s is on cuda:%d, other tensors are on cuda:%d", name, index, device);
+        throw Refused();
+    }
     const at::Tensor& tensor(int i, const char* name, at::ScalarType type) const {
         if (!THPVariable_Check(at[i])) refuse(PyExc_TypeError, name, "is not a tensor");
         const at::Tensor& x = THPVariable_Unpack(at[i]);
@@ -43,6 +58,7 @@ struct Args {
                          c10::toString(x.scalar_type()), x.device().str().c_str());
             throw Refused();
         }
+        on(x.get_device(), name);
         return x;
     }
     at::ScalarType type(int i, const char* name) const {
@@ -64,10 +80,17 @@ struct Args {
     const clove_kv_cache_t* cache(int i) const {
         const void* p = PyLong_AsVoidPtr(at[i]);
         if (!p && PyErr_Occurred()) throw Refused();
-        return static_cast<const clove_kv_cache_t*>(p);
+        const CacheAt* x = static_cast<const CacheAt*>(p);
+        on(x->device, "the cache");
+        return &x->c;
     }
-    // None: torch's current one
+    // None: torch's current one.  (The library works on the current device, so the
+    // tensors have to be there.)
     void* stream(int i) const {
+        if (const int now = c10::hip::current_device(); device >= 0 && device != now) {
+            PyErr_Format(PyExc_ValueError, "the tensors are on cuda:%d, the current device is cuda:%d", device, now);
+            throw Refused();
+        }
         if (none(i)) return c10::hip::getCurrentHIPStream().stream();
         PyObject* x = PyLong_Check(at[i]) ? (Py_INCREF(at[i]), at[i]) : PyObject_GetAttrString(at[i], "cuda_stream");
         if (!x) throw Refused();

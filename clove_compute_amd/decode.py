@@ -6,9 +6,10 @@ Buffers are torch tensors on the current HIP device, passed with their sizes as
 in ``gemm``; every call goes through the C ABI (include/clove/gemm_c.h states
 the formulas), is asynchronous on ``stream`` (default: torch's current stream)
 and raises CloveError where the library refuses it.  What the C ABI cannot see
--- device, element type, number of elements, inner strides -- is checked on the
-way (ValueError), in compiled code: it is most of a small call's time.  A tensor's rows may be further apart than they are long; the
-elements of a row are adjacent.
+-- device (the current one), element type, number of elements, inner strides -- is
+checked on the way (ValueError), in compiled code: it is most of a small call's
+time.  A tensor's rows may be further apart than they are long; the elements of a
+row are adjacent.
 """
 from __future__ import annotations
 
@@ -46,6 +47,11 @@ class _Bound:
 _b = _Bound()
 
 
+class _CacheAt(_lib.KVCacheDesc):
+    """What the compiled module takes: the description and the device of its tensors."""
+    _fields_ = [("device", ctypes.c_int)]
+
+
 class KVCache:
     """The paged key-value cache of one layer: ``k``, ``v``
     [num_pages, kv_heads, page_size, head_dim], fp16 or bf16.  Pages are dense
@@ -62,15 +68,15 @@ class KVCache:
             raise ValueError("the pages of k and v must be equally far apart")
         if k.shape[0] > 1 and k.stride(0) < k[0].numel():  # (the library takes 0 for dense pages)
             raise ValueError("the pages of k and v must lie apart: an expanded tensor has one page only")
-        if not (k.is_cuda and v.is_cuda):
-            raise ValueError("k and v must be on the GPU")
+        if not (k.is_cuda and v.is_cuda and k.device == v.device):
+            raise ValueError("k and v must be on the GPU, on the same one")
         if str(k.dtype) not in _CODES:
             raise ValueError(f"element type {k.dtype} is not fp16, bf16 or fp32")
         self.k, self.v = k, v
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype = k.dtype
-        self._c = _lib.KVCacheDesc(k.data_ptr(), v.data_ptr(), k.stride(0) if k.shape[0] > 1 else 0, self.num_pages,
-                                   self.page_size, self.kv_heads, self.head_dim, _CODES[str(k.dtype)])
+        self._c = _CacheAt(k.data_ptr(), v.data_ptr(), k.stride(0) if k.shape[0] > 1 else 0, self.num_pages, self.page_size,
+                           self.kv_heads, self.head_dim, _CODES[str(k.dtype)], k.get_device())
         self._at = ctypes.addressof(self._c)
 
 

@@ -943,3 +943,14 @@ def test_rope_in_place_of_one_token(dtype, D):
     _close(x[:, :Hq * D], q64.reshape(1, -1), dtype, 1e-5)
     _close(x[:, Hq * D:(Hq + Hk) * D], k64.reshape(1, -1), dtype, 1e-5)
     assert np.array_equal(_f64(x)[:, (Hq + Hk) * D:], v64.reshape(1, -1))
+
+
+def test_tensors_of_another_device_than_the_current_are_refused():
+    import torch
+    from tests.test_decode_binding import _Elsewhere
+    x = _Elsewhere("cuda:1", 2, 64)  # (has no memory, and need not be there)
+    with pytest.raises(ValueError, match="the tensors are on cuda:1, the current device is cuda:0"):
+        _cg().penalize_logits(x, x, 2, 64)
+    y = torch.ones(2, 64, device="cuda")
+    with pytest.raises(ValueError, match="out is on cuda:1"):
+        _cg().penalize_logits(y, x, 2, 64)
