@@ -1,6 +1,7 @@
 """Builds the gfx950 GEMM library libclove_gemm.so in-tree with hipcc, and with
 the host compiler the module through which Python calls the decode step's
-operators with torch tensors (lib/_decode.so, from csrc/decode_binding.cpp).
+operators with torch tensors (lib/_decode.so, from csrc/decode_binding.cpp; left
+out where there is no torch).
 
 Each .hip source under csrc/ is compiled to an object for gfx950 only, then
 linked into clove_compute_amd/lib/libclove_gemm.so.  Objects are rebuilt when
@@ -13,6 +14,7 @@ states a gfx9 hazard requires (hazards.py).
 from __future__ import annotations
 
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
@@ -80,11 +82,23 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _binding_for(torch_version: str) -> str:
+    """What a built module runs with: this Python's ABI and that torch's."""
+    return f"{sysconfig.get_config_var('SOABI')} torch {torch_version}"
+
+
 def _build_binding(force: bool) -> None:
-    if (not force and os.path.exists(BINDING)
-            and os.path.getmtime(BINDING) >= max(os.path.getmtime(BINDING_SRC), _headers_mtime())):
+    spec = importlib.util.find_spec("torch")  # (found, not imported: that takes seconds)
+    if spec is None:
+        print(f"no torch: {os.path.basename(BINDING)} is not built (the C and C++ library needs none)", file=sys.stderr)
         return
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]  # (found, not imported: that takes seconds)
+    torch, wanted = spec.submodule_search_locations[0], _binding_for(importlib.metadata.version("torch"))
+    told = os.path.join(OBJ, "decode_binding.for")
+    if (not force and os.path.exists(BINDING) and os.path.exists(told)
+            and os.path.getmtime(BINDING) >= max(os.path.getmtime(BINDING_SRC), _headers_mtime())):
+        with open(told) as f:
+            if f.read() == wanted:
+                return
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
            "-I", os.path.join(ROOT, "include"), "-isystem", os.path.join(torch, "include"),
            "-isystem", os.path.join(torch, "include", "torch", "csrc", "api", "include"),
@@ -96,6 +110,8 @@ def _build_binding(force: bool) -> None:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("compiling decode_binding.cpp failed")
     os.replace(BINDING + ".tmp", BINDING)
+    with open(told, "w") as f:
+        f.write(wanted)
 
 
 def build(force: bool = False, jobs: int = 8) -> str:
@@ -105,13 +121,13 @@ def build(force: bool = False, jobs: int = 8) -> str:
     with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + 1))) as ex:
         binding = ex.submit(_build_binding, force)
         objs = list(ex.map(lambda s: _compile(s, force), srcs))
-        binding.result()
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB + ".tmp", *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("link of libclove_gemm.so failed")
     os.replace(LIB + ".tmp", LIB)
+    binding.result()  # (the library is there even where the module fails)
     dsrcs = sorted(glob.glob(os.path.join(DIAG_SRC, "*.hip")))
     dobjs = [_compile(s, force) for s in dsrcs]
     if dobjs:
