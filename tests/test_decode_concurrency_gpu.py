@@ -114,3 +114,22 @@ def test_threads_on_one_stream():
     torch.cuda.synchronize()
     one = torch.cuda.current_stream()
     _same(jobs, _at_once(jobs, 40, lambda i: one), want)
+
+
+def test_two_streams_on_library_scratch():
+    """Each stream has buffers and counters of its own: calls that run beside each other
+    on the device do not meet in them."""
+    import torch
+    cg = _cg()
+    jobs = _jobs(cg)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[] for _ in jobs]
+    for _ in range(10):  # one thread, the streams in turn
+        for i, job in enumerate(jobs):
+            with torch.cuda.stream(streams[i % 2]):
+                got[i].append(job())
+    torch.cuda.synchronize()
+    _same(jobs, got, want)
+    _same(jobs, _at_once(jobs, 10, lambda i: streams[i % 2]), want)
