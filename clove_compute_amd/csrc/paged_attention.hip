@@ -35,6 +35,7 @@ struct Params {
     // the kernel cuts each sequence by the lengths it finds (Cut)
     bool cuts;
     int fill;            // workgroups that the CUs hold at once
+    int rounds;          // most times as many that there are
     int slots;           // most workgroups with keys: all of them, where it does not cut
     float* partials;     // [slots] slabs of `slab` floats, then as many for joined ones
     unsigned* counters;  // [sequence, KV head, tile], then [slots] of groups of `fan` splits
@@ -320,7 +321,8 @@ __device__ __forceinline__ void merge(float& m, float& l, f32x4& o, float m2, fl
 }
 
 // How the kernel shares out the keys: into `chunk`s of so many 32s of keys that
-// there are about `fill` of them (with KV heads and tiles), a sequence's of one length.
+// there are about `fill` of them (with KV heads and tiles), or up to `rounds` times
+// that where they would be longer than kLongest, a sequence's chunks of one length.
 // Every wave works it out for itself from the lengths, 64 sequences at a time.
 // (By the bound of the lengths alone, most workgroups of 48 mixed sequences had no
 // keys, and those that had some waited for them to pass: 55 us instead of 49.)
@@ -348,7 +350,7 @@ __device__ __forceinline__ Cut cut(const Params& p, int i, int per) {
         if (b0 == 0) t0 = t;
         sum += wave_sum((unsigned)t);  // (64 of at most 2^25)
     }
-    const int chunk = chunk_of(sum, per, p.fill);
+    const int chunk = chunk_of(sum, per, p.fill, p.rounds);
     int before = 0;
     Cut c{-1, 0, 0, 0, 0};
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
@@ -860,6 +862,7 @@ clove_status_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s
         const paged::Plan plan = paged::plan(a.batch, per, span, p.fill);
         p.cuts = waves == paged::kW && plan.cuts;
         if (p.cuts) {
+            p.rounds = (int)plan.rounds;
             p.slots = (int)plan.slots;
             // what a workgroup reads in about 3 us; another round of arrivals takes as long
             p.fan = std::max(16, std::min(64, (128 << 10) / (std::min(p.group, 16) * c.head_dim * 4)));
