@@ -252,12 +252,12 @@ __device__ __forceinline__ float groups_sum(float x) {
 // 16-bit numbers that a softmax weight is the sum of
 template <int DT>
 constexpr int kParts = DT == CLOVE_DTYPE_BF16 ? 3 : 2;
-// What it is multiplied by for them, taken out of the wave's sums after the keys.
-// fp16's steps end at 2^-24: of a weight 2^(t - m) <= 1 as it is, the two parts hold
-// fewer than 22 bits from 2^-3 down and nothing below 2^-25, and many keys far below
-// one whose value is small are then lost (4096 positive ones 2^-24 below it came out
-// 3e-3 off, and more the more they cancel).  Times 2^15 they are whole down to
-// 2^-18, and what is lost of any weight is at most 2^-40 of the wave's largest.
+// What it is multiplied by for them, in both sums, O and l, whose quotient is the
+// result.  fp16's steps end at 2^-24: of a weight 2^(t - m) <= 1 as it is, the two
+// parts hold fewer than 22 bits from 2^-3 down and nothing below 2^-25, and many keys
+// far below one whose value is small are then lost (4096 positive ones 2^-24 below it
+// came out 3e-3 off, and more the more they cancel).  Times 2^15 they are whole down
+// to 2^-18, and what is lost of any weight is at most 2^-40 of the wave's largest.
 template <int DT>
 constexpr float kPScale = DT == CLOVE_DTYPE_FP16 ? 32768.0f : 1.0f;
 
@@ -622,10 +622,8 @@ __global__ void __launch_bounds__(64 * W, (resident<NC, TAIL, W>())) attend(cons
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                float x = exp2_(s[r][i] - sub), y = exp2_(s[r][i + 1] - sub);
+                float x = exp2_(s[r][i] - sub) * kPScale<DT>, y = exp2_(s[r][i + 1] - sub) * kPScale<DT>;
                 l += x + y;
-                x *= kPScale<DT>;
-                y *= kPScale<DT>;
 #pragma unroll
                 for (int k = 0; k < kParts<DT>; ++k) {  // each part what the ones before it leave, rounded
                     const unsigned h = pack2<DT>(x, y);
@@ -708,12 +706,6 @@ __global__ void __launch_bounds__(64 * W, (resident<NC, TAIL, W>())) attend(cons
             for (int i = 0; i < 4; ++i) o[c][i] = special[c][i] != 0.0f ? special[c][i] : o[c][i];
     }
     l = groups_sum(l);
-    if constexpr (kPScale<DT> != 1.0f) {
-#pragma unroll
-        for (int c = 0; c < 2 * NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[c][i] *= 1.0f / kPScale<DT>;
-    }
 
     // the waves, merged in their order
     __syncthreads();
@@ -730,7 +722,7 @@ __global__ void __launch_bounds__(64 * W, (resident<NC, TAIL, W>())) attend(cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = L == 0.0f ? 0.0f : O[i] / L;
         store4<DT>(a.out + b * a.out_stride + (int64_t)(h0 + h) * D, 4 * quad, D, vec, x);
-        if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L};
+        if (p.stats && quad == 0) p.stats[(int64_t)b * a.q_heads + h0 + h] = float2{finite_max(M), L * (1.0f / kPScale<DT>)};
     };
     const __amdgpu_buffer_rsrc_t slabs = slabs_of(p);
     for (int i = threadIdx.x; i < items; i += 64 * W) {
