@@ -6,9 +6,9 @@
 // in base 2 (t = s log2 e), p_j = 2^(t_j - m) / l.  The bytes are K and V once;
 // everything else is small, so long caches are bound by HBM: 65536 keys of one
 // sequence, 8 KV heads of 128 (268 MB), 53 us, 5.0 TB/s; 16 x 4096 keys of 32 KV
-// heads of 128 (1.07 GB) 187 us, 5.7 TB/s, where a copy reaches 5.1.  Short ones are
+// heads of 128 (1.07 GB) 188 us, 5.7 TB/s, where a copy reaches 5.1.  Short ones are
 // bound by the latencies from the lengths to the page table to the rows, and of the
-// join: 411 keys 7.7 us, 20 keys 4.3.
+// join: 411 keys 7.8 us, 20 keys 4.3.
 //
 // Accumulated weights need every head's final m and l, so the scores go to
 // scratch (fp32, one per query head and key) and a second kernel adds
@@ -73,7 +73,9 @@ __device__ __forceinline__ int64_t row_at(const Params& p, int b, int kh, int j)
 __device__ __forceinline__ float finite_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
 // Any head_dim up to 64 E and any alignment: a workgroup per (sequence, query
-// head), a key per wave, element lane + 64 e per lane.
+// head), a key per wave, element lane + 64 e per lane.  For head_dim outside 8 .. 256
+// only, and slow there: nothing is split over the length, K and V are read once for
+// each query head (32768 keys, 16 heads on one KV head of 512, 67 MB: 38 ms).
 template <int DT, int E>
 __global__ void __launch_bounds__(256) attend_any(const Params p) {
     using T = Elem<DT>;

@@ -28,7 +28,7 @@ struct Plan {
 // one does not fill: 17 x 32 heads of 128 with 8192 keys 456 us in one, 419 in up to
 // four, 407 in up to six, 406 in eight; 33 x 8 of 256 567, 431, 416, 416.  But their
 // number goes by the bound of the lengths, and workgroups without keys take time: 32
-// sequences of 1000 keys, 8 heads of 128, behind a bound of 131072, 29, 30, 32, 35 us,
+// sequences of 1000 keys, 8 heads of 128, behind a bound of 131072, 29, 30, 34, 35 us,
 // and 58 with the 31 that the bound has.  Where counters have no room for six there are
 // fewer; where they have none for one, from about 7900 sequences x KV heads x tiles on,
 // each of those is one workgroup's.

@@ -252,7 +252,7 @@ clove_status_t clove_w4a16_swiglu(const void* X, const uint8_t* W_q, const void*
  * replaced (the reference declares a paged_attention in include/clove/kernels/
  * attention.cuh:85-100 and never defines it).  Element type `dtype`: see
  * clove_dtype_t; every sum, norm and softmax statistic is fp32 and a result is
- * rounded once.  Row strides count elements.  All of these take their scratch
+ * rounded once (what a softmax weight keeps: clove_paged_attention).  Row strides count elements.  All of these take their scratch
  * as the GEMMs do (library buffers, a bound workspace, or a size query).
  * ------------------------------------------------------------------------ */
 typedef enum clove_dtype {
@@ -330,7 +330,8 @@ clove_status_t clove_qk_norm_rope(const void* qkv, int64_t qkv_stride, const voi
  * page_size (and weights_stride), and a row of the table has ceil(max_context /
  * page_size) entries, of which those past the length may be anything.  The work
  * is shared out on the device by the lengths themselves, so a recorded call may
- * be replayed with others.  Sums run in a fixed order: a call gives the same
+ * be replayed with others; with more than about 7900 sequences x KV heads x 16
+ * query heads of one, long sequences are not split.  Sums run in a fixed order: a call gives the same
  * bits every time.  With `weights` the call takes a buffer of batch * q_heads *
  * max_context floats of scratch.
  */
