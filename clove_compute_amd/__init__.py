@@ -7,7 +7,8 @@ GEMM API over torch device tensors, and the INT4 packing/quantisation helpers.
 """
 from ._lib import (  # noqa: F401
     CloveError, CLOVE_ERR_SCRATCH_LIMIT, CLOVE_ERR_WORKSPACE, CLOVE_INT4_GROUPWISE,
-    CLOVE_INT4_REFERENCE_LITERAL, CLOVE_INT8_EXACT, CLOVE_INT8_REFERENCE_LITERAL, CLOVE_MAX_HEAD_DIM, CLOVE_NOALLOC_SCRATCH_BYTES,
+    CLOVE_INT4_REFERENCE_LITERAL, CLOVE_INT8_EXACT, CLOVE_INT8_REFERENCE_LITERAL, CLOVE_MAX_EXPERTS, CLOVE_MAX_HEAD_DIM,
+    CLOVE_MAX_NORM_DIM, CLOVE_MAX_TOP_K, CLOVE_NOALLOC_SCRATCH_BYTES, CLOVE_ROUTE_SIGMOID, CLOVE_ROUTE_SOFTMAX,
     CLOVE_WORKSPACE_MIN_BYTES,
 )
 from .gemm import (  # noqa: F401
@@ -36,5 +37,11 @@ from .decode import (  # noqa: F401
     paged_attention,
     penalize_logits,
     qk_norm_rope,
+)
+from .moe import (  # noqa: F401
+    block_norm,
+    moe_route,
+    moe_w4a16,
+    moe_w4a16_swiglu,
 )
 from . import quant  # noqa: F401

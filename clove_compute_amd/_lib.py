@@ -35,6 +35,12 @@ CLOVE_DTYPE_BF16 = 1
 CLOVE_DTYPE_FP32 = 2
 CLOVE_MAX_HEAD_DIM = 1024
 
+CLOVE_ROUTE_SOFTMAX = 0
+CLOVE_ROUTE_SIGMOID = 1
+CLOVE_MAX_NORM_DIM = 32768
+CLOVE_MAX_EXPERTS = 1024
+CLOVE_MAX_TOP_K = 64
+
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
@@ -72,6 +78,10 @@ SIGNATURES = {
     "clove_paged_attention": ([P, L, KV, P, L, P, P, L, P, L, I, I, I, F, F, I, P], I),
     "clove_cache_evict": ([KV, P, L, P, P, L, P, L, P, L, P, L, P, I, I, I, I, I, P], I),
     "clove_penalize_logits": ([P, L, I, P, L, I, I, I, P, L, P, P, P, P, P, P, P, L, P, P, L, P], I),
+    "clove_block_norm": ([P, L, P, L, P, P, L, F, P, P, L, P, L, I, I, F, I, I, P], I),
+    "clove_moe_route": ([P, L, I, P, I, I, I, I, I, I, F, P, P, I, I, P], I),
+    "clove_moe_w4a16_swiglu": ([P, P, P, P, P, P, I, I, I, I, I, P], I),
+    "clove_moe_w4a16": ([P, P, P, P, P, P, P, I, I, I, I, I, F, F, P], I),
     "clove_workspace_bind": ([P, ctypes.c_size_t], I),
     "clove_workspace_query_begin": ([], I),
     "clove_workspace_query_end": ([], ctypes.c_size_t),

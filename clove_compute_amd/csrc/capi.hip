@@ -13,6 +13,7 @@
 #include "common.hpp"
 #include "decode.hpp"
 #include "dispatch.hpp"
+#include "moe.hpp"
 
 namespace clove {
 using hw::cdiv64;
@@ -886,6 +887,158 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
     a.allowed = allowed;
     a.allowed_stride = allowed_stride;
     return launch_penalize_logits(a, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_block_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                const void* post_weight, const void* gate, int64_t gate_stride, float scale,
+                                const void* pre_weight, void* y_out, int64_t y_out_stride, void* h_out,
+                                int64_t h_out_stride, int T, int D, float eps, int dtype, int residual_dtype,
+                                void* stream) {
+    CallScope scope;
+    if (dtype != CLOVE_DTYPE_FP16 && dtype != CLOVE_DTYPE_BF16) return CLOVE_ERR_INVALID_ARG;
+    if (residual_dtype != dtype && residual_dtype != CLOVE_DTYPE_FP32) return CLOVE_ERR_INVALID_ARG;
+    if (T < 0 || D < 0 || D > CLOVE_MAX_NORM_DIM) return CLOVE_ERR_INVALID_DIM;
+    if (T == 0 || D == 0) return CLOVE_OK;
+    if ((!x && !residual) || (!y_out && !h_out)) return CLOVE_ERR_NULL_POINTER;
+    if ((x && x_stride < D) || (residual && residual_stride < D) || (gate && gate_stride != 0 && gate_stride < D) ||
+        (y_out && y_out_stride < D) || (h_out && h_out_stride < D))
+        return CLOVE_ERR_INVALID_ARG;
+    const bool wide = residual_dtype == CLOVE_DTYPE_FP32;
+    if (!aligned2(x) || !aligned2(gate) || !aligned2(post_weight) || !aligned2(pre_weight) || !aligned2(h_out) ||
+        !(wide ? aligned4(residual) && aligned4(y_out) : aligned2(residual) && aligned2(y_out)))
+        return CLOVE_ERR_INVALID_ARG;
+    const int64_t rs = wide ? 4 : 2;
+    // (an output may be the input that each thread has read all of before it writes)
+    struct In {
+        Rows r;
+        bool by_y, by_h;
+    };
+    const In in[] = {{{x, x_stride * 2, (int64_t)D * 2, T}, !wide, true},
+                     {{residual, residual_stride * rs, D * rs, T}, true, !wide},
+                     {{gate, gate_stride * 2, (int64_t)D * 2, gate_stride ? T : 1}, !wide && (gate_stride || T == 1),
+                      gate_stride || T == 1},
+                     {{post_weight, 0, (int64_t)D * 2, 1}, false, false},
+                     {{pre_weight, 0, (int64_t)D * 2, 1}, false, false}};
+    const Rows oy{y_out, y_out_stride * rs, D * rs, T}, oh{h_out, h_out_stride * 2, (int64_t)D * 2, T};
+    for (const In& i : in) {
+        if (overlaps(oy, i.r) && !(i.by_y && same_rows(oy, i.r))) return CLOVE_ERR_ALIASING;
+        if (overlaps(oh, i.r) && !(i.by_h && same_rows(oh, i.r))) return CLOVE_ERR_ALIASING;
+    }
+    if (overlaps(oy, oh)) return CLOVE_ERR_ALIASING;
+    BlockNormArgs a;
+    a.x = x;
+    a.x_stride = x_stride;
+    a.residual = residual;
+    a.residual_stride = residual_stride;
+    a.post_weight = x ? post_weight : nullptr;
+    a.gate = x ? gate : nullptr;
+    a.gate_stride = gate_stride;
+    a.scale = scale;
+    a.pre_weight = pre_weight;
+    a.y_out = y_out;
+    a.y_out_stride = y_out_stride;
+    a.h_out = h_out;
+    a.h_out_stride = h_out_stride;
+    a.T = T; a.D = D;
+    a.eps = eps;
+    a.dtype = dtype;
+    a.residual_dtype = residual_dtype;
+    return launch_block_norm(a, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_moe_route(const void* logits, int64_t logits_stride, int dtype, const float* bias, int score,
+                               int groups, int top_groups, int group_top, int top_k, int renormalize, float scale,
+                               int32_t* ids, float* weights, int T, int experts, void* stream) {
+    CallScope scope;
+    if (dtype < CLOVE_DTYPE_FP16 || dtype > CLOVE_DTYPE_FP32 ||
+        (score != CLOVE_ROUTE_SOFTMAX && score != CLOVE_ROUTE_SIGMOID) || (group_top != 1 && group_top != 2))
+        return CLOVE_ERR_INVALID_ARG;
+    if (T < 0 || experts < 1 || experts > CLOVE_MAX_EXPERTS || top_k < 1 || top_k > CLOVE_MAX_TOP_K || groups < 1 ||
+        top_groups < 1)
+        return CLOVE_ERR_INVALID_DIM;
+    if (top_k > experts || experts % groups != 0 || top_groups > groups || groups > 64) return CLOVE_ERR_INVALID_ARG;
+    if (T == 0) return CLOVE_OK;
+    if (!logits || !ids || !weights) return CLOVE_ERR_NULL_POINTER;
+    if (logits_stride < experts) return CLOVE_ERR_INVALID_ARG;
+    const int64_t es = dtype == CLOVE_DTYPE_FP32 ? 4 : 2;
+    if (!(es == 4 ? aligned4(logits) : aligned2(logits)) || !aligned4(bias) || !aligned4(ids) || !aligned4(weights))
+        return CLOVE_ERR_INVALID_ARG;
+    const int64_t out = (int64_t)T * top_k * 4;
+    const Rows in[] = {{logits, logits_stride * es, experts * es, T}, {bias, 0, (int64_t)experts * 4, 1}};
+    const Rows outs[] = {{ids, 0, out, 1}, {weights, 0, out, 1}};
+    for (const Rows& o : outs)
+        for (const Rows& i : in)
+            if (overlaps(o, i)) return CLOVE_ERR_ALIASING;
+    if (overlaps(outs[0], outs[1])) return CLOVE_ERR_ALIASING;
+    RouteArgs a;
+    a.logits = logits;
+    a.logits_stride = logits_stride;
+    a.dtype = dtype;
+    a.bias = bias;
+    a.score = score;
+    a.groups = groups; a.top_groups = top_groups; a.group_top = group_top; a.top_k = top_k;
+    a.renormalize = renormalize != 0;
+    a.scale = scale;
+    a.ids = ids;
+    a.weights = weights;
+    a.T = T; a.experts = experts;
+    return launch_moe_route(a, static_cast<hipStream_t>(stream));
+}
+
+// Both products of a sparse MLP block (MoeArgs): `rows` weight rows an expert
+static clove_status_t moe_common(MoeArgs& a, bool swiglu, void* stream) {
+    CallScope scope;
+    if (a.T < 0 || a.O < 0 || a.K < 0 || a.top_k < 1 || a.top_k > CLOVE_MAX_TOP_K || a.experts < 1 ||
+        a.experts > CLOVE_MAX_EXPERTS)
+        return CLOVE_ERR_INVALID_DIM;
+    if (a.K % 2 != 0) return CLOVE_ERR_INVALID_ARG;
+    if (a.T == 0 || a.O == 0) return CLOVE_OK;
+    // (pairs, and rows in tiles of them, are counted in 31 bits; a row of weights is at most 2^30 bytes)
+    const int64_t pairs = (int64_t)a.T * a.top_k, rows = (int64_t)a.O * (swiglu ? 2 : 1), G = cdiv64(a.K, 128);
+    if (pairs > 0x3fffffff || rows > 0x7fffffff || (pairs / 32 + a.experts + 1) * cdiv64(rows, 32) > 0x7fffffff)
+        return CLOVE_ERR_INVALID_DIM;
+    if (rows * (a.K / 2) > ((int64_t)1 << 50) / a.experts) return CLOVE_ERR_INVALID_DIM;
+    if (!a.Y || !a.ids || (a.K > 0 && (!a.X || !a.W || !a.scale || !a.zero))) return CLOVE_ERR_NULL_POINTER;
+    if (!aligned2(a.X) || !aligned2(a.Y) || !aligned2(a.scale) || !aligned2(a.zero) || !aligned4(a.ids) ||
+        !aligned4(a.weights))
+        return CLOVE_ERR_INVALID_ARG;
+    const int64_t all = a.experts * rows;
+    const Rows y{a.Y, 0, (swiglu ? pairs : a.T) * a.O * 2, 1};
+    const Rows in[] = {{a.X, 0, (swiglu ? a.T : pairs) * a.K * 2, 1}, {a.ids, 0, pairs * 4, 1}, {a.weights, 0, pairs * 4, 1},
+                       {a.W, 0, all * (a.K / 2), 1}, {a.scale, 0, all * G * 2, 1}, {a.zero, 0, all * G * 2, 1}};
+    for (const Rows& i : in)
+        if (overlaps(y, i)) return CLOVE_ERR_ALIASING;
+    return launch_moe_w4a16(a, swiglu, static_cast<hipStream_t>(stream));
+}
+
+clove_status_t clove_moe_w4a16_swiglu(const void* X, const int32_t* expert_ids, const uint8_t* W_q,
+                                      const void* W_scale, const void* W_zero, void* H, int T, int top_k, int experts,
+                                      int I, int K, void* stream) {
+    MoeArgs a;
+    a.X = static_cast<const uint16_t*>(X);
+    a.ids = expert_ids;
+    a.W = W_q;
+    a.scale = static_cast<const uint16_t*>(W_scale);
+    a.zero = static_cast<const uint16_t*>(W_zero);
+    a.Y = static_cast<uint16_t*>(H);
+    a.T = T; a.top_k = top_k; a.experts = experts; a.O = I; a.K = K;
+    return moe_common(a, true, stream);
+}
+
+clove_status_t clove_moe_w4a16(const void* H, const int32_t* expert_ids, const float* weights, const uint8_t* W_q,
+                               const void* W_scale, const void* W_zero, void* Y, int T, int top_k, int experts, int O,
+                               int K, float alpha, float beta, void* stream) {
+    MoeArgs a;
+    a.X = static_cast<const uint16_t*>(H);
+    a.ids = expert_ids;
+    a.weights = weights;
+    a.W = W_q;
+    a.scale = static_cast<const uint16_t*>(W_scale);
+    a.zero = static_cast<const uint16_t*>(W_zero);
+    a.Y = static_cast<uint16_t*>(Y);
+    a.T = T; a.top_k = top_k; a.experts = experts; a.O = O; a.K = K;
+    a.alpha = alpha; a.beta = beta;
+    return moe_common(a, false, stream);
 }
 
 clove_status_t clove_workspace_bind(void* ptr, size_t bytes) {

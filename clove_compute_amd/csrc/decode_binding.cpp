@@ -1,11 +1,12 @@
-// The decode step's operators for Python: tensors in, calls of the C ABI out.
+// The decode step's and the sparse MLP block's operators for Python: tensors in, calls
+// of the C ABI out.
 //
 // The C ABI cannot see a tensor's device, element type, number of elements and
 // inner strides: they are checked here, which in Python (five attributes of up to
 // nine tensors, and twenty-odd numbers through ctypes) cost 3 to 5 of the 7.5 us
-// of a call whose kernel runs 3.  A function takes what its namesake in decode.py
-// does, in order, and returns the library's status; a tensor that does not fit is
-// a ValueError.  The library's functions come as addresses (bind), so the one
+// of a call whose kernel runs 3.  A function takes what its namesake in decode.py or
+// moe.py does, in order, and returns the library's status; a tensor that does not fit
+// is a ValueError.  The library's functions come as addresses (bind), so the one
 // that ctypes has loaded is the one called.
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -31,6 +32,10 @@ decltype(&clove_qk_norm_rope) g_rope;
 decltype(&clove_paged_attention) g_attend;
 decltype(&clove_cache_evict) g_evict;
 decltype(&clove_penalize_logits) g_penalize;
+decltype(&clove_block_norm) g_norm;
+decltype(&clove_moe_route) g_route;
+decltype(&clove_moe_w4a16_swiglu) g_up;
+decltype(&clove_moe_w4a16) g_down;
 
 constexpr auto kInt = at::kInt, kFloat = at::kFloat;
 
@@ -272,6 +277,97 @@ clove_status_t penalize(const Args& a) {
     return st;
 }
 
+clove_status_t block_norm(const Args& a) {
+    const int T = a.number(3, "T"), D = a.number(4, "D");
+    const float scale = a.real(9), eps = a.real(10);
+    // x and h_out, the weights and the gate are one type; the residual and y_out one, that or fp32
+    const at::ScalarType t = !a.none(0) ? a.type(0, "x") : !a.none(2) ? a.type(2, "h_out") : !a.none(1) ? a.type(1, "residual") : at::kHalf;
+    const at::ScalarType tr = !a.none(1) ? a.type(1, "residual") : !a.none(5) ? a.type(5, "y_out") : t;
+    const Rows x = a.none(0) ? Rows{} : rows(a, 0, "x", t, T, D), r = a.none(1) ? Rows{} : rows(a, 1, "residual", tr, T, D);
+    const Rows h = a.none(2) ? Rows{} : rows(a, 2, "h_out", t, T, D), y = a.none(5) ? Rows{} : rows(a, 5, "y_out", tr, T, D);
+    Rows g;
+    if (!a.none(8)) {
+        const at::Tensor& gate = a.tensor(8, "gate", t);
+        if (gate.dim() == 1) g = {flat<void>(a, 8, "gate", t, D), 0};
+        else g = rows(gate, "gate", T, D);
+    }
+    const void *wo = flat<void>(a, 6, "post_weight", t, D), *wi = flat<void>(a, 7, "pre_weight", t, D);
+    const int dt = code(t), dtr = code(tr);
+    void* stream = a.stream(11);
+    clove_status_t st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_norm(x.at, x.stride, r.at, r.stride, wo, g.at, g.stride, scale, wi, y.at, y.stride, h.at, h.stride, T, D, eps, dt, dtr, stream);
+    Py_END_ALLOW_THREADS
+    return st;
+}
+
+clove_status_t moe_route(const Args& a) {
+    const int T = a.number(3, "T"), E = a.number(4, "experts"), k = a.number(5, "top_k"), score = a.number(6, "score");
+    const int groups = a.number(8, "groups"), top = a.number(9, "top_groups"), of = a.number(10, "group_top");
+    const int renorm = PyObject_IsTrue(a.at[11]);
+    if (renorm < 0) throw Refused();
+    const float scale = a.real(12);
+    const at::ScalarType t = a.type(0, "logits");
+    const Rows x = rows(a, 0, "logits", t, T, E);
+    if (a.none(1) || a.none(2)) refuse(PyExc_TypeError, a.none(1) ? "ids" : "weights", "is not a tensor");
+    int32_t* ids = flat<int32_t>(a, 1, "ids", kInt, times(T, k));
+    float* w = flat<float>(a, 2, "weights", kFloat, times(T, k));
+    const float* bias = flat<float>(a, 7, "bias", kFloat, E);
+    const int dt = code(t);
+    void* stream = a.stream(13);
+    clove_status_t st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_route(x.at, x.stride, dt, bias, score, groups, top, of, k, renorm, scale, ids, w, T, E, stream);
+    Py_END_ALLOW_THREADS
+    return st;
+}
+
+// What both products of the experts take: ids and weights of `rows` rows an expert
+struct Experts {
+    const int32_t* ids;
+    const uint8_t* q;
+    const void *scale, *zero;
+};
+Experts experts(const Args& a, int i, int q, int64_t pairs, int64_t all, int K) {
+    const int64_t G = ((int64_t)K + 127) / 128;
+    for (int j : {i, q, q + 1, q + 2})
+        if (a.none(j)) refuse(PyExc_TypeError, j == i ? "ids" : j == q ? "W_q" : j == q + 1 ? "W_scale" : "W_zero", "is not a tensor");
+    return {flat<int32_t>(a, i, "ids", kInt, pairs), flat<uint8_t>(a, q, "W_q", at::kByte, times(all, K / 2)),
+            flat<void>(a, q + 1, "W_scale", at::kHalf, times(all, G)), flat<void>(a, q + 2, "W_zero", at::kHalf, times(all, G))};
+}
+
+clove_status_t moe_up(const Args& a) {
+    const int T = a.number(6, "T"), k = a.number(7, "top_k"), E = a.number(8, "experts"), I = a.number(9, "I"), K = a.number(10, "K");
+    if (a.none(0) || a.none(5)) refuse(PyExc_TypeError, a.none(0) ? "X" : "H", "is not a tensor");
+    const int64_t pairs = times(T, k);
+    const void* x = flat<void>(a, 0, "X", at::kHalf, times(T, K));
+    const Experts w = experts(a, 1, 2, pairs, times(E, times(2, I)), K);
+    void* h = flat<void>(a, 5, "H", at::kHalf, times(pairs, I));
+    void* stream = a.stream(11);
+    clove_status_t st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_up(x, w.ids, w.q, w.scale, w.zero, h, T, k, E, I, K, stream);
+    Py_END_ALLOW_THREADS
+    return st;
+}
+
+clove_status_t moe_down(const Args& a) {
+    const int T = a.number(7, "T"), k = a.number(8, "top_k"), E = a.number(9, "experts"), O = a.number(10, "O"), K = a.number(11, "K");
+    const float alpha = a.real(12), beta = a.real(13);
+    if (a.none(0) || a.none(6)) refuse(PyExc_TypeError, a.none(0) ? "H" : "Y", "is not a tensor");
+    const int64_t pairs = times(T, k);
+    const void* h = flat<void>(a, 0, "H", at::kHalf, times(pairs, K));
+    const float* weights = flat<float>(a, 2, "weights", kFloat, pairs);
+    const Experts w = experts(a, 1, 3, pairs, times(E, O), K);
+    void* y = flat<void>(a, 6, "Y", at::kHalf, times(T, O));
+    void* stream = a.stream(14);
+    clove_status_t st;
+    Py_BEGIN_ALLOW_THREADS
+    st = g_down(h, w.ids, weights, w.q, w.scale, w.zero, y, T, k, E, O, K, alpha, beta, stream);
+    Py_END_ALLOW_THREADS
+    return st;
+}
+
 // the status as a Python number; no exception leaves
 template <clove_status_t (*F)(const Args&), int N>
 PyObject* entry(PyObject*, PyObject* const* at, Py_ssize_t n) {
@@ -286,15 +382,20 @@ PyObject* entry(PyObject*, PyObject* const* at, Py_ssize_t n) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* at, Py_ssize_t n) {
-    void* p[4];
-    if (n != 4) return PyErr_Format(PyExc_TypeError, "4 addresses are wanted, not %zd", n);
-    for (int i = 0; i < 4; ++i)
+    constexpr int N = 8;
+    void* p[N];
+    if (n != N) return PyErr_Format(PyExc_TypeError, "%d addresses are wanted, not %zd", N, n);
+    for (int i = 0; i < N; ++i)
         if (!(p[i] = PyLong_AsVoidPtr(at[i])))
             return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "address %d is null", i);
     g_rope = reinterpret_cast<decltype(g_rope)>(p[0]);
     g_attend = reinterpret_cast<decltype(g_attend)>(p[1]);
     g_evict = reinterpret_cast<decltype(g_evict)>(p[2]);
     g_penalize = reinterpret_cast<decltype(g_penalize)>(p[3]);
+    g_norm = reinterpret_cast<decltype(g_norm)>(p[4]);
+    g_route = reinterpret_cast<decltype(g_route)>(p[5]);
+    g_up = reinterpret_cast<decltype(g_up)>(p[6]);
+    g_down = reinterpret_cast<decltype(g_down)>(p[7]);
     Py_RETURN_NONE;
 }
 
@@ -307,6 +408,10 @@ PyMethodDef methods[] = {{"bind", fast(bind), METH_FASTCALL, nullptr},
                          {"paged_attention", fast(entry<attend, 13>), METH_FASTCALL, nullptr},
                          {"cache_evict", fast(entry<evict, 14>), METH_FASTCALL, nullptr},
                          {"penalize_logits", fast(entry<penalize, 15>), METH_FASTCALL, nullptr},
+                         {"block_norm", fast(entry<block_norm, 12>), METH_FASTCALL, nullptr},
+                         {"moe_route", fast(entry<moe_route, 14>), METH_FASTCALL, nullptr},
+                         {"moe_w4a16_swiglu", fast(entry<moe_up, 12>), METH_FASTCALL, nullptr},
+                         {"moe_w4a16", fast(entry<moe_down, 15>), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -38,9 +38,12 @@ class _Bound:
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_decode", loader))
         loader.exec_module(module)
         module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in
-                      (lib.clove_qk_norm_rope, lib.clove_paged_attention, lib.clove_cache_evict, lib.clove_penalize_logits)))
+                      (lib.clove_qk_norm_rope, lib.clove_paged_attention, lib.clove_cache_evict, lib.clove_penalize_logits,
+                       lib.clove_block_norm, lib.clove_moe_route, lib.clove_moe_w4a16_swiglu, lib.clove_moe_w4a16)))
         self.rope, self.attend, self.evict, self.penalize = (module.qk_norm_rope, module.paged_attention, module.cache_evict,
                                                              module.penalize_logits)
+        self.block_norm, self.moe_route, self.moe_up, self.moe_down = (module.block_norm, module.moe_route,
+                                                                       module.moe_w4a16_swiglu, module.moe_w4a16)
         return self.__dict__[name]
 
 

@@ -187,4 +187,37 @@ inline void penalize_logits(const void* logits, int64_t logits_stride, clove_dty
                                              allowed, allowed_stride, stream));
 }
 
+// A sparse MLP block (see <clove/gemm_c.h> for each formula).
+inline void block_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                       const void* post_weight, const void* gate, int64_t gate_stride, float scale,
+                       const void* pre_weight, void* y_out, int64_t y_out_stride, void* h_out, int64_t h_out_stride,
+                       int T, int D, float eps, clove_dtype_t dtype, clove_dtype_t residual_dtype,
+                       hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_block_norm(x, x_stride, residual, residual_stride, post_weight, gate, gate_stride, scale,
+                                        pre_weight, y_out, y_out_stride, h_out, h_out_stride, T, D, eps, (int)dtype,
+                                        (int)residual_dtype, stream));
+}
+
+inline void moe_route(const void* logits, int64_t logits_stride, clove_dtype_t dtype, int32_t* ids, float* weights,
+                      int T, int experts, int top_k, clove_route_score_t score = CLOVE_ROUTE_SOFTMAX,
+                      const float* bias = nullptr, int groups = 1, int top_groups = 1, int group_top = 1,
+                      bool renormalize = false, float scale = 1.0f, hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_moe_route(logits, logits_stride, (int)dtype, bias, (int)score, groups, top_groups,
+                                       group_top, top_k, renormalize ? 1 : 0, scale, ids, weights, T, experts, stream));
+}
+
+inline void moe_w4a16_swiglu(const half* X, const int32_t* expert_ids, const uint8_t* W_q, const half* W_scale,
+                             const half* W_zero, half* H, int T, int top_k, int experts, int I, int K,
+                             hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(
+        clove_moe_w4a16_swiglu(X, expert_ids, W_q, W_scale, W_zero, H, T, top_k, experts, I, K, stream));
+}
+
+inline void moe_w4a16(const half* H, const int32_t* expert_ids, const float* weights, const uint8_t* W_q,
+                      const half* W_scale, const half* W_zero, half* Y, int T, int top_k, int experts, int O, int K,
+                      float alpha = 1.0f, float beta = 0.0f, hipStream_t stream = 0) {
+    CLOVE_CHECK_STATUS(clove_moe_w4a16(H, expert_ids, weights, W_q, W_scale, W_zero, Y, T, top_k, experts, O, K, alpha,
+                                       beta, stream));
+}
+
 }  // namespace clove

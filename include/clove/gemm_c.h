@@ -400,6 +400,100 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
                                      const int32_t* bias_counts, const uint32_t* allowed,
                                      int64_t allowed_stride, void* stream);
 
+/* ------------------------------------------------------------------------
+ * A sparse MLP block around the linear layers: the norms before and after a
+ * block with its residual, the router, and the products of the experts it
+ * chose.  No reference counterpart.  Element types, strides, rounding and
+ * scratch as for the decode step above.
+ * ------------------------------------------------------------------------ */
+
+/* Largest D of clove_block_norm, experts and top_k of the others. */
+#define CLOVE_MAX_NORM_DIM 32768
+#define CLOVE_MAX_EXPERTS 1024
+#define CLOVE_MAX_TOP_K 64
+
+/*
+ * What a block gave joins the residual stream, and the next block's input
+ * leaves it, in one pass:
+ *   u = x / sqrt(mean(x^2) + eps) * post_weight, where post_weight is not
+ *       NULL, else u = x
+ *   y = residual + scale * gate * u
+ *   h = y / sqrt(mean(y^2) + eps) * pre_weight
+ * x, gate, the weights and h are `dtype` (FP16 or BF16), residual and y are
+ * residual_dtype (the same, or FP32).  h comes from the fp32 y, not from the
+ * rounded one.  gate is one row for all tokens (gate_stride 0) or a row for
+ * each, NULL: 1; pre_weight NULL: 1; x NULL: y = residual (a stack's first
+ * norm); residual NULL: 0 (not both).  y_out or h_out may be NULL: not wanted.
+ * Rows [T, D], strides in elements.  y_out may be residual, y_out or h_out may
+ * be x or gate (same rows and type; of several rows the same stride); else
+ * outputs overlap neither inputs nor each other.  T == 0 or D == 0 is a no-op.
+ */
+clove_status_t clove_block_norm(const void* x, int64_t x_stride, const void* residual,
+                                int64_t residual_stride, const void* post_weight, const void* gate,
+                                int64_t gate_stride, float scale, const void* pre_weight, void* y_out,
+                                int64_t y_out_stride, void* h_out, int64_t h_out_stride, int T, int D,
+                                float eps, int dtype, int residual_dtype, void* stream);
+
+typedef enum clove_route_score {
+    CLOVE_ROUTE_SOFTMAX = 0, /* exp(x_e) / the sum of it over the token's available experts */
+    CLOVE_ROUTE_SIGMOID = 1  /* 1 / (1 + exp(-x_e)) */
+} clove_route_score_t;
+
+/*
+ * The experts of each token and their weights, from the router's logits
+ * [T, experts] (`dtype`: FP16, BF16 or FP32; rows logits_stride apart):
+ *   s_e = score of x_e;  c_e = s_e + bias_e (bias [experts] fp32, NULL: none)
+ *   groups > 1: the experts are that many equal runs; the value of a run is the
+ *   sum of its group_top (1 or 2) largest c, and only those of the top_groups
+ *   largest values are left
+ *   ids[t, 0 : top_k]  = the experts of the largest c (without a bias: of the
+ *   largest x), largest first
+ *   weights[t, j]      = scale * s of that expert, where `renormalize` divided
+ *   by the sum of the chosen ones' (a sum of 0 divides nothing)
+ * Equal values go to the lowest index.  s, c and the sums are 64 bits: only
+ * the weights (fp32) are rounded.  An expert whose logit or bias is NaN or
+ * -infinity is not available; a place for which no expert is left has id -1
+ * and weight 0.  +infinity counts as the limit (softmax: shared equally among
+ * those that have it).
+ */
+clove_status_t clove_moe_route(const void* logits, int64_t logits_stride, int dtype, const float* bias,
+                               int score, int groups, int top_groups, int group_top, int top_k,
+                               int renormalize, float scale, int32_t* ids, float* weights, int T,
+                               int experts, void* stream);
+
+/*
+ * clove_w4a16_swiglu with weights of its own for every (token, place) pair
+ * p = t * top_k + j, those of expert e = expert_ids[p]:
+ *   H[p, i] = fp16(silu(g) * u),  g = X[t] . dequant(W[e, i]),
+ *                                 u = X[t] . dequant(W[e, I + i])
+ * X [T, K] fp16, expert_ids [T, top_k], W_q [experts, 2 I, K / 2] in gemm_int4's
+ * A layout (of each expert the I gate rows, then the I up rows), W_scale /
+ * W_zero [experts, 2 I, ceil(K / 128)] fp16, H [T top_k, I] fp16.  g and u stay
+ * fp32 (no rounding before SwiGLU).  A pair whose id lies outside [0, experts)
+ * (a padding token, an expert of another device) has no product and its row of
+ * H is left as it is; an expert may come twice in a row.  K is even.  Which
+ * kernel runs goes by the sizes and alignments alone, and a row's bits do not
+ * depend on what other tokens chose.
+ */
+clove_status_t clove_moe_w4a16_swiglu(const void* X, const int32_t* expert_ids, const uint8_t* W_q,
+                                      const void* W_scale, const void* W_zero, void* H, int T, int top_k,
+                                      int experts, int I, int K, void* stream);
+
+/*
+ * clove_gemm_w4a16 with weights of its own for every pair, summed over the
+ * token's places:
+ *   Y[t, o] = alpha * sum_j weights[t, j] * (H[p] . dequant(W[e, o]))
+ *             + beta * Y[t, o],   p = t * top_k + j, e = expert_ids[p]
+ * H [T top_k, K] fp16, expert_ids [T, top_k], weights [T, top_k] fp32 (NULL: 1),
+ * W_q [experts, O, K / 2], W_scale / W_zero [experts, O, ceil(K / 128)] fp16,
+ * Y [T, O] fp16, rounded once.  The row of H and the weight of a pair without a
+ * product (see above) are not used; a token without any gets beta * Y.
+ * beta == 0 never reads Y.  K is even.
+ */
+clove_status_t clove_moe_w4a16(const void* H, const int32_t* expert_ids, const float* weights,
+                               const uint8_t* W_q, const void* W_scale, const void* W_zero, void* Y, int T,
+                               int top_k, int experts, int O, int K, float alpha, float beta, void* stream);
+
 /* Caller-owned workspace (no reference counterpart: the reference allocates no
  * scratch).  Per host thread, three modes:
  *

@@ -1,0 +1,563 @@
+"""The sparse MLP block's operators against their plain 64-bit definitions (_moe_ref).
+
+Tolerances.  An output is rounded once: half a unit in the last place.  What fp32
+leaves before that:
+ * norms: a sum of D <= 32768 squares in a tree of at most 32 + 6 + 16 additions, at
+   most 54 2^-24 of it, half of that in its root, and a handful of roundings more:
+   below 40 2^-24 = 2.4e-6 of the terms an element is made of; 4e-6 is taken.
+ * products: a group's sum adds at most 128 exact products, each addition off by at
+   most 2^-23 of the partial sum (MFMA may truncate), the fold of G groups, K splits
+   and places by 2^-24 each: (256 + 2 G + 64) 2^-24 of the sum of the terms' sizes,
+   and 8 2^-24 for SwiGLU.
+ * routing: ids are equal; weights are 64-bit results rounded to fp32.
+"""
+import numpy as np
+import pytest
+
+from tests import _moe_ref as ref
+from tests._util import rng
+from tests.test_decode_gpu import HALF_ULP, TINY, _dev, _dt, _f64, _rounded
+
+pytestmark = pytest.mark.gpu
+
+
+def _cg():
+    import clove_compute_amd as cg
+    return cg
+
+
+def _close(got, want, dtype, extra):
+    got, want = _f64(got), np.asarray(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = np.isfinite(want)
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    err = np.abs(got - np.where(ok, want, 0.0))[ok]
+    bound = HALF_ULP[dtype] * np.abs(want[ok]) * 1.0001 + TINY[dtype] + np.broadcast_to(extra, want.shape)[ok]
+    assert np.all(err <= bound), (float(np.max(err - bound)), float(err.max()))
+
+
+# ---- block_norm ---------------------------------------------------------------
+
+FP32 = 4e-6
+
+
+def _norm_bounds(x, residual, post, gate, scale, pre, eps, y, h):
+    """What fp32 may leave in y and h."""
+    term = np.zeros_like(y)
+    if x is not None:
+        u = np.abs(x) if post is None else np.abs(x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * post)
+        term = np.abs(scale) * u * (1.0 if gate is None else np.abs(gate))
+    size = term + (0.0 if residual is None else np.abs(residual))
+    r = 1.0 / np.sqrt((y * y).mean(-1, keepdims=True) + eps)
+    return FP32 * size, FP32 * (size * r * (1.0 if pre is None else np.abs(pre)) + np.abs(h))
+
+
+@pytest.mark.parametrize("dtype,wide", [("fp16", False), ("bf16", False), ("fp16", True), ("bf16", True)])
+@pytest.mark.parametrize("T,D,post,gate,pre", [
+    (1, 2048, True, "row", True), (1, 1, True, "row", True), (3, 7, True, "rows", True), (5, 8, False, "none", True), (2, 64, True, "none", False),
+    (4, 129, False, "rows", False), (3, 1000, True, "rows", True), (2, 4100, True, "row", True), (7, 5120, True, "rows", True),
+    (2, 8192, False, "none", True), (2, 8195, True, "rows", True), (1, 16384, True, "row", True), (2, 32768, True, "rows", True),
+    (1, 32767, True, "row", True), (300, 512, True, "none", True), (2, 16391, True, "rows", True), (70, 4096, True, "row", True)])
+def test_norm_values(dtype, wide, T, D, post, gate, pre):
+    import torch
+    cg = _cg()
+    g = rng("norm", T, D, dtype, wide)
+    rt = "fp32" if wide else dtype
+    x, x64 = _rounded(g, dtype, T, D, scale=2.0)
+    r, r64 = _rounded(g, rt, T, D, scale=3.0)
+    wo, wo64 = _rounded(g, dtype, D) if post else (None, None)
+    wi, wi64 = _rounded(g, dtype, D) if pre else (None, None)
+    ga, ga64 = _rounded(g, dtype, *((T, D) if gate == "rows" else (D,))) if gate != "none" else (None, None)
+    y, h = torch.full((T, D), 7.0, dtype=_dt(rt), device="cuda"), torch.full((T, D), 7.0, dtype=_dt(dtype), device="cuda")
+    cg.block_norm(x, r, h, T, D, y_out=y, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
+    y64, h64 = ref.block_norm(x64, r64, wo64, ga64, 0.5, wi64, 1e-5)
+    by, bh = _norm_bounds(x64, r64, wo64, ga64, 0.5, wi64, 1e-5, y64, h64)
+    _close(y, y64, rt, by)
+    _close(h, h64, dtype, bh)
+    # parts left out
+    h2, y2 = torch.empty_like(h), torch.empty_like(y)
+    cg.block_norm(x, r, h2, T, D, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
+    cg.block_norm(x, r, None, T, D, y_out=y2, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
+    assert torch.equal(h, h2) and torch.equal(y, y2)
+    # in place
+    x3, r3 = x.clone(), r.clone()
+    cg.block_norm(x3, r3, x3, T, D, y_out=r3, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
+    assert torch.equal(h, x3) and torch.equal(y, r3)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D,pad,at", [(64, 8, 0), (100, 3, 1), (2050, 1, 5), (8192, 8, 8), (333, 0, 1)])
+def test_norm_strides_and_absent_inputs(dtype, D, pad, at):
+    import torch
+    cg = _cg()
+    T = 5
+    g = rng("norm-strides", D, pad)
+    wide, wide64 = _rounded(g, dtype, 3, T, D + pad + at)
+    x, r, ga = (w[:, at:at + D] for w in wide)
+    x64, r64, ga64 = (w[:, at:at + D] for w in wide64)
+    both = torch.full((T, 2 * D + 5), 3.0, dtype=_dt(dtype), device="cuda")
+    y, h = both[:, 1:1 + D], both[:, D + 3:2 * D + 3]  # rows of one tensor
+    for args, plain in [(dict(x=x, residual=r, gate=ga), (x64, r64, ga64)), (dict(x=None, residual=r), (None, r64, None)),
+                        (dict(x=x, residual=None, gate=ga), (x64, None, ga64))]:
+        both.fill_(3.0)
+        cg.block_norm(args["x"], args["residual"], h, T, D, y_out=y, gate=args.get("gate"), scale=1.5)
+        px, pr, pg = plain
+        y64, h64 = ref.block_norm(px, pr, None, pg, 1.5, None, 1e-6)
+        by, bh = _norm_bounds(px, pr, None, pg, 1.5, None, 1e-6, y64, h64)
+        _close(y, y64, dtype, by)
+        _close(h, h64, dtype, bh)
+        rest = torch.cat((both[:, :1], both[:, 1 + D:D + 3], both[:, 2 * D + 3:]), 1)
+        assert bool((rest == 3.0).all())
+    assert np.array_equal(_f64(wide), wide64)
+
+
+def test_norm_rows_do_not_meet():
+    """A row of zeros, of infinities or NaN and of the type's largest values changes no other."""
+    import torch
+    cg = _cg()
+    T, D = 6, 200
+    g = rng("norm-odd-rows")
+    x, x64 = _rounded(g, "fp16", T, D)
+    x[1], x[2, 7], x[3, 199], x[4] = 0.0, float("inf"), float("nan"), 65504.0
+    x64 = _f64(x)
+    w, w64 = _rounded(g, "fp16", D)
+    r = torch.zeros(T, D, device="cuda")
+    h, y = torch.empty_like(x), torch.empty_like(r)
+    cg.block_norm(x, r, h, T, D, y_out=y, pre_weight=w)
+    y64, h64 = ref.block_norm(x64, np.zeros((T, D)), None, None, 1.0, w64, 1e-6)
+    keep = [0, 1, 4, 5]
+    _close(y[keep], y64[keep], "fp32", 0.0)
+    _close(h[keep], h64[keep], "fp16", FP32 * np.abs(h64[keep]))
+    assert not bool(torch.isfinite(h[3]).any())
+    # an infinite scale past the end of an odd row
+    cg.block_norm(x[:1, :199].contiguous(), None, None, 1, 199, y_out=y[:1, :199].contiguous(), scale=float("inf"))
+
+
+# ---- moe_route ----------------------------------------------------------------
+
+def _route(cg, x, bias, k, E=None, **kw):
+    import torch
+    T = x.shape[0]
+    ids = torch.full((T, k), 77, dtype=torch.int32, device="cuda")
+    w = torch.full((T, k), 7.0, device="cuda")
+    cg.moe_route(x, ids, w, T, x.shape[1] if E is None else E, k, bias=bias, **kw)
+    return ids, w
+
+
+def _check_route(x, bias, got, k, score, groups=1, top_groups=1, group_top=1, renormalize=False, scale=1.0):
+    ids, w = got
+    want, w64 = ref.route(_f64(x), None if bias is None else _f64(bias), score, groups, top_groups, group_top, k, renormalize, scale)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    _close(w, w64, "fp32", 1e-12 * np.abs(w64) + 1e-45)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("T,E,k,groups,top_groups,group_top,biased", [
+    (1, 1, 1, 1, 1, 1, False), (1, 8, 2, 1, 1, 1, False), (9, 8, 8, 1, 1, 1, True), (5, 7, 3, 1, 1, 1, True), (33, 64, 6, 1, 1, 1, False),
+    (17, 60, 4, 1, 1, 1, False), (12, 65, 9, 5, 2, 2, True), (40, 128, 8, 8, 3, 1, False), (21, 160, 6, 8, 3, 2, False), (50, 256, 8, 8, 4, 2, True),
+    (3, 384, 12, 1, 1, 1, True), (4, 1024, 64, 64, 32, 2, True), (2, 1000, 10, 8, 8, 1, False), (3, 64, 64, 64, 64, 1, True), (300, 16, 4, 4, 2, 2, True),
+    (5, 513, 5, 27, 4, 2, False), (130, 32, 1, 2, 1, 1, True)])
+def test_route_values(score, dtype, T, E, k, groups, top_groups, group_top, biased):
+    cg = _cg()
+    g = rng("route", T, E, k, score)
+    x, _ = _rounded(g, dtype, T, E, scale=2.0)
+    bias = _dev((g.standard_normal(E) * 0.2).astype(np.float32)) if biased else None
+    for renorm, scale in [(False, 1.0), (True, 2.5)]:
+        how = dict(groups=groups, top_groups=top_groups, group_top=group_top, renormalize=renorm, scale=scale)
+        got = _route(cg, x, bias, k, score=getattr(cg, "CLOVE_ROUTE_" + score.upper()), **how)
+        _check_route(x, bias, got, k, score, **how)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased,groups", [(False, 1), (True, 1), (False, 4), (True, 4)])
+def test_route_ties_and_masks(score, biased, groups):
+    """Equal values, -inf, +inf and NaN logits, rows with few experts left or none, values
+    far from each other (scores that underflow)."""
+    cg = _cg()
+    E, k = 48, 6
+    g = rng("route-ties", score, biased, groups)
+    x = np.round(g.standard_normal((14, E)) * 2).astype(np.float32)  # many equal
+    x[1] = 0.0
+    x[2] = -np.inf
+    x[3, 5:] = -np.inf
+    x[4, ::2] = np.nan
+    x[5] = np.nan
+    x[6, 7], x[6, 30] = np.inf, np.inf
+    x[7] = np.where(np.arange(E) % 5 == 0, x[7], -np.inf)
+    x[8] = np.linspace(-2000, 2000, E)
+    x[9] = np.linspace(100, -200, E)
+    x[10] = -np.arange(E)[::-1] * 40.0
+    x[11, 1:] = -np.inf
+    x[12] = 1e30
+    x[13] = -3.0e38
+    bias = None
+    if biased:
+        b = np.round(g.standard_normal(E) * 4).astype(np.float32) / 8
+        b[3], b[9], b[20] = -np.inf, np.nan, np.inf
+        bias = _dev(b)
+    t = _dev(x)
+    for renorm in (False, True):
+        how = dict(groups=groups, top_groups=2 if groups > 1 else 1, group_top=2 if groups > 1 else 1, renormalize=renorm)
+        got = _route(cg, t, bias, k, score=getattr(cg, "CLOVE_ROUTE_" + score.upper()), **how)
+        _check_route(t, bias, got, k, score, **how)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_values_that_nearly_agree(score):
+    """Scores plus bias one part in 2^30 apart: 32 bits cannot tell them, 64 can."""
+    cg = _cg()
+    T, E, k = 64, 64, 8
+    g = rng("route-near", score)
+    x = g.standard_normal((T, E)).astype(np.float32)
+    x[:, 32:] = x[:, :32] + (g.integers(-2, 3, (T, 32)) * 2.0 ** -22).astype(np.float32)
+    b = np.zeros(E, np.float32)
+    b[::2], b[1::2] = 2.0 ** -40, -2.0 ** -40
+    got = _route(cg, _dev(x), _dev(b), k, score=getattr(cg, "CLOVE_ROUTE_" + score.upper()))
+    _check_route(_dev(x), _dev(b), got, k, score)
+
+
+def test_route_rows_of_wider_tensors():
+    cg = _cg()
+    g = rng("route-wide")
+    wide, _ = _rounded(g, "fp16", 9, 101)
+    x = wide[:, 3:3 + 60]
+    _check_route(x, None, _route(cg, x, None, 4), 4, "softmax")
+
+
+# ---- the experts' products ------------------------------------------------------
+
+def _ids(g, T, k, E, absent=0.0, distinct=True):
+    ids = np.stack([g.permutation(E)[:k] if distinct and k <= E else g.integers(0, E, k) for _ in range(T)]).astype(np.int32)
+    if absent:
+        ids[g.random((T, k)) < absent] = -1
+    return ids
+
+
+class Case:
+    def __init__(self, key, T, k, E, R, K, absent=0.0, distinct=True, offset=0, whole=True):
+        import torch
+        g = self.g = rng("moe", key, T, k, E, R, K)
+        self.T, self.k, self.E, self.R, self.K = T, k, E, R, K
+        G = -(-K // ref.GROUP)
+        self.ids = _ids(g, T, k, E, absent, distinct)
+        q = g.integers(0, 256, (E, R, K // 2)).astype(np.uint8)
+        s = g.uniform(0.5, 1.5, (E, R, G)).astype(np.float16) / np.float16(max(1.0, 4.6 * K ** 0.5))
+        z = g.integers(0, 16, (E, R, G)).astype(np.float16)
+        if not whole:
+            z = (z + g.uniform(-0.4, 0.4, z.shape)).astype(np.float16)  # rounded to whole numbers by the call
+        self.w = ref.dequantized(q, s, z, K)
+        flat = torch.zeros(q.size + offset, dtype=torch.uint8, device="cuda")
+        flat[offset:] = _dev(q).flatten()
+        self.q, self.s, self.z, self.dev_ids = flat[offset:].view(E, R, K // 2), _dev(s), _dev(z), _dev(self.ids)
+        self.slack = (256 + 2 * G + 64) * 2.0 ** -24
+
+
+def _up(cg, c, x, h):
+    cg.moe_w4a16_swiglu(x, c.dev_ids, c.q, c.s, c.z, h, c.T, c.k, c.E, c.R // 2, c.K)
+
+
+def _check_up(cg, c, x=None):
+    import torch
+    if x is None:
+        x, _ = _rounded(c.g, "fp16", c.T, c.K)
+    h = torch.full((c.T * c.k, c.R // 2), 5.0, dtype=torch.float16, device="cuda")
+    want, size = ref.swiglu_up(_f64(x), c.ids, c.w, _f64(h))
+    _up(cg, c, x, h)
+    _close(h, want, "fp16", c.slack * size)
+    again = torch.full_like(h, 5.0)
+    _up(cg, c, x, again)
+    assert torch.equal(h.view(torch.int16), again.view(torch.int16))
+    return h, want
+
+
+def _check_down(cg, c, beta=1.0, alpha=1.0, weighted=True):
+    import torch
+    h, h64 = _rounded(c.g, "fp16", c.T * c.k, c.K)
+    w = _dev(c.g.uniform(-0.5, 1.0, (c.T, c.k)).astype(np.float32)) if weighted else None
+    y0, y64 = _rounded(c.g, "fp16", c.T, c.R)
+    if beta == 0.0:
+        y0.fill_(float("nan"))  # never read
+    want, size = ref.down(h64, c.ids, None if w is None else _f64(w), c.w, y64, alpha, beta)
+    y = y0.clone()
+    cg.moe_w4a16(h, c.dev_ids, w, c.q, c.s, c.z, y, c.T, c.k, c.E, c.R, c.K, alpha=alpha, beta=beta)
+    _close(y, want, "fp16", c.slack * size)
+    again = y0.clone()
+    cg.moe_w4a16(h, c.dev_ids, w, c.q, c.s, c.z, again, c.T, c.k, c.E, c.R, c.K, alpha=alpha, beta=beta)
+    assert torch.equal(y, again)
+    return y, want
+
+
+# T, top_k, experts, outputs, K
+SIZES = [(1, 1, 1, 1, 2), (1, 2, 4, 3, 128), (1, 8, 128, 64, 256), (1, 8, 16, 768, 1024), (2, 4, 8, 100, 160), (3, 2, 4, 33, 130), (5, 8, 16, 64, 256),
+         (4, 2, 8, 48, 2048), (16, 2, 64, 80, 512), (33, 1, 2, 40, 96), (70, 3, 5, 100, 384), (130, 6, 64, 96, 192), (257, 4, 3, 48, 160),
+         (40, 8, 8, 130, 1024), (600, 2, 2, 64, 256), (64, 4, 4, 513, 640), (300, 1, 9, 256, 128), (100, 8, 256, 64, 256), (1, 1, 3, 16, 14336),
+         (20, 64, 64, 32, 128), (512, 2, 4, 320, 544), (7, 3, 4, 31, 62), (1100, 2, 8, 128, 256), (150, 2, 1024, 16, 64)]
+
+
+@pytest.mark.parametrize("T,k,E,O,K", SIZES)
+def test_up_values(T, k, E, O, K):
+    c = Case("up", T, k, E, 2 * O, K, absent=0.1 if T > 2 else 0.0)
+    got, want = _check_up(_cg(), c)
+    if K <= 1024 and got.numel() > 2000:
+        # one rounding only: an fp32 sum off by some 2^-20 moves few of them over a boundary
+        assert np.mean(_f64(got) == want.astype(np.float16).astype(np.float64)) > 0.97
+
+
+@pytest.mark.parametrize("T,k,E,O,K", SIZES)
+@pytest.mark.parametrize("beta,alpha,weighted", [(1.0, 1.0, True), (0.0, 0.5, False)])
+def test_down_values(T, k, E, O, K, beta, alpha, weighted):
+    c = Case("down", T, k, E, O, K, absent=0.1 if T > 2 else 0.0)
+    got, want = _check_down(_cg(), c, beta, alpha, weighted)
+    if K <= 1024 and got.numel() > 2000:
+        assert np.mean(_f64(got) == want.astype(np.float16).astype(np.float64)) > 0.97
+
+
+@pytest.mark.parametrize("T", [1, 3, 40, 300])
+@pytest.mark.parametrize("offset,K", [(1, 128), (4, 256), (8, 96), (16, 256), (2, 66)])
+def test_weights_at_any_alignment(T, offset, K):
+    cg = _cg()
+    _check_up(cg, Case("up-offset", T, 2, 5, 2 * 40, K, offset=offset, whole=False))
+    _check_down(cg, Case("down-offset", T, 2, 5, 72, K, offset=offset, whole=False))
+
+
+@pytest.mark.parametrize("T", [1, 2, 20, 200])
+def test_the_same_expert_twice_and_ids_that_are_none(T):
+    import torch
+    cg = _cg()
+    for key in ("up", "down"):
+        c = Case("odd-ids", T, 4, 3, 96, 256, distinct=False)
+        c.ids[:, 1] = c.ids[:, 0]
+        c.ids[T // 2, 2:] = [3, 2 ** 31 - 1]
+        c.ids[0, 3] = -2 ** 31
+        c.ids[T - 1] = -1  # a token without experts
+        c.dev_ids = torch.from_numpy(c.ids).cuda()
+        _check_up(cg, c) if key == "up" else _check_down(cg, c)
+    c.ids[:] = -1
+    c.dev_ids = torch.from_numpy(c.ids).cuda()
+    _check_up(cg, c)
+    _check_down(cg, c)
+    _check_down(cg, c, beta=0.0)
+
+
+@pytest.mark.parametrize("T,E", [(1, 4), (6, 4), (80, 4), (300, 2)])
+def test_rows_do_not_meet(T, E):
+    """NaN and infinities stay in their token's rows, and what no expert reads is not used."""
+    import torch
+    cg = _cg()
+    k, K, O = 2, 256, 48
+    c = Case("nan", T, k, E, 2 * O, K)
+    c.ids[0, 1] = -1
+    c.dev_ids = torch.from_numpy(c.ids).cuda()
+    x, _ = _rounded(c.g, "fp16", T, K)
+    if T > 1:
+        x[T // 2, 3], x[T - 1, 0] = float("nan"), float("inf")
+    h = torch.full((T * k, O), 5.0, dtype=torch.float16, device="cuda")
+    _up(cg, c, x, h)
+    want, size = ref.swiglu_up(_f64(x), c.ids, c.w, np.full((T * k, O), 5.0))
+    rows = [p for p in range(T * k) if T == 1 or p // k not in (T // 2, T - 1)]
+    _close(h[rows], want[rows], "fp16", c.slack * size[rows])
+    if T > 1:
+        assert bool(torch.isnan(h[T // 2 * k:T // 2 * k + k]).all())
+    d = Case("nan-down", T, k, E, O, K)
+    d.ids[0, 1] = -1
+    d.dev_ids = torch.from_numpy(d.ids).cuda()
+    hin, _ = _rounded(d.g, "fp16", T * k, K)
+    w = torch.rand(T, k, device="cuda")
+    hin[1], w[0, 1] = float("nan"), float("nan")  # a pair without a product
+    if T > 1:
+        hin[(T // 2) * k + 1, 5] = float("inf")
+    y = torch.zeros(T, O, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16(hin, d.dev_ids, w, d.q, d.s, d.z, y, T, k, E, O, K)
+    clean = torch.where(torch.isfinite(hin), hin, 0.0)
+    want, size = ref.down(_f64(clean), d.ids, np.nan_to_num(_f64(w)), d.w, np.zeros((T, O)), 1.0, 0.0)
+    rows = [t for t in range(T) if T == 1 or t != T // 2]
+    _close(y[rows], want[rows], "fp16", d.slack * size[rows])
+    if T > 1:
+        assert not bool(torch.isfinite(y[T // 2]).all())
+
+
+@pytest.mark.parametrize("O,K", [(40, 0), (5, 0)])
+def test_no_k(O, K):
+    import torch
+    cg = _cg()
+    T, k, E = 3, 2, 4
+    ids = torch.tensor([[0, 1], [2, -1], [3, 3]], dtype=torch.int32, device="cuda")
+    none, half = torch.empty(0, dtype=torch.uint8, device="cuda"), torch.empty(0, dtype=torch.float16, device="cuda")
+    h = torch.full((T * k, O), 5.0, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16_swiglu(half, ids, none, half, half, h, T, k, E, O, K)
+    assert bool((h[[0, 1, 2, 4, 5]] == 0).all()) and bool((h[3] == 5).all())
+    y = torch.full((T, O), 3.0, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16(half, ids, None, none, half, half, y, T, k, E, O, K, beta=2.0)
+    assert bool((y == 6).all())
+
+
+@pytest.mark.parametrize("T", [1, 50])
+def test_experts_past_four_gigabytes(T):
+    """The last of 1024 experts lies past 2^32 bytes of weights."""
+    import torch
+    cg = _cg()
+    E, R, K, k = 1024, 4096, 2304, 1
+    q = torch.zeros(E, R, K // 2, dtype=torch.uint8, device="cuda")
+    s, z = torch.ones(E, R, K // 128, dtype=torch.float16, device="cuda"), torch.zeros(E, R, K // 128, dtype=torch.float16, device="cuda")
+    g = rng("far", T)
+    last = g.integers(0, 256, (R, K // 2)).astype(np.uint8)
+    q[-1] = _dev(last)
+    s[-1] = 2.0 ** -9
+    ids = torch.full((T, k), E - 1, dtype=torch.int32, device="cuda")
+    x, x64 = _rounded(g, "fp16", T, K)
+    w = ref.dequantized(last, np.full((R, K // 128), 2.0 ** -9), np.zeros((R, K // 128)), K)[None]
+    zeros = np.zeros((T, k), np.int32)
+    slack = (256 + 2 * 18 + 64) * 2.0 ** -24
+    h = torch.zeros(T, R // 2, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16_swiglu(x, ids, q, s, z, h, T, k, E, R // 2, K)
+    want, size = ref.swiglu_up(x64, zeros, w, np.zeros((T, R // 2)))
+    ok = np.abs(want) < 65000
+    _close(h[torch.from_numpy(ok).cuda()], want[ok], "fp16", (slack * size)[ok])
+    y = torch.zeros(T, R, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16(x, ids, None, q, s, z, y, T, k, E, R, K)
+    want, size = ref.down(x64, zeros, None, w, np.zeros((T, R)), 1.0, 0.0)
+    _close(y, want, "fp16", slack * size)
+
+
+# ---- workspaces, graphs, streams, the block as a whole ----------------------------
+
+@pytest.mark.parametrize("T", [1, 4, 40, 400])
+def test_bound_workspace_and_its_size(T):
+    import torch
+    cg = _cg()
+    c = Case("workspace", T, 4, 8, 128, 256)
+    x, _ = _rounded(c.g, "fp16", T, 256)
+    hin, _ = _rounded(c.g, "fp16", T * 4, 256)
+    w = torch.rand(T, 4, device="cuda")
+    h, y = torch.zeros(T * 4, 64, dtype=torch.float16, device="cuda"), torch.zeros(T, 128, dtype=torch.float16, device="cuda")
+
+    def calls():
+        _up(cg, c, x, h)
+        cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, 256)
+        return h.clone(), y.clone()
+
+    want = calls()
+    h.zero_(), y.zero_()
+    with cg.workspace_query() as q:
+        calls()
+    torch.cuda.synchronize()
+    assert not bool(h.any()) and not bool(y.any())  # only planned
+    if q.bytes == 0:
+        return
+    ws = torch.zeros(q.bytes, dtype=torch.uint8, device="cuda")
+    cg.workspace_bind(ws)
+    try:
+        got = calls()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert not bool(ws[:cg.CLOVE_WORKSPACE_MIN_BYTES].any())
+        cg.workspace_bind(ws[:cg.CLOVE_WORKSPACE_MIN_BYTES])
+        h.fill_(3.0), y.fill_(3.0)
+        with pytest.raises(cg.CloveError) as e:
+            for call in (lambda: _up(cg, c, x, h), lambda: cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, 256)):
+                call()
+        assert e.value.status == cg.CLOVE_ERR_WORKSPACE
+    finally:
+        cg.workspace_bind()
+
+
+class Block:
+    """norm, router, experts and the norm after them, as a decoder's sparse MLP block calls them."""
+
+    def __init__(self, T, hidden=256, inter=192, E=16, k=4, seed=0):
+        import torch
+        g = self.g = rng("block", T, seed)
+        self.T, self.D, self.I, self.E, self.k = T, hidden, inter, E, k
+        self.up, self.down = Case(("block-up", seed), T, k, E, 2 * inter, hidden), Case(("block-down", seed), T, k, E, hidden, inter)
+        self.router, self.router64 = _rounded(g, "fp16", hidden, E, scale=hidden ** -0.5)
+        self.pre, self.pre64 = _rounded(g, "fp16", hidden)
+        self.post, self.post64 = _rounded(g, "fp16", hidden)
+        self.next, self.next64 = _rounded(g, "fp16", hidden)
+        self.residual, _ = _rounded(g, "fp32", T, hidden, scale=2.0)
+        half = dict(dtype=torch.float16, device="cuda")
+        self.x, self.y = torch.empty(T, hidden, **half), torch.empty(T, hidden, **half)
+        self.logits, self.h = torch.empty(T, E, **half), torch.zeros(T * k, inter, **half)
+        self.ids, self.w = torch.empty(T, k, dtype=torch.int32, device="cuda"), torch.empty(T, k, device="cuda")
+        self.stream, self.out = torch.empty_like(self.residual), torch.empty_like(self.x)
+
+    def __call__(self):
+        cg, T, D = _cg(), self.T, self.D
+        cg.block_norm(None, self.residual, self.x, T, D, pre_weight=self.pre)
+        cg.gemm_fp16(self.x, self.router, self.logits, T, self.E, D)
+        cg.moe_route(self.logits, self.ids, self.w, T, self.E, self.k, renormalize=True)
+        u, d = self.up, self.down
+        cg.moe_w4a16_swiglu(self.x, self.ids, u.q, u.s, u.z, self.h, T, self.k, self.E, self.I, D)
+        cg.moe_w4a16(self.h, self.ids, self.w, d.q, d.s, d.z, self.y, T, self.k, self.E, D, self.I)
+        cg.block_norm(self.y, self.residual, self.out, T, D, y_out=self.stream, post_weight=self.post, pre_weight=self.next, scale=0.7)
+        return [t.clone() for t in (self.x, self.ids, self.w, self.h, self.y, self.stream, self.out)]
+
+    def check(self):
+        """Each operator against its definition on what it was given."""
+        r, x = _f64(self.residual), _f64(self.x)
+        zero, x64 = ref.block_norm(None, r, None, None, 1.0, self.pre64, 1e-6)
+        _close(self.x, x64, "fp16", _norm_bounds(None, r, None, None, 1.0, self.pre64, 1e-6, zero, x64)[1])
+        _check_route(self.logits, None, (self.ids, self.w), self.k, "softmax", renormalize=True)
+        ids = self.ids.cpu().numpy()
+        h64, size = ref.swiglu_up(x, ids, self.up.w, np.zeros(self.h.shape))
+        _close(self.h, h64, "fp16", self.up.slack * size)
+        y64, size = ref.down(_f64(self.h), ids, _f64(self.w), self.down.w, np.zeros(self.y.shape), 1.0, 0.0)
+        _close(self.y, y64, "fp16", self.down.slack * size)
+        s64, o64 = ref.block_norm(_f64(self.y), r, self.post64, None, 0.7, self.next64, 1e-6)
+        by, bh = _norm_bounds(_f64(self.y), r, self.post64, None, 0.7, self.next64, 1e-6, s64, o64)
+        _close(self.stream, s64, "fp32", by)
+        _close(self.out, o64, "fp16", bh)
+
+
+@pytest.mark.parametrize("T", [1, 3, 24, 200])
+def test_block(T):
+    block = Block(T)
+    block()
+    block.check()
+
+
+def _bits(ts):
+    return [t.cpu().numpy().tobytes() for t in ts]
+
+
+@pytest.mark.parametrize("T", [1, 24, 200])
+def test_block_in_a_graph(T):
+    """Replays with other inputs, eager work between them, two graphs of one stream."""
+    import torch
+    blocks = [Block(T, seed=s) for s in (0, 1)]
+    side = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(side):
+        for b in blocks:
+            b()  # (scratch of this stream)
+        side.synchronize()
+        for b in blocks:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                b()
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for i in range(4):
+        for b, graph in zip(blocks, graphs):
+            b.residual.copy_(torch.randn_like(b.residual))
+            want = _bits(b())
+            for t in (b.x, b.h, b.y, b.stream, b.out, b.ids):
+                t.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert _bits((b.x, b.ids, b.w, b.h, b.y, b.stream, b.out)) == want, i
+            b.check()
+
+
+def test_blocks_on_two_streams_and_threads():
+    import torch
+
+    from tests.test_decode_concurrency_gpu import _at_once
+    blocks = [Block(T, seed=s) for s, T in enumerate((1, 24, 200, 3))]
+    want = [_bits(b()) for b in blocks]
+    torch.cuda.synchronize()
+    one, streams = torch.cuda.current_stream(), [torch.cuda.Stream(), torch.cuda.Stream()]
+    for stream_of in (lambda i: one, lambda i: streams[i % 2]):
+        got = _at_once(blocks, 10, stream_of)
+        for i, runs in enumerate(got):
+            assert all(_bits(run) == want[i] for run in runs), i
