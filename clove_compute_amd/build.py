@@ -55,6 +55,7 @@ CFLAGS = [
 # separate v_accvgpr_read), as the attention kernel does its output sums, which
 # a new maximum rescales
 EXTRA = {"paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "moe_w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "i4w_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "i4i4_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 

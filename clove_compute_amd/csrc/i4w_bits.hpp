@@ -32,15 +32,14 @@ __device__ __forceinline__ void dma4(const u32x4& rsrc, unsigned lds_addr, int v
                  : "memory");
 }
 
-// (q - z) * 2^-9 for the 8 nibbles of one dword, in k order; zz = -z * 2^-9.
+// (q - z) * 2^-9 for the 8 nibbles of one dword, in k order; zz = -z * 2^-9, mul what
+// takes the two subnormals of a byte to q * 2^-9 (0, and zz 0: makes all of them 0).
 // Byte b holds k = 2b and 2b + 1: in the high and low nibble (the weights'
 // packing), or with LO_FIRST in the low and high nibble (the order in which
 // ds_read_b64_tr_b4 returns k rows)
 template <bool LO_FIRST = false>
-__device__ __forceinline__ f16x8 unpack8(unsigned w, f16x2 zz) {
+__device__ __forceinline__ f16x8 unpack8(unsigned w, f16x2 mul, f16x2 zz) {
     const unsigned hr = w & 0xf0f0f0f0u, lo = w & 0x0f0f0f0fu;
-    const f16x2 mul = LO_FIRST ? f16x2{(_Float16)32768.0f, (_Float16)2048.0f}
-                               : f16x2{(_Float16)2048.0f, (_Float16)32768.0f};
     f16x2 v[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -55,6 +54,13 @@ __device__ __forceinline__ f16x8 unpack8(unsigned w, f16x2 zz) {
     r.s45 = v[2];
     r.s67 = v[3];
     return r;
+}
+template <bool LO_FIRST = false>
+__device__ __forceinline__ f16x8 unpack8(unsigned w, f16x2 zz) {
+    return unpack8<LO_FIRST>(w,
+                             LO_FIRST ? f16x2{(_Float16)32768.0f, (_Float16)2048.0f}
+                                      : f16x2{(_Float16)2048.0f, (_Float16)32768.0f},
+                             zz);
 }
 
 // A 16-byte LDS read serves 16 lanes per clock from one 256-byte window of

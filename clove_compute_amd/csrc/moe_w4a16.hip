@@ -13,6 +13,8 @@
 // meets the pairs of one expert (moe_any), and the places of a token are added
 // up from fp32 partial results in place order (moe_combine), so that a call
 // gives the same bits every time.
+#include <cstdlib>
+
 #include "i4w_bits.hpp"
 #include "moe.hpp"
 
@@ -25,48 +27,63 @@ struct Params {
     MoeArgs a;
     int* off;      // [experts + 1]: where an expert's pairs begin in `order`
     int* order;    // [T top_k]: pairs, those of one expert after those of the one before
-    float* part;   // down: [T top_k, O] products
+    float* part;   // down: [T top_k, ldp] products with the outputs o0 .. o0 + on - 1
+    int o0, on, ldp;
     FastDiv k;     // by top_k
     int rows_t;    // tiles of weight rows
     int P, G;
+    int64_t x_bytes;  // of X
 };
 
-// Workgroup e lists the pairs of expert e in order; where they begin is the
-// number of pairs of lower experts, which it counts itself: no workgroup waits
-// for another.  (128 experts read 65536 ids each from the L2s.)
-__global__ void __launch_bounds__(256) moe_sort(const int32_t* ids, int P, int E, int* off, int* order) {
-    __shared__ int lds[2][4];
-    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Workgroup e lists the pairs of expert e; where they begin is the number of pairs of
+// lower experts, which it counts itself: no workgroup waits for another.  A thread
+// lists its own pairs behind those of the threads before it, so the ids are read
+// twice and nothing waits but for the one scan of the counts between.
+constexpr int kSortThreads = 1024;
+__global__ void __launch_bounds__(kSortThreads) moe_sort(const int32_t* ids, int P, int E, int* off, int* order) {
+    __shared__ int lds[2][kSortThreads / 64];
+    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, step = 4 * blockDim.x;
     int less = 0, mine = 0;
-    for (int p = tid; p < P; p += 256) {
-        const int id = ids[p];
-        less += id >= 0 && id < e;
-        mine += id == e;
-    }
-    less = wave_sum(less), mine = wave_sum(mine);
-    if (lane == 0) lds[0][wave] = less, lds[1][wave] = mine;
-    __syncthreads();
-    int at = lds[0][0] + lds[0][1] + lds[0][2] + lds[0][3];
-    const int count = lds[1][0] + lds[1][1] + lds[1][2] + lds[1][3];
-    if (tid == 0) {
-        off[e] = at;
-        if (e == E - 1) off[E] = at + count;
-    }
-    if (count == 0) return;
-    for (int p0 = 0; p0 < P; p0 += 256) {
-        const int p = p0 + tid;
-        const bool is = p < P && ids[p] == e;
-        const uint64_t m = __ballot(is);
-        __syncthreads();
-        if (lane == 0) lds[0][wave] = __popcll(m);
-        __syncthreads();
-        int before = at;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) before += lds[0][w];
-            at += lds[0][w];
+    const int whole = P & ~3;
+    auto load = [&](int p) { return *reinterpret_cast<const u32x4u*>(ids + p); };
+#pragma unroll 4
+    for (int p = 4 * tid; p < whole; p += step) {
+        const u32x4 v = load(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            less += v[i] < (unsigned)e;
+            mine += v[i] == (unsigned)e;
         }
-        if (is) order[before + __popcll(m & (((uint64_t)1 << lane) - 1))] = p;
     }
+    const bool tail = tid < P - whole;  // of the last, partial four ids one a thread
+    const unsigned last = tail ? (unsigned)ids[whole + tid] : ~0u;
+    less += last < (unsigned)e;
+    mine += last == (unsigned)e;
+    const int upto = wave_scan(mine);
+    less = wave_sum(less);
+    if (lane == 63) lds[0][wave] = upto;
+    if (lane == 0) lds[1][wave] = less;
+    __syncthreads();
+    int begin = 0, count = 0, at = upto - mine;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+        begin += lds[1][w];
+        if (w < wave) at += lds[0][w];
+        count += lds[0][w];
+    }
+    if (tid == 0) {
+        off[e] = begin;
+        if (e == E - 1) off[E] = begin + count;
+    }
+    if (mine == 0) return;
+    at += begin;
+#pragma unroll 4
+    for (int p = 4 * tid; p < whole; p += step) {
+        const u32x4 v = load(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (v[i] == (unsigned)e) order[at++] = p + i;
+    }
+    if (last == (unsigned)e) order[at] = whole + tid;
 }
 
 // Tile `tile` of BC pairs.  Expert e's tiles are numbered off[e] / BC + e and on:
@@ -104,7 +121,7 @@ __global__ void __launch_bounds__(256) moe_any(const Params p) {
     if (tid < AC) pair[tid] = p.order[t.first + min(tid, t.count - 1)];
     __syncthreads();
     constexpr int OR = SWIGLU ? AR / 2 : AR;  // outputs of a tile
-    const int r0 = tr * OR, O = a.O, K = a.K, G = p.G;
+    const int r0 = p.o0 + tr * OR, O = a.O, K = a.K, G = p.G;
     const int64_t R = SWIGLU ? 2 * (int64_t)O : O;
     // weight row of tile row i (past the end: the last one, whose results go nowhere)
     auto row = [&](int i) { return (SWIGLU && i >= OR ? (int64_t)O : 0) + min(r0 + i % OR, O - 1) + t.e * R; };
@@ -183,39 +200,336 @@ __global__ void __launch_bounds__(256) moe_any(const Params p) {
             }
     } else {
         const int o = r0 + 16 * wave + l16;
-        if (o >= O) return;
+        if (o >= p.o0 + p.on) return;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const int c = 16 * j + 4 * h + v;
-                if (c < t.count) p.part[(int64_t)pair[c] * O + o] = acc[j][v];
+                if (c < t.count) p.part[(int64_t)pair[c] * p.ldp + o - p.o0] = acc[j][v];
             }
     }
 }
 
-// Y[t] = alpha sum_j w[t, j] part[t top_k + j] + beta Y[t], places in order; a
-// place without an expert is left out.
-__global__ void __launch_bounds__(256) moe_combine(const Params p) {
+// ---------------------------------------------------------------------------
+// K % 32 == 0, 16-byte aligned X and W: tiles of BR weight rows by BC pairs of one
+// expert, everything a stage needs (a 128-k group or half of one) by LDS DMA, in the
+// layout of i4w_gemm.hpp: X rows and weight rows in 16-byte chunks swizzled by the
+// row, then the aligned dwords that hold each row's scale and zero point.  The rows
+// of X are those of the tile's pairs, gathered by the DMA's per-lane offsets.
+//
+// A wave owns 32 FW weight rows by 32 FX pairs on v_mfma_f32_32x32x16_f16 with X
+// as the "A" operand: a lane holds one weight row of each block and 16 pairs.
+// SwiGLU: of every 32 rows 16 are gate rows and 16 the up rows of the same
+// outputs, which meet through v_permlane16_swap.
+//
+// The accumulators are kept in units of the current group's scale: at a group's
+// start they are multiplied by (last scale / this scale), and the group's MFMAs add
+// to them.  That is as many VALU operations as folding group sums into a second
+// set of accumulators, and half the registers: a wave holds 64 x 128 outputs with
+// two waves on a SIMD, so that an unpacked weight meets four blocks of pairs.  A
+// group whose scale is 0 leaves the unit as it is and its weights are made 0.
+// ---------------------------------------------------------------------------
+template <int WR_, int WC_, int FW_, int FX_, int S_, int KS_>
+struct Cfg {
+    static constexpr int WR = WR_, WC = WC_, FW = FW_, FX = FX_, S = S_, KS = KS_;  // KS: 16-k steps a stage
+    static constexpr int NW = WR * WC, NT = 64 * NW, BR = 32 * FW * WR, BC = 32 * FX * WC, SPG = 8 / KS;
+    static constexpr int XRB = 32 * KS, WRB = 8 * KS;  // bytes of an X row and a weight row
+    static constexpr int X_BYTES = BC * XRB, W_BYTES = BR * WRB, SC_BYTES = BR * 4;
+    static constexpr int OFF_W = X_BYTES, OFF_SC = OFF_W + W_BYTES, OFF_ZR = OFF_SC + SC_BYTES, STAGE = OFF_ZR + SC_BYTES;
+    static constexpr int DX = X_BYTES / (1024 * NW), DW = W_BYTES / (1024 * NW), DS = 2 * BR / (64 * NW);
+    static constexpr int OFF_P = S * STAGE, LDS = OFF_P + 4 * BC;  // then the tile's pairs
+    // DMA instructions of stage t of a wave (scales and zero points with a group's first)
+    static constexpr int dmas(int t) { return DX + DW + (t % SPG == 0 ? DS : 0); }
+    static_assert(KS == 8 || KS == 4, "k-steps");
+    static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && (2 * BR) % (64 * NW) == 0, "DMA split");
+    static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT, "stages");
+};
+
+template <class CF, bool SWIGLU>
+__global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
+    using namespace i4w;
+    constexpr int FW = CF::FW, FX = CF::FX, S = CF::S, BR = CF::BR, BC = CF::BC, KS = CF::KS, SPG = CF::SPG;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const MoeArgs& a = p.a;
-    const int64_t n = (int64_t)a.T * a.O, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-        const int t = (int)(i / a.O), o = (int)(i - (int64_t)t * a.O);
-        float sum = 0.0f;
-        for (int j = 0; j < a.top_k; ++j) {
-            const int q = t * a.top_k + j;
-            if ((unsigned)a.ids[q] >= (unsigned)a.experts) continue;
-            sum = fmaf(a.weights ? a.weights[q] : 1.0f, p.part[(int64_t)q * a.O + o], sum);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % CF::WR, wc = wave / CF::WR;
+
+    // ---- the tile: workgroups are dealt to the 8 XCDs in turn, and each XCD takes a
+    // contiguous run of the tiles there are, the pair tiles of one row tile after each
+    // other (they share its weights in the XCD's L2) ----
+    const int E = a.experts;
+    int tiles = 0;
+    for (int e = lane; e - lane < E; e += 64) tiles += e < E ? cdiv(p.off[min(e, E - 1) + 1] - p.off[min(e, E - 1)], BC) : 0;
+    tiles = wave_sum(tiles);
+    const int64_t items = (int64_t)tiles * p.rows_t, per = cdiv64(items, 8);
+    const int64_t slot = blockIdx.x / 8, item = (blockIdx.x % 8) * per + slot;
+    if (slot >= per || item >= items) return;
+    const int number = (int)(item / p.rows_t);  // some tile of its expert
+    int e = 0, before = 0, nt = 1, done = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+        const int x = min(e0 + lane, E - 1);
+        const int n = e0 + lane < E ? cdiv(p.off[x + 1] - p.off[x], BC) : 0, upto = done + wave_scan(n);
+        const uint64_t m = __ballot(upto > number);
+        if (m) {
+            const int l = __builtin_ctzll(m);
+            e = e0 + l;
+            nt = __builtin_amdgcn_readlane(n, l);
+            before = __builtin_amdgcn_readlane(upto, l) - nt;
+            break;
         }
-        float y = a.alpha * sum;
-        if (a.beta != 0.0f) y = fmaf(a.beta, h2f(a.Y[i]), y);
-        a.Y[i] = f2h(y);
+        done = __builtin_amdgcn_readlane(upto, 63);
+    }
+    const int in = (int)(item - (int64_t)before * p.rows_t), tr = in / nt;
+    const int first = p.off[e] + (in - tr * nt) * BC, count = min(BC, p.off[e + 1] - first);
+
+    constexpr int OR = SWIGLU ? BR / 2 : BR;  // outputs of a tile
+    const int r0 = p.o0 + tr * OR, O = a.O, K = a.K, G = p.G;
+    const int end = SWIGLU ? O : p.o0 + p.on;
+    const int R = SWIGLU ? 2 * O : O;
+    // weight row of tile row i (past the end: the last one, whose results go nowhere)
+    auto row = [&](int i) {
+        if constexpr (SWIGLU) return ((i & 16) ? O : 0) + min(r0 + 16 * (i >> 5) + (i & 15), O - 1);
+        else return min(r0 + i, O - 1);
+    };
+    const unsigned lds0 =
+        __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) unsigned char*)smem));
+
+    // ---- DMA descriptors and per-lane offsets.  An offset of 2^31 lies past every
+    // buffer (all are shorter) and reads zeros ----
+    constexpr unsigned kPast = 0x80000000u;
+    const int64_t srow0 = (int64_t)e * R * G * 2;
+    const uintptr_t sb = reinterpret_cast<uintptr_t>(a.scale) + srow0, zb = reinterpret_cast<uintptr_t>(a.zero) + srow0;
+    const int so = (int)(sb & 3), zo = (int)(zb & 3);
+    const unsigned sbytes = ((unsigned)R * G * 2 + 2u + 3u) & ~3u;
+    const u32x4 rx = make_rsrc(a.X, (unsigned)p.x_bytes);
+    const u32x4 rw = make_rsrc(a.W + (int64_t)e * R * (K / 2), (unsigned)R * (K / 2));
+    const u32x4 rs = make_rsrc(reinterpret_cast<const void*>(sb & ~(uintptr_t)3), sbytes);
+    const u32x4 rz = make_rsrc(reinterpret_cast<const void*>(zb & ~(uintptr_t)3), sbytes);
+    constexpr int XC = CF::XRB / 16, WC16 = CF::WRB / 16;  // 16-byte chunks of a row
+    int offx[CF::DX], offw[CF::DW], offs[CF::DS];
+    auto xrow = [&](int i) { return 64 / XC * (wave * CF::DX + i) + lane / XC; };
+    auto xchunk = [&](int i) { return (lane % XC) ^ swz_x<KS>(xrow(i)); };
+#pragma unroll
+    for (int i = 0; i < CF::DX; ++i) {
+        const int q = p.order[first + min(xrow(i), count - 1)];
+        offx[i] = (SWIGLU ? p.k.div(q) : q) * K * 2 + 16 * xchunk(i);
+    }
+#pragma unroll
+    for (int i = 0; i < CF::DW; ++i) {
+        const int r = 64 / WC16 * (wave * CF::DW + i) + lane / WC16;
+        offw[i] = row(r) * (K / 2) + 16 * ((lane % WC16) ^ swz_w<KS>(r));
+    }
+#pragma unroll
+    for (int i = 0; i < CF::DS; ++i) {
+        const int j = wave * CF::DS + i;
+        offs[i] = row(64 * (j % (BR / 64)) + lane) * G * 2 + (j >= BR / 64 ? zo : so);
+    }
+    int* pairs = reinterpret_cast<int*>(smem + CF::OFF_P);  // (read after the K loop's barriers)
+    if (tid < BC) pairs[tid] = p.order[first + min(tid, count - 1)];
+
+    const int NS = cdiv(K, 16 * KS);  // stages
+    // stage t to buffer b; HS: its place in the group
+    auto issue = [&](int t, int b, bool starts) {
+        const unsigned st = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(b * CF::STAGE));
+        if (16 * KS * (t + 1) > K) {
+#pragma unroll
+            for (int i = 0; i < CF::DX; ++i)
+                dma16(rx, st + (wave * CF::DX + i) * 1024, 16 * KS * t + 8 * xchunk(i) < K ? offx[i] : (int)kPast, t * CF::XRB);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CF::DX; ++i) dma16(rx, st + (wave * CF::DX + i) * 1024, offx[i], t * CF::XRB);
+        }
+#pragma unroll
+        for (int i = 0; i < CF::DW; ++i) dma16(rw, st + CF::OFF_W + (wave * CF::DW + i) * 1024, offw[i], t * CF::WRB);
+        if (starts) {
+            const int g = t / SPG;
+#pragma unroll
+            for (int i = 0; i < CF::DS; ++i) {
+                const int j = wave * CF::DS + i;
+                const bool is_zero = j >= BR / 64;
+                dma4(is_zero ? rz : rs, st + (is_zero ? CF::OFF_ZR : CF::OFF_SC) + (j % (BR / 64)) * 256, (offs[i] + 2 * g) & ~3, 0);
+            }
+        }
+    };
+
+    // ---- fragments: X row x, step s at XRB x + 16 ((KS h + s) ^ swz(x)); weight row r,
+    // 32-k chunk c at WRB r + 16 ((NWC h + c) ^ swz(r)) ----
+    const int h = lane >> 5, l32 = lane & 31;
+    const int xrow0 = wc * 32 * FX + l32, wrow0 = wr * 32 * FW + l32;
+    constexpr int NWC = KS / 4;
+    unsigned xoff[KS], woff[NWC];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) xoff[s] = xrow0 * CF::XRB + 16 * ((KS * h + s) ^ swz_x<KS>(xrow0));
+#pragma unroll
+    for (int c = 0; c < NWC; ++c) woff[c] = CF::OFF_W + wrow0 * CF::WRB + 16 * ((NWC * h + c) ^ swz_w<KS>(wrow0));
+    int soff[FW];  // bit 1: which half of the dword holds the scale at group 0, bit 0: the zero point
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+        const int at = row(wrow0 + 32 * i) * G * 2;
+        soff[i] = ((at + so) & 2) | (((at + zo) >> 1) & 1);
+    }
+
+    f32x16 acc[FW][FX] = {};
+    float unit[FW];
+    f16x2 zz[FW], mul[FW];
+#pragma unroll
+    for (int i = 0; i < FW; ++i) unit[i] = 1.0f;
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t)
+        if (t < NS) issue(t, t, t % SPG == 0);
+    int stage = 0, stage_next = S - 1;
+    for (int t0 = 0; t0 < NS; t0 += SPG) {
+#pragma unroll
+        for (int hs = 0; hs < SPG; ++hs) {
+            const int t = t0 + hs;
+            if (SPG > 1 && t >= NS) break;
+            // stage t landed (what was issued after it may stay in flight), then the
+            // barrier: every wave's part of it has, and every wave has read stage t - 1,
+            // whose buffer the next issue writes
+            const int ahead = min(S - 2, NS - 1 - t);
+            if (S > 3 && ahead >= 2) wait_vm<vmcnt_imm(CF::dmas(0) + CF::dmas(1))>();
+            else if (S > 2 && ahead >= 1 && hs == 0) wait_vm<vmcnt_imm(CF::dmas(1))>();
+            else if (S > 2 && ahead >= 1) wait_vm<vmcnt_imm(CF::dmas(0))>();
+            else wait_vm<vmcnt_imm(0)>();
+            dma::stage_barrier<0xc07f>();
+            if (t + S - 1 < NS) issue(t + S - 1, stage_next, (hs + S - 1) % SPG == 0);
+            const unsigned st = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(stage * CF::STAGE));
+            stage_next = stage;
+            stage = stage + 1 == S ? 0 : stage + 1;
+            float ratio[FW];
+            u32x4 wraw[FW][NWC];
+#pragma unroll
+            for (int c = 0; c < NWC; ++c)
+#pragma unroll
+                for (int i = 0; i < FW; ++i) wraw[i][c] = lds_read16(st + woff[c] + 32 * CF::WRB * i);
+            if (hs == 0) {
+                const int odd = (t / SPG) & 1;
+#pragma unroll
+                for (int i = 0; i < FW; ++i) {
+                    const unsigned sd = lds_read4(st + CF::OFF_SC + (wrow0 + 32 * i) * 4);
+                    const unsigned zd = lds_read4(st + CF::OFF_ZR + (wrow0 + 32 * i) * 4);
+                    const float sc = h2f((uint16_t)((soff[i] >> 1) ^ odd ? sd >> 16 : sd));
+                    const float z = rintf(h2f((uint16_t)((soff[i] & 1) ^ odd ? zd >> 16 : zd)));
+                    const bool none = sc == 0.0f;
+                    ratio[i] = none ? 1.0f : unit[i] / sc;
+                    unit[i] = none ? unit[i] : sc;
+                    const _Float16 nz = (_Float16)(none ? 0.0f : z * (-1.0f / 512.0f));
+                    zz[i] = f16x2{nz, nz};
+                    mul[i] = none ? f16x2{(_Float16)0.0f, (_Float16)0.0f} : f16x2{(_Float16)2048.0f, (_Float16)32768.0f};
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                f16x8 xf[FX], wf[FW];
+#pragma unroll
+                for (int j = 0; j < FX; ++j) xf[j] = bitcast<f16x8>(lds_read16(st + xoff[s] + 32 * CF::XRB * j));
+#pragma unroll
+                for (int i = 0; i < FW; ++i) {
+                    const u32x4& q = wraw[i][s >> 2];
+                    wf[i] = unpack8((s & 3) == 0 ? q.x : (s & 3) == 1 ? q.y : (s & 3) == 2 ? q.z : q.w, mul[i], zz[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < FW; ++i)
+#pragma unroll
+                    for (int j = 0; j < FX; ++j) {
+                        if (hs == 0 && s == 0) acc[i][j] *= ratio[i];
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[j], wf[i], acc[i][j], 0, 0, 0);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FW; ++i) unit[i] *= 512.0f;  // (q - z) 2^-9 back to q - z
+#pragma unroll
+    for (int i = 0; i < FW; ++i)
+#pragma unroll
+        for (int j = 0; j < FX; ++j) acc[i][j] *= unit[i];
+
+    // ---- stores: pairs 8 q + 4 h + e of each 32 ----
+    const bool up_lane = (l32 & 16) != 0;
+#pragma unroll
+    for (int j = 0; j < FX; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int v = 0; v < 4; v += SWIGLU ? 2 : 1) {
+                const int c = wc * 32 * FX + 32 * j + 8 * q + 4 * h + v + (SWIGLU && up_lane ? 1 : 0);
+                const int64_t to = (int64_t)pairs[c] * (SWIGLU ? O : p.ldp);
+#pragma unroll
+                for (int i = 0; i < FW; ++i) {
+                    if constexpr (SWIGLU) {
+                        // (gate, up) of pair v to lane l, of pair v + 1 to lane l ^ 16
+                        const auto sw = __builtin_amdgcn_permlane16_swap(bitcast<unsigned>(acc[i][j][4 * q + v]),
+                                                                         bitcast<unsigned>(acc[i][j][4 * q + v + 1]), false, false);
+                        const float x = bitcast<float>(sw[0]), u = bitcast<float>(sw[1]);
+                        const int o = r0 + 16 * (wr * FW + i) + (l32 & 15);
+                        if (o < O && c < count) a.Y[to + o] = f2h(x / (1.0f + expf(-x)) * u);
+                    } else {
+                        const int o = r0 + wrow0 + 32 * i;
+                        if (o < end && c < count) p.part[to + o - p.o0] = acc[i][j][4 * q + v];
+                    }
+                }
+            }
+}
+
+// Y[t, o0 + o] = alpha sum_j w[t, j] part[t top_k + j, o] + beta Y, places in order; a
+// place without an expert is left out.  A thread takes four outputs of one token, and
+// eight places' parts are in flight at once.
+__global__ void __launch_bounds__(128) moe_combine(const Params p) {
+    const MoeArgs& a = p.a;
+    const int t = blockIdx.x, o = 512 * blockIdx.y + 4 * threadIdx.x;
+    const int n = min(4, p.on - o);
+    if (n <= 0) return;
+    const float* part = p.part + (int64_t)t * a.top_k * p.ldp + o;
+    const int32_t* ids = a.ids + (int64_t)t * a.top_k;
+    f32x4 sum = {};
+    for (int j0 = 0; j0 < a.top_k; j0 += 8) {
+        f32x4 v[8];
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool there = j0 + j < a.top_k && (unsigned)ids[min(j0 + j, a.top_k - 1)] < (unsigned)a.experts;
+            w[j] = 0.0f;
+            v[j] = f32x4{};
+            if (there) {
+                w[j] = a.weights ? a.weights[(int64_t)t * a.top_k + j0 + j] : 1.0f;
+                v[j] = *reinterpret_cast<const f32x4*>(part + (int64_t)(j0 + j) * p.ldp);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = fmaf(w[j], v[j][i], sum[i]);
+    }
+    uint16_t* y = a.Y + (int64_t)t * a.O + p.o0 + o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum[i] *= a.alpha;
+        if (a.beta != 0.0f && i < n) sum[i] = fmaf(a.beta, h2f(y[i]), sum[i]);
+    }
+    if (n == 4) {
+        *reinterpret_cast<u32x2u*>(y) = u32x2{pack2h(sum[0], sum[1]), pack2h(sum[2], sum[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) y[i] = f2h(sum[i]);
     }
 }
 
 namespace {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+template <class CF, bool SWIGLU>
+clove_status_t run_tile(Params p, hipStream_t stream) {
+    p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR);
+    const int64_t tiles = ((int64_t)p.P / CF::BC + p.a.experts) * p.rows_t;
+    auto k = moe_tile<CF, SWIGLU>;
+    if (ensure_lds(reinterpret_cast<const void*>(k), CF::LDS) != CLOVE_OK) return CLOVE_ERR_LAUNCH;
+    CLOVE_LAUNCH(k, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(CF::NT), CF::LDS, stream, p);
+    return check_launch();
+}
 
 }  // namespace
 }  // namespace moe
@@ -229,8 +543,21 @@ clove_status_t launch_moe_w4a16(const MoeArgs& a, bool swiglu, hipStream_t strea
     p.P = a.T * a.top_k;
     p.G = cdiv(a.K, 128);
     p.k = FastDiv(a.top_k);
+    p.x_bytes = (int64_t)(swiglu ? a.T : p.P) * a.K * 2;
+    const int64_t expert_bytes = (int64_t)(swiglu ? 2 : 1) * a.O * (a.K / 2);
+    const bool dma = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W) && p.x_bytes < ((int64_t)1 << 31) &&
+                     expert_bytes < ((int64_t)1 << 31);
     const size_t off = round256((size_t)(a.experts + 1) * 4), order = round256((size_t)p.P * 4);
-    const size_t part = swiglu ? 0 : (size_t)p.P * a.O * 4;
+    // down: the products of so many outputs at a time that they stay in the Infinity Cache
+    const int64_t chunk_bytes = (int64_t)(getenv("MOE_CHUNK") ? atoi(getenv("MOE_CHUNK")) : 128) << 20;
+    int chunk = a.O;
+    if (!swiglu) {
+        const int64_t most = chunk_bytes / ((int64_t)p.P * 4) / 256 * 256;
+        const int n = cdiv(a.O, (int)(most < 256 ? 256 : most > a.O ? a.O : most));
+        chunk = min(a.O, cdiv(cdiv(a.O, n), 256) * 256);
+    }
+    p.ldp = (chunk + 3) & ~3;
+    const size_t part = swiglu ? 0 : (size_t)p.P * p.ldp * 4;
     void* buf = nullptr;
     clove_status_t st = acquire_buffer(stream, kBufMoe, off + order + part, &buf);
     if (st != CLOVE_OK) return st;
@@ -238,14 +565,43 @@ clove_status_t launch_moe_w4a16(const MoeArgs& a, bool swiglu, hipStream_t strea
     p.off = reinterpret_cast<int*>(at);
     p.order = reinterpret_cast<int*>(at + off);
     p.part = reinterpret_cast<float*>(at + off + order);
-    CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3(256), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
-    p.rows_t = cdiv(a.O, swiglu ? AR / 2 : AR);
-    const int64_t tiles = ((int64_t)p.P / AC + a.experts) * p.rows_t;
-    if (swiglu) CLOVE_LAUNCH(moe_any<true>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
-    else CLOVE_LAUNCH(moe_any<false>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
-    if (!swiglu) {
-        const int64_t n = cdiv64((int64_t)a.T * a.O, 256);
-        CLOVE_LAUNCH(moe_combine, dim3((unsigned)(n < 16384 ? n : 16384)), dim3(256), 0, stream, p);
+    const int st_threads = p.P >= 4 * kSortThreads ? kSortThreads : max(64, cdiv(p.P, 256) * 64);
+    CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)st_threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
+    for (p.o0 = 0; p.o0 < a.O; p.o0 += chunk) {
+        p.on = min(chunk, a.O - p.o0);
+        if (dma) {
+            const int cfg = getenv("MOE_CFG") ? atoi(getenv("MOE_CFG")) : 0;
+#define GO(...) (swiglu ? run_tile<__VA_ARGS__, true>(p, stream) : run_tile<__VA_ARGS__, false>(p, stream))
+            using C0 = Cfg<4, 1, 2, 4, 2, 4>;
+            using C1 = Cfg<4, 1, 2, 4, 3, 4>;
+            using C2 = Cfg<4, 2, 2, 2, 2, 8>;
+            using C3 = Cfg<4, 1, 2, 2, 2, 8>;
+            using C4 = Cfg<4, 1, 1, 2, 2, 8>;
+            using C5 = Cfg<4, 1, 2, 2, 3, 4>;
+            using C6 = Cfg<4, 1, 1, 1, 4, 8>;
+            using C7 = Cfg<4, 1, 2, 1, 3, 8>;
+            using C8 = Cfg<4, 2, 2, 4, 3, 4>;
+            using C9 = Cfg<4, 1, 1, 4, 3, 4>;
+            switch (cfg) {
+                case 0: st = GO(C0); break;
+                case 1: st = GO(C1); break;
+                case 2: st = GO(C2); break;
+                case 3: st = GO(C3); break;
+                case 4: st = GO(C4); break;
+                case 5: st = GO(C5); break;
+                case 6: st = GO(C6); break;
+                case 7: st = GO(C7); break;
+                case 8: st = GO(C8); break;
+                default: st = GO(C9); break;
+            }
+            if (st != CLOVE_OK) return st;
+        } else {
+            p.rows_t = cdiv(p.on, swiglu ? AR / 2 : AR);
+            const int64_t tiles = ((int64_t)p.P / AC + a.experts) * p.rows_t;
+            if (swiglu) CLOVE_LAUNCH(moe_any<true>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
+            else CLOVE_LAUNCH(moe_any<false>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
+        }
+        if (!swiglu) CLOVE_LAUNCH(moe_combine, dim3((unsigned)a.T, (unsigned)cdiv(p.on, 512)), dim3(128), 0, stream, p);
     }
     return check_launch();
 }
