@@ -5,6 +5,8 @@
 //
 // s and c are 64 bits: of some hundred experts two often agree to 2^-24, and
 // which of them comes first must not depend on an exponential's last bit.
+#include <type_traits>
+
 #include "moe.hpp"
 
 namespace clove {
@@ -12,116 +14,211 @@ namespace route {
 
 using namespace hw;
 
-constexpr int WAVES = 4;      // tokens a workgroup
+constexpr int WAVES = 4;  // tokens a workgroup
 constexpr double NONE = -__builtin_inf();
 
-// The larger value, of equal ones the lower index, over the wave.
-__device__ __forceinline__ void wave_best(double& v, int& at) {
+// Reductions over the wave in the VALU: inside each row of 16 lanes by DPP (row_ror 8
+// and 4, quad_perm 2301 and 1032), then across the rows by v_permlane16_swap and
+// v_permlane32_swap.  Every lane has the result.
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t u = bitcast<uint64_t>(v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_mov_dpp((int)(unsigned)u, CTRL, 0xf, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_mov_dpp((int)(unsigned)(u >> 32), CTRL, 0xf, 0xf, false);
+    return bitcast<double>((uint64_t)hi << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return bitcast<float>(__builtin_amdgcn_mov_dpp(bitcast<int>(v), CTRL, 0xf, 0xf, false));
+}
+template <bool FAR>
+__device__ __forceinline__ void swap_rows(float v, float* a, float* b) {
+    const unsigned u = bitcast<unsigned>(v);
+    const auto s = FAR ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    *a = bitcast<float>(s[0]);
+    *b = bitcast<float>(s[1]);
+}
+template <bool FAR>
+__device__ __forceinline__ void swap_rows(double v, double* a, double* b) {
+    const uint64_t u = bitcast<uint64_t>(v);
+    float l0, l1, h0, h1;
+    swap_rows<FAR>(bitcast<float>((unsigned)u), &l0, &l1);
+    swap_rows<FAR>(bitcast<float>((unsigned)(u >> 32)), &h0, &h1);
+    *a = bitcast<double>((uint64_t)bitcast<unsigned>(h0) << 32 | bitcast<unsigned>(l0));
+    *b = bitcast<double>((uint64_t)bitcast<unsigned>(h1) << 32 | bitcast<unsigned>(l1));
+}
+template <class T, class F>
+__device__ __forceinline__ T reduce(T v, F f) {
+    v = f(v, dpp<0x128>(v));
+    v = f(v, dpp<0x124>(v));
+    v = f(v, dpp<0x4e>(v));
+    v = f(v, dpp<0xb1>(v));
+    T a, b;
+    swap_rows<false>(v, &a, &b);
+    v = f(a, b);
+    swap_rows<true>(v, &a, &b);
+    return f(a, b);
+}
+__device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // (never NaN)
+__device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
+template <class T>
+__device__ __forceinline__ T wave_most(T v) {
+    return reduce(v, [](T a, T b) { return most(a, b); });
+}
+__device__ __forceinline__ double wave_total(double v) {
+    return reduce(v, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const uint64_t u = bitcast<uint64_t>(v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, lane);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), lane);
+    return bitcast<double>((uint64_t)hi << 32 | lo);
+}
+
+// The lowest lane of those with the largest value; -1 if that is -infinity.  Doubles by
+// their fp32 roundings first, which keep the order: only where several lanes share the
+// largest of them are the doubles compared, at more than twice the instructions.
+__device__ __forceinline__ int best_lane(float v) {
+    const float u = wave_most(v);
+    return u > -__builtin_inff() ? __builtin_ctzll(__ballot(v == u)) : -1;
+}
+__device__ __forceinline__ int best_lane(double v) {
+    const float f = (float)v, u = wave_most(f);
+    if (!(u > -__builtin_inff())) return -1;
+    const uint64_t m = __ballot(f == u);
+    if ((m & (m - 1)) == 0) return __builtin_ctzll(m);
+    const double w = wave_most(f == u ? v : NONE);
+    return __builtin_ctzll(__ballot(f == u && v == w));
+}
+
+// Elements [0, n) of `V` adjacent ones at any alignment of their type; -infinity for the others.
+template <int DT, int V>
+__device__ __forceinline__ void load(float (&v)[V], const typename Elem<DT>::raw* p, int n) {
+    using E = Elem<DT>;
+    typedef typename E::raw raw;
+    struct __attribute__((packed, aligned(sizeof(raw)))) Run {
+        raw x[V];
+    };
+    if (n >= V) {
+        const Run r = *reinterpret_cast<const Run*>(p);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const double u = __shfl_xor(v, d);
-        const int b = __shfl_xor(at, d);
-        if (u > v || (u == v && b < at)) {
-            v = u;
-            at = b;
-        }
+        for (int i = 0; i < V; ++i) v[i] = E::load(r.x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = i < n ? E::load(p[i]) : -__builtin_inff();
     }
 }
 
-// One token a wave; lane l holds experts l + 64 i, i < VPL.
-template <int DT, int VPL>
-__global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a) {
-    using E = Elem<DT>;
-    __shared__ double lds[WAVES][64 * VPL];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = blockIdx.x * WAVES + wave, N = a.experts;
+// One token a wave; lane l holds experts l V .. l V + V - 1, so that of equal values
+// the lowest lane, and in it the lowest entry, is the lowest index.  C: what the choice
+// goes by, the logits themselves (float) or score + bias (double).
+//
+// A round of the choice is the lanes' own best (kept up to date), one reduction, one
+// ballot: some 40 instructions of one wave, which is the time (E = 64, top 6, 16384
+// tokens: 16 waves a SIMD of 300 each).
+template <int DT, int V, bool BIAS>
+__global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const FastDiv group) {
+    typedef typename std::conditional<BIAS, double, float>::type C;
+    constexpr C none = -__builtin_inff();
+    __shared__ double lds[WAVES][64 * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, N = a.experts, e0 = lane * V;
+    const int t = blockIdx.x * WAVES + wave;
     if (t >= a.T) return;
-    const typename E::raw* x = static_cast<const typename E::raw*>(a.logits) + (int64_t)t * a.logits_stride;
-    double s[VPL], c[VPL];  // scores; what the choice goes by, NONE: not available
-    double most = NONE;
+    const typename Elem<DT>::raw* row = static_cast<const typename Elem<DT>::raw*>(a.logits) + (int64_t)t * a.logits_stride;
+    float x[V], bias[V];
+    load<DT, V>(x, row + e0, N - e0);
+    if constexpr (BIAS) load<CLOVE_DTYPE_FP32, V>(bias, a.bias + e0, N - e0);
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const int e = lane + 64 * i;
-        const float f = e < N ? E::load(x[e]) : -__builtin_inff();
-        const float b = a.bias && e < N ? a.bias[e] : 0.0f;
-        const bool here = f > -__builtin_inff() && b > -__builtin_inff();  // (false for NaN)
-        s[i] = here ? (double)f : NONE;
-        c[i] = (double)b;
-        most = s[i] > most ? s[i] : most;
+    for (int i = 0; i < V; ++i) {
+        bool here = x[i] > -__builtin_inff();  // (false for NaN)
+        if constexpr (BIAS) here = here && bias[i] > -__builtin_inff();
+        x[i] = here ? x[i] : -__builtin_inff();
+        top = most(top, x[i]);
     }
+    const bool softmax = a.score == CLOVE_ROUTE_SOFTMAX;
+    double s[V];
+    if (softmax) {
+        top = wave_most(top);
+        double total = 0.0;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const double u = __shfl_xor(most, d);
-        most = u > most ? u : most;
+        for (int i = 0; i < V; ++i) {
+            s[i] = x[i] == top ? 1.0 : x[i] > -__builtin_inff() ? exp((double)x[i] - (double)top) : 0.0;
+            if (!(x[i] > -__builtin_inff())) s[i] = 0.0;
+            total += s[i];
+        }
+        const double inv = 1.0 / wave_total(total);  // (infinity if no expert is there: not used then)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] *= inv;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = 1.0 / (1.0 + exp(-(double)x[i]));
     }
-    double total = 0.0;
-    const bool every_x = a.score == CLOVE_ROUTE_SOFTMAX;
+    C c[V];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const double f = s[i];
-        const bool here = f > NONE;
-        if (every_x) s[i] = !here ? 0.0 : f == most ? 1.0 : exp(f - most);
-        else s[i] = here ? 1.0 / (1.0 + exp(-f)) : 0.0;
-        total += s[i];
-        c[i] = here ? (a.bias ? 0.0 : f) + c[i] : NONE;  // (the score joins a bias below)
-    }
-    if (every_x) {
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) s[i] = total > 0.0 ? s[i] / total : 0.0;
-    }
-    if (a.bias) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) c[i] = c[i] > NONE ? s[i] + c[i] : NONE;
+    for (int i = 0; i < V; ++i) {
+        if constexpr (BIAS) c[i] = x[i] > -__builtin_inff() ? s[i] + (double)bias[i] : none;
+        else c[i] = x[i];
     }
     if (a.groups > 1) {
-        // lane g: the value of group g
-        const int n = N / a.groups;
+        // `per` lanes to a group, a power of two: each the two largest of its share, then
+        // the lanes' pairs merged
+        const int n = group.d, per = 1 << (31 - __builtin_clz(64 / a.groups)), g = lane / per, sub = lane % per;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) lds[wave][lane + 64 * i] = c[i] > NONE ? (a.bias ? c[i] : s[i]) : NONE;
+        for (int i = 0; i < V; ++i) lds[wave][e0 + i] = c[i] > none ? (BIAS ? (double)c[i] : s[i]) : NONE;
         asm volatile("" ::: "memory");  // (one wave's LDS accesses take effect in order)
-        double v = NONE;
-        if (lane < a.groups) {
-            double first = NONE, second = NONE;
-            for (int j = 0; j < n; ++j) {
-                const double u = lds[wave][lane * n + j];
-                if (u > first) second = first, first = u;
-                else if (u > second) second = u;
+        double first = NONE, second = NONE;
+        if (g < a.groups) {
+#pragma unroll 4
+            for (int j = sub; j < n; j += per) {
+                const double u = lds[wave][g * n + j];
+                second = most(second, u > first ? first : u);
+                first = most(first, u);
             }
-            v = a.group_top > 1 && second > NONE ? first + second : first;
         }
+        for (int d = 1; d < per; d <<= 1) {
+            const double f = __shfl_xor(first, d), u = __shfl_xor(second, d);
+            second = most(most(second, u), f > first ? first : f);
+            first = most(first, f);
+        }
+        // (one lane of each group stands for it)
+        double v = sub != 0 || g >= a.groups ? NONE : a.group_top > 1 && second > NONE ? first + second : first;
         uint64_t kept = 0;
         for (int j = 0; j < a.top_groups; ++j) {
-            double u = v;
-            int g = lane;
-            wave_best(u, g);
-            if (!(u > NONE)) break;
-            kept |= (uint64_t)1 << g;
-            if (lane == g) v = NONE;
+            const int l = best_lane(v);
+            if (l < 0) break;
+            kept |= (uint64_t)1 << (l / per);
+            if (lane == l) v = NONE;
         }
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int e = lane + 64 * i;
-            if (e < N && !((kept >> (e / n)) & 1)) c[i] = NONE;
-        }
+        for (int i = 0; i < V; ++i)
+            if (!((kept >> group.div(min(e0 + i, N - 1))) & 1)) c[i] = none;
     }
     int id = -1;
     double w = 0.0, sum = 0.0;
+    C best = none;
+    int at = 0;
+    auto update = [&] {
+        best = c[0];
+        at = 0;
+#pragma unroll
+        for (int i = 1; i < V; ++i)
+            if (c[i] > best) best = c[i], at = i;
+    };
+    update();
     for (int j = 0; j < a.top_k; ++j) {
-        double v = NONE, mine = 0.0;
-        int at = 0x7fffffff;
+        const int l = best_lane(best);
+        if (l < 0) break;
+        const int i0 = __builtin_amdgcn_readlane(at, l);
+        double mine = s[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (c[i] > v) v = c[i], at = lane + 64 * i, mine = s[i];
-        wave_best(v, at);
-        if (!(v > NONE)) break;
-        mine = __shfl(mine, at & 63);
+        for (int i = 1; i < V; ++i) mine = i0 == i ? s[i] : mine;
+        mine = lane_value(mine, l);
         sum += mine;
-        if (lane == j) id = at, w = mine;
+        if (lane == j) id = l * V + i0, w = mine;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (at == lane + 64 * i) c[i] = NONE;
+        for (int i = 0; i < V; ++i) c[i] = lane == l && i0 == i ? none : c[i];
+        update();
     }
     if (lane >= a.top_k) return;
     if (a.renormalize && sum > 0.0) w /= sum;
@@ -131,12 +228,17 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a) {
 
 namespace {
 
-template <int DT>
+template <int DT, bool BIAS>
 clove_status_t run(const RouteArgs& a, hipStream_t stream) {
     const int v = cdiv(a.experts, 64);
-    auto k = v <= 1 ? moe_route<DT, 1> : v <= 2 ? moe_route<DT, 2> : v <= 4 ? moe_route<DT, 4> : v <= 8 ? moe_route<DT, 8> : moe_route<DT, 16>;
-    CLOVE_LAUNCH(k, dim3((unsigned)cdiv(a.T, WAVES)), dim3(64 * WAVES), 0, stream, a);
+    auto k = v <= 1 ? moe_route<DT, 1, BIAS> : v <= 2 ? moe_route<DT, 2, BIAS> : v <= 4 ? moe_route<DT, 4, BIAS>
+             : v <= 8 ? moe_route<DT, 8, BIAS> : moe_route<DT, 16, BIAS>;
+    CLOVE_LAUNCH(k, dim3((unsigned)cdiv(a.T, WAVES)), dim3(64 * WAVES), 0, stream, a, FastDiv(a.experts / a.groups));
     return check_launch();
+}
+template <int DT>
+clove_status_t run(const RouteArgs& a, hipStream_t stream) {
+    return a.bias ? run<DT, true>(a, stream) : run<DT, false>(a, stream);
 }
 
 }  // namespace

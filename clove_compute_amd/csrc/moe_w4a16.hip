@@ -33,6 +33,8 @@ struct Params {
     int rows_t;    // tiles of weight rows
     int P, G;
     int64_t x_bytes;  // of X
+    bool by_expert;   // moe_few
+    int ng;           // moe_few*: groups of a unit
 };
 
 // Workgroup e lists the pairs of expert e; where they begin is the number of pairs of
@@ -209,6 +211,249 @@ __global__ void __launch_bounds__(256) moe_any(const Params p) {
                 if (c < t.count) p.part[(int64_t)pair[c] * p.ldp + o - p.o0] = acc[j][v];
             }
     }
+}
+
+// ---------------------------------------------------------------------------
+// Few pairs (K % 32 == 0, 16-byte aligned X and W): the weights are the time.  A wave
+// takes 16 WF weight rows and up to NG = 4 groups of K at once, all their loads in
+// flight together and straight to registers (16 bytes a lane: lane group h of 16
+// holds k = 32 h .. 32 h + 31 of a row's group); the rows of X it meets and the
+// groups' constants, loaded ahead of them, go through a part of LDS that is the
+// wave's own, so no wave waits for another before the sums meet at the end.  On
+// v_mfma_f32_16x16x32_f16 with X as the "A" operand: a lane holds weight row
+// l % 16 and X rows 4 h .. 4 h + 3; step q of a group takes dword q of every lane,
+// k = 32 h + 8 q .. + 7 of lane group h.
+// ---------------------------------------------------------------------------
+constexpr int NG = 4;                 // groups of a unit
+constexpr int XLD = 128 * NG + 8;     // halves of a row of X in LDS
+
+template <int WF, int TB>
+struct Unit {
+    u32x4 x[TB], w[WF][NG];
+    uint16_t s[WF], z[WF];  // entry lane + 64 i: row (lane + 64 i) / NG, group (lane + 64 i) % NG
+};
+template <int WF, int TB>
+struct UnitLds {
+    uint16_t x[TB][XLD];
+    unsigned c[16 * WF][NG];  // scale, zero point
+    static constexpr int BYTES = TB * XLD * 2 + 16 * WF * NG * 4;
+};
+
+// Groups g0 .. g0 + ng - 1 of rows row(i) (i < 16 WF, rows of all experts' weights) and
+// of n rows of X that begin at element xrow(i).  Everything unconditional, from
+// clamped addresses.
+template <int WF, int TB, class Row, class XRow>
+__device__ __forceinline__ void load_unit(Unit<WF, TB>& u, const MoeArgs& a, int G, int g0, int ng, int n, int lane, Row row,
+                                          XRow xrow) {
+    const int K = a.K, l16 = lane & 15, h = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < WF; ++i) {
+        const int r = (lane + 64 * i) / NG, g = min(g0 + min(lane % NG, ng - 1), G - 1);
+        const int64_t at = row(r) * G + g;
+        u.s[i] = a.scale[at];
+        u.z[i] = a.zero[at];
+    }
+#pragma unroll
+    for (int f = 0; f < WF; ++f) {
+        const uint8_t* w = a.W + row(16 * f + l16) * (K / 2);
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+            if (j < ng)
+                u.w[f][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w + min(64 * (g0 + j) + 16 * h, K / 2 - 16)));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (the weights, which come from farthest away, first)
+#pragma unroll
+    for (int i = 0; i < TB; ++i)
+        if (i < n) u.x[i] = *reinterpret_cast<const u32x4*>(a.X + xrow(i) + min(128 * g0 + 8 * lane, K - 8));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The constants and X to the wave's part of LDS: past K, and past the unit's groups, 0.
+template <int WF, int TB>
+__device__ __forceinline__ void stage_unit(const Unit<WF, TB>& u, UnitLds<WF, TB>& l, int K, int g0, int ng, int n, int lane) {
+#pragma unroll
+    for (int i = 0; i < WF; ++i) {
+        const int e = lane + 64 * i;
+        l.c[e / NG][e % NG] = e % NG < ng ? (unsigned)u.s[i] | ((unsigned)u.z[i] << 16) : 0u;
+    }
+    const bool in = 8 * lane < 128 * ng && 128 * g0 + 8 * lane < K;
+#pragma unroll
+    for (int i = 0; i < TB; ++i)
+        if (i < n) *reinterpret_cast<u32x4*>(&l.x[i][8 * lane]) = in ? u.x[i] : u32x4{0u, 0u, 0u, 0u};
+    asm volatile("" ::: "memory");  // (one wave's LDS accesses take effect in order)
+}
+
+// acc += factor * the unit's products
+template <int WF, int TB>
+__device__ __forceinline__ void add_unit(const Unit<WF, TB>& u, const UnitLds<WF, TB>& l, int ng, int n, int lane, float factor,
+                                         f32x4 (&acc)[WF]) {
+    const int l16 = lane & 15, h = lane >> 4;
+    const uint16_t* x = l.x[min(l16, n - 1)] + 32 * h;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+        if (j >= ng) break;
+        f16x8 xf[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) xf[q] = bitcast<f16x8>(*reinterpret_cast<const u32x4*>(x + 128 * j + 8 * q));
+#pragma unroll
+        for (int f = 0; f < WF; ++f) {
+            const unsigned c = l.c[16 * f + l16][j];
+            const _Float16 nz = (_Float16)(-rintf(h2f((uint16_t)(c >> 16))) * (1.0f / 512.0f));
+            const f16x2 zz = {nz, nz};
+            f32x4 P = {};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                P = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[q], i4w::unpack8(u.w[f][j][q], zz), P, 0, 0, 0);
+            const float sc = h2f((uint16_t)c) * 512.0f * factor;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) acc[f][v] = fmaf(sc, P[v], acc[f][v]);
+        }
+    }
+}
+
+// A workgroup takes the pairs of one expert, TB at a time, and 32 weight rows (SwiGLU:
+// 16 gate rows and the up rows of the same outputs); its waves share K.  The expert is
+// `slot` (p.by_expert), or that of pair `slot`, whose other pairs' workgroups end.
+template <bool SWIGLU, int TB, bool PF>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3))) moe_few(const Params p) {
+    constexpr int WF = 2, OR = SWIGLU ? 16 : 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const MoeArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), KS = blockDim.x >> 6;
+    const int l16 = lane & 15, h = lane >> 4;
+    const int slot = blockIdx.x / p.rows_t, r0 = p.o0 + (blockIdx.x - slot * p.rows_t) * OR, O = a.O, K = a.K, G = p.G;
+    int id = a.ids[min(lane, p.P - 1)];  // (beside the slot's own id, not behind it)
+    const int e = p.by_expert ? slot : __builtin_amdgcn_readfirstlane(a.ids[slot]);
+    if ((unsigned)e >= (unsigned)a.experts) return;
+    // [KS] units, then each wave's list of pairs, then the sums of the waves
+    UnitLds<WF, TB>& l = reinterpret_cast<UnitLds<WF, TB>*>(smem)[wave];
+    int* list = reinterpret_cast<int*>(smem + KS * UnitLds<WF, TB>::BYTES) + wave * p.P;
+    float* red = reinterpret_cast<float*>(smem + KS * UnitLds<WF, TB>::BYTES + (KS * p.P * 4 + 15) / 16 * 16);
+    int count = 0;
+    for (int q0 = 0; q0 < p.P; q0 += 64) {
+        const bool is = q0 + lane < p.P && id == e;
+        const uint64_t m = __ballot(is);
+        if (q0 + 64 < p.P) id = a.ids[min(q0 + 64 + lane, p.P - 1)];
+        if (m && count == 0 && !p.by_expert && q0 + __builtin_ctzll(m) != slot) return;
+        if (is) list[count + __popcll(m & (((uint64_t)1 << lane) - 1))] = q0 + lane;
+        count += __popcll(m);
+    }
+    asm volatile("" ::: "memory");
+    const int64_t base = (int64_t)e * (SWIGLU ? 2 : 1) * O;
+    auto row = [&](int i) { return base + (SWIGLU && i >= 16 ? O : 0) + min(r0 + (SWIGLU ? i & 15 : i), O - 1); };
+    for (int b0 = 0; b0 < count; b0 += TB) {
+        const int n = min(TB, count - b0);
+        auto xrow = [&](int i) {
+            const int q = __builtin_amdgcn_readfirstlane(list[b0 + min(i, n - 1)]);
+            return (int64_t)(SWIGLU ? p.k.div(q) : q) * K;
+        };
+        f32x4 acc[WF] = {};
+        const int ng = p.ng;
+        int g0 = wave * ng;
+        Unit<WF, TB> u;
+        if (g0 < G) load_unit(u, a, G, g0, min(ng, G - g0), n, lane, row, xrow);
+        while (g0 < G) {
+            const int m = min(ng, G - g0);
+            stage_unit(u, l, K, g0, m, n, lane);
+            const int g1 = g0 + KS * ng;
+            if constexpr (PF) {
+                Unit<WF, TB> next;
+                if (g1 < G) load_unit(next, a, G, g1, min(ng, G - g1), n, lane, row, xrow);
+                add_unit(u, l, m, n, lane, 1.0f, acc);
+                u = next;
+            } else {
+                add_unit(u, l, m, n, lane, 1.0f, acc);
+                if (g1 < G) load_unit(u, a, G, g1, min(ng, G - g1), n, lane, row, xrow);
+            }
+            g0 = g1;
+        }
+        __syncthreads();  // (the sums of the pairs before have been read)
+#pragma unroll
+        for (int f = 0; f < WF; ++f)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) red[((wave * WF + f) * 4 + v) * 64 + lane] = acc[f][v];
+        __syncthreads();
+        // thread: weight row l16, X row 4 h + v with v = its wave (modulo the waves there are)
+        for (int v = wave; v < 4; v += KS) {
+            const int c = 4 * h + v;
+            float sum[WF];
+#pragma unroll
+            for (int f = 0; f < WF; ++f) {
+                sum[f] = red[(f * 4 + v) * 64 + lane];
+                for (int w = 1; w < KS; ++w) sum[f] += red[((w * WF + f) * 4 + v) * 64 + lane];
+            }
+            if (c >= n) continue;
+            const int64_t q = list[b0 + c];
+            if constexpr (SWIGLU) {
+                const float x = sum[0];
+                if (r0 + l16 < O) a.Y[q * O + r0 + l16] = f2h(x / (1.0f + expf(-x)) * sum[1]);
+            } else {
+#pragma unroll
+                for (int f = 0; f < WF; ++f)
+                    if (r0 + 16 * f + l16 < p.o0 + p.on) p.part[q * p.ldp + r0 - p.o0 + 16 * f + l16] = sum[f];
+            }
+        }
+    }
+}
+
+// Down for few tokens: a workgroup takes one token and 16 WF outputs, its waves the
+// (place, K part) units in turn, each weighted as it is added; no partial results in
+// memory and one launch.
+template <int WF>
+__global__ void __launch_bounds__(1024) moe_few_down(const Params p) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const MoeArgs& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), KS = blockDim.x >> 6;
+    const int l16 = lane & 15;
+    const int t = blockIdx.x / p.rows_t, r0 = (blockIdx.x - t * p.rows_t) * 16 * WF, O = a.O, K = a.K, G = p.G;
+    UnitLds<WF, 1>& l = reinterpret_cast<UnitLds<WF, 1>*>(smem)[wave];
+    float* red = reinterpret_cast<float*>(smem + KS * UnitLds<WF, 1>::BYTES);
+    const int ng = p.ng, parts = cdiv(G, ng), units = a.top_k * parts;
+    f32x4 acc[WF] = {};
+    // unit i: place i / parts, groups from ng (i % parts); those without an expert are passed over
+    auto at = [&](int i, int64_t* q, int* e, int* g0) {
+        for (; i < units; i += KS) {
+            const int j = i / parts;
+            *q = (int64_t)t * a.top_k + j;
+            *e = __builtin_amdgcn_readfirstlane(a.ids[*q]);
+            *g0 = (i - j * parts) * ng;
+            if ((unsigned)*e < (unsigned)a.experts) break;
+        }
+        return i;
+    };
+    int64_t q = 0, q1 = 0;
+    int e = 0, g0 = 0, e1 = 0, g1 = 0;
+    auto load = [&](Unit<WF, 1>& u, int64_t pair, int expert, int g) {
+        load_unit(u, a, G, g, min(ng, G - g), 1, lane, [&](int i) { return (int64_t)expert * O + min(r0 + i, O - 1); },
+                  [&](int) { return pair * K; });
+    };
+    Unit<WF, 1> u;
+    int i = at(wave, &q, &e, &g0);
+    if (i < units) load(u, q, e, g0);
+    while (i < units) {
+        const int m = min(ng, G - g0);
+        const float weight = a.weights ? a.weights[q] : 1.0f;
+        stage_unit(u, l, K, g0, m, 1, lane);
+        Unit<WF, 1> next;
+        const int i1 = at(i + KS, &q1, &e1, &g1);
+        if (i1 < units) load(next, q1, e1, g1);
+        add_unit(u, l, m, 1, lane, weight, acc);
+        u = next;
+        i = i1, q = q1, e = e1, g0 = g1;
+    }
+    // X row 0: entry 0 of lanes 0 .. 15
+    if (lane < 16) {
+#pragma unroll
+        for (int f = 0; f < WF; ++f) red[(wave * WF + f) * 16 + lane] = acc[f][0];
+    }
+    __syncthreads();
+    if (tid >= 16 * WF || r0 + tid >= O) return;
+    float sum = red[tid];
+    for (int w = 1; w < KS; ++w) sum += red[w * 16 * WF + tid];
+    uint16_t* y = a.Y + (int64_t)t * O + r0 + tid;
+    sum *= a.alpha;
+    if (a.beta != 0.0f) sum = fmaf(a.beta, h2f(*y), sum);
+    *y = f2h(sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -521,6 +766,42 @@ namespace {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// ---- few pairs ----
+// Units of K: a wave takes one of ng <= NG groups after the other.
+int few_waves(const Params& p, int64_t workgroups, int cus) { return workgroups >= 8 * (int64_t)cus ? 2 : 4; }
+
+template <bool SWIGLU, int TB, bool PF>
+clove_status_t run_few(Params p, int cus, hipStream_t stream) {
+    p.rows_t = cdiv(p.on, SWIGLU ? 16 : 32);
+    p.by_expert = p.P > p.a.experts;
+    const int64_t grid = (int64_t)(p.by_expert ? p.a.experts : p.P) * p.rows_t;
+    const int KS = few_waves(p, grid, cus);
+    p.ng = min(NG, cdiv(p.G, KS));
+    // (units, lists, sums: see the kernel)
+    const int lds = KS * UnitLds<2, TB>::BYTES + (KS * p.P * 4 + 15) / 16 * 16 + KS * 2048;
+    auto k = moe_few<SWIGLU, TB, PF>;
+    if (ensure_lds(reinterpret_cast<const void*>(k), lds) != CLOVE_OK) return CLOVE_ERR_LAUNCH;
+    CLOVE_LAUNCH(k, dim3((unsigned)grid), dim3(64 * KS), lds, stream, p);
+    return check_launch();
+}
+
+template <int WF>
+clove_status_t run_few_down(Params p, int KS, hipStream_t stream) {
+    p.rows_t = cdiv(p.a.O, 16 * WF);
+    // as many units as waves where the groups allow it
+    const int parts = max(cdiv(p.G, NG), min(p.G, cdiv(KS, p.a.top_k)));
+    p.ng = cdiv(p.G, parts);
+    KS = min(KS, p.a.top_k * cdiv(p.G, p.ng));
+    CLOVE_LAUNCH(moe_few_down<WF>, dim3((unsigned)(p.a.T * p.rows_t)), dim3(64 * KS), KS * (UnitLds<WF, 1>::BYTES + 64 * WF), stream, p);
+    return check_launch();
+}
+
+// ---- tiles ----
+template <class CF>
+int64_t items(const Params& p, bool swiglu) {
+    return cdiv64(p.on, swiglu ? CF::BR / 2 : CF::BR) * (p.P / CF::BC + (p.a.experts + 1) / 2);
+}
+
 template <class CF, bool SWIGLU>
 clove_status_t run_tile(Params p, hipStream_t stream) {
     p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR);
@@ -531,6 +812,88 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
     return check_launch();
 }
 
+template <bool SWIGLU>
+clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
+    using Many = Cfg<4, 1, 2, 4, 2, 4>;    // 256 x 128
+    using Some = Cfg<4, 1, 1, 2, 2, 8>;    // 128 x 64
+    using Wide = Cfg<4, 1, 2, 1, 3, 8>;    // 256 x 32
+    using Narrow = Cfg<4, 1, 1, 1, 4, 8>;  // 128 x 32
+    using Small = Cfg<2, 1, 1, 1, 4, 8>;   // 64 x 32
+    const int avg = p.P / p.a.experts;
+    const int cfg = getenv("MOE_CFG") ? atoi(getenv("MOE_CFG")) : -1;
+    switch (cfg) {
+        case 0: return run_tile<Many, SWIGLU>(p, stream);
+        case 4: return run_tile<Some, SWIGLU>(p, stream);
+        case 7: return run_tile<Wide, SWIGLU>(p, stream);
+        case 6: return run_tile<Narrow, SWIGLU>(p, stream);
+        case 17: return run_tile<Small, SWIGLU>(p, stream);
+        case 18: return run_tile<Cfg<2, 1, 1, 2, 3, 8>, SWIGLU>(p, stream);
+        case 19: return run_tile<Cfg<2, 1, 2, 1, 3, 8>, SWIGLU>(p, stream);
+    }
+    if (avg >= 110 && items<Many>(p, SWIGLU) >= cus) return run_tile<Many, SWIGLU>(p, stream);
+    if (avg >= 25 && 2 * items<Some>(p, SWIGLU) >= cus) return run_tile<Some, SWIGLU>(p, stream);
+    if (avg < 25 && items<Wide>(p, SWIGLU) >= cus) return run_tile<Wide, SWIGLU>(p, stream);
+    if (2 * items<Narrow>(p, SWIGLU) >= cus) return run_tile<Narrow, SWIGLU>(p, stream);
+    return run_tile<Small, SWIGLU>(p, stream);
+}
+
+template <bool SWIGLU>
+clove_status_t run(Params& p, int cus, hipStream_t stream) {
+    const MoeArgs& a = p.a;
+    const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
+    p.x_bytes = (int64_t)(SWIGLU ? a.T : p.P) * a.K * 2;
+    const bool aligned = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W);
+    const bool tiles = aligned && p.x_bytes < ((int64_t)1 << 31) && expert_bytes < ((int64_t)1 << 31);
+    const int fewenv = getenv("MOE_FEW") ? atoi(getenv("MOE_FEW")) : 3;
+    const bool few = aligned && p.P < fewenv * (int64_t)a.experts;
+    if (few && !SWIGLU && 4 * (int64_t)p.P <= 3 * (int64_t)a.experts) {
+        const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
+        if (grid <= cus) return run_few_down<1>(p, 16, stream);
+        if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
+        return run_few_down<1>(p, 4, stream);
+    }
+    // the lists of the pairs by expert, and for down the products of as many outputs at a
+    // time as 512 MB hold
+    const size_t off = few ? 0 : round256((size_t)(a.experts + 1) * 4), order = few ? 0 : round256((size_t)p.P * 4);
+    int chunk = a.O;
+    if constexpr (!SWIGLU) {
+        const int64_t most = max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)p.P * 4) / 256 * 256);
+        if (most < a.O) chunk = cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256;
+        p.ldp = (min(chunk, a.O) + 3) & ~3;
+    }
+    const size_t bytes = off + order + (SWIGLU ? 0 : (size_t)p.P * p.ldp * 4);
+    if (bytes) {
+        void* buf = nullptr;
+        const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &buf);
+        if (st != CLOVE_OK) return st;
+        p.off = static_cast<int*>(buf);
+        p.order = reinterpret_cast<int*>(static_cast<char*>(buf) + off);
+        p.part = reinterpret_cast<float*>(static_cast<char*>(buf) + off + order);
+    }
+    if (!few) {
+        const int threads = min(kSortThreads, cdiv(p.P, 256) * 64);
+        CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
+    }
+    for (p.o0 = 0; p.o0 < a.O; p.o0 += chunk) {
+        p.on = min(chunk, a.O - p.o0);
+        clove_status_t st;
+        if (few) {
+            // (2 pairs of an expert at a time while most have one or none, else 8)
+            st = 2 * (int64_t)p.P <= a.experts ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
+        } else if (tiles) {
+            st = tile_by_shape<SWIGLU>(p, cus, stream);
+        } else {
+            p.rows_t = cdiv(p.on, SWIGLU ? AR / 2 : AR);
+            CLOVE_LAUNCH(moe_any<SWIGLU>, dim3((unsigned)(((int64_t)p.P / AC + a.experts) * p.rows_t)), dim3(256), 0, stream, p);
+            st = check_launch();
+        }
+        if (st != CLOVE_OK) return st;
+        if constexpr (!SWIGLU)
+            CLOVE_LAUNCH(moe_combine, dim3((unsigned)a.T, (unsigned)cdiv(p.on, 512)), dim3(128), 0, stream, p);
+    }
+    return check_launch();
+}
+
 }  // namespace
 }  // namespace moe
 
@@ -538,72 +901,12 @@ clove_status_t launch_moe_w4a16(const MoeArgs& a, bool swiglu, hipStream_t strea
     using namespace moe;
     DeviceInfo dev;
     if (const clove_status_t st = current_device_info(&dev); st != CLOVE_OK) return st;
-    Params p;
+    Params p{};
     p.a = a;
     p.P = a.T * a.top_k;
     p.G = cdiv(a.K, 128);
     p.k = FastDiv(a.top_k);
-    p.x_bytes = (int64_t)(swiglu ? a.T : p.P) * a.K * 2;
-    const int64_t expert_bytes = (int64_t)(swiglu ? 2 : 1) * a.O * (a.K / 2);
-    const bool dma = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W) && p.x_bytes < ((int64_t)1 << 31) &&
-                     expert_bytes < ((int64_t)1 << 31);
-    const size_t off = round256((size_t)(a.experts + 1) * 4), order = round256((size_t)p.P * 4);
-    // down: the products of so many outputs at a time that they stay in the Infinity Cache
-    const int64_t chunk_bytes = (int64_t)(getenv("MOE_CHUNK") ? atoi(getenv("MOE_CHUNK")) : 128) << 20;
-    int chunk = a.O;
-    if (!swiglu) {
-        const int64_t most = chunk_bytes / ((int64_t)p.P * 4) / 256 * 256;
-        const int n = cdiv(a.O, (int)(most < 256 ? 256 : most > a.O ? a.O : most));
-        chunk = min(a.O, cdiv(cdiv(a.O, n), 256) * 256);
-    }
-    p.ldp = (chunk + 3) & ~3;
-    const size_t part = swiglu ? 0 : (size_t)p.P * p.ldp * 4;
-    void* buf = nullptr;
-    clove_status_t st = acquire_buffer(stream, kBufMoe, off + order + part, &buf);
-    if (st != CLOVE_OK) return st;
-    char* at = static_cast<char*>(buf);
-    p.off = reinterpret_cast<int*>(at);
-    p.order = reinterpret_cast<int*>(at + off);
-    p.part = reinterpret_cast<float*>(at + off + order);
-    const int st_threads = p.P >= 4 * kSortThreads ? kSortThreads : max(64, cdiv(p.P, 256) * 64);
-    CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)st_threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
-    for (p.o0 = 0; p.o0 < a.O; p.o0 += chunk) {
-        p.on = min(chunk, a.O - p.o0);
-        if (dma) {
-            const int cfg = getenv("MOE_CFG") ? atoi(getenv("MOE_CFG")) : 0;
-#define GO(...) (swiglu ? run_tile<__VA_ARGS__, true>(p, stream) : run_tile<__VA_ARGS__, false>(p, stream))
-            using C0 = Cfg<4, 1, 2, 4, 2, 4>;
-            using C1 = Cfg<4, 1, 2, 4, 3, 4>;
-            using C2 = Cfg<4, 2, 2, 2, 2, 8>;
-            using C3 = Cfg<4, 1, 2, 2, 2, 8>;
-            using C4 = Cfg<4, 1, 1, 2, 2, 8>;
-            using C5 = Cfg<4, 1, 2, 2, 3, 4>;
-            using C6 = Cfg<4, 1, 1, 1, 4, 8>;
-            using C7 = Cfg<4, 1, 2, 1, 3, 8>;
-            using C8 = Cfg<4, 2, 2, 4, 3, 4>;
-            using C9 = Cfg<4, 1, 1, 4, 3, 4>;
-            switch (cfg) {
-                case 0: st = GO(C0); break;
-                case 1: st = GO(C1); break;
-                case 2: st = GO(C2); break;
-                case 3: st = GO(C3); break;
-                case 4: st = GO(C4); break;
-                case 5: st = GO(C5); break;
-                case 6: st = GO(C6); break;
-                case 7: st = GO(C7); break;
-                case 8: st = GO(C8); break;
-                default: st = GO(C9); break;
-            }
-            if (st != CLOVE_OK) return st;
-        } else {
-            p.rows_t = cdiv(p.on, swiglu ? AR / 2 : AR);
-            const int64_t tiles = ((int64_t)p.P / AC + a.experts) * p.rows_t;
-            if (swiglu) CLOVE_LAUNCH(moe_any<true>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
-            else CLOVE_LAUNCH(moe_any<false>, dim3((unsigned)tiles), dim3(256), 0, stream, p);
-        }
-        if (!swiglu) CLOVE_LAUNCH(moe_combine, dim3((unsigned)a.T, (unsigned)cdiv(p.on, 512)), dim3(128), 0, stream, p);
-    }
-    return check_launch();
+    return swiglu ? run<true>(p, dev.num_cus, stream) : run<false>(p, dev.num_cus, stream);
 }
 
 }  // namespace clove
