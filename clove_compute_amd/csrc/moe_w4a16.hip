@@ -483,12 +483,14 @@ struct Cfg {
     static constexpr int X_BYTES = BC * XRB, W_BYTES = BR * WRB, SC_BYTES = BR * 4;
     static constexpr int OFF_W = X_BYTES, OFF_SC = OFF_W + W_BYTES, OFF_ZR = OFF_SC + SC_BYTES, STAGE = OFF_ZR + SC_BYTES;
     static constexpr int DX = X_BYTES / (1024 * NW), DW = W_BYTES / (1024 * NW), DS = 2 * BR / (64 * NW);
+    // elements of a row of one wave's 32 turned pairs (outputs: fp16 with SwiGLU, else fp32)
+    static constexpr int turned_row(bool swiglu) { return swiglu ? 16 * FW + 8 : 32 * FW + 4; }
     static constexpr int OFF_P = S * STAGE, LDS = OFF_P + 4 * BC;  // then the tile's pairs
     // DMA instructions of stage t of a wave (scales and zero points with a group's first)
     static constexpr int dmas(int t) { return DX + DW + (t % SPG == 0 ? DS : 0); }
     static_assert(KS == 8 || KS == 4, "k-steps");
     static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && (2 * BR) % (64 * NW) == 0, "DMA split");
-    static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT, "stages");
+    static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT && NW * 32 * (32 * FW + 4) * 4 <= OFF_P, "stages");
 };
 
 template <class CF, bool SWIGLU>
@@ -691,31 +693,71 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
 #pragma unroll
         for (int j = 0; j < FX; ++j) acc[i][j] *= unit[i];
 
-    // ---- stores: pairs 8 q + 4 h + e of each 32 ----
-    const bool up_lane = (l32 & 16) != 0;
+    // ---- stores.  A lane holds one weight row of pairs 8 q + 4 h + v of each 32: the wave
+    // turns them in LDS, 32 pairs at a time in a part of its own, and stores 16 bytes of a
+    // pair's row a lane (4-byte stores, four times as many, were 20 % of the call that
+    // multiplies 65536 pairs by rows of 768) ----
+    __syncthreads();  // (the last stage has been read)
+    const int c0 = wc * 32 * FX;
+    if constexpr (SWIGLU) {
+        constexpr int LD = CF::turned_row(true), LPP = 2 * FW;  // halves of a turned row, lanes a pair
+        uint16_t* turned = reinterpret_cast<uint16_t*>(smem) + wave * 32 * LD;
 #pragma unroll
-    for (int j = 0; j < FX; ++j)
+        for (int j = 0; j < FX; ++j) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int v = 0; v < 4; v += SWIGLU ? 2 : 1) {
-                const int c = wc * 32 * FX + 32 * j + 8 * q + 4 * h + v + (SWIGLU && up_lane ? 1 : 0);
-                const int64_t to = (int64_t)pairs[c] * (SWIGLU ? O : p.ldp);
+                for (int v = 0; v < 4; v += 2)
 #pragma unroll
-                for (int i = 0; i < FW; ++i) {
-                    if constexpr (SWIGLU) {
+                    for (int i = 0; i < FW; ++i) {
                         // (gate, up) of pair v to lane l, of pair v + 1 to lane l ^ 16
                         const auto sw = __builtin_amdgcn_permlane16_swap(bitcast<unsigned>(acc[i][j][4 * q + v]),
                                                                          bitcast<unsigned>(acc[i][j][4 * q + v + 1]), false, false);
                         const float x = bitcast<float>(sw[0]), u = bitcast<float>(sw[1]);
-                        const int o = r0 + 16 * (wr * FW + i) + (l32 & 15);
-                        if (o < O && c < count) a.Y[to + o] = f2h(x / (1.0f + expf(-x)) * u);
-                    } else {
-                        const int o = r0 + wrow0 + 32 * i;
-                        if (o < end && c < count) p.part[to + o - p.o0] = acc[i][j][4 * q + v];
+                        turned[(8 * q + 4 * h + v + (l32 >> 4)) * LD + 16 * i + (l32 & 15)] = f2h(x / (1.0f + expf(-x)) * u);
                     }
+            asm volatile("" ::: "memory");  // (one wave's LDS accesses take effect in order)
+            const int o = r0 + 16 * FW * wr + 8 * (lane % LPP), n = O - o;
+#pragma unroll
+            for (int k = 0; k < 32; k += 64 / LPP) {
+                const int c = k + lane / LPP, at = c0 + 32 * j + c;
+                if (c >= 32 || at >= count || n <= 0) continue;
+                const u32x4 y = *reinterpret_cast<const u32x4*>(turned + c * LD + 8 * (lane % LPP));
+                uint16_t* to = a.Y + (int64_t)pairs[at] * O + o;
+                if (n >= 8) {
+                    *reinterpret_cast<u32x4u*>(to) = y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < n) to[i] = (uint16_t)(y[i >> 1] >> (16 * (i & 1)));
                 }
             }
+            asm volatile("" ::: "memory");
+        }
+    } else {
+        constexpr int LD = CF::turned_row(false), LPP = 8 * FW;  // floats of a turned row, lanes a pair
+        float* turned = reinterpret_cast<float*>(smem) + wave * 32 * LD;
+#pragma unroll
+        for (int j = 0; j < FX; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int i = 0; i < FW; ++i) turned[(8 * q + 4 * h + v) * LD + 32 * i + l32] = acc[i][j][4 * q + v];
+            asm volatile("" ::: "memory");
+            const int o = r0 + 32 * FW * wr + 4 * (lane % LPP);
+#pragma unroll
+            for (int k = 0; k < 32; k += 64 / LPP) {
+                const int c = k + lane / LPP, at = c0 + 32 * j + c;
+                if (at >= count || o >= end) continue;
+                // (rows of the products have room for whole fours)
+                *reinterpret_cast<f32x4*>(p.part + (int64_t)pairs[at] * p.ldp + o - p.o0) =
+                    *reinterpret_cast<const f32x4*>(turned + c * LD + 4 * (lane % LPP));
+            }
+            asm volatile("" ::: "memory");
+        }
+    }
 }
 
 // Y[t, o0 + o] = alpha sum_j w[t, j] part[t top_k + j, o] + beta Y, places in order; a
