@@ -506,29 +506,43 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
     // contiguous run of the tiles there are, the pair tiles of one row tile after each
     // other (they share its weights in the XCD's L2) ----
     const int E = a.experts;
-    int tiles = 0;
-    for (int e = lane; e - lane < E; e += 64) tiles += e < E ? cdiv(p.off[min(e, E - 1) + 1] - p.off[min(e, E - 1)], BC) : 0;
+    constexpr int CHUNKS = CLOVE_MAX_EXPERTS / 64;
+    int begin[CHUNKS], n[CHUNKS], tiles = 0;  // lane l: of expert 64 i + l (all loads in flight together)
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        if (64 * i >= E) break;
+        const int x = min(64 * i + lane, E - 1);
+        begin[i] = p.off[x];
+        n[i] = 64 * i + lane < E ? p.off[x + 1] - begin[i] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+        if (64 * i < E) tiles += cdiv(n[i], BC);
     tiles = wave_sum(tiles);
     const int64_t items = (int64_t)tiles * p.rows_t, per = cdiv64(items, 8);
     const int64_t slot = blockIdx.x / 8, item = (blockIdx.x % 8) * per + slot;
     if (slot >= per || item >= items) return;
     const int number = (int)(item / p.rows_t);  // some tile of its expert
-    int e = 0, before = 0, nt = 1, done = 0;
-    for (int e0 = 0; e0 < E; e0 += 64) {
-        const int x = min(e0 + lane, E - 1);
-        const int n = e0 + lane < E ? cdiv(p.off[x + 1] - p.off[x], BC) : 0, upto = done + wave_scan(n);
+    int e = 0, before = 0, first = 0, count = 0, done = 0;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        if (64 * i >= E) break;
+        const int upto = done + wave_scan(cdiv(n[i], BC));
         const uint64_t m = __ballot(upto > number);
         if (m) {
             const int l = __builtin_ctzll(m);
-            e = e0 + l;
-            nt = __builtin_amdgcn_readlane(n, l);
-            before = __builtin_amdgcn_readlane(upto, l) - nt;
+            e = 64 * i + l;
+            first = __builtin_amdgcn_readlane(begin[i], l);
+            count = __builtin_amdgcn_readlane(n[i], l);
+            before = __builtin_amdgcn_readlane(upto, l) - cdiv(count, BC);
             break;
         }
         done = __builtin_amdgcn_readlane(upto, 63);
     }
+    const int nt = cdiv(count, BC);  // tiles of pairs of the expert
     const int in = (int)(item - (int64_t)before * p.rows_t), tr = in / nt;
-    const int first = p.off[e] + (in - tr * nt) * BC, count = min(BC, p.off[e + 1] - first);
+    first += (in - tr * nt) * BC;
+    count = min(BC, count - (in - tr * nt) * BC);
 
     constexpr int OR = SWIGLU ? BR / 2 : BR;  // outputs of a tile
     const int r0 = p.o0 + tr * OR, O = a.O, K = a.K, G = p.G;
