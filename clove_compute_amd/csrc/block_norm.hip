@@ -73,10 +73,10 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
 
 // One row a workgroup, CPT chunks a thread (chunk c of the row: thread c % threads).
 template <int DT, int RT, int CPT>
-__global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a) {
+__global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a, int64_t t0) {
     __shared__ float lds[2][16];
     const int tid = threadIdx.x, NT = blockDim.x, D = a.D;
-    const int64_t t = blockIdx.x;
+    const int64_t t = t0 + blockIdx.x;
     float y[CPT][CH];
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
@@ -155,7 +155,9 @@ clove_status_t run(const BlockNormArgs& a, hipStream_t stream) {
     const int cpt = cdiv(chunks, 1024) <= 1 ? 1 : cdiv(chunks, 1024) <= 2 ? 2 : 4;
     const int nt = 64 * cdiv(chunks, 64 * cpt);
     auto k = cpt == 1 ? block_norm<DT, RT, 1> : cpt == 2 ? block_norm<DT, RT, 2> : block_norm<DT, RT, 4>;
-    CLOVE_LAUNCH(k, dim3((unsigned)a.T), dim3((unsigned)nt), 0, stream, a);
+    // (a launch counts fewer than 2^32 threads)
+    for (int64_t t = 0, most = ((int64_t)1 << 31) / nt; t < a.T; t += most)
+        CLOVE_LAUNCH(k, dim3((unsigned)min(most, a.T - t)), dim3((unsigned)nt), 0, stream, a, t);
     return check_launch();
 }
 

@@ -117,14 +117,14 @@ __device__ __forceinline__ void load(float (&v)[V], const typename Elem<DT>::raw
 // ballot: some 40 instructions of one wave, which is the time (E = 64, top 6, 16384
 // tokens: 16 waves a SIMD of 300 each).
 template <int DT, int V, bool BIAS>
-__global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const FastDiv group) {
+__global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const FastDiv group, int t0) {
     typedef typename std::conditional<BIAS, double, float>::type C;
     constexpr C none = -__builtin_inff();
     __shared__ double lds[WAVES][64 * V];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, N = a.experts, e0 = lane * V;
-    const int t = blockIdx.x * WAVES + wave;
+    const int64_t t = (int64_t)t0 + blockIdx.x * WAVES + wave;
     if (t >= a.T) return;
-    const typename Elem<DT>::raw* row = static_cast<const typename Elem<DT>::raw*>(a.logits) + (int64_t)t * a.logits_stride;
+    const typename Elem<DT>::raw* row = static_cast<const typename Elem<DT>::raw*>(a.logits) + t * a.logits_stride;
     float x[V], bias[V];
     load<DT, V>(x, row + e0, N - e0);
     if constexpr (BIAS) load<CLOVE_DTYPE_FP32, V>(bias, a.bias + e0, N - e0);
@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
     }
     if (lane >= a.top_k) return;
     if (a.renormalize && sum > 0.0) w /= sum;
-    a.ids[(int64_t)t * a.top_k + lane] = id;
-    a.weights[(int64_t)t * a.top_k + lane] = (float)(w * (double)a.scale);
+    a.ids[t * a.top_k + lane] = id;
+    a.weights[t * a.top_k + lane] = (float)(w * (double)a.scale);
 }
 
 namespace {
@@ -233,7 +233,10 @@ clove_status_t run(const RouteArgs& a, hipStream_t stream) {
     const int v = cdiv(a.experts, 64);
     auto k = v <= 1 ? moe_route<DT, 1, BIAS> : v <= 2 ? moe_route<DT, 2, BIAS> : v <= 4 ? moe_route<DT, 4, BIAS>
              : v <= 8 ? moe_route<DT, 8, BIAS> : moe_route<DT, 16, BIAS>;
-    CLOVE_LAUNCH(k, dim3((unsigned)cdiv(a.T, WAVES)), dim3(64 * WAVES), 0, stream, a, FastDiv(a.experts / a.groups));
+    // (a launch counts fewer than 2^32 threads)
+    for (int64_t t = 0, most = (int64_t)1 << 25; t < a.T; t += most)
+        CLOVE_LAUNCH(k, dim3((unsigned)cdiv64(min(most, a.T - t), WAVES)), dim3(64 * WAVES), 0, stream, a,
+                     FastDiv(a.experts / a.groups), (int)t);
     return check_launch();
 }
 template <int DT>

@@ -9,12 +9,15 @@
 // products, folded into the fp32 accumulator with its scale; SwiGLU and the
 // weighted sum over a token's places are fp32, and a result is rounded once.
 //
-// The pairs are sorted by expert first (moe_sort), a tile of weight rows then
-// meets the pairs of one expert (moe_any), and the places of a token are added
-// up from fp32 partial results in place order (moe_combine), so that a call
-// gives the same bits every time.
-#include <cstdlib>
-
+// What bounds it is the weights of the experts hit for few tokens, the matrix
+// instructions for many.  Three ways, by shape (run() below):
+//  * few pairs: moe_few_down (a token's places added up by one workgroup) and
+//    moe_few (an expert's pairs meet its weights, straight from memory);
+//  * moe_sort lists the pairs by expert, moe_tile multiplies tiles of weight rows
+//    by tiles of one expert's pairs;
+//  * moe_any, the same for any K and alignment.
+// Down without moe_few_down: the places of a token are added up from fp32 partial
+// results in place order (moe_combine), so that a call gives the same bits every time.
 #include "i4w_bits.hpp"
 #include "moe.hpp"
 
@@ -822,16 +825,22 @@ namespace {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
+// More threads than a launch counts (2^32 in a dimension): refused
+bool too_many(int64_t workgroups, int threads) { return workgroups > ((int64_t)0xffffffff) / threads; }
+
 // ---- few pairs ----
-// Units of K: a wave takes one of ng <= NG groups after the other.
-int few_waves(const Params& p, int64_t workgroups, int cus) { return workgroups >= 8 * (int64_t)cus ? 2 : 4; }
+// Waves that share K: four, two once workgroups of two cover the CUs eight times (32 tokens
+// on 8 of 128 experts of 2 x 768 rows of 2048: 47 us against 54; 8 tokens 24 and 24.6; 1
+// token 8.5 against 7.0).
+int few_waves(int64_t workgroups, int cus) { return workgroups >= 8 * (int64_t)cus ? 2 : 4; }
 
 template <bool SWIGLU, int TB, bool PF>
 clove_status_t run_few(Params p, int cus, hipStream_t stream) {
     p.rows_t = cdiv(p.on, SWIGLU ? 16 : 32);
     p.by_expert = p.P > p.a.experts;
     const int64_t grid = (int64_t)(p.by_expert ? p.a.experts : p.P) * p.rows_t;
-    const int KS = few_waves(p, grid, cus);
+    const int KS = few_waves(grid, cus);
+    if (too_many(grid, 64 * KS)) return CLOVE_ERR_INVALID_DIM;
     p.ng = min(NG, cdiv(p.G, KS));
     // (units, lists, sums: see the kernel)
     const int lds = KS * UnitLds<2, TB>::BYTES + (KS * p.P * 4 + 15) / 16 * 16 + KS * 2048;
@@ -848,6 +857,7 @@ clove_status_t run_few_down(Params p, int KS, hipStream_t stream) {
     const int parts = max(cdiv(p.G, NG), min(p.G, cdiv(KS, p.a.top_k)));
     p.ng = cdiv(p.G, parts);
     KS = min(KS, p.a.top_k * cdiv(p.G, p.ng));
+    if (too_many((int64_t)p.a.T * p.rows_t, 64 * KS)) return CLOVE_ERR_INVALID_DIM;
     CLOVE_LAUNCH(moe_few_down<WF>, dim3((unsigned)(p.a.T * p.rows_t)), dim3(64 * KS), KS * (UnitLds<WF, 1>::BYTES + 64 * WF), stream, p);
     return check_launch();
 }
@@ -862,12 +872,24 @@ template <class CF, bool SWIGLU>
 clove_status_t run_tile(Params p, hipStream_t stream) {
     p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR);
     const int64_t tiles = ((int64_t)p.P / CF::BC + p.a.experts) * p.rows_t;
+    if (too_many(tiles + 7, CF::NT)) return CLOVE_ERR_INVALID_DIM;
     auto k = moe_tile<CF, SWIGLU>;
     if (ensure_lds(reinterpret_cast<const void*>(k), CF::LDS) != CLOVE_OK) return CLOVE_ERR_LAUNCH;
     CLOVE_LAUNCH(k, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(CF::NT), CF::LDS, stream, p);
     return check_launch();
 }
 
+// Tiles by the pairs an expert has on average (us per call, weights from HBM; SwiGLU of
+// 64 experts of 2 x 1408 rows of 2048, 6 of them a token; the other sides in brackets):
+//   256 x 128 from 110 pairs: 240 pairs 253 [128 x 64: 266], 120 154 [155]; 8 experts of
+//   2 x 11008 rows of 4096, 512 pairs: 754 [128 x 64: 920, 256 x 64 868, 128 x 128 862]
+//   128 x 64 from 25: 60 pairs 99 [256 x 128: 119, 256 x 32 115], 30 76 [113, 80]
+//   256 x 32 below: 15 pairs 64 [128 x 32: 64.5, 128 x 64 72], 7 62 [63, 70]
+// and smaller row tiles where those leave CUs idle (8 experts of 4096 rows of 14336, 4
+// pairs: 128 x 32 86 [256 x 32: 135, 64 x 32 100]; 4 experts of 2 x 1024 rows of 4096, 25
+// pairs: 64 x 32 23.6 [128 x 32: 24.3, 256 x 32 36]).  Half-group stages pay where two
+// stages of whole groups leave a CU one workgroup (256 x 128); elsewhere their 32-byte
+// pieces of weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
 template <bool SWIGLU>
 clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
     using Many = Cfg<4, 1, 2, 4, 2, 4>;    // 256 x 128
@@ -876,16 +898,6 @@ clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
     using Narrow = Cfg<4, 1, 1, 1, 4, 8>;  // 128 x 32
     using Small = Cfg<2, 1, 1, 1, 4, 8>;   // 64 x 32
     const int avg = p.P / p.a.experts;
-    const int cfg = getenv("MOE_CFG") ? atoi(getenv("MOE_CFG")) : -1;
-    switch (cfg) {
-        case 0: return run_tile<Many, SWIGLU>(p, stream);
-        case 4: return run_tile<Some, SWIGLU>(p, stream);
-        case 7: return run_tile<Wide, SWIGLU>(p, stream);
-        case 6: return run_tile<Narrow, SWIGLU>(p, stream);
-        case 17: return run_tile<Small, SWIGLU>(p, stream);
-        case 18: return run_tile<Cfg<2, 1, 1, 2, 3, 8>, SWIGLU>(p, stream);
-        case 19: return run_tile<Cfg<2, 1, 2, 1, 3, 8>, SWIGLU>(p, stream);
-    }
     if (avg >= 110 && items<Many>(p, SWIGLU) >= cus) return run_tile<Many, SWIGLU>(p, stream);
     if (avg >= 25 && 2 * items<Some>(p, SWIGLU) >= cus) return run_tile<Some, SWIGLU>(p, stream);
     if (avg < 25 && items<Wide>(p, SWIGLU) >= cus) return run_tile<Wide, SWIGLU>(p, stream);
@@ -893,23 +905,38 @@ clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
     return run_tile<Small, SWIGLU>(p, stream);
 }
 
+// The call's scratch, kept from one part of its tokens to the next
+struct Held {
+    void* p = nullptr;
+    size_t bytes = 0;
+};
+
 template <bool SWIGLU>
-clove_status_t run(Params& p, int cus, hipStream_t stream) {
-    const MoeArgs& a = p.a;
-    const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
+clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
+    Params p{};
+    p.a = a;
+    p.P = a.T * a.top_k;
+    p.G = cdiv(a.K, 128);
+    p.k = FastDiv(a.top_k);
     p.x_bytes = (int64_t)(SWIGLU ? a.T : p.P) * a.K * 2;
+    const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
     const bool aligned = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W);
-    const bool tiles = aligned && p.x_bytes < ((int64_t)1 << 31) && expert_bytes < ((int64_t)1 << 31);
-    const int fewenv = getenv("MOE_FEW") ? atoi(getenv("MOE_FEW")) : 3;
-    const bool few = aligned && p.P < fewenv * (int64_t)a.experts;
-    if (few && !SWIGLU && 4 * (int64_t)p.P <= 3 * (int64_t)a.experts) {
+    // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
+    // 2048, 6 a token: 20 tokens 40 us against 51 with tiles of 256 x 32, 40 56 and 58, 80 83 and 62)
+    const bool few = aligned && p.P < 3 * a.experts;
+    if (few && !SWIGLU && 4 * p.P <= 3 * a.experts) {
+        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that
+        // leaves one a CU), which reads the weights of an expert hit twice twice but takes one launch
+        // and no memory between (64 experts, 2048 rows of 1408, 6 a token: 1 token 7.0 us against 9.2
+        // by expert and 16 with tiles, 6 16.9, 18.6 and 22, 10 23.4, 22.2 and 25).
         const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
         if (grid <= cus) return run_few_down<1>(p, 16, stream);
         if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
         return run_few_down<1>(p, 4, stream);
     }
-    // the lists of the pairs by expert, and for down the products of as many outputs at a
-    // time as 512 MB hold
+    const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
+    // scratch: the lists of the pairs by expert, and for down the products with as many outputs at
+    // a time as 512 MB hold
     const size_t off = few ? 0 : round256((size_t)(a.experts + 1) * 4), order = few ? 0 : round256((size_t)p.P * 4);
     int chunk = a.O;
     if constexpr (!SWIGLU) {
@@ -918,29 +945,31 @@ clove_status_t run(Params& p, int cus, hipStream_t stream) {
         p.ldp = (min(chunk, a.O) + 3) & ~3;
     }
     const size_t bytes = off + order + (SWIGLU ? 0 : (size_t)p.P * p.ldp * 4);
-    if (bytes) {
-        void* buf = nullptr;
-        const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &buf);
-        if (st != CLOVE_OK) return st;
-        p.off = static_cast<int*>(buf);
-        p.order = reinterpret_cast<int*>(static_cast<char*>(buf) + off);
-        p.part = reinterpret_cast<float*>(static_cast<char*>(buf) + off + order);
+    if (bytes > held.bytes) {
+        if (const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &held.p); st != CLOVE_OK) return st;
+        held.bytes = bytes;
     }
+    p.off = static_cast<int*>(held.p);
+    p.order = reinterpret_cast<int*>(static_cast<char*>(held.p) + off);
+    p.part = reinterpret_cast<float*>(static_cast<char*>(held.p) + off + order);
     if (!few) {
         const int threads = min(kSortThreads, cdiv(p.P, 256) * 64);
         CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
     }
     for (p.o0 = 0; p.o0 < a.O; p.o0 += chunk) {
         p.on = min(chunk, a.O - p.o0);
-        clove_status_t st;
+        clove_status_t st = CLOVE_OK;
         if (few) {
-            // (2 pairs of an expert at a time while most have one or none, else 8)
-            st = 2 * (int64_t)p.P <= a.experts ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
+            // (2 pairs of an expert at a time while most have one or none, else 8: 1 token on 2 of 8
+            // experts of 2 x 14336 rows of 4096 28.3 us against 32.2, 32 on 8 of 128 71 against 47)
+            st = 2 * p.P <= a.experts ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
         } else if (tiles) {
             st = tile_by_shape<SWIGLU>(p, cus, stream);
         } else {
             p.rows_t = cdiv(p.on, SWIGLU ? AR / 2 : AR);
-            CLOVE_LAUNCH(moe_any<SWIGLU>, dim3((unsigned)(((int64_t)p.P / AC + a.experts) * p.rows_t)), dim3(256), 0, stream, p);
+            const int64_t grid = ((int64_t)p.P / AC + a.experts) * p.rows_t;
+            if (too_many(grid, 256)) return CLOVE_ERR_INVALID_DIM;
+            CLOVE_LAUNCH(moe_any<SWIGLU>, dim3((unsigned)grid), dim3(256), 0, stream, p);
             st = check_launch();
         }
         if (st != CLOVE_OK) return st;
@@ -957,12 +986,26 @@ clove_status_t launch_moe_w4a16(const MoeArgs& a, bool swiglu, hipStream_t strea
     using namespace moe;
     DeviceInfo dev;
     if (const clove_status_t st = current_device_info(&dev); st != CLOVE_OK) return st;
-    Params p{};
-    p.a = a;
-    p.P = a.T * a.top_k;
-    p.G = cdiv(a.K, 128);
-    p.k = FastDiv(a.top_k);
-    return swiglu ? run<true>(p, dev.num_cus, stream) : run<false>(p, dev.num_cus, stream);
+    // as many tokens at a time as keep X below the 2^31 bytes that a buffer's offsets reach, and
+    // the lists and launches small beside the products
+    const int64_t per_token = (int64_t)(swiglu ? 1 : a.top_k) * a.K * 2;
+    const int64_t most = min((int64_t)1 << 19, per_token ? (((int64_t)1 << 31) - 1) / per_token * a.top_k : (int64_t)1 << 19) / a.top_k;
+    if (most < 1) return CLOVE_ERR_INVALID_DIM;
+    Held held;
+    for (int64_t t = 0; t < a.T;) {
+        // (equal parts)
+        const int n = (int)cdiv64(a.T - t, cdiv64(a.T - t, most));
+        MoeArgs part = a;
+        part.T = n;
+        part.X = a.X ? a.X + t * (per_token / 2) : nullptr;
+        part.ids = a.ids + t * a.top_k;
+        part.weights = a.weights ? a.weights + t * a.top_k : nullptr;
+        part.Y = a.Y + t * (swiglu ? a.top_k : 1) * a.O;
+        const clove_status_t st = swiglu ? run<true>(part, dev.num_cus, stream, held) : run<false>(part, dev.num_cus, stream, held);
+        if (st != CLOVE_OK) return st;
+        t += n;
+    }
+    return CLOVE_OK;
 }
 
 }  // namespace clove

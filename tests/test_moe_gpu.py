@@ -8,7 +8,12 @@ leaves before that:
  * products: a group's sum adds at most 128 exact products, each addition off by at
    most 2^-23 of the partial sum (MFMA may truncate), the fold of G groups, K splits
    and places by 2^-24 each: (256 + 2 G + 64) 2^-24 of the sum of the terms' sizes,
-   and 8 2^-24 for SwiGLU.
+   and 8 2^-24 for SwiGLU.  Accumulators that go on from group to group in units of
+   the group's scale have 2 G 2^-24 for the units (a quotient and a product each), and
+   partial sums that are no longer a group's: with terms of random sign, as here, one
+   of n terms of size s is about s sqrt(n), so K / 16 additions of 2^-23 each leave
+   2^-23 s K^1.5 / 24, of the terms' K s a part of 2^-23 sqrt(K) / 24: 10 2^-24 at K =
+   14336, far below the 256.
  * routing: ids are equal; weights are 64-bit results rounded to fp32.
 """
 import numpy as np
@@ -375,6 +380,98 @@ def test_rows_do_not_meet(T, E):
     _close(y[rows], want[rows], "fp16", d.slack * size[rows])
     if T > 1:
         assert not bool(torch.isfinite(y[T // 2]).all())
+
+
+@pytest.mark.parametrize("T,k,E,O,K", [(1, 2, 4, 48, 512), (3, 2, 64, 48, 512), (6, 2, 4, 48, 512), (30, 2, 4, 80, 768), (200, 2, 4, 80, 768),
+                                       (700, 2, 4, 200, 512), (3, 2, 4, 33, 322)])
+def test_scales_of_any_size_and_sign(T, k, E, O, K):
+    """Groups with a scale of 0, of either sign, subnormal or large, one after another: the
+    accumulators' unit changes by up to 2^34 from a group to the next, and back."""
+    import torch
+    cg = _cg()
+    for key in ("up", "down"):
+        c = Case("scales-" + key, T, k, E, 2 * O if key == "up" else O, K)
+        g = c.g
+        s = (g.choice([0.0, -0.0, 1.0, -1.0, 2.0 ** -24, -(2.0 ** -20), 0.37, 3.0, 0.01], c.s.shape) * 0.05).astype(np.float16)
+        s[:, 0] = 0.0  # a row of nothing
+        s[:, 1:, -1] = np.where(g.random(s[:, 1:, -1].shape) < 0.5, 0.0, s[:, 1:, -1])
+        q, z = c.q.cpu().numpy(), c.z.cpu().numpy()
+        c.w, c.s = ref.dequantized(q, s, z, K), _dev(s)
+        if key == "up":
+            _check_up(cg, c)
+        else:
+            _check_down(cg, c)
+
+
+def test_infinite_and_nan_scales_stay_in_their_row():
+    import torch
+    cg = _cg()
+    for T in (1, 40, 300):
+        c = Case("bad-scales", T, 2, 4, 64, 384)
+        c.s[:, 5, 1], c.s[:, 9, 2] = float("inf"), float("nan")
+        h, _ = _rounded(c.g, "fp16", T * 2, 384)
+        y = torch.zeros(T, 64, dtype=torch.float16, device="cuda")
+        cg.moe_w4a16(h, c.dev_ids, None, c.q, c.s, c.z, y, T, 2, 4, 64, 384)
+        want, size = ref.down(_f64(h), c.ids, None, c.w, np.zeros((T, 64)), 1.0, 0.0)
+        rows = [r for r in range(64) if r not in (5, 9)]
+        _close(y[:, rows], want[:, rows], "fp16", c.slack * size[:, rows])
+        assert not bool(torch.isfinite(y[:, [5, 9]]).any())
+
+
+def _device_products(x, w):
+    """x [n, K] by each w [E, R, K], all in 64 bits on the device: [E, n, R]."""
+    import torch
+    return torch.stack([x @ e.T.contiguous() for e in torch.from_numpy(w).cuda()])
+
+
+@pytest.mark.parametrize("T,k,E,O,K", [(70001, 8, 4, 32, 64), (150001, 2, 2, 16, 4096)])
+def test_more_pairs_than_one_part_takes(T, k, E, O, K):
+    """More than 2^19 pairs, and rows of X past 2^31 bytes: parts of the tokens one after another."""
+    import torch
+    cg = _cg()
+    g = torch.Generator(device="cuda").manual_seed(T)
+    ids = torch.randint(-1, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    part = slice(T // 2 - 100, T // 2 + 200)  # (where the parts meet) and both ends
+    c = Case("parts", 1, k, E, 2 * O, K)
+    x = torch.empty(T, K, dtype=torch.float16, device="cuda").normal_(generator=g)
+    h = torch.full((T * k, O), 5.0, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16_swiglu(x, ids, c.q, c.s, c.z, h, T, k, E, O, K)
+    for rows in (slice(0, 50), part, slice(T - 50, T)):
+        y = _device_products(x[rows].double(), c.w)
+        gate, up = y[..., :O], y[..., O:]
+        want = (gate * torch.sigmoid(gate) * up)[ids[rows].clamp(min=0).long().T, torch.arange(y.shape[1], device="cuda")]
+        want = torch.where(ids[rows].T[..., None] >= 0, want, 5.0).transpose(0, 1)
+        got = h.view(T, k, O)[rows].double()
+        assert float((got - want).abs().max()) <= 2.0 ** -11 * float(want.abs().max()) * 1.01 + 1e-4
+    d = Case("parts-down", 1, k, E, O, K)
+    hin = torch.empty(T * k, K, dtype=torch.float16, device="cuda").normal_(generator=g)
+    w = torch.rand(T, k, generator=g, device="cuda")
+    out = torch.empty(T, O, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16(hin, ids, w, d.q, d.s, d.z, out, T, k, E, O, K)
+    for rows in (slice(0, 50), part, slice(T - 50, T)):
+        n = rows.stop - rows.start
+        y = _device_products(hin.view(T, k, K)[rows].reshape(n * k, K).double(), d.w).view(E, n, k, O)
+        y = y.permute(1, 2, 0, 3).gather(2, ids[rows].clamp(min=0).long()[:, :, None, None].expand(n, k, 1, O))[:, :, 0]
+        want = (torch.where(ids[rows][..., None] >= 0, y, 0.0) * w[rows].double()[..., None]).sum(1)
+        assert float((out[rows].double() - want).abs().max()) <= 2.0 ** -11 * float(want.abs().max()) * 1.01 + 1e-4
+
+
+def test_rows_past_one_launch():
+    """More rows than a launch of the norm, and of the router, counts threads for."""
+    import torch
+    cg = _cg()
+    T, D = 2 ** 31 // 64 + 3, 8
+    x = torch.empty(T, D, dtype=torch.float16, device="cuda").normal_()
+    h = torch.empty_like(x)
+    cg.block_norm(None, x, h, T, D)
+    for rows in (slice(0, 5), slice(T - 8, T)):
+        _, want = ref.block_norm(None, _f64(x[rows]), None, None, 1.0, None, 1e-6)
+        _close(h[rows], want, "fp16", FP32 * np.abs(want))
+    T, E = 2 ** 25 + 5, 4
+    x = x.flatten()[:T * E].view(T, E)
+    ids, w = _route(cg, x, None, 1)
+    assert bool((ids[:, 0] == x.float().argmax(1)).all())
+    _check_route(x[-9:], None, (ids[-9:], w[-9:]), 1, "softmax")
 
 
 @pytest.mark.parametrize("O,K", [(40, 0), (5, 0)])
