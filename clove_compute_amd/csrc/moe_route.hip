@@ -47,48 +47,55 @@ __device__ __forceinline__ void swap_rows(double v, double* a, double* b) {
     *a = bitcast<double>((uint64_t)bitcast<unsigned>(h0) << 32 | bitcast<unsigned>(l0));
     *b = bitcast<double>((uint64_t)bitcast<unsigned>(h1) << 32 | bitcast<unsigned>(l1));
 }
-template <class T, class F>
+// over each L = 16, 32 or 64 lanes
+template <int L, class T, class F>
 __device__ __forceinline__ T reduce(T v, F f) {
     v = f(v, dpp<0x128>(v));
     v = f(v, dpp<0x124>(v));
     v = f(v, dpp<0x4e>(v));
     v = f(v, dpp<0xb1>(v));
     T a, b;
-    swap_rows<false>(v, &a, &b);
-    v = f(a, b);
-    swap_rows<true>(v, &a, &b);
-    return f(a, b);
+    if constexpr (L >= 32) {
+        swap_rows<false>(v, &a, &b);
+        v = f(a, b);
+    }
+    if constexpr (L == 64) {
+        swap_rows<true>(v, &a, &b);
+        v = f(a, b);
+    }
+    return v;
 }
 __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }  // (never NaN)
 __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
-template <class T>
-__device__ __forceinline__ T wave_most(T v) {
-    return reduce(v, [](T a, T b) { return most(a, b); });
-}
-__device__ __forceinline__ double wave_total(double v) {
-    return reduce(v, [](double a, double b) { return a + b; });
-}
-__device__ __forceinline__ double lane_value(double v, int lane) {
-    const uint64_t u = bitcast<uint64_t>(v);
-    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, lane);
-    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), lane);
-    return bitcast<double>((uint64_t)hi << 32 | lo);
+template <int L, class T>
+__device__ __forceinline__ T lanes_most(T v) {
+    return reduce<L>(v, [](T a, T b) { return most(a, b); });
 }
 
-// The lowest lane of those with the largest value; -1 if that is -infinity.  Doubles by
+// The bits of this lane's L lanes
+template <int L>
+__device__ __forceinline__ uint64_t own_lanes(uint64_t m) {
+    if constexpr (L == 64) return m;
+    return (m >> (threadIdx.x & 63 & ~(L - 1))) & (((uint64_t)1 << L) - 1);
+}
+
+// Of each L lanes the lowest with the largest value, -1 if that is -infinity.  Doubles by
 // their fp32 roundings first, which keep the order: only where several lanes share the
 // largest of them are the doubles compared, at more than twice the instructions.
+template <int L>
 __device__ __forceinline__ int best_lane(float v) {
-    const float u = wave_most(v);
-    return u > -__builtin_inff() ? __builtin_ctzll(__ballot(v == u)) : -1;
+    const float u = lanes_most<L>(v);
+    return u > -__builtin_inff() ? __builtin_ctzll(own_lanes<L>(__ballot(v == u))) : -1;
 }
+template <int L>
 __device__ __forceinline__ int best_lane(double v) {
-    const float f = (float)v, u = wave_most(f);
-    if (!(u > -__builtin_inff())) return -1;
-    const uint64_t m = __ballot(f == u);
-    if ((m & (m - 1)) == 0) return __builtin_ctzll(m);
-    const double w = wave_most(f == u ? v : NONE);
-    return __builtin_ctzll(__ballot(f == u && v == w));
+    const float f = (float)v, u = lanes_most<L>(f);
+    uint64_t m = own_lanes<L>(__ballot(f == u));
+    if (__any((m & (m - 1)) != 0 && u > -__builtin_inff())) {
+        const double w = lanes_most<L>(f == u ? v : NONE);
+        m = own_lanes<L>(__ballot(f == u && v == w));
+    }
+    return u > -__builtin_inff() ? __builtin_ctzll(m) : -1;
 }
 
 // Elements [0, n) of `V` adjacent ones at any alignment of their type; -infinity for the others.
@@ -109,24 +116,26 @@ __device__ __forceinline__ void load(float (&v)[V], const typename Elem<DT>::raw
     }
 }
 
-// One token a wave; lane l holds experts l V .. l V + V - 1, so that of equal values
+// L lanes a token; its lane l holds experts l V .. l V + V - 1, so that of equal values
 // the lowest lane, and in it the lowest entry, is the lowest index.  C: what the choice
 // goes by, the logits themselves (float) or score + bias (double).
 //
-// A round of the choice is the lanes' own best (kept up to date), one reduction, one
-// ballot: some 40 instructions of one wave, which is the time (E = 64, top 6, 16384
-// tokens: 16 waves a SIMD of 300 each).
-template <int DT, int V, bool BIAS>
+// A round of the choice is one reduction, one ballot, and the chosen lane's next best:
+// some 30 instructions for all tokens of a wave, which is the time (E = 64, top 6, 16384
+// tokens: 7.7 us with two tokens a wave, 12.0 with one, 27 with reductions through LDS).
+template <int DT, int V, int L, bool BIAS>
 __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const FastDiv group, int t0) {
     typedef typename std::conditional<BIAS, double, float>::type C;
     constexpr C none = -__builtin_inff();
-    __shared__ double lds[WAVES][64 * V];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, N = a.experts, e0 = lane * V;
-    const int64_t t = (int64_t)t0 + blockIdx.x * WAVES + wave;
-    if (t >= a.T) return;
-    const typename Elem<DT>::raw* row = static_cast<const typename Elem<DT>::raw*>(a.logits) + t * a.logits_stride;
+    __shared__ double values[WAVES][64 * V];  // of the groups' experts, then the chosen ones' scores
+    __shared__ int chosen[WAVES][64 * V];
+    const int lane = threadIdx.x & 63, l = lane % L, wave = threadIdx.x >> 6, N = a.experts, e0 = l * V;
+    const int64_t t = (int64_t)t0 + (blockIdx.x * WAVES + wave) * (64 / L) + lane / L;
+    const int64_t row = t < a.T ? t : a.T - 1;  // (past the last token: its row again, stored nowhere)
+    double* mine = values[wave] + (lane - l) * V;  // this token's L V
+    int* picks = chosen[wave] + (lane - l) * V;
     float x[V], bias[V];
-    load<DT, V>(x, row + e0, N - e0);
+    load<DT, V>(x, static_cast<const typename Elem<DT>::raw*>(a.logits) + row * a.logits_stride + e0, N - e0);
     if constexpr (BIAS) load<CLOVE_DTYPE_FP32, V>(bias, a.bias + e0, N - e0);
     float top = -__builtin_inff();
 #pragma unroll
@@ -136,18 +145,17 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
         x[i] = here ? x[i] : -__builtin_inff();
         top = most(top, x[i]);
     }
-    const bool softmax = a.score == CLOVE_ROUTE_SOFTMAX;
     double s[V];
-    if (softmax) {
-        top = wave_most(top);
+    if (a.score == CLOVE_ROUTE_SOFTMAX) {
+        top = lanes_most<L>(top);
         double total = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            s[i] = x[i] == top ? 1.0 : x[i] > -__builtin_inff() ? exp((double)x[i] - (double)top) : 0.0;
-            if (!(x[i] > -__builtin_inff())) s[i] = 0.0;
+            s[i] = !(x[i] > -__builtin_inff()) ? 0.0 : x[i] == top ? 1.0 : exp((double)x[i] - (double)top);
             total += s[i];
         }
-        const double inv = 1.0 / wave_total(total);  // (infinity if no expert is there: not used then)
+        total = reduce<L>(total, [](double u, double v) { return u + v; });
+        const double inv = 1.0 / total;  // (infinity if no expert is there: not used then)
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] *= inv;
     } else {
@@ -163,15 +171,15 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
     if (a.groups > 1) {
         // `per` lanes to a group, a power of two: each the two largest of its share, then
         // the lanes' pairs merged
-        const int n = group.d, per = 1 << (31 - __builtin_clz(64 / a.groups)), g = lane / per, sub = lane % per;
+        const int n = group.d, per = 1 << (31 - __builtin_clz(L / a.groups)), g = l / per, sub = l % per;
 #pragma unroll
-        for (int i = 0; i < V; ++i) lds[wave][e0 + i] = c[i] > none ? (BIAS ? (double)c[i] : s[i]) : NONE;
+        for (int i = 0; i < V; ++i) mine[e0 + i] = c[i] > none ? (BIAS ? (double)c[i] : s[i]) : NONE;
         asm volatile("" ::: "memory");  // (one wave's LDS accesses take effect in order)
         double first = NONE, second = NONE;
         if (g < a.groups) {
 #pragma unroll 4
             for (int j = sub; j < n; j += per) {
-                const double u = lds[wave][g * n + j];
+                const double u = mine[g * n + j];
                 second = most(second, u > first ? first : u);
                 first = most(first, u);
             }
@@ -185,17 +193,15 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
         double v = sub != 0 || g >= a.groups ? NONE : a.group_top > 1 && second > NONE ? first + second : first;
         uint64_t kept = 0;
         for (int j = 0; j < a.top_groups; ++j) {
-            const int l = best_lane(v);
-            if (l < 0) break;
-            kept |= (uint64_t)1 << (l / per);
-            if (lane == l) v = NONE;
+            const int at = best_lane<L>(v);
+            if (at >= 0) kept |= (uint64_t)1 << (at / per);
+            if (l == at) v = NONE;
         }
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (!((kept >> group.div(min(e0 + i, N - 1))) & 1)) c[i] = none;
+        asm volatile("" ::: "memory");
     }
-    int id = -1;
-    double w = 0.0, sum = 0.0;
     C best = none;
     int at = 0;
     auto update = [&] {
@@ -206,38 +212,60 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
             if (c[i] > best) best = c[i], at = i;
     };
     update();
+    int found = 0;
     for (int j = 0; j < a.top_k; ++j) {
-        const int l = best_lane(best);
-        if (l < 0) break;
-        const int i0 = __builtin_amdgcn_readlane(at, l);
-        double mine = s[0];
+        const int won = best_lane<L>(best);
+        if (!__any(won >= 0)) break;
+        found += won >= 0;
+        if (l == won) {
+            double score = s[0];
 #pragma unroll
-        for (int i = 1; i < V; ++i) mine = i0 == i ? s[i] : mine;
-        mine = lane_value(mine, l);
-        sum += mine;
-        if (lane == j) id = l * V + i0, w = mine;
+            for (int i = 1; i < V; ++i) score = at == i ? s[i] : score;
+            mine[j] = score;
+            picks[j] = e0 + at;
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = lane == l && i0 == i ? none : c[i];
-        update();
+            for (int i = 0; i < V; ++i) c[i] = at == i ? none : c[i];
+            update();
+        }
     }
-    if (lane >= a.top_k) return;
-    if (a.renormalize && sum > 0.0) w /= sum;
-    a.ids[t * a.top_k + lane] = id;
-    a.weights[t * a.top_k + lane] = (float)(w * (double)a.scale);
+    asm volatile("" ::: "memory");
+    double sum = 0.0;
+    if (a.renormalize)
+        for (int j = 0; j < found; ++j) sum += mine[j];
+    if (t >= a.T) return;
+    for (int j = l; j < a.top_k; j += L) {
+        double w = j < found ? mine[j] : 0.0;
+        if (sum > 0.0) w /= sum;
+        a.ids[t * a.top_k + j] = j < found ? picks[j] : -1;
+        a.weights[t * a.top_k + j] = (float)(w * (double)a.scale);
+    }
 }
 
 namespace {
 
-template <int DT, bool BIAS>
-clove_status_t run(const RouteArgs& a, hipStream_t stream) {
-    const int v = cdiv(a.experts, 64);
-    auto k = v <= 1 ? moe_route<DT, 1, BIAS> : v <= 2 ? moe_route<DT, 2, BIAS> : v <= 4 ? moe_route<DT, 4, BIAS>
-             : v <= 8 ? moe_route<DT, 8, BIAS> : moe_route<DT, 16, BIAS>;
+template <int DT, int V, int L, bool BIAS>
+clove_status_t launch(const RouteArgs& a, hipStream_t stream) {
+    constexpr int TOKENS = WAVES * (64 / L);  // of a workgroup
     // (a launch counts fewer than 2^32 threads)
     for (int64_t t = 0, most = (int64_t)1 << 25; t < a.T; t += most)
-        CLOVE_LAUNCH(k, dim3((unsigned)cdiv64(min(most, a.T - t), WAVES)), dim3(64 * WAVES), 0, stream, a,
+        CLOVE_LAUNCH((moe_route<DT, V, L, BIAS>), dim3((unsigned)cdiv64(min(most, a.T - t), TOKENS)), dim3(64 * WAVES), 0, stream, a,
                      FastDiv(a.experts / a.groups), (int)t);
     return check_launch();
+}
+
+// Lanes a token: 16 for up to 32 experts, 32 for up to 128 (where there are as many as
+// groups), else 64
+template <int DT, bool BIAS>
+clove_status_t run(const RouteArgs& a, hipStream_t stream) {
+    const int n = a.experts;
+    if (n <= 16) return launch<DT, 1, 16, BIAS>(a, stream);
+    if (n <= 32 && a.groups <= 16) return launch<DT, 2, 16, BIAS>(a, stream);
+    if (n <= 64 && a.groups <= 32) return launch<DT, 2, 32, BIAS>(a, stream);
+    if (n <= 128 && a.groups <= 32) return launch<DT, 4, 32, BIAS>(a, stream);
+    if (n <= 128) return launch<DT, 2, 64, BIAS>(a, stream);
+    if (n <= 256) return launch<DT, 4, 64, BIAS>(a, stream);
+    if (n <= 512) return launch<DT, 8, 64, BIAS>(a, stream);
+    return launch<DT, 16, 64, BIAS>(a, stream);
 }
 template <int DT>
 clove_status_t run(const RouteArgs& a, hipStream_t stream) {
