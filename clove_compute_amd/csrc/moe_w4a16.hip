@@ -28,7 +28,7 @@ using namespace hw;
 
 struct Params {
     MoeArgs a;
-    int* off;      // [experts + 1]: where an expert's pairs begin in `order`
+    int* off;      // [experts + 1] or null: where an expert's pairs begin in `order`
     int* order;    // [T top_k]: pairs, those of one expert after those of the one before
     float* part;   // down: [T top_k, ldp] products with the outputs o0 .. o0 + on - 1
     int o0, on, ldp;
@@ -493,8 +493,11 @@ struct Cfg {
     static constexpr int dmas(int t) { return DX + DW + (t % SPG == 0 ? DS : 0); }
     static_assert(KS == 8 || KS == 4, "k-steps");
     static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && (2 * BR) % (64 * NW) == 0, "DMA split");
-    static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT && NW * 32 * (32 * FW + 4) * 4 <= OFF_P, "stages");
+    static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT && OFF_P >= (CLOVE_MAX_EXPERTS + 8) * 4 && NW * 32 * (32 * FW + 4) * 4 <= OFF_P, "stages");
 };
+
+// Ids that a thread holds where the workgroups make their tile's list themselves
+constexpr int SCAN = 16;
 
 template <class CF, bool SWIGLU>
 __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
@@ -510,13 +513,45 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
     // other (they share its weights in the XCD's L2) ----
     const int E = a.experts;
     constexpr int CHUNKS = CLOVE_MAX_EXPERTS / 64;
+    int* const pairs = reinterpret_cast<int*>(smem + CF::OFF_P);
+    // (no lists: the workgroup counts the pairs of every expert itself, each thread holds
+    // its ids until the tile is known; where a DMA has not written yet)
+    int* const counts = reinterpret_cast<int*>(smem);
+    u32x4 id[SCAN / 4];
     int begin[CHUNKS], n[CHUNKS], tiles = 0;  // lane l: of expert 64 i + l (all loads in flight together)
+    if (p.off) {
 #pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-        if (64 * i >= E) break;
-        const int x = min(64 * i + lane, E - 1);
-        begin[i] = p.off[x];
-        n[i] = 64 * i + lane < E ? p.off[x + 1] - begin[i] : 0;
+        for (int i = 0; i < CHUNKS; ++i) {
+            if (64 * i >= E) break;
+            const int x = min(64 * i + lane, E - 1);
+            begin[i] = p.off[x];
+            n[i] = 64 * i + lane < E ? p.off[x + 1] - begin[i] : 0;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < SCAN / 4; ++i) {
+            const int q = 4 * (i * CF::NT + tid);
+            id[i] = u32x4{~0u, ~0u, ~0u, ~0u};
+            if (q + 4 <= p.P) id[i] = *reinterpret_cast<const u32x4u*>(a.ids + q);
+            else
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    if (q + v < p.P) id[i][v] = (unsigned)a.ids[q + v];
+        }
+        for (int e = tid; e < E; e += CF::NT) counts[e] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SCAN / 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (id[i][v] < (unsigned)E) atomicAdd(&counts[id[i][v]], 1);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            if (64 * i >= E) break;
+            begin[i] = 0;
+            n[i] = 64 * i + lane < E ? counts[64 * i + lane] : 0;
+        }
     }
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i)
@@ -543,9 +578,37 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
         done = __builtin_amdgcn_readlane(upto, 63);
     }
     const int nt = cdiv(count, BC);  // tiles of pairs of the expert
-    const int in = (int)(item - (int64_t)before * p.rows_t), tr = in / nt;
-    first += (in - tr * nt) * BC;
-    count = min(BC, count - (in - tr * nt) * BC);
+    const int in = (int)(item - (int64_t)before * p.rows_t), tr = in / nt, skip = (in - tr * nt) * BC;
+    first += skip;
+    count = min(BC, count - skip);
+    // the tile's pairs to LDS
+    if (p.off) {
+        if (tid < BC) pairs[tid] = p.order[first + min(tid, count - 1)];
+    } else {
+        // a thread's matches come after those of the threads before it
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < SCAN / 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) mine += id[i][v] == (unsigned)e;
+        const int upto = wave_scan(mine);
+        int* const waves = counts + CLOVE_MAX_EXPERTS;
+        if (lane == 63) waves[wave] = upto;
+        __syncthreads();
+        int at = upto - mine - skip;
+#pragma unroll
+        for (int w = 0; w < CF::NW; ++w)
+            if (w < wave) at += waves[w];
+#pragma unroll
+        for (int i = 0; i < SCAN / 4; ++i)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (id[i][v] == (unsigned)e) {
+                    if ((unsigned)at < (unsigned)count) pairs[at] = 4 * (i * CF::NT + tid) + v;
+                    ++at;
+                }
+    }
+    __syncthreads();
 
     constexpr int OR = SWIGLU ? BR / 2 : BR;  // outputs of a tile
     const int r0 = p.o0 + tr * OR, O = a.O, K = a.K, G = p.G;
@@ -576,7 +639,7 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
     auto xchunk = [&](int i) { return (lane % XC) ^ swz_x<KS>(xrow(i)); };
 #pragma unroll
     for (int i = 0; i < CF::DX; ++i) {
-        const int q = p.order[first + min(xrow(i), count - 1)];
+        const int q = pairs[min(xrow(i), count - 1)];
         offx[i] = (SWIGLU ? p.k.div(q) : q) * K * 2 + 16 * xchunk(i);
     }
 #pragma unroll
@@ -589,9 +652,6 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
         const int j = wave * CF::DS + i;
         offs[i] = row(64 * (j % (BR / 64)) + lane) * G * 2 + (j >= BR / 64 ? zo : so);
     }
-    int* pairs = reinterpret_cast<int*>(smem + CF::OFF_P);  // (read after the K loop's barriers)
-    if (tid < BC) pairs[tid] = p.order[first + min(tid, count - 1)];
-
     const int NS = cdiv(K, 16 * KS);  // stages
     // stage t to buffer b; HS: its place in the group
     auto issue = [&](int t, int b, bool starts) {
@@ -937,7 +997,8 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
     // scratch: the lists of the pairs by expert, and for down the products with as many outputs at
     // a time as 512 MB hold
-    const size_t off = few ? 0 : round256((size_t)(a.experts + 1) * 4), order = few ? 0 : round256((size_t)p.P * 4);
+    const bool lists = !few && (!tiles || p.P > SCAN * 128);
+    const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
     int chunk = a.O;
     if constexpr (!SWIGLU) {
         const int64_t most = max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)p.P * 4) / 256 * 256);
@@ -949,10 +1010,10 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
         if (const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &held.p); st != CLOVE_OK) return st;
         held.bytes = bytes;
     }
-    p.off = static_cast<int*>(held.p);
+    p.off = lists ? static_cast<int*>(held.p) : nullptr;
     p.order = reinterpret_cast<int*>(static_cast<char*>(held.p) + off);
     p.part = reinterpret_cast<float*>(static_cast<char*>(held.p) + off + order);
-    if (!few) {
+    if (lists) {
         const int threads = min(kSortThreads, cdiv(p.P, 256) * 64);
         CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
     }
