@@ -942,26 +942,25 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
 // Tiles by the pairs an expert has on average (us per call, weights from HBM; SwiGLU of
 // 64 experts of 2 x 1408 rows of 2048, 6 of them a token; the other sides in brackets):
 //   256 x 128 from 110 pairs: 240 pairs 253 [128 x 64: 266], 120 154 [155]; 8 experts of
-//   2 x 11008 rows of 4096, 512 pairs: 754 [128 x 64: 920, 256 x 64 868, 128 x 128 862]
-//   128 x 64 from 25: 60 pairs 99 [256 x 128: 119, 256 x 32 115], 30 76 [113, 80]
-//   256 x 32 below: 15 pairs 64 [128 x 32: 64.5, 128 x 64 72], 7 62 [63, 70]
-// and smaller row tiles where those leave CUs idle (8 experts of 4096 rows of 14336, 4
-// pairs: 128 x 32 86 [256 x 32: 135, 64 x 32 100]; 4 experts of 2 x 1024 rows of 4096, 25
-// pairs: 64 x 32 23.6 [128 x 32: 24.3, 256 x 32 36]).  Half-group stages pay where two
-// stages of whole groups leave a CU one workgroup (256 x 128); elsewhere their 32-byte
-// pieces of weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
+//   2 x 11008 rows of 4096, 512 pairs: 741 [128 x 64: 915, 256 x 64 861, 256 x 32 1222]
+//   128 x 64 from 40: 60 pairs 96 [256 x 128: 119, 128 x 32 109]
+//   128 x 32 below: 30 pairs 76 [128 x 64: 77], 15 59 [73], 4 54 [67; 256 x 32 57]; three
+//   workgroups a CU with two stages ahead (15 pairs of 2048 rows of 1408 down 38.6 us, two
+//   with three stages 42.5)
+// and 64 x 32 where those leave half of the CUs idle (4 experts of 2 x 1024 rows of 4096,
+// 25 pairs: 23.6 [128 x 32: 24.3, 256 x 32 36]).  Half-group stages pay where stages of
+// whole groups leave a CU one workgroup (256 x 128); elsewhere their 32-byte pieces of
+// weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
 template <bool SWIGLU>
 clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
-    using Many = Cfg<4, 1, 2, 4, 2, 4>;    // 256 x 128
-    using Some = Cfg<4, 1, 1, 2, 2, 8>;    // 128 x 64
-    using Wide = Cfg<4, 1, 2, 1, 3, 8>;    // 256 x 32
-    using Narrow = Cfg<4, 1, 1, 1, 4, 8>;  // 128 x 32
-    using Small = Cfg<2, 1, 1, 1, 4, 8>;   // 64 x 32
+    using Many = Cfg<4, 1, 2, 4, 2, 4>;   // 256 x 128
+    using Some = Cfg<4, 1, 1, 2, 2, 8>;   // 128 x 64
+    using Thin = Cfg<4, 1, 1, 1, 3, 8>;   // 128 x 32
+    using Small = Cfg<2, 1, 1, 1, 4, 8>;  // 64 x 32
     const int avg = p.P / p.a.experts;
     if (avg >= 110 && items<Many>(p, SWIGLU) >= cus) return run_tile<Many, SWIGLU>(p, stream);
-    if (avg >= 25 && 2 * items<Some>(p, SWIGLU) >= cus) return run_tile<Some, SWIGLU>(p, stream);
-    if (avg < 25 && items<Wide>(p, SWIGLU) >= cus) return run_tile<Wide, SWIGLU>(p, stream);
-    if (2 * items<Narrow>(p, SWIGLU) >= cus) return run_tile<Narrow, SWIGLU>(p, stream);
+    if (avg >= 40 && 2 * items<Some>(p, SWIGLU) >= cus) return run_tile<Some, SWIGLU>(p, stream);
+    if (2 * items<Thin>(p, SWIGLU) >= cus) return run_tile<Thin, SWIGLU>(p, stream);
     return run_tile<Small, SWIGLU>(p, stream);
 }
 
