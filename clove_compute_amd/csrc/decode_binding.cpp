@@ -281,8 +281,14 @@ clove_status_t block_norm(const Args& a) {
     const int T = a.number(3, "T"), D = a.number(4, "D");
     const float scale = a.real(9), eps = a.real(10);
     // x and h_out, the weights and the gate are one type; the residual and y_out one, that or fp32
-    const at::ScalarType t = !a.none(0) ? a.type(0, "x") : !a.none(2) ? a.type(2, "h_out") : !a.none(1) ? a.type(1, "residual") : at::kHalf;
+    at::ScalarType t = at::kHalf;
+    for (int i : {0, 2, 6, 7, 8})
+        if (!a.none(i)) {
+            t = a.type(i, i == 0 ? "x" : i == 2 ? "h_out" : i == 6 ? "post_weight" : i == 7 ? "pre_weight" : "gate");
+            break;
+        }
     const at::ScalarType tr = !a.none(1) ? a.type(1, "residual") : !a.none(5) ? a.type(5, "y_out") : t;
+    if (a.none(0) && a.none(2) && tr != at::kFloat) t = tr;  // (only the residual stream is there)
     const Rows x = a.none(0) ? Rows{} : rows(a, 0, "x", t, T, D), r = a.none(1) ? Rows{} : rows(a, 1, "residual", tr, T, D);
     const Rows h = a.none(2) ? Rows{} : rows(a, 2, "h_out", t, T, D), y = a.none(5) ? Rows{} : rows(a, 5, "y_out", tr, T, D);
     Rows g;

@@ -5,7 +5,8 @@ a key-value cache of bounded size.
 Each step takes one token per sequence through a Llama-style decoder -- fused QKV
 projection, norms and rotation of queries and keys with the cache write, attention
 over the pages (which also adds up what each cached token is attended with), output
-projection into the residual stream, SwiGLU MLP -- and through the logits'
+projection into the residual stream, SwiGLU MLP, or with --experts a sparse one: a
+router and the products of the experts it chose -- and through the logits'
 penalties and grammar mask to the next token.  A sequence that outgrows the budget
 loses the token of the least accumulated attention weight in every layer, so the
 cache never holds more than `budget` tokens a sequence however long the answer is.
@@ -13,6 +14,7 @@ cache never holds more than `budget` tokens a sequence however long the answer i
 Weights are random: the point is the calls and what they share.
 
     python examples/decode_step.py --steps 64 --batch 4 --budget 48
+    python examples/decode_step.py --experts 32 --top-k 4 --inter 1024
 """
 from __future__ import annotations
 
@@ -32,10 +34,11 @@ GROUP = cg.INT4_GROUP_SIZE
 
 class Config:
     def __init__(self, hidden=2048, q_heads=32, kv_heads=8, head_dim=64, inter=8192, layers=2, vocab=32000, page=16, budget=48,
-                 sinks=4, recent=16, longest=4096):
+                 sinks=4, recent=16, longest=4096, experts=0, top_k=2):
         self.hidden, self.q_heads, self.kv_heads, self.head_dim, self.inter = hidden, q_heads, kv_heads, head_dim, inter
         self.layers, self.vocab, self.page, self.budget, self.sinks, self.recent = layers, vocab, page, budget, sinks, recent
         self.longest = longest
+        self.experts, self.top_k = experts, top_k  # 0 experts: a dense MLP
 
 
 class Decoder:
@@ -54,8 +57,7 @@ class Decoder:
         for _ in range(c.layers):
             k, v = (torch.zeros(batch * per, c.kv_heads, c.page, c.head_dim, dtype=half, device="cuda") for _ in range(2))
             self.layers.append(dict(
-                qkv=self._int4(qkv, c.hidden), o=self._int4(c.hidden, c.q_heads * c.head_dim), up=self._int4(2 * c.inter, c.hidden),
-                down=self._int4(c.hidden, c.inter), qn=1.0 + self._normal(c.head_dim, std=0.1), kn=1.0 + self._normal(c.head_dim, std=0.1),
+                qkv=self._int4(qkv, c.hidden), o=self._int4(c.hidden, c.q_heads * c.head_dim), **self._mlp(), qn=1.0 + self._normal(c.head_dim, std=0.1), kn=1.0 + self._normal(c.head_dim, std=0.1),
                 cache=cg.KVCache(k, v), weights=torch.zeros(batch, self.capacity, device="cuda"),
                 positions=torch.full((batch, self.capacity), -1, dtype=torch.int32, device="cuda")))
         angle = torch.arange(c.longest, dtype=torch.float64, device="cuda")[:, None] * 10000.0 ** (
@@ -72,7 +74,11 @@ class Decoder:
 
         self.hidden, self.x = buffer(batch, c.hidden), buffer(batch, c.hidden)
         self.proj, self.q = buffer(batch, qkv), buffer(batch, c.q_heads, c.head_dim)
-        self.attn, self.act = buffer(batch, c.q_heads, c.head_dim), buffer(batch, c.inter)
+        self.attn, self.act = buffer(batch, c.q_heads, c.head_dim), buffer(batch * (c.top_k if c.experts else 1), c.inter)
+        if c.experts:
+            self.route = buffer(batch, c.experts)
+            self.chosen = torch.empty(batch, c.top_k, dtype=torch.int32, device="cuda")
+            self.share = torch.empty(batch, c.top_k, device="cuda")
         self.logits, self.scores = buffer(batch, c.vocab), torch.empty(batch, c.vocab, device="cuda")
 
     def _normal(self, *shape, std=1.0):
@@ -84,9 +90,16 @@ class Decoder:
         scale = torch.full((out, k // GROUP), 1.0 / (4.6 * k ** 0.5), device="cuda").half()
         return q, scale, torch.full_like(scale, 8.0)
 
+    def _mlp(self):
+        c = self.cfg
+        if not c.experts:
+            return dict(up=self._int4(2 * c.inter, c.hidden), down=self._int4(c.hidden, c.inter))
+        up, down = ([torch.stack(x) for x in zip(*(self._int4(r, k) for _ in range(c.experts)))]
+                    for r, k in ((2 * c.inter, c.hidden), (c.hidden, c.inter)))
+        return dict(up=up, down=down, router=self._normal(c.hidden, c.experts, std=c.hidden ** -0.5))
+
     def _norm(self, out):
-        h = self.hidden.float()
-        out.copy_(h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6))
+        cg.block_norm(None, self.hidden, out, self.batch, self.cfg.hidden)
 
     def step(self, tokens, **penalties):
         """The tokens [batch] through the model: fp32 scores [batch, vocab] of the next
@@ -109,8 +122,14 @@ class Decoder:
             cg.cache_evict(L["cache"], self.table, self.lens, L["weights"], L["positions"], L["weights"], L["positions"], self.lens_out, B,
                            self.capacity, c.budget, sinks=c.sinks, recent=c.recent)
             self._norm(self.x)
-            cg.w4a16_swiglu(self.x, *L["up"], self.act, B, c.inter, c.hidden)
-            cg.gemm_w4a16(self.act, *L["down"], self.hidden, B, c.hidden, c.inter, 1.0, 1.0)
+            if c.experts:
+                cg.gemm_fp16(self.x, L["router"], self.route, B, c.experts, c.hidden)
+                cg.moe_route(self.route, self.chosen, self.share, B, c.experts, c.top_k, renormalize=True)
+                cg.moe_w4a16_swiglu(self.x, self.chosen, *L["up"], self.act, B, c.top_k, c.experts, c.inter, c.hidden)
+                cg.moe_w4a16(self.act, self.chosen, self.share, *L["down"], self.hidden, B, c.top_k, c.experts, c.hidden, c.inter, beta=1.0)
+            else:
+                cg.w4a16_swiglu(self.x, *L["up"], self.act, B, c.inter, c.hidden)
+                cg.gemm_w4a16(self.act, *L["down"], self.hidden, B, c.hidden, c.inter, 1.0, 1.0)
         self.lens.copy_(self.lens_out)  # every layer keeps as many
         self.position += 1
         self._norm(self.x)
@@ -140,8 +159,11 @@ def main():
     ap.add_argument("--batch", type=int, default=4)
     ap.add_argument("--budget", type=int, default=48)
     ap.add_argument("--layers", type=int, default=2)
+    ap.add_argument("--inter", type=int, default=8192, help="width of the MLP, or of one expert")
+    ap.add_argument("--experts", type=int, default=0, help="of a sparse MLP (0: a dense one)")
+    ap.add_argument("--top-k", type=int, default=2, help="experts a token")
     a = ap.parse_args()
-    cfg = Config(budget=a.budget, layers=a.layers)
+    cfg = Config(budget=a.budget, layers=a.layers, inter=a.inter, experts=a.experts, top_k=a.top_k)
     dec = Decoder(cfg, a.batch)
     prompt = torch.randint(0, cfg.vocab, (a.batch, 8), generator=dec.g, device="cuda")
     # a grammar that allows even tokens only

@@ -84,6 +84,10 @@ def test_norm_values(dtype, wide, T, D, post, gate, pre):
     cg.block_norm(x, r, h2, T, D, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
     cg.block_norm(x, r, None, T, D, y_out=y2, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
     assert torch.equal(h, h2) and torch.equal(y, y2)
+    # the residual stream alone, a copy of it, in any type
+    y4 = torch.empty_like(y)
+    cg.block_norm(None, r, None, T, D, y_out=y4)
+    assert torch.equal(y4, r)
     # in place
     x3, r3 = x.clone(), r.clone()
     cg.block_norm(x3, r3, x3, T, D, y_out=r3, post_weight=wo, pre_weight=wi, gate=ga, scale=0.5, eps=1e-5)
@@ -252,9 +256,15 @@ class Case:
         if not whole:
             z = (z + g.uniform(-0.4, 0.4, z.shape)).astype(np.float16)  # rounded to whole numbers by the call
         self.w = ref.dequantized(q, s, z, K)
-        flat = torch.zeros(q.size + offset, dtype=torch.uint8, device="cuda")
-        flat[offset:] = _dev(q).flatten()
-        self.q, self.s, self.z, self.dev_ids = flat[offset:].view(E, R, K // 2), _dev(s), _dev(z), _dev(self.ids)
+        def shifted(x, by):  # the same values, `by` elements into an allocation
+            t = _dev(x)
+            flat = torch.zeros(x.size + by, dtype=t.dtype, device="cuda")
+            flat[by:] = t.flatten()
+            return flat[by:].view(*x.shape)
+
+        odd = 1 if offset else 0  # (scales and zero points off a dword's start, not by as much)
+        self.q, self.s, self.z = shifted(q, offset), shifted(s, odd), shifted(z, 3 * odd)
+        self.dev_ids = shifted(self.ids, odd)
         self.slack = (256 + 2 * G + 64) * 2.0 ** -24
 
 
@@ -297,7 +307,7 @@ def _check_down(cg, c, beta=1.0, alpha=1.0, weighted=True):
 SIZES = [(1, 1, 1, 1, 2), (1, 2, 4, 3, 128), (1, 8, 128, 64, 256), (1, 8, 16, 768, 1024), (2, 4, 8, 100, 160), (3, 2, 4, 33, 130), (5, 8, 16, 64, 256),
          (4, 2, 8, 48, 2048), (16, 2, 64, 80, 512), (33, 1, 2, 40, 96), (70, 3, 5, 100, 384), (130, 6, 64, 96, 192), (257, 4, 3, 48, 160),
          (40, 8, 8, 130, 1024), (600, 2, 2, 64, 256), (64, 4, 4, 513, 640), (300, 1, 9, 256, 128), (100, 8, 256, 64, 256), (1, 1, 3, 16, 14336),
-         (20, 64, 64, 32, 128), (512, 2, 4, 320, 544), (7, 3, 4, 31, 62), (1100, 2, 8, 128, 256), (150, 2, 1024, 16, 64)]
+         (20, 64, 64, 32, 128), (512, 2, 4, 320, 544), (7, 3, 4, 31, 62), (2, 2, 4, 40, 32), (50, 2, 4, 40, 32), (400, 2, 4, 40, 32), (1100, 2, 8, 128, 256), (150, 2, 1024, 16, 64)]
 
 
 @pytest.mark.parametrize("T,k,E,O,K", SIZES)
