@@ -5,6 +5,7 @@
 //
 // s and c are 64 bits: of some hundred experts two often agree to 2^-24, and
 // which of them comes first must not depend on an exponential's last bit.
+#include <cfloat>
 #include <type_traits>
 
 #include "moe.hpp"
@@ -88,14 +89,18 @@ __device__ __forceinline__ int best_lane(float v) {
     return u > -__builtin_inff() ? __builtin_ctzll(own_lanes<L>(__ballot(v == u))) : -1;
 }
 template <int L>
-__device__ __forceinline__ int best_lane(double v) {
-    const float f = (float)v, u = lanes_most<L>(f);
+__device__ __forceinline__ int best_lane(double v, float f) {
+    const float u = lanes_most<L>(f);
     uint64_t m = own_lanes<L>(__ballot(f == u));
     if (__any((m & (m - 1)) != 0 && u > -__builtin_inff())) {
         const double w = lanes_most<L>(f == u ? v : NONE);
         m = own_lanes<L>(__ballot(f == u && v == w));
     }
     return u > -__builtin_inff() ? __builtin_ctzll(m) : -1;
+}
+template <int L>
+__device__ __forceinline__ int best_lane(double v) {
+    return best_lane<L>(v, (float)v);
 }
 
 // Elements [0, n) of `V` adjacent ones at any alignment of their type; -infinity for the others.
@@ -193,7 +198,8 @@ __global__ void __launch_bounds__(64 * WAVES) moe_route(const RouteArgs a, const
         double v = sub != 0 || g >= a.groups ? NONE : a.group_top > 1 && second > NONE ? first + second : first;
         uint64_t kept = 0;
         for (int j = 0; j < a.top_groups; ++j) {
-            const int at = best_lane<L>(v);
+            // (two biases of fp32's lowest value add up to less than it: still more than none)
+            const int at = best_lane<L>(v, v > NONE ? fmaxf((float)v, -FLT_MAX) : -__builtin_inff());
             if (at >= 0) kept |= (uint64_t)1 << (at / per);
             if (l == at) v = NONE;
         }
