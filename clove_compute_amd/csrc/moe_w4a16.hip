@@ -1000,7 +1000,8 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
     int chunk = a.O;
     if constexpr (!SWIGLU) {
-        const int64_t most = max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)p.P * 4) / 256 * 256);
+        // (and no more than moe_combine's grid has room for: 65535 workgroups of 512 outputs)
+        const int64_t most = min((int64_t)512 * 65535, max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)p.P * 4) / 256 * 256));
         if (most < a.O) chunk = cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256;
         p.ldp = (min(chunk, a.O) + 3) & ~3;
     }

@@ -226,6 +226,24 @@ def test_route_values_that_nearly_agree(score):
     _check_route(_dev(x), _dev(b), got, k, score)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(48, 4), (16, 8), (64, 2), (256, 8)])
+def test_route_biases_of_the_lowest_value(score, E, groups):
+    """Experts masked by fp32's lowest value, whose sum over two leaves fp32: they come after
+    the others, but before none, and whole groups of them too."""
+    cg = _cg()
+    k, n = 6, E // groups
+    g = rng("route-lowest", score, E, groups)
+    x = _dev(g.standard_normal((9, E)).astype(np.float32))
+    low = np.finfo(np.float32).min
+    for masked in (np.arange(E) >= n, np.arange(E) % n != 0, np.arange(E) >= 0, np.arange(E) < n):
+        b = np.where(masked, low, (g.standard_normal(E) * 0.2)).astype(np.float32)
+        for top_groups in (1, 2, groups):
+            how = dict(groups=groups, top_groups=top_groups, group_top=2)
+            got = _route(cg, x, _dev(b), k, score=getattr(cg, "CLOVE_ROUTE_" + score.upper()), **how)
+            _check_route(x, _dev(b), got, k, score, **how)
+
+
 def test_route_rows_of_wider_tensors():
     cg = _cg()
     g = rng("route-wide")
@@ -482,6 +500,22 @@ def test_rows_past_one_launch():
     ids, w = _route(cg, x, None, 1)
     assert bool((ids[:, 0] == x.float().argmax(1)).all())
     _check_route(x[-9:], None, (ids[-9:], w[-9:]), 1, "softmax")
+
+
+def test_outputs_past_one_grid():
+    """More outputs of one pair than a launch's second dimension counts in blocks of 512."""
+    import torch
+    cg = _cg()
+    O = 512 * 65535 + 700
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randint(0, 256, (1, O, 1), generator=g, device="cuda", dtype=torch.uint8)
+    one = torch.ones(1, O, 1, dtype=torch.float16, device="cuda")
+    y = torch.full((1, O), 7.0, dtype=torch.float16, device="cuda")
+    x = torch.tensor([[2.0, 3.0]], dtype=torch.float16, device="cuda")
+    cg.moe_w4a16(x, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), None, q, one, one * 8, y, 1, 1, 1, O, 2)
+    byte = q.view(-1).to(torch.int16)
+    want = 2 * (byte // 16 - 8) + 3 * (byte % 16 - 8)  # whole numbers: exact
+    assert bool((y.view(-1) == want).all())
 
 
 @pytest.mark.parametrize("O,K", [(40, 0), (5, 0)])
