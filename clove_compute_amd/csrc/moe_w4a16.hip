@@ -964,10 +964,11 @@ clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
     return run_tile<Small, SWIGLU>(p, stream);
 }
 
-// The call's scratch, kept from one part of its tokens to the next
+// The call's scratch, taken for the first of its parts, whose pairs are the most
 struct Held {
     void* p = nullptr;
     size_t bytes = 0;
+    int pairs = 0;
 };
 
 template <bool SWIGLU>
@@ -998,10 +999,11 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     // a time as 512 MB hold
     const bool lists = !few && (!tiles || p.P > SCAN * 128);
     const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
+    if (held.pairs == 0) held.pairs = p.P;
     int chunk = a.O;
     if constexpr (!SWIGLU) {
         // (and no more than moe_combine's grid has room for: 65535 workgroups of 512 outputs)
-        const int64_t most = min((int64_t)512 * 65535, max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)p.P * 4) / 256 * 256));
+        const int64_t most = min((int64_t)512 * 65535, max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)held.pairs * 4) / 256 * 256));
         if (most < a.O) chunk = cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256;
         p.ldp = (min(chunk, a.O) + 3) & ~3;
     }

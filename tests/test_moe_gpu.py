@@ -373,6 +373,19 @@ def test_the_same_expert_twice_and_ids_that_are_none(T):
     _check_down(cg, c, beta=0.0)
 
 
+@pytest.mark.parametrize("T,k,E", [(9, 2, 64), (40, 8, 128), (70, 4, 16), (300, 2, 16)])
+def test_all_pairs_of_one_expert(T, k, E):
+    """The shapes are those of many experts hit, the pairs all the last one's, but for one of the first's."""
+    import torch
+    cg = _cg()
+    for key in ("up", "down"):
+        c = Case("one-" + key, T, k, E, 64, 128)
+        c.ids[:] = E - 1
+        c.ids[T // 2, 0] = 0
+        c.dev_ids = torch.from_numpy(c.ids).cuda()
+        _check_up(cg, c) if key == "up" else _check_down(cg, c)
+
+
 @pytest.mark.parametrize("T,E", [(1, 4), (6, 4), (80, 4), (300, 2)])
 def test_rows_do_not_meet(T, E):
     """NaN and infinities stay in their token's rows, and what no expert reads is not used."""
@@ -482,6 +495,41 @@ def test_more_pairs_than_one_part_takes(T, k, E, O, K):
         y = y.permute(1, 2, 0, 3).gather(2, ids[rows].clamp(min=0).long()[:, :, None, None].expand(n, k, 1, O))[:, :, 0]
         want = (torch.where(ids[rows][..., None] >= 0, y, 0.0) * w[rows].double()[..., None]).sum(1)
         assert float((out[rows].double() - want).abs().max()) <= 2.0 ** -11 * float(want.abs().max()) * 1.01 + 1e-4
+
+
+def test_parts_share_one_plan():
+    """65537 tokens go in parts of 32769 and 32768, and the second's products alone would come
+    with twice as many outputs at a time: the call needs what its first part needs, no more."""
+    import torch
+    cg = _cg()
+    T, k, E, O, K = 65537, 8, 2, 512, 32
+    c = Case("plan", 1, k, E, O, K)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    h = torch.empty(T * k, K, dtype=torch.float16, device="cuda").normal_(generator=g)
+    y = torch.zeros(T, O, dtype=torch.float16, device="cuda")
+
+    def down(n):
+        cg.moe_w4a16(h[:n * k], ids[:n], None, c.q, c.s, c.z, y[:n], n, k, E, O, K)
+
+    need = []
+    for n in (32769, T):
+        with cg.workspace_query() as q:
+            down(n)
+        need.append(q.bytes)
+    assert need[0] == need[1] < 2 ** 29
+    down(T)
+    want = y.clone()
+    cg.workspace_bind(torch.zeros(need[1], dtype=torch.uint8, device="cuda"))
+    try:
+        y.zero_()
+        down(T)
+    finally:
+        cg.workspace_bind(None)
+    assert torch.equal(y, want)
+    products = _device_products(h[-80:].double(), c.w)[ids[-10:].flatten().long(), torch.arange(80, device="cuda")]
+    exact = products.view(10, k, O).sum(1)
+    assert float((y[-10:].double() - exact).abs().max()) <= 2.0 ** -11 * float(exact.abs().max()) * 1.01 + 1e-4
 
 
 def test_rows_past_one_launch():
