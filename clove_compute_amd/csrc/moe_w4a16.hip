@@ -13,8 +13,8 @@
 // instructions for many.  Three ways, by shape (run() below):
 //  * few pairs: moe_few_down (a token's places added up by one workgroup) and
 //    moe_few (an expert's pairs meet its weights, straight from memory);
-//  * moe_sort lists the pairs by expert, moe_tile multiplies tiles of weight rows
-//    by tiles of one expert's pairs;
+//  * moe_tile multiplies tiles of weight rows by tiles of one expert's pairs, which
+//    moe_sort has listed by expert (up to 2048 pairs each workgroup finds its own);
 //  * moe_any, the same for any K and alignment.
 // Down without moe_few_down: the places of a token are added up from fp32 partial
 // results in place order (moe_combine), so that a call gives the same bits every time.
@@ -43,7 +43,9 @@ struct Params {
 // Workgroup e lists the pairs of expert e; where they begin is the number of pairs of
 // lower experts, which it counts itself: no workgroup waits for another.  A thread
 // lists its own pairs behind those of the threads before it, so the ids are read
-// twice and nothing waits but for the one scan of the counts between.
+// twice and nothing waits but for the one scan of the counts between.  65536 ids of
+// 128 experts: 11 us, of 8 experts and 4096 ids 4.8, latencies of the two passes.  (Every
+// workgroup reads all ids, from the L2 after the first: 262 KB each, 34 MB together.)
 constexpr int kSortThreads = 1024;
 __global__ void __launch_bounds__(kSortThreads) moe_sort(const int32_t* ids, int P, int E, int* off, int* order) {
     __shared__ int lds[2][kSortThreads / 64];
@@ -110,7 +112,10 @@ __device__ __forceinline__ bool find_tile(const int* off, int E, int tile, int B
 
 // Any K and alignment.  64 weight rows (SwiGLU: 32 gate and the 32 up rows of the
 // same outputs) by 32 pairs, four waves of 16 rows; a 128-k group at a time comes
-// through registers to LDS, the weights unpacked on the way.
+// through registers to LDS, the weights unpacked on the way.  No stage is loaded ahead
+// and its unpacking is scalar: 100 tokens on 6 of 64 experts of 2 x 1408 rows of 2046 123 us
+// (of 2048, with moe_tile, 57), 1 on 8 of 128 of 2 x 768 rows of 2046 37 (moe_few 6.8), 2048
+// on 2 of 8 of 2 x 11008 rows of 4094 2590 (747).
 constexpr int AR = 64, AC = 32, ALD = 136;
 
 template <bool SWIGLU>
@@ -221,8 +226,11 @@ __global__ void __launch_bounds__(256) moe_any(const Params p) {
 // takes 16 WF weight rows and up to NG = 4 groups of K at once, all their loads in
 // flight together and straight to registers (16 bytes a lane: lane group h of 16
 // holds k = 32 h .. 32 h + 31 of a row's group); the rows of X it meets and the
-// groups' constants, loaded ahead of them, go through a part of LDS that is the
-// wave's own, so no wave waits for another before the sums meet at the end.  On
+// groups' constants go through a part of LDS that is the wave's own, so no wave
+// waits for another before the sums meet at the end.  One token on 8 of 128 experts,
+// with weights from HBM: 2 x 768 rows of 2048 (13.4 MB) 6.8 us, 2048 rows of 768 back
+// (6.7 MB) 5.9, of which a launch takes 4; 20 tokens on 6 of 64 experts of 2 x 1408 rows
+// of 2048 (55 experts hit, 169 MB) 40 us, 4.2 TB/s.  On
 // v_mfma_f32_16x16x32_f16 with X as the "A" operand: a lane holds weight row
 // l % 16 and X rows 4 h .. 4 h + 3; step q of a group takes dword q of every lane,
 // k = 32 h + 8 q .. + 7 of lane group h.
@@ -477,6 +485,12 @@ __global__ void __launch_bounds__(1024) moe_few_down(const Params p) {
 // set of accumulators, and half the registers: a wave holds 64 x 128 outputs with
 // two waves on a SIMD, so that an unpacked weight meets four blocks of pairs.  A
 // group whose scale is 0 leaves the unit as it is and its weights are made 0.
+//
+// 4096 pairs on 8 experts of 2 x 11008 rows of 4096 take 747 us, 0.99 PFLOP/s (a library
+// product of fp16 weights reaches 1.20): the matrix pipe is busy 56 % of the cycles, the
+// VALU, mostly with unpacking, 55 %.  65536 pairs on 128 experts of 2048 rows of 768: 291
+// us, as much of it the 537 MB of fp32 products as the six groups of K.  540 pairs on 64
+// experts of 2 x 1408 rows of 2048 (197 MB): 57 us, 3.5 TB/s, the VALU busy for 54 %.
 // ---------------------------------------------------------------------------
 template <int WR_, int WC_, int FW_, int FX_, int S_, int KS_>
 struct Cfg {
@@ -839,7 +853,8 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
 
 // Y[t, o0 + o] = alpha sum_j w[t, j] part[t top_k + j, o] + beta Y, places in order; a
 // place without an expert is left out.  A thread takes four outputs of one token, and
-// eight places' parts are in flight at once.
+// eight places' parts are in flight at once: 8192 tokens of 8 places and 2048 outputs, 570
+// MB, 120 us, 4.7 TB/s.
 __global__ void __launch_bounds__(128) moe_combine(const Params p) {
     const MoeArgs& a = p.a;
     const int t = blockIdx.x, o = 512 * blockIdx.y + 4 * threadIdx.x;
@@ -885,7 +900,7 @@ namespace {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// More threads than a launch counts (2^32 in a dimension): refused
+// More threads than a launch counts (2^32 in a dimension)
 bool too_many(int64_t workgroups, int threads) { return workgroups > ((int64_t)0xffffffff) / threads; }
 
 // ---- few pairs ----
@@ -984,7 +999,7 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
     // 2048, 6 a token: 20 tokens 40 us against 51 with tiles of 256 x 32, 40 56 and 58, 80 83 and 62)
     const bool few = aligned && p.P < 3 * a.experts;
-    if (few && !SWIGLU && 4 * p.P <= 3 * a.experts) {
+    if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
         // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that
         // leaves one a CU), which reads the weights of an expert hit twice twice but takes one launch
         // and no memory between (64 experts, 2048 rows of 1408, 6 a token: 1 token 7.0 us against 9.2
@@ -995,18 +1010,17 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
         return run_few_down<1>(p, 4, stream);
     }
     const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
-    // scratch: the lists of the pairs by expert, and for down the products with as many outputs at
-    // a time as 512 MB hold
+    // As many outputs at a time as workgroups of 256 threads for 16 of them and 32 pairs make a
+    // launch; scratch: the lists of the pairs by expert, and for down the products with as many
+    // outputs at a time as 512 MB hold
     const bool lists = !few && (!tiles || p.P > SCAN * 128);
     const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
     if (held.pairs == 0) held.pairs = p.P;
-    int chunk = a.O;
-    if constexpr (!SWIGLU) {
-        // (and no more than moe_combine's grid has room for: 65535 workgroups of 512 outputs)
-        const int64_t most = min((int64_t)512 * 65535, max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)held.pairs * 4) / 256 * 256));
-        if (most < a.O) chunk = cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256;
-        p.ldp = (min(chunk, a.O) + 3) & ~3;
-    }
+    int64_t most = (int64_t)16 * ((1 << 24) - 8) / (held.pairs / 32 + a.experts) / 256 * 256;
+    // (moe_combine: 65535 workgroups of 512 outputs)
+    if (!SWIGLU) most = min(min(most, (int64_t)512 * 65535), max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)held.pairs * 4) / 256 * 256));
+    const int chunk = most < a.O ? cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256 : a.O;
+    if (!SWIGLU) p.ldp = (min(chunk, a.O) + 3) & ~3;
     const size_t bytes = off + order + (SWIGLU ? 0 : (size_t)p.P * p.ldp * 4);
     if (bytes > held.bytes) {
         if (const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &held.p); st != CLOVE_OK) return st;

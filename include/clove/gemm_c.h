@@ -404,7 +404,7 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
  * A sparse MLP block around the linear layers: the norms before and after a
  * block with its residual, the router, and the products of the experts it
  * chose.  No reference counterpart.  Element types, strides, rounding and
- * scratch as for the decode step above.
+ * scratch as for the decode step above; only the products take scratch.
  * ------------------------------------------------------------------------ */
 
 /* Largest D of clove_block_norm, experts and top_k of the others. */
@@ -423,7 +423,8 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
  * residual_dtype (the same, or FP32).  h comes from the fp32 y, not from the
  * rounded one.  gate is one row for all tokens (gate_stride 0) or a row for
  * each, NULL: 1; pre_weight NULL: 1; x NULL: y = residual (a stack's first
- * norm); residual NULL: 0 (not both).  y_out or h_out may be NULL: not wanted.
+ * norm; post_weight, gate and scale are not used); residual NULL: 0 (not both).
+ * y_out or h_out may be NULL: not wanted.
  * Rows [T, D], strides in elements.  y_out may be residual, y_out or h_out may
  * be x or gate (same rows and type; of several rows the same stride); else
  * outputs overlap neither inputs nor each other.  T == 0 or D == 0 is a no-op.
@@ -473,7 +474,14 @@ clove_status_t clove_moe_route(const void* logits, int64_t logits_stride, int dt
  * (a padding token, an expert of another device) has no product and its row of
  * H is left as it is; an expert may come twice in a row.  K is even.  Which
  * kernel runs goes by the sizes and alignments alone, and a row's bits do not
- * depend on what other tokens chose.
+ * depend on what other tokens chose.  Fastest with K % 32 == 0 and 16-byte
+ * aligned X and W_q.
+ * Zero points round to the nearest integer, as clove_gemm_w4a16's; q - z is
+ * exact up to 2048 in magnitude and rounded to fp16 past that.
+ * Scratch: 4 bytes a pair, at most 2 MB (more pairs than 2^19, or an X of 2^31
+ * bytes, go in parts).  2^31 tiles of 32 rows by 32 pairs and more, or one
+ * token's X of 2^31 bytes (here a row, below top_k rows), are
+ * CLOVE_ERR_INVALID_DIM.
  */
 clove_status_t clove_moe_w4a16_swiglu(const void* X, const int32_t* expert_ids, const uint8_t* W_q,
                                       const void* W_scale, const void* W_zero, void* H, int T, int top_k,
@@ -488,7 +496,10 @@ clove_status_t clove_moe_w4a16_swiglu(const void* X, const int32_t* expert_ids, 
  * W_q [experts, O, K / 2], W_scale / W_zero [experts, O, ceil(K / 128)] fp16,
  * Y [T, O] fp16, rounded once.  The row of H and the weight of a pair without a
  * product (see above) are not used; a token without any gets beta * Y.
- * beta == 0 never reads Y.  K is even.
+ * beta == 0 never reads Y.  K is even.  The rest as above, but for the scratch:
+ * the pairs' fp32 products besides, T top_k O * 4 bytes up to 512 MB (with more,
+ * as many outputs at a time as fit there; at least 256), which library scratch
+ * rounds up to a power of two.
  */
 clove_status_t clove_moe_w4a16(const void* H, const int32_t* expert_ids, const float* weights,
                                const uint8_t* W_q, const void* W_scale, const void* W_zero, void* Y, int T,

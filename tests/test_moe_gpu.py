@@ -550,6 +550,35 @@ def test_rows_past_one_launch():
     _check_route(x[-9:], None, (ids[-9:], w[-9:]), 1, "softmax")
 
 
+@pytest.mark.parametrize("K,T", [(32, 550), (32, 384), (2, 1)])
+def test_more_workgroups_than_one_launch_counts(K, T):
+    """1024 experts of 2 x 262400 rows: 2^32 threads are less than the outputs call for."""
+    import torch
+    cg = _cg()
+    k, E, I = 2, 1024, 262400
+    R = 2 * I
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q = torch.empty(E, R, K // 2, dtype=torch.uint8, device="cuda")
+    for e in range(0, E, 64):
+        q[e:e + 64] = torch.randint(0, 256, (64, R, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    s, z = torch.full((E, R, 1), 2.0 ** -6, dtype=torch.float16, device="cuda"), torch.full((E, R, 1), 8.0, dtype=torch.float16, device="cuda")
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.randint(-4, 5, (T * k, K), generator=g, device="cuda").half()
+    h, y = torch.full((T * k, I), 5.0, dtype=torch.float16, device="cuda"), torch.full((T, R), 5.0, dtype=torch.float16, device="cuda")
+    cg.moe_w4a16_swiglu(x[:T], ids, q, s, z, h, T, k, E, I, K)
+    cg.moe_w4a16(x, ids, None, q, s, z, y, T, k, E, R, K)
+    for t in sorted({0, T // 2, T - 1}):
+        want = 0.0
+        for j in range(k):
+            b = q[int(ids[t, j])]
+            w = (torch.stack([b // 16, b % 16], -1).view(R, K).double() - 8) / 64
+            gate, up = (w @ x[t].double()).view(2, I)
+            v = gate * torch.sigmoid(gate) * up
+            assert bool(((h[t * k + j].double() - v).abs() <= 2.0 ** -11 * v.abs() + 2.0 ** -18 * (1 + v.abs())).all())
+            want = want + w @ x[t * k + j].double()
+        assert torch.equal(y[t].double(), want.half().double())  # (exact in fp32)
+
+
 def test_outputs_past_one_grid():
     """More outputs of one pair than a launch's second dimension counts in blocks of 512."""
     import torch
