@@ -18,6 +18,8 @@
 //  * moe_any, the same for any K and alignment.
 // Down without moe_few_down: the places of a token are added up from fp32 partial
 // results in place order (moe_combine), so that a call gives the same bits every time.
+#include <type_traits>
+
 #include "i4w_bits.hpp"
 #include "moe.hpp"
 
@@ -505,7 +507,7 @@ struct Cfg {
     static constexpr int OFF_P = S * STAGE, LDS = OFF_P + 4 * BC;  // then the tile's pairs
     // DMA instructions of stage t of a wave (scales and zero points with a group's first)
     static constexpr int dmas(int t) { return DX + DW + (t % SPG == 0 ? DS : 0); }
-    static_assert(KS == 8 || KS == 4, "k-steps");
+    static_assert((KS == 8 || KS == 4) && WC == 1, "k-steps, waves");
     static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && (2 * BR) % (64 * NW) == 0, "DMA split");
     static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT && OFF_P >= (CLOVE_MAX_EXPERTS + 8) * 4 && NW * 32 * (32 * FW + 4) * 4 <= OFF_P, "stages");
 };
@@ -717,66 +719,74 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
     for (int t = 0; t < S - 1; ++t)
         if (t < NS) issue(t, t, t % SPG == 0);
     int stage = 0, stage_next = S - 1;
-    for (int t0 = 0; t0 < NS; t0 += SPG) {
+    // (FXU blocks of 32 pairs; the others of a ragged tile multiply nothing)
+    auto k_loop = [&](auto blocks) {
+        constexpr int FXU = decltype(blocks)::value;
+        for (int t0 = 0; t0 < NS; t0 += SPG) {
 #pragma unroll
-        for (int hs = 0; hs < SPG; ++hs) {
-            const int t = t0 + hs;
-            if (SPG > 1 && t >= NS) break;
-            // stage t landed (what was issued after it may stay in flight), then the
-            // barrier: every wave's part of it has, and every wave has read stage t - 1,
-            // whose buffer the next issue writes
-            const int ahead = min(S - 2, NS - 1 - t);
-            if (S > 3 && ahead >= 2) wait_vm<vmcnt_imm(CF::dmas(0) + CF::dmas(1))>();
-            else if (S > 2 && ahead >= 1 && hs == 0) wait_vm<vmcnt_imm(CF::dmas(1))>();
-            else if (S > 2 && ahead >= 1) wait_vm<vmcnt_imm(CF::dmas(0))>();
-            else wait_vm<vmcnt_imm(0)>();
-            dma::stage_barrier<0xc07f>();
-            if (t + S - 1 < NS) issue(t + S - 1, stage_next, (hs + S - 1) % SPG == 0);
-            const unsigned st = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(stage * CF::STAGE));
-            stage_next = stage;
-            stage = stage + 1 == S ? 0 : stage + 1;
-            float ratio[FW];
-            u32x4 wraw[FW][NWC];
+            for (int hs = 0; hs < SPG; ++hs) {
+                const int t = t0 + hs;
+                if (SPG > 1 && t >= NS) break;
+                // stage t landed (what was issued after it may stay in flight), then the
+                // barrier: every wave's part of it has, and every wave has read stage t - 1,
+                // whose buffer the next issue writes
+                const int ahead = min(S - 2, NS - 1 - t);
+                if (S > 3 && ahead >= 2) wait_vm<vmcnt_imm(CF::dmas(0) + CF::dmas(1))>();
+                else if (S > 2 && ahead >= 1 && hs == 0) wait_vm<vmcnt_imm(CF::dmas(1))>();
+                else if (S > 2 && ahead >= 1) wait_vm<vmcnt_imm(CF::dmas(0))>();
+                else wait_vm<vmcnt_imm(0)>();
+                dma::stage_barrier<0xc07f>();
+                if (t + S - 1 < NS) issue(t + S - 1, stage_next, (hs + S - 1) % SPG == 0);
+                const unsigned st = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(stage * CF::STAGE));
+                stage_next = stage;
+                stage = stage + 1 == S ? 0 : stage + 1;
+                float ratio[FW];
+                u32x4 wraw[FW][NWC];
 #pragma unroll
-            for (int c = 0; c < NWC; ++c)
+                for (int c = 0; c < NWC; ++c)
 #pragma unroll
-                for (int i = 0; i < FW; ++i) wraw[i][c] = lds_read16(st + woff[c] + 32 * CF::WRB * i);
-            if (hs == 0) {
-                const int odd = (t / SPG) & 1;
+                    for (int i = 0; i < FW; ++i) wraw[i][c] = lds_read16(st + woff[c] + 32 * CF::WRB * i);
+                if (hs == 0) {
+                    const int odd = (t / SPG) & 1;
 #pragma unroll
-                for (int i = 0; i < FW; ++i) {
-                    const unsigned sd = lds_read4(st + CF::OFF_SC + (wrow0 + 32 * i) * 4);
-                    const unsigned zd = lds_read4(st + CF::OFF_ZR + (wrow0 + 32 * i) * 4);
-                    const float sc = h2f((uint16_t)((soff[i] >> 1) ^ odd ? sd >> 16 : sd));
-                    const float z = rintf(h2f((uint16_t)((soff[i] & 1) ^ odd ? zd >> 16 : zd)));
-                    const bool none = sc == 0.0f;
-                    ratio[i] = none ? 1.0f : unit[i] / sc;
-                    unit[i] = none ? unit[i] : sc;
-                    const _Float16 nz = (_Float16)(none ? 0.0f : z * (-1.0f / 512.0f));
-                    zz[i] = f16x2{nz, nz};
-                    mul[i] = none ? f16x2{(_Float16)0.0f, (_Float16)0.0f} : f16x2{(_Float16)2048.0f, (_Float16)32768.0f};
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                f16x8 xf[FX], wf[FW];
-#pragma unroll
-                for (int j = 0; j < FX; ++j) xf[j] = bitcast<f16x8>(lds_read16(st + xoff[s] + 32 * CF::XRB * j));
-#pragma unroll
-                for (int i = 0; i < FW; ++i) {
-                    const u32x4& q = wraw[i][s >> 2];
-                    wf[i] = unpack8((s & 3) == 0 ? q.x : (s & 3) == 1 ? q.y : (s & 3) == 2 ? q.z : q.w, mul[i], zz[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < FW; ++i)
-#pragma unroll
-                    for (int j = 0; j < FX; ++j) {
-                        if (hs == 0 && s == 0) acc[i][j] *= ratio[i];
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[j], wf[i], acc[i][j], 0, 0, 0);
+                    for (int i = 0; i < FW; ++i) {
+                        const unsigned sd = lds_read4(st + CF::OFF_SC + (wrow0 + 32 * i) * 4);
+                        const unsigned zd = lds_read4(st + CF::OFF_ZR + (wrow0 + 32 * i) * 4);
+                        const float sc = h2f((uint16_t)((soff[i] >> 1) ^ odd ? sd >> 16 : sd));
+                        const float z = rintf(h2f((uint16_t)((soff[i] & 1) ^ odd ? zd >> 16 : zd)));
+                        const bool none = sc == 0.0f;
+                        ratio[i] = none ? 1.0f : unit[i] / sc;
+                        unit[i] = none ? unit[i] : sc;
+                        const _Float16 nz = (_Float16)(none ? 0.0f : z * (-1.0f / 512.0f));
+                        zz[i] = f16x2{nz, nz};
+                        mul[i] = none ? f16x2{(_Float16)0.0f, (_Float16)0.0f} : f16x2{(_Float16)2048.0f, (_Float16)32768.0f};
                     }
+                }
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    f16x8 xf[FXU], wf[FW];
+#pragma unroll
+                    for (int j = 0; j < FXU; ++j) xf[j] = bitcast<f16x8>(lds_read16(st + xoff[s] + 32 * CF::XRB * j));
+#pragma unroll
+                    for (int i = 0; i < FW; ++i) {
+                        const u32x4& q = wraw[i][s >> 2];
+                        wf[i] = unpack8((s & 3) == 0 ? q.x : (s & 3) == 1 ? q.y : (s & 3) == 2 ? q.z : q.w, mul[i], zz[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < FW; ++i)
+#pragma unroll
+                        for (int j = 0; j < FXU; ++j) {
+                            if (hs == 0 && s == 0) acc[i][j] *= ratio[i];
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xf[j], wf[i], acc[i][j], 0, 0, 0);
+                        }
+                }
             }
         }
-    }
+    };
+    // An expert's last tile may be half empty (4096 pairs on 8 experts: 762 us without the
+    // second loop, 748 with it; 65536 on 128 426 and 418)
+    if (FX > 1 && count <= 16 * FX) k_loop(std::integral_constant<int, (FX + 1) / 2>());
+    else k_loop(std::integral_constant<int, FX>());
 #pragma unroll
     for (int i = 0; i < FW; ++i) unit[i] *= 512.0f;  // (q - z) 2^-9 back to q - z
 #pragma unroll
@@ -938,9 +948,10 @@ clove_status_t run_few_down(Params p, int KS, hipStream_t stream) {
 }
 
 // ---- tiles ----
+// (about: half of an expert's last tile is empty, and an expert hit has one)
 template <class CF>
 int64_t items(const Params& p, bool swiglu) {
-    return cdiv64(p.on, swiglu ? CF::BR / 2 : CF::BR) * (p.P / CF::BC + (p.a.experts + 1) / 2);
+    return cdiv64(p.on, swiglu ? CF::BR / 2 : CF::BR) * max(p.P / CF::BC + (p.a.experts + 1) / 2, min(p.P, p.a.experts));
 }
 
 template <class CF, bool SWIGLU>
@@ -954,27 +965,43 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
     return check_launch();
 }
 
-// Tiles by the pairs an expert has on average (us per call, weights from HBM; SwiGLU of
-// 64 experts of 2 x 1408 rows of 2048, 6 of them a token; the other sides in brackets):
-//   256 x 128 from 110 pairs: 240 pairs 253 [128 x 64: 266], 120 154 [155]; 8 experts of
-//   2 x 11008 rows of 4096, 512 pairs: 741 [128 x 64: 915, 256 x 64 861, 256 x 32 1222]
-//   128 x 64 from 40: 60 pairs 96 [256 x 128: 119, 128 x 32 109]
-//   128 x 32 below: 30 pairs 76 [128 x 64: 77], 15 59 [73], 4 54 [67; 256 x 32 57]; three
-//   workgroups a CU with two stages ahead (15 pairs of 2048 rows of 1408 down 38.6 us, two
-//   with three stages 42.5)
-// and 64 x 32 where those leave half of the CUs idle (4 experts of 2 x 1024 rows of 4096,
-// 25 pairs: 23.6 [128 x 32: 24.3, 256 x 32 36]).  Half-group stages pay where stages of
-// whole groups leave a CU one workgroup (256 x 128); elsewhere their 32-byte pieces of
-// weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
+// The shape whose workgroups come first to an end: whole rounds of as many as the CUs hold,
+// and the rest, which takes less time the fewer of them share a CU.  `time`: of a workgroup
+// beside 0, 1, 2 others, 1 for a 128 x 64 tile alone on its CU.  Measured over 144 shapes of 3
+// to 1100 pairs an expert, 8 to 128 experts, 256 to 16384 rows of 256 to 8192, of the three
+// shapes' times; the choice is 0.6 % off the best of them on average, one by the pairs an
+// expert has on average 2.3 %.  Some (us, weights from HBM):
+//                                             256 x 128  128 x 64  128 x 32
+//   up 4096 on 8 experts of 22016 rows of 4096     747       898
+//   up 20000 on 128 of 768 of 4896                 296       229
+//   up 7388 on 16 of 1536 of 8192                  257       288       411
+//   up 4736 on 128 of 11008 of 512                 219       171       176
+//   up 1090 on 64 of 1024 of 1024, 5 an expert                37        34
+//   down 3000 on 64 of 2048 of 1408                           52        57
+//   up 600 on 64 of 2816 of 2048                              71        57
+// (the last with two stages ahead and three workgroups a CU; two with three stages 42.5
+// against 38.6 for 15 pairs of 2048 rows of 1408 down.)  And 64 x 32 where 128 x 32 leaves half
+// of the CUs idle (4 experts of 2 x 1024 rows of 4096, 25 pairs: 23.6, 24.3).  Half-group stages
+// pay where stages of whole groups leave a CU one workgroup (256 x 128); elsewhere their
+// 32-byte pieces of weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
+using Many = Cfg<4, 1, 2, 4, 2, 4>;   // 256 x 128
+using Some = Cfg<4, 1, 1, 2, 2, 8>;   // 128 x 64
+using Thin = Cfg<4, 1, 1, 1, 3, 8>;   // 128 x 32
+using Small = Cfg<2, 1, 1, 1, 4, 8>;  // 64 x 32
+
+template <int SLOTS>
+float rounds(int64_t items, int cus, const float (&time)[SLOTS]) {
+    const int64_t full = items / (SLOTS * cus), rest = items - full * SLOTS * cus;
+    return full * time[SLOTS - 1] + (rest ? time[cdiv64(rest, cus) - 1] : 0.0f);
+}
+
 template <bool SWIGLU>
 clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
-    using Many = Cfg<4, 1, 2, 4, 2, 4>;   // 256 x 128
-    using Some = Cfg<4, 1, 1, 2, 2, 8>;   // 128 x 64
-    using Thin = Cfg<4, 1, 1, 1, 3, 8>;   // 128 x 32
-    using Small = Cfg<2, 1, 1, 1, 4, 8>;  // 64 x 32
-    const int avg = p.P / p.a.experts;
-    if (avg >= 110 && items<Many>(p, SWIGLU) >= cus) return run_tile<Many, SWIGLU>(p, stream);
-    if (avg >= 40 && 2 * items<Some>(p, SWIGLU) >= cus) return run_tile<Some, SWIGLU>(p, stream);
+    const float many = rounds(items<Many>(p, SWIGLU), cus, {2.2f, 3.3f});
+    const float some = rounds(items<Some>(p, SWIGLU), cus, {1.0f, 1.25f, 1.6f});
+    const float thin = rounds(items<Thin>(p, SWIGLU), cus, {0.7f, 1.15f, 1.25f});
+    if (many <= some && many <= thin) return run_tile<Many, SWIGLU>(p, stream);
+    if (some <= thin) return run_tile<Some, SWIGLU>(p, stream);
     if (2 * items<Thin>(p, SWIGLU) >= cus) return run_tile<Thin, SWIGLU>(p, stream);
     return run_tile<Small, SWIGLU>(p, stream);
 }
@@ -997,8 +1024,12 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
     const bool aligned = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W);
     // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
-    // 2048, 6 a token: 20 tokens 40 us against 51 with tiles of 256 x 32, 40 56 and 58, 80 83 and 62)
-    const bool few = aligned && p.P < 3 * a.experts;
+    // 2048, 6 a token: 20 tokens 45 us against 47 with tiles, 40 60 and 55, 80 89 and 59); below
+    // seven where there are fewer tiles than half of the CUs, as waves share K then (8 experts: 28
+    // pairs down to 1408 from 4096 14 us and 25, 48 up to 2 x 256 from 2048 6 and 14, 52 up to 2 x
+    // 1408 13 and 18; 16 experts, 126 pairs down to 768 from 768 13.4 and 11)
+    p.on = a.O;
+    const bool few = aligned && (p.P < 3 * a.experts || (p.P < 7 * a.experts && 2 * items<Thin>(p, SWIGLU) < cus));
     if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
         // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that
         // leaves one a CU), which reads the weights of an expert hit twice twice but takes one launch
