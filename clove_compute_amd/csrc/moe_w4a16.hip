@@ -1031,14 +1031,21 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     p.on = a.O;
     const bool few = aligned && (p.P < 3 * a.experts || (p.P < 7 * a.experts && 2 * items<Thin>(p, SWIGLU) < cus));
     if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
-        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that
-        // leaves one a CU), which reads the weights of an expert hit twice twice but takes one launch
-        // and no memory between (64 experts, 2048 rows of 1408, 6 a token: 1 token 7.0 us against 9.2
-        // by expert and 16 with tiles, 6 16.9, 18.6 and 22, 10 23.4, 22.2 and 25).
-        const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
-        if (grid <= cus) return run_few_down<1>(p, 16, stream);
-        if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
-        return run_few_down<1>(p, 4, stream);
+        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 in large grids,
+        // or where that leaves one a CU) takes one launch and no memory between.  It reads the weights
+        // of an expert hit twice twice, and all of a token's places through one CU: by expert where that
+        // takes more than the second launch's 4 us, at the 19 GB/s of a CU and 4.2 TB/s of all that both
+        // kernels reach (us, down and by expert: 1 token on 8 of 16 experts, 704 rows of 8192 31.6 and 15.2,
+        // of 64, 2048 of 2048 9.7 and 10.3, 6 of 16, 1472 of 2048 8.6 and 10.0; 12 on 6 of 128, 5120 of 3072
+        // 127 and 97; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
+        const float mb = (float)a.O * a.K * 0.53e-6f, places = min(a.top_k, a.experts), units = cdiv(p.G, NG);
+        const float hit = a.experts * (1.0f - powf(1.0f - places / a.experts, a.T));
+        if (max(units * a.top_k * 0.215f, p.P * mb / 4.2f) <= max(units * 0.43f, hit * mb / 4.2f) + 4.0f) {
+            const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
+            if (grid <= cus) return run_few_down<1>(p, 16, stream);
+            if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
+            return grid <= 3 * cus ? run_few_down<1>(p, 4, stream) : run_few_down<2>(p, 4, stream);
+        }
     }
     const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
     // As many outputs at a time as workgroups of 256 threads for 16 of them and 32 pairs make a
