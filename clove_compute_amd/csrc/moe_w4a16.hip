@@ -489,10 +489,10 @@ __global__ void __launch_bounds__(1024) moe_few_down(const Params p) {
 // group whose scale is 0 leaves the unit as it is and its weights are made 0.
 //
 // 4096 pairs on 8 experts of 2 x 11008 rows of 4096 take 747 us, 0.99 PFLOP/s (a library
-// product of fp16 weights reaches 1.20): the matrix pipe is busy 56 % of the cycles, the
-// VALU, mostly with unpacking, 55 %.  65536 pairs on 128 experts of 2048 rows of 768: 291
+// product of fp16 weights reaches 1.20): the matrix pipe is busy 55 % of the cycles, and
+// the VALU, mostly with unpacking.  65536 pairs on 128 experts of 2048 rows of 768: 282
 // us, as much of it the 537 MB of fp32 products as the six groups of K.  540 pairs on 64
-// experts of 2 x 1408 rows of 2048 (197 MB): 57 us, 3.4 TB/s, the VALU busy for 54 %.
+// experts of 2 x 1408 rows of 2048 (197 MB): 57 us, 3.4 TB/s, the VALU busy for 55 %.
 // ---------------------------------------------------------------------------
 template <int WR_, int WC_, int FW_, int FX_, int S_, int KS_>
 struct Cfg {
