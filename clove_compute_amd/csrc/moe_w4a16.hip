@@ -18,6 +18,8 @@
 //  * moe_any, the same for any K and alignment.
 // Down without moe_few_down: the places of a token are added up from fp32 partial
 // results in place order (moe_combine), so that a call gives the same bits every time.
+// Where tiles leave CUs idle they split K, and the parts are added up in order, by
+// moe_combine or, before SwiGLU, moe_swiglu.
 #include <type_traits>
 
 #include "i4w_bits.hpp"
@@ -32,9 +34,11 @@ struct Params {
     MoeArgs a;
     int* off;      // [experts + 1] or null: where an expert's pairs begin in `order`
     int* order;    // [T top_k]: pairs, those of one expert after those of the one before
-    float* part;   // down: [T top_k, ldp] products with the outputs o0 .. o0 + on - 1
+    float* part;   // down: [splits][T top_k, ldp] products with the outputs o0 .. o0 + on - 1
     int o0, on, ldp;
     FastDiv k;     // by top_k
+    FastDiv x;     // a pair's row of X: by top_k, or 1
+    int splits, split_groups;  // moe_tile: parts of K, groups of a part
     int rows_t;    // tiles of weight rows
     int P, G;
     int64_t x_bytes;  // of X
@@ -594,7 +598,8 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
         done = __builtin_amdgcn_readlane(upto, 63);
     }
     const int nt = cdiv(count, BC);  // tiles of pairs of the expert
-    const int in = (int)(item - (int64_t)before * p.rows_t), tr = in / nt, skip = (in - tr * nt) * BC;
+    const int in = (int)(item - (int64_t)before * p.rows_t), tk = in / nt, skip = (in - tk * nt) * BC;
+    const int tr = SWIGLU ? tk : tk / p.splits, split = SWIGLU ? 0 : tk - tr * p.splits;
     first += skip;
     count = min(BC, count - skip);
     // the tile's pairs to LDS
@@ -656,7 +661,7 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
 #pragma unroll
     for (int i = 0; i < CF::DX; ++i) {
         const int q = pairs[min(xrow(i), count - 1)];
-        offx[i] = (SWIGLU ? p.k.div(q) : q) * K * 2 + 16 * xchunk(i);
+        offx[i] = p.x.div(q) * K * 2 + 16 * xchunk(i);
     }
 #pragma unroll
     for (int i = 0; i < CF::DW; ++i) {
@@ -668,7 +673,8 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
         const int j = wave * CF::DS + i;
         offs[i] = row(64 * (j % (BR / 64)) + lane) * G * 2 + (j >= BR / 64 ? zo : so);
     }
-    const int NS = cdiv(K, 16 * KS);  // stages
+    // stages of the tile
+    const int first_stage = split * p.split_groups * SPG, NS = min(cdiv(K, 16 * KS), first_stage + p.split_groups * SPG);
     // stage t to buffer b; HS: its place in the group
     auto issue = [&](int t, int b, bool starts) {
         const unsigned st = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)(b * CF::STAGE));
@@ -717,12 +723,12 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
     for (int i = 0; i < FW; ++i) unit[i] = 1.0f;
 #pragma unroll
     for (int t = 0; t < S - 1; ++t)
-        if (t < NS) issue(t, t, t % SPG == 0);
+        if (first_stage + t < NS) issue(first_stage + t, t, t % SPG == 0);
     int stage = 0, stage_next = S - 1;
     // (FXU blocks of 32 pairs; the others of a ragged tile multiply nothing)
     auto k_loop = [&](auto blocks) {
         constexpr int FXU = decltype(blocks)::value;
-        for (int t0 = 0; t0 < NS; t0 += SPG) {
+        for (int t0 = first_stage; t0 < NS; t0 += SPG) {
 #pragma unroll
             for (int hs = 0; hs < SPG; ++hs) {
                 const int t = t0 + hs;
@@ -853,7 +859,7 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
                 const int c = k + lane / LPP, at = c0 + 32 * j + c;
                 if (at >= count || o >= end) continue;
                 // (rows of the products have room for whole fours)
-                *reinterpret_cast<f32x4*>(p.part + (int64_t)pairs[at] * p.ldp + o - p.o0) =
+                *reinterpret_cast<f32x4*>(p.part + ((int64_t)split * p.P + pairs[at]) * p.ldp + o - p.o0) =
                     *reinterpret_cast<const f32x4*>(turned + c * LD + 4 * (lane % LPP));
             }
             asm volatile("" ::: "memory");
@@ -876,15 +882,26 @@ __global__ void __launch_bounds__(128) moe_combine(const Params p) {
     for (int j0 = 0; j0 < a.top_k; j0 += 8) {
         f32x4 v[8];
         float w[8];
+        bool there[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const bool there = j0 + j < a.top_k && (unsigned)ids[min(j0 + j, a.top_k - 1)] < (unsigned)a.experts;
+            there[j] = j0 + j < a.top_k && (unsigned)ids[min(j0 + j, a.top_k - 1)] < (unsigned)a.experts;
             w[j] = 0.0f;
             v[j] = f32x4{};
-            if (there) {
+            if (there[j]) {
                 w[j] = a.weights ? a.weights[(int64_t)t * a.top_k + j0 + j] : 1.0f;
                 v[j] = *reinterpret_cast<const f32x4*>(part + (int64_t)(j0 + j) * p.ldp);
             }
+        }
+#pragma unroll 2
+        for (int s = 1; s < p.splits; ++s) {
+            const float* more = part + ((int64_t)s * p.P + j0) * p.ldp;
+            f32x4 m[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[j] = *reinterpret_cast<const f32x4*>(more + (int64_t)min(j, a.top_k - 1 - j0) * p.ldp);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (there[j]) v[j] += m[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -904,6 +921,26 @@ __global__ void __launch_bounds__(128) moe_combine(const Params p) {
         for (int i = 0; i < 4; ++i)
             if (i < n) y[i] = f2h(sum[i]);
     }
+}
+
+// H[q, i] from the parts of K of the pairs' gate and up products, part[s][q][i] and
+// [I + i], in order: some 4 us, a launch and a memory latency for two parts
+__global__ void __launch_bounds__(128) moe_swiglu(const Params p) {
+    const MoeArgs& a = p.a;
+    const int q = blockIdx.x, i = 512 * blockIdx.y + 4 * threadIdx.x, I = a.O / 2, n = min(4, I - i);
+    if (n <= 0 || (unsigned)a.ids[q] >= (unsigned)a.experts) return;
+    const float* part = p.part + (int64_t)q * p.ldp + i;
+    f32x4 g = {}, u = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s, part += (int64_t)p.P * p.ldp) {
+        g += *reinterpret_cast<const f32x4*>(part);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] += part[I + min(j, n - 1)];
+    }
+    uint16_t* h = a.Y + (int64_t)q * I + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < n) h[j] = f2h(g[j] / (1.0f + expf(-g[j])) * u[j]);
 }
 
 namespace {
@@ -956,7 +993,7 @@ int64_t items(const Params& p, bool swiglu) {
 
 template <class CF, bool SWIGLU>
 clove_status_t run_tile(Params p, hipStream_t stream) {
-    p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR);
+    p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR) * p.splits;
     const int64_t tiles = ((int64_t)p.P / CF::BC + p.a.experts) * p.rows_t;
     if (too_many(tiles + 7, CF::NT)) return CLOVE_ERR_INVALID_DIM;
     auto k = moe_tile<CF, SWIGLU>;
@@ -965,12 +1002,14 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
     return check_launch();
 }
 
-// The shape whose workgroups come first to an end: whole rounds of as many as the CUs hold,
-// and the rest, which takes less time the fewer of them share a CU.  `time`: of a workgroup
-// beside 0, 1, 2 others, 1 for a 128 x 64 tile alone on its CU.  Measured over 144 shapes of 3
-// to 1100 pairs an expert, 8 to 128 experts, 256 to 16384 rows of 256 to 8192, of the three
-// shapes' times; the choice is 0.6 % off the best of them on average, one by the pairs an
-// expert has on average 2.3 %.  Some (us, weights from HBM):
+// What runs first to its end by an estimate.  Workgroups: whole rounds of as many as the CUs
+// hold, and the rest, which takes less time the fewer of them share a CU (`time`: of one beside
+// 0, 1, 2 others, 1 for a 128 x 64 tile alone on its CU, which takes 0.8 us for a group and ten
+// groups' worth to begin and end).  Where they leave CUs idle K is split: more workgroups, and
+// fp32 sums of the parts to write and add up (for SwiGLU by a launch more).  Over 276 shapes
+// of 3 to 1100 pairs an expert, 4 to 128 experts, 256 to 16384 rows of 256 to 14336 the choice
+// is 1 % off the best of the shapes and splits on average; by the pairs an expert has on
+// average, without splits, 7 %.  Some (us, weights from HBM):
 //                                             256 x 128  128 x 64  128 x 32
 //   up 4096 on 8 experts of 22016 rows of 4096     747       898
 //   up 20000 on 128 of 768 of 4896                 296       229
@@ -979,7 +1018,13 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
 //   up 1090 on 64 of 1024 of 1024, 5 an expert                37        34
 //   down 3000 on 64 of 2048 of 1408                           52        57
 //   up 600 on 64 of 2816 of 2048                              71        57
-// (the last with two stages ahead and three workgroups a CU; two with three stages 42.5
+//                                              parts of K:  1    2    4    8
+//   down 107 on 8 of 256 of 8192, 128 x 32                  42   26   19   16
+//   down 42 on 8 of 2048 of 8192                            43   28   28   31
+//   down 184 on 8 of 1408 of 14336                          75   44   45   41
+//   up 216 on 8 of 1536 of 14336                            73   54   50   49
+//   down 722 on 16 of 2816 of 3072                          42   44   54   80
+// (128 x 32 with two stages ahead and three workgroups a CU; two with three stages 42.5
 // against 38.6 for 15 pairs of 2048 rows of 1408 down.)  And 64 x 32 where 128 x 32 leaves half
 // of the CUs idle (4 experts of 2 x 1024 rows of 4096, 25 pairs: 23.6, 24.3).  Half-group stages
 // pay where stages of whole groups leave a CU one workgroup (256 x 128); elsewhere their
@@ -995,14 +1040,35 @@ float rounds(int64_t items, int cus, const float (&time)[SLOTS]) {
     return full * time[SLOTS - 1] + (rest ? time[cdiv64(rest, cus) - 1] : 0.0f);
 }
 
+enum class Shape { kMany, kSome, kThin, kSmall };
+struct Plan {
+    Shape shape = Shape::kThin;
+    int splits = 1;
+    float us = 0.0f;
+};
+
+Plan plan(const Params& p, bool swiglu, int cus) {
+    Plan best;
+    auto take = [&](Shape shape, int splits, float time) {
+        const float sums = splits > 1 ? (float)splits * (0.5f + (float)p.P * p.on * (swiglu ? 16 : 8) / 4.5e6f) + (swiglu ? 4.0f : 0.0f) : 0.0f;
+        const float us = 0.8f * time * (cdiv(p.G, splits) + 10) + sums;
+        if (best.us == 0.0f || us < best.us) best = {shape, splits, us};
+    };
+    take(Shape::kMany, 1, rounds(items<Many>(p, swiglu), cus, {2.0f, 3.2f}));
+    for (int splits : {1, 2, 3, 4, 6, 8}) {
+        if (splits > 1 && ((int64_t)splits * p.P * p.on * (swiglu ? 8 : 4) > (64 << 20) || p.G < 4 * splits)) break;
+        take(Shape::kSome, splits, rounds(splits * items<Some>(p, swiglu), cus, {1.0f, 1.15f, 1.5f}));
+        take(Shape::kThin, splits, rounds(splits * items<Thin>(p, swiglu), cus, {0.8f, 1.05f, 1.3f}));
+    }
+    if (best.shape == Shape::kThin && best.splits == 1 && 2 * items<Thin>(p, swiglu) < cus) best.shape = Shape::kSmall;
+    return best;
+}
+
 template <bool SWIGLU>
-clove_status_t tile_by_shape(const Params& p, int cus, hipStream_t stream) {
-    const float many = rounds(items<Many>(p, SWIGLU), cus, {2.2f, 3.3f});
-    const float some = rounds(items<Some>(p, SWIGLU), cus, {1.0f, 1.25f, 1.6f});
-    const float thin = rounds(items<Thin>(p, SWIGLU), cus, {0.7f, 1.15f, 1.25f});
-    if (many <= some && many <= thin) return run_tile<Many, SWIGLU>(p, stream);
-    if (some <= thin) return run_tile<Some, SWIGLU>(p, stream);
-    if (2 * items<Thin>(p, SWIGLU) >= cus) return run_tile<Thin, SWIGLU>(p, stream);
+clove_status_t run_shape(Shape s, const Params& p, hipStream_t stream) {
+    if (s == Shape::kMany) return run_tile<Many, SWIGLU>(p, stream);
+    if (s == Shape::kSome) return run_tile<Some, SWIGLU>(p, stream);
+    if (s == Shape::kThin) return run_tile<Thin, SWIGLU>(p, stream);
     return run_tile<Small, SWIGLU>(p, stream);
 }
 
@@ -1011,6 +1077,7 @@ struct Held {
     void* p = nullptr;
     size_t bytes = 0;
     int pairs = 0;
+    Plan plan;
 };
 
 template <bool SWIGLU>
@@ -1020,46 +1087,58 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     p.P = a.T * a.top_k;
     p.G = cdiv(a.K, 128);
     p.k = FastDiv(a.top_k);
+    p.x = FastDiv(SWIGLU ? a.top_k : 1);
+    p.splits = 1;
+    p.split_groups = p.G;
     p.x_bytes = (int64_t)(SWIGLU ? a.T : p.P) * a.K * 2;
     const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
     const bool aligned = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W);
     // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
     // 2048, 6 a token: 20 tokens 45 us against 47 with tiles, 40 60 and 55, 80 89 and 59); below
-    // seven where there are fewer tiles than half of the CUs, as waves share K then (8 experts: 28
-    // pairs down to 1408 from 4096 14 us and 25, 48 up to 2 x 256 from 2048 6 and 14, 52 up to 2 x
-    // 1408 13 and 18; 16 experts, 126 pairs down to 768 from 768 13.4 and 11)
+    // eight where there are fewer tiles than half of the CUs and K is too short to be split (8
+    // experts: 28 pairs down to 768 from 768 7.9 us and 11.0, 54 from 3072 to 1024 18.3 and 14.2)
     p.on = a.O;
-    const bool few = aligned && (p.P < 3 * a.experts || (p.P < 7 * a.experts && 2 * items<Thin>(p, SWIGLU) < cus));
+    const bool few = aligned && (p.P < 3 * a.experts || (p.P < 8 * a.experts && p.G <= 16 && 2 * items<Thin>(p, SWIGLU) < cus));
     if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
-        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 in large grids,
-        // or where that leaves one a CU) takes one launch and no memory between.  It reads the weights
-        // of an expert hit twice twice, and all of a token's places through one CU: by expert where that
-        // takes more than the second launch's 4 us, at the 19 GB/s of a CU and 4.2 TB/s of all that both
-        // kernels reach (us, down and by expert: 1 token on 8 of 16 experts, 704 rows of 8192 31.6 and 15.2,
-        // of 64, 2048 of 2048 9.7 and 10.3, 6 of 16, 1472 of 2048 8.6 and 10.0; 12 on 6 of 128, 5120 of 3072
-        // 127 and 97; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
+        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that leaves
+        // one a CU, or the waves with little: 41 tokens on 1 of 128, 2752 rows of 256 7.3 and 9.4 us)
+        // takes one launch and no memory between.  It reads the weights of an expert hit twice twice, and
+        // all of a token's places through one CU: by expert where that takes more than the second launch's
+        // 4 us, at the 19 GB/s of a CU and 4.2 TB/s of all that both kernels reach (us, by token and by
+        // expert: 1 token on 8 of 16 experts, 704 rows of 8192 31.6 and 15.2, 6 of 16, 1472 of 2048 8.6
+        // and 10.0; 12 on 6 of 128, 5120 of 3072 127 and 97; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
         const float mb = (float)a.O * a.K * 0.53e-6f, places = min(a.top_k, a.experts), units = cdiv(p.G, NG);
         const float hit = a.experts * (1.0f - powf(1.0f - places / a.experts, a.T));
         if (max(units * a.top_k * 0.215f, p.P * mb / 4.2f) <= max(units * 0.43f, hit * mb / 4.2f) + 4.0f) {
             const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
             if (grid <= cus) return run_few_down<1>(p, 16, stream);
             if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
-            return grid <= 3 * cus ? run_few_down<1>(p, 4, stream) : run_few_down<2>(p, 4, stream);
+            return units * a.top_k <= 2 ? run_few_down<2>(p, 4, stream) : run_few_down<1>(p, 4, stream);
         }
     }
     const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
     // As many outputs at a time as workgroups of 256 threads for 16 of them and 32 pairs make a
     // launch; scratch: the lists of the pairs by expert, and for down the products with as many
-    // outputs at a time as 512 MB hold
+    // outputs at a time as 512 MB hold, the products of parts of K up to 64 MB.  The first part of
+    // the tokens settles it for all
     const bool lists = !few && (!tiles || p.P > SCAN * 128);
     const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
-    if (held.pairs == 0) held.pairs = p.P;
+    const bool begins = held.pairs == 0;
+    if (begins) held.pairs = p.P;
     int64_t most = (int64_t)16 * ((1 << 24) - 8) / (held.pairs / 32 + a.experts) / 256 * 256;
     // (moe_combine: 65535 workgroups of 512 outputs)
     if (!SWIGLU) most = min(min(most, (int64_t)512 * 65535), max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)held.pairs * 4) / 256 * 256));
     const int chunk = most < a.O ? cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256 : a.O;
-    if (!SWIGLU) p.ldp = (min(chunk, a.O) + 3) & ~3;
-    const size_t bytes = off + order + (SWIGLU ? 0 : (size_t)p.P * p.ldp * 4);
+    if (begins && tiles && !few) {
+        p.on = chunk;
+        held.plan = plan(p, SWIGLU, cus);
+    }
+    if (tiles && !few) {
+        p.split_groups = cdiv(p.G, held.plan.splits);
+        p.splits = cdiv(p.G, p.split_groups);
+    }
+    if (!SWIGLU || p.splits > 1) p.ldp = ((SWIGLU ? 2 * a.O : min(chunk, a.O)) + 3) & ~3;
+    const size_t bytes = off + order + (size_t)p.splits * p.P * p.ldp * 4;
     if (bytes > held.bytes) {
         if (const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &held.p); st != CLOVE_OK) return st;
         held.bytes = bytes;
@@ -1071,7 +1150,15 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
         const int threads = min(kSortThreads, cdiv(p.P, 256) * 64);
         CLOVE_LAUNCH(moe_sort, dim3((unsigned)a.experts), dim3((unsigned)threads), 0, stream, a.ids, p.P, a.experts, p.off, p.order);
     }
-    for (p.o0 = 0; p.o0 < a.O; p.o0 += chunk) {
+    if (SWIGLU && p.splits > 1) {
+        // (the products of gate and up rows as of any others, and SwiGLU of their sums)
+        p.a.O = p.on = 2 * a.O;
+        if (const clove_status_t st = run_shape<false>(held.plan.shape, p, stream); st != CLOVE_OK) return st;
+        CLOVE_LAUNCH(moe_swiglu, dim3((unsigned)p.P, (unsigned)cdiv(a.O, 512)), dim3(128), 0, stream, p);
+        return check_launch();
+    }
+    for (int64_t o = 0; o < a.O; o += chunk) {
+        p.o0 = (int)o;
         p.on = min(chunk, a.O - p.o0);
         clove_status_t st = CLOVE_OK;
         if (few) {
@@ -1079,7 +1166,7 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
             // experts of 2 x 14336 rows of 4096 28.3 us against 32.2, 32 on 8 of 128 71 against 47)
             st = 2 * p.P <= a.experts ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
         } else if (tiles) {
-            st = tile_by_shape<SWIGLU>(p, cus, stream);
+            st = run_shape<SWIGLU>(held.plan.shape, p, stream);
         } else {
             p.rows_t = cdiv(p.on, SWIGLU ? AR / 2 : AR);
             const int64_t grid = ((int64_t)p.P / AC + a.experts) * p.rows_t;

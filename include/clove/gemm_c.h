@@ -479,7 +479,7 @@ clove_status_t clove_moe_route(const void* logits, int64_t logits_stride, int dt
  * Zero points round to the nearest integer, as clove_gemm_w4a16's; q - z is
  * exact up to 2048 in magnitude and rounded to fp16 past that.
  * Scratch: 4 bytes a pair, at most 2 MB (more pairs than 2^19, or an X of 2^31
- * bytes, go in parts).  2^31 tiles of 32 rows by 32 pairs and more, or one
+ * bytes, go in parts), and up to 64 MB of fp32 products where K is split.  2^31 tiles of 32 rows by 32 pairs and more, or one
  * token's X of 2^31 bytes (here a row, below top_k rows), are
  * CLOVE_ERR_INVALID_DIM.
  */

@@ -346,6 +346,17 @@ def test_down_values(T, k, E, O, K, beta, alpha, weighted):
         assert np.mean(_f64(got) == want.astype(np.float16).astype(np.float64)) > 0.97
 
 
+# few tiles and a long K: the products go in parts of K (of 2 to 8, the last one shorter)
+@pytest.mark.parametrize("T,k,E,O,K", [(14, 7, 8, 128, 8192), (20, 2, 4, 200, 4096), (21, 2, 8, 1023, 8192), (13, 3, 4, 61, 4000), (300, 2, 8, 96, 2080),
+                                       (9, 3, 8, 70, 10880), (90, 12, 16, 130, 3136)])
+def test_parts_of_k(T, k, E, O, K):
+    cg = _cg()
+    for absent in (0.0, 0.2):
+        _check_up(cg, Case("up-parts", T, k, E, 2 * O, K, absent=absent))
+        _check_down(cg, Case("down-parts", T, k, E, O, K, absent=absent))
+        _check_down(cg, Case("down-parts-0", T, k, E, O, K, absent=absent), beta=0.0, alpha=-1.5, weighted=False)
+
+
 @pytest.mark.parametrize("T", [1, 3, 40, 300])
 @pytest.mark.parametrize("offset,K", [(1, 128), (4, 256), (8, 96), (16, 256), (2, 66)])
 def test_weights_at_any_alignment(T, offset, K):
@@ -640,19 +651,19 @@ def test_experts_past_four_gigabytes(T):
 
 # ---- workspaces, graphs, streams, the block as a whole ----------------------------
 
-@pytest.mark.parametrize("T", [1, 4, 40, 400])
-def test_bound_workspace_and_its_size(T):
+@pytest.mark.parametrize("T,K", [(1, 256), (4, 256), (40, 256), (400, 256), (20, 6144)])
+def test_bound_workspace_and_its_size(T, K):
     import torch
     cg = _cg()
-    c = Case("workspace", T, 4, 8, 128, 256)
-    x, _ = _rounded(c.g, "fp16", T, 256)
-    hin, _ = _rounded(c.g, "fp16", T * 4, 256)
+    c = Case("workspace", T, 4, 8, 128, K)
+    x, _ = _rounded(c.g, "fp16", T, K)
+    hin, _ = _rounded(c.g, "fp16", T * 4, K)
     w = torch.rand(T, 4, device="cuda")
     h, y = torch.zeros(T * 4, 64, dtype=torch.float16, device="cuda"), torch.zeros(T, 128, dtype=torch.float16, device="cuda")
 
     def calls():
         _up(cg, c, x, h)
-        cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, 256)
+        cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, K)
         return h.clone(), y.clone()
 
     want = calls()
@@ -672,7 +683,7 @@ def test_bound_workspace_and_its_size(T):
         cg.workspace_bind(ws[:cg.CLOVE_WORKSPACE_MIN_BYTES])
         h.fill_(3.0), y.fill_(3.0)
         with pytest.raises(cg.CloveError) as e:
-            for call in (lambda: _up(cg, c, x, h), lambda: cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, 256)):
+            for call in (lambda: _up(cg, c, x, h), lambda: cg.moe_w4a16(hin, c.dev_ids, w, c.q, c.s, c.z, y, T, 4, 8, 128, K)):
                 call()
         assert e.value.status == cg.CLOVE_ERR_WORKSPACE
     finally:
