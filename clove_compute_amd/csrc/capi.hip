@@ -993,9 +993,10 @@ static clove_status_t moe_common(MoeArgs& a, bool swiglu, void* stream) {
         return CLOVE_ERR_INVALID_DIM;
     if (a.K % 2 != 0) return CLOVE_ERR_INVALID_ARG;
     if (a.T == 0 || a.O == 0) return CLOVE_OK;
-    // (pairs, and rows in tiles of them, are counted in 31 bits; a row of weights is at most 2^30 bytes)
+    // (pairs, and rows in tiles that may end past the last one, are counted in 31 bits; a row of
+    // weights is at most 2^30 bytes)
     const int64_t pairs = (int64_t)a.T * a.top_k, rows = (int64_t)a.O * (swiglu ? 2 : 1), G = cdiv64(a.K, 128);
-    if (pairs > 0x3fffffff || rows > 0x7fffffff || (pairs / 32 + a.experts + 1) * cdiv64(rows, 32) > 0x7fffffff)
+    if (pairs > 0x3fffffff || rows > 0x7fff0000 || (pairs / 32 + a.experts + 1) * cdiv64(rows, 32) > 0x7fffffff)
         return CLOVE_ERR_INVALID_DIM;
     if (rows * (a.K / 2) > ((int64_t)1 << 50) / a.experts) return CLOVE_ERR_INVALID_DIM;
     if (!a.Y || !a.ids || (a.K > 0 && (!a.X || !a.W || !a.scale || !a.zero))) return CLOVE_ERR_NULL_POINTER;

@@ -63,7 +63,7 @@ def test_product_refusals(L, name):  # noqa: F811
                         ({src: args[src] + 1}, ARG), (dict(ids=I + 2), ARG), (dict(W_scale=S + 1), ARG), ({out: args[out] + 1}, ARG),
                         ({out: args[src] + 2}, ALIASING), ({out: W + 64}, ALIASING), ({out: S}, ALIASING), ({out: Z}, ALIASING),
                         ({out: I}, ALIASING), ({rows: 2 ** 31 - 1, "K": 2 ** 31 - 2, "experts": 1024}, DIM), (dict(T=2 ** 31 - 1), DIM),
-                        (dict(T=2 ** 25, top_k=32), DIM)]:
+                        (dict(T=2 ** 25, top_k=32), DIM), ({rows: 2 ** 31 - 64, "K": 2, "experts": 1, "T": 1, "top_k": 1}, DIM)]:
         assert call(f, args, **bad) == status, bad
     assert call(f, args, T=0, ids=None) == OK
     assert call(f, args, **{rows: 0}) == OK
