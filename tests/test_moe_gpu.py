@@ -778,6 +778,46 @@ def test_block_in_a_graph(T):
             b.check()
 
 
+def test_parts_of_k_in_a_graph():
+    """Parts of K and their sums, replayed with other ids and rows, eager calls of other sizes between."""
+    import torch
+    cg = _cg()
+    T, k, E, O, K = 20, 4, 8, 64, 6144
+    c = Case("graph-parts", T, k, E, 2 * O, K)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.empty(T * k, K, dtype=torch.float16, device="cuda")
+    ids = torch.zeros(T, k, dtype=torch.int32, device="cuda")
+    h, y = torch.zeros(T * k, O, dtype=torch.float16, device="cuda"), torch.zeros(T, 2 * O, dtype=torch.float16, device="cuda")
+
+    def calls(n=T):
+        cg.moe_w4a16_swiglu(x[:n], ids[:n], c.q, c.s, c.z, h[:n * k], n, k, E, O, K)
+        cg.moe_w4a16(x[:n * k], ids[:n], None, c.q, c.s, c.z, y[:n], n, k, E, 2 * O, K)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            calls()
+    torch.cuda.synchronize()
+    for i in range(4):
+        x.normal_(generator=g)
+        ids.copy_(torch.randint(-1, E, (T, k), generator=g, device="cuda"))
+        h.zero_(), y.zero_()
+        calls()
+        want = _bits((h, y))
+        calls(5)
+        h.zero_(), y.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _bits((h, y)) == want, i
+        exact, size = ref.down(_f64(x), ids.cpu().numpy(), None, c.w, np.zeros((T, 2 * O)), 1.0, 0.0)
+        _close(y, exact, "fp16", c.slack * size)
+
+
 def test_blocks_on_two_streams_and_threads():
     import torch
 
