@@ -1023,7 +1023,7 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
 //   down 42 on 8 of 2048 of 8192                            43   28   28   31
 //   down 184 on 8 of 1408 of 14336                          75   44   45   41
 //   up 216 on 8 of 1536 of 14336                            73   54   50   49
-//   down 722 on 16 of 2816 of 3072                          42   44   54   80
+//   up 857 on 16 of 4096 of 1408                            32   43   57   75
 // (128 x 32 with two stages ahead and three workgroups a CU; two with three stages 42.5
 // against 38.6 for 15 pairs of 2048 rows of 1408 down.)  And 64 x 32 where 128 x 32 leaves half
 // of the CUs idle (4 experts of 2 x 1024 rows of 4096, 25 pairs: 23.6, 24.3).  Half-group stages
@@ -1096,7 +1096,7 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
     // 2048, 6 a token: 20 tokens 45 us against 47 with tiles, 40 60 and 55, 80 89 and 59); below
     // eight where there are fewer tiles than half of the CUs and K is too short to be split (8
-    // experts: 28 pairs down to 768 from 768 7.9 us and 11.0, 54 from 3072 to 1024 18.3 and 14.2)
+    // experts: 28 pairs down to 768 from 768 7.9 us and 11.0, 50 from 14336 to 1408 59 and 40)
     p.on = a.O;
     const bool few = aligned && (p.P < 3 * a.experts || (p.P < 8 * a.experts && p.G <= 16 && 2 * items<Thin>(p, SWIGLU) < cus));
     if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
@@ -1106,7 +1106,7 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
         // all of a token's places through one CU: by expert where that takes more than the second launch's
         // 4 us, at the 19 GB/s of a CU and 4.2 TB/s of all that both kernels reach (us, by token and by
         // expert: 1 token on 8 of 16 experts, 704 rows of 8192 31.6 and 15.2, 6 of 16, 1472 of 2048 8.6
-        // and 10.0; 12 on 6 of 128, 5120 of 3072 127 and 97; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
+        // and 10.0; 10 on 6 of 128, 2048 of 8192 128 and 107; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
         const float mb = (float)a.O * a.K * 0.53e-6f, places = min(a.top_k, a.experts), units = cdiv(p.G, NG);
         const float hit = a.experts * (1.0f - powf(1.0f - places / a.experts, a.T));
         if (max(units * a.top_k * 0.215f, p.P * mb / 4.2f) <= max(units * 0.43f, hit * mb / 4.2f) + 4.0f) {
