@@ -294,8 +294,17 @@ clove_status_t block_norm(const Args& a) {
     Rows g;
     if (!a.none(8)) {
         const at::Tensor& gate = a.tensor(8, "gate", t);
-        if (gate.dim() == 1) g = {flat<void>(a, 8, "gate", t, D), 0};
-        else g = rows(gate, "gate", T, D);
+        // Of one dimension it is one row for all tokens, or as long as all rows those, as x; of
+        // any other length neither
+        if (gate.dim() != 1 || gate.numel() == times(T, D)) {
+            g = rows(gate, "gate", T, D);
+        } else {
+            if (T > 1 && gate.numel() > D) {
+                PyErr_Format(PyExc_ValueError, "gate must be %d elements or %d rows of them, not %lld", D, T, (long long)gate.numel());
+                throw Refused();
+            }
+            g = {flat<void>(a, 8, "gate", t, D), 0};
+        }
     }
     const void *wo = flat<void>(a, 6, "post_weight", t, D), *wi = flat<void>(a, 7, "pre_weight", t, D);
     const int dt = code(t), dtr = code(tr);

@@ -15,7 +15,7 @@ def block_norm(x, residual, h_out, T: int, D: int, y_out=None, post_weight=None,
                scale: float = 1.0, eps: float = 1e-6, stream=None) -> None:
     """y = residual + scale * gate * norm(x; post_weight), h = norm(y; pre_weight), rows [T, D] of the
     residual stream (the type of x, or fp32).  ``post_weight`` None: x is not normed; ``pre_weight``
-    None: weight 1; ``gate`` [D] or [T, D]; ``x`` None: y = residual; ``residual`` None: 0.  ``y_out`` or
+    None: weight 1; ``gate`` [D] (one row for all) or [T, D]; ``x`` None: y = residual; ``residual`` None: 0.  ``y_out`` or
     ``h_out`` may be None; they may be the residual and x themselves."""
     st = _b.block_norm(x, residual, h_out, T, D, y_out, post_weight, pre_weight, gate, scale, eps, stream)
     if st:

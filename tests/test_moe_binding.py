@@ -53,6 +53,22 @@ def test_types_and_sizes_are_checked():
                 f(**{**args, name: None})
 
 
+@pytest.mark.parametrize("T,D", [(2, 64), (3, 1), (5, 7)])
+def test_a_flat_gate_is_one_row_or_all_of_them(T, D):
+    """A gate of one dimension is a row for all tokens or, as long as all rows, a row for each, as x is;
+    of any other length it would be read as something it is not."""
+    cg, x = _cg(), _half(T, D)
+    for n in (D + 1, T * D - 1, T * D + 1, 2 * T * D):
+        if n in (D, T * D):
+            continue
+        with pytest.raises(ValueError, match=f"gate must be {D} .*not {n}"):
+            cg.block_norm(x, x, x, T, D, gate=_half(n), post_weight=_half(D - 1))
+    # taken, and refused only for the next argument
+    for n in (D, T * D):
+        with pytest.raises(ValueError, match="post_weight must be"):
+            cg.block_norm(x, x, x, T, D, gate=_half(n), post_weight=_half(D - 1))
+
+
 def test_entry_points_take_their_number_of_arguments():
     from clove_compute_amd.decode import _b
     for f in (_b.block_norm, _b.moe_route, _b.moe_up, _b.moe_down):

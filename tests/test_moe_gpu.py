@@ -142,6 +142,23 @@ def test_norm_rows_do_not_meet():
     cg.block_norm(x[:1, :199].contiguous(), None, None, 1, 199, y_out=y[:1, :199].contiguous(), scale=float("inf"))
 
 
+@pytest.mark.parametrize("T,D", [(3, 64), (5, 101)])
+def test_norm_flat_gate(T, D):
+    """A gate of one dimension as long as all rows is a row for each, not the first for all."""
+    import torch
+    cg = _cg()
+    g = rng("norm-flat-gate", T, D)
+    x, x64 = _rounded(g, "fp16", T, D)
+    ga, ga64 = _rounded(g, "fp16", T, D)
+    y, h = torch.empty_like(x), torch.empty_like(x)
+    for gate, gate64 in ((ga.flatten(), ga64), (ga[1].clone(), ga64[1])):
+        cg.block_norm(x, None, h, T, D, y_out=y, gate=gate)
+        y64, h64 = ref.block_norm(x64, None, None, gate64, 1.0, None, 1e-6)
+        by, bh = _norm_bounds(x64, None, None, gate64, 1.0, None, 1e-6, y64, h64)
+        _close(y, y64, "fp16", by)
+        _close(h, h64, "fp16", bh)
+
+
 # ---- moe_route ----------------------------------------------------------------
 
 def _route(cg, x, bias, k, E=None, **kw):
