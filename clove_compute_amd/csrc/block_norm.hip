@@ -73,13 +73,39 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
     return s;
 }
 
+// 1 / sqrt(mean(y^2) + eps) for the row whose chunks the threads hold.  Squares past fp32, and a
+// mean so small that fp32 lost part of them (below 2^-100, so with such an eps only), are taken
+// of y 2^-80 or y 2^88 instead, which y becomes: the result fits what it became.  That is a
+// branch of the whole workgroup (every thread has the same sum) that no usual row takes.
+template <int CPT>
+__device__ __forceinline__ float inverse_rms(float (&y)[CPT][CH], int D, float eps, float (*lds)[16]) {
+    auto mean = [&](float* to) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CPT; ++c)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) sum = fmaf(y[c][i], y[c][i], sum);
+        return block_sum(sum, to) / (float)D;
+    };
+    float m = mean(lds[0]) + eps;
+    if (__builtin_amdgcn_readfirstlane((m >= 0.0f && m < 0x1p-100f) || m == __builtin_inff())) {
+        const float f = m < 1.0f ? 0x1p88f : 0x1p-80f;
+#pragma unroll
+        for (int c = 0; c < CPT; ++c)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) y[c][i] *= f;
+        m = mean(lds[1]) + eps * f * f;
+    }
+    return 1.0f / sqrtf(m);
+}
+
 // One row a workgroup, CPT chunks a thread (chunk c of the row: thread c % threads): as
 // few as 1024 threads allow, so that a row's loads are all in flight at once and its sums
 // are short.  A workgroup of its own per row, not a loop over rows: 8192 rows keep HBM busy
 // by the workgroups that wait beside each other on a CU (four of 512 threads).
 template <int DT, int RT, int CPT>
 __global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a, int64_t t0) {
-    __shared__ float lds[2][16];
+    __shared__ float lds[4][16];
     const int tid = threadIdx.x, NT = blockDim.x, D = a.D;
     const int64_t t = t0 + blockIdx.x;
     float y[CPT][CH];
@@ -92,14 +118,7 @@ __global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a, int64_
             for (int i = 0; i < CH; ++i) y[c][i] = 0.0f;
     }
     float r = 1.0f;
-    if (a.post_weight) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < CPT; ++c)
-#pragma unroll
-            for (int i = 0; i < CH; ++i) sum = fmaf(y[c][i], y[c][i], sum);
-        r = 1.0f / sqrtf(block_sum(sum, lds[0]) / (float)D + a.eps);
-    }
+    if (a.post_weight) r = inverse_rms(y, D, a.eps, lds);
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
         const int d = (c * NT + tid) * CH;
@@ -130,12 +149,7 @@ __global__ void __launch_bounds__(1024) block_norm(const BlockNormArgs a, int64_
         if (a.y_out) store<RT>(y[c], a.y_out, t * a.y_out_stride + d, D - d);
     }
     if (!a.h_out) return;
-    float sum = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-#pragma unroll
-        for (int i = 0; i < CH; ++i) sum = fmaf(y[c][i], y[c][i], sum);
-    r = 1.0f / sqrtf(block_sum(sum, lds[1]) / (float)D + a.eps);
+    r = inverse_rms(y, D, a.eps, lds + 2);
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
         const int d = (c * NT + tid) * CH;

@@ -421,7 +421,8 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
  *   h = y / sqrt(mean(y^2) + eps) * pre_weight
  * x, gate, the weights and h are `dtype` (FP16 or BF16), residual and y are
  * residual_dtype (the same, or FP32).  h comes from the fp32 y, not from the
- * rounded one.  gate is one row for all tokens (gate_stride 0) or a row for
+ * rounded one; squares that leave fp32 are taken of scaled rows, so a finite row
+ * of any size has its norm.  gate is one row for all tokens (gate_stride 0) or a row for
  * each, NULL: 1; pre_weight NULL: 1; x NULL: y = residual (a stack's first
  * norm; post_weight, gate and scale are not used); residual NULL: 0 (not both).
  * y_out or h_out may be NULL: not wanted.

@@ -159,6 +159,34 @@ def test_norm_flat_gate(T, D):
         _close(h, h64, "fp16", bh)
 
 
+@pytest.mark.parametrize("dtype,stream", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp32")])
+@pytest.mark.parametrize("T,D", [(3, 1), (2, 100), (2, 2048), (2, 8195), (1, 32768)])
+@pytest.mark.parametrize("size,eps", [(1e20, 1e-6), (2e38, 1e-6), (1e25, 1e30), (1e-25, 0.0), (1e-38, 0.0), (1e-30, 1e-36), (1e-15, 1e-34)])
+def test_norm_squares_that_leave_fp32(dtype, stream, T, D, size, eps):
+    """Rows whose squares are infinite or nothing in fp32 have norms like all others.  Magnitudes are
+    size / 48 to size / 1.5: the smallest at 1e-38, 2^-132, is not below bf16's least."""
+    import torch
+    cg = _cg()
+    g = rng("norm-far", T, D, size)
+    rt = torch.float32 if stream == "fp32" else _dt(dtype)
+    v = torch.from_numpy(g.integers(64, 257, (2, T, D)) * g.choice([-1.0, 1.0], (2, T, D)) * 2.0 ** -g.integers(0, 4, (2, T, D)))
+    v = v * (size / 1.5 / 256)
+    r = v[0].to(rt).cuda()
+    w, w64 = _rounded(g, dtype, D)
+    y, h = torch.empty_like(r), torch.empty(T, D, dtype=_dt(dtype), device="cuda")
+    cg.block_norm(None, r, h, T, D, y_out=y, pre_weight=w, eps=eps)
+    y64, h64 = ref.block_norm(None, _f64(r), None, None, 1.0, w64, eps)
+    assert torch.equal(y, r) and np.all(np.isfinite(h64))
+    _close(h, h64, dtype, FP32 * np.abs(h64))
+    if dtype == "bf16":  # and the block's output
+        x = v[1].to(torch.bfloat16).cuda()
+        cg.block_norm(x, None, h, T, D, y_out=y, post_weight=w, scale=0.5, eps=eps)
+        y64, h64 = ref.block_norm(_f64(x), None, w64, None, 0.5, None, eps)
+        by, bh = _norm_bounds(_f64(x), None, w64, None, 0.5, None, eps, y64, h64)
+        _close(y, y64, stream, by)
+        _close(h, h64, dtype, bh)
+
+
 # ---- moe_route ----------------------------------------------------------------
 
 def _route(cg, x, bias, k, E=None, **kw):
