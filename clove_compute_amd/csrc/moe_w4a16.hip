@@ -10,7 +10,7 @@
 // weighted sum over a token's places are fp32, and a result is rounded once.
 //
 // What bounds it is the weights of the experts hit for few tokens, the matrix
-// instructions for many.  Three ways, by shape (run() below):
+// instructions for many.  Three ways, by shape (choose() in moe_plan.hpp):
 //  * few pairs: moe_few_down (a token's places added up by one workgroup) and
 //    moe_few (an expert's pairs meet its weights, straight from memory);
 //  * moe_tile multiplies tiles of weight rows by tiles of one expert's pairs, which
@@ -24,6 +24,7 @@
 
 #include "i4w_bits.hpp"
 #include "moe.hpp"
+#include "moe_plan.hpp"
 
 namespace clove {
 namespace moe {
@@ -122,7 +123,7 @@ __device__ __forceinline__ bool find_tile(const int* off, int E, int tile, int B
 // and its unpacking is scalar: 100 tokens on 6 of 64 experts of 2 x 1408 rows of 2046 123 us
 // (of 2048, with moe_tile, 57), 1 on 8 of 128 of 2 x 768 rows of 2046 37 (moe_few 6.8), 2048
 // on 2 of 8 of 2 x 11008 rows of 4094 2590 (747).
-constexpr int AR = 64, AC = 32, ALD = 136;
+constexpr int ALD = 136;
 
 template <bool SWIGLU>
 __global__ void __launch_bounds__(256) moe_any(const Params p) {
@@ -241,7 +242,6 @@ __global__ void __launch_bounds__(256) moe_any(const Params p) {
 // l % 16 and X rows 4 h .. 4 h + 3; step q of a group takes dword q of every lane,
 // k = 32 h + 8 q .. + 7 of lane group h.
 // ---------------------------------------------------------------------------
-constexpr int NG = 4;                 // groups of a unit
 constexpr int XLD = 128 * NG + 8;     // halves of a row of X in LDS
 
 template <int WF, int TB>
@@ -515,9 +515,6 @@ struct Cfg {
     static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && (2 * BR) % (64 * NW) == 0, "DMA split");
     static_assert(S >= 2 && S <= 4 && LDS <= 160 * 1024 && BC <= NT && OFF_P >= (CLOVE_MAX_EXPERTS + 8) * 4 && NW * 32 * (32 * FW + 4) * 4 <= OFF_P, "stages");
 };
-
-// Ids that a thread holds where the workgroups make their tile's list themselves
-constexpr int SCAN = 16;
 
 template <class CF, bool SWIGLU>
 __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
@@ -947,9 +944,6 @@ namespace {
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// More threads than a launch counts (2^32 in a dimension)
-bool too_many(int64_t workgroups, int threads) { return workgroups > ((int64_t)0xffffffff) / threads; }
-
 // ---- few pairs ----
 // Waves that share K: four, two once workgroups of two cover the CUs eight times (32 tokens
 // on 8 of 128 experts of 2 x 768 rows of 2048: 47 us against 54; 8 tokens 24 and 24.6; 1
@@ -985,12 +979,6 @@ clove_status_t run_few_down(Params p, int KS, hipStream_t stream) {
 }
 
 // ---- tiles ----
-// (about: half of an expert's last tile is empty, and an expert hit has one)
-template <class CF>
-int64_t items(const Params& p, bool swiglu) {
-    return cdiv64(p.on, swiglu ? CF::BR / 2 : CF::BR) * max(p.P / CF::BC + (p.a.experts + 1) / 2, min(p.P, p.a.experts));
-}
-
 template <class CF, bool SWIGLU>
 clove_status_t run_tile(Params p, hipStream_t stream) {
     p.rows_t = cdiv(p.on, SWIGLU ? CF::BR / 2 : CF::BR) * p.splits;
@@ -1002,67 +990,17 @@ clove_status_t run_tile(Params p, hipStream_t stream) {
     return check_launch();
 }
 
-// What runs first to its end by an estimate.  Workgroups: whole rounds of as many as the CUs
-// hold, and the rest, which takes less time the fewer of them share a CU (`time`: of one beside
-// 0, 1, 2 others, 1 for a 128 x 64 tile alone on its CU, which takes 0.8 us for a group and ten
-// groups' worth to begin and end).  Where they leave CUs idle K is split: more workgroups, and
-// fp32 sums of the parts to write and add up (for SwiGLU by a launch more).  Over 276 shapes
-// of 3 to 1100 pairs an expert, 4 to 128 experts, 256 to 16384 rows of 256 to 14336 the choice
-// is 1 % off the best of the shapes and splits on average; by the pairs an expert has on
-// average, without splits, 7 %.  Some (us, weights from HBM):
-//                                             256 x 128  128 x 64  128 x 32
-//   up 4096 on 8 experts of 22016 rows of 4096     747       898
-//   up 20000 on 128 of 768 of 4896                 296       229
-//   up 7388 on 16 of 1536 of 8192                  257       288       411
-//   up 4736 on 128 of 11008 of 512                 219       171       176
-//   up 1090 on 64 of 1024 of 1024, 5 an expert                37        34
-//   down 3000 on 64 of 2048 of 1408                           52        57
-//   up 600 on 64 of 2816 of 2048                              71        57
-//                                              parts of K:  1    2    4    8
-//   down 107 on 8 of 256 of 8192, 128 x 32                  42   26   19   16
-//   down 42 on 8 of 2048 of 8192                            43   28   28   31
-//   down 184 on 8 of 1408 of 14336                          75   44   45   41
-//   up 216 on 8 of 1536 of 14336                            73   54   50   49
-//   up 857 on 16 of 4096 of 1408                            32   43   57   75
-// (128 x 32 with two stages ahead and three workgroups a CU; two with three stages 42.5
-// against 38.6 for 15 pairs of 2048 rows of 1408 down.)  And 64 x 32 where 128 x 32 leaves half
-// of the CUs idle (4 experts of 2 x 1024 rows of 4096, 25 pairs: 23.6, 24.3).  Half-group stages
-// pay where stages of whole groups leave a CU one workgroup (256 x 128); elsewhere their
-// 32-byte pieces of weight rows cost more than they bring (256 x 32, 7 pairs: 66 against 57).
+// Shapes (plan() chooses)
 using Many = Cfg<4, 1, 2, 4, 2, 4>;   // 256 x 128
 using Some = Cfg<4, 1, 1, 2, 2, 8>;   // 128 x 64
 using Thin = Cfg<4, 1, 1, 1, 3, 8>;   // 128 x 32
 using Small = Cfg<2, 1, 1, 1, 4, 8>;  // 64 x 32
 
-template <int SLOTS>
-float rounds(int64_t items, int cus, const float (&time)[SLOTS]) {
-    const int64_t full = items / (SLOTS * cus), rest = items - full * SLOTS * cus;
-    return full * time[SLOTS - 1] + (rest ? time[cdiv64(rest, cus) - 1] : 0.0f);
+template <class CF>
+constexpr bool is(Shape s) {
+    return CF::BR == dims(s).rows && CF::BC == dims(s).pairs;
 }
-
-enum class Shape { kMany, kSome, kThin, kSmall };
-struct Plan {
-    Shape shape = Shape::kThin;
-    int splits = 1;
-    float us = 0.0f;
-};
-
-Plan plan(const Params& p, bool swiglu, int cus) {
-    Plan best;
-    auto take = [&](Shape shape, int splits, float time) {
-        const float sums = splits > 1 ? (float)splits * (0.5f + (float)p.P * p.on * (swiglu ? 16 : 8) / 4.5e6f) + (swiglu ? 4.0f : 0.0f) : 0.0f;
-        const float us = 0.8f * time * (cdiv(p.G, splits) + 10) + sums;
-        if (best.us == 0.0f || us < best.us) best = {shape, splits, us};
-    };
-    take(Shape::kMany, 1, rounds(items<Many>(p, swiglu), cus, {2.0f, 3.2f}));
-    for (int splits : {1, 2, 3, 4, 6, 8}) {
-        if (splits > 1 && ((int64_t)splits * p.P * p.on * (swiglu ? 8 : 4) > (64 << 20) || p.G < 4 * splits)) break;
-        take(Shape::kSome, splits, rounds(splits * items<Some>(p, swiglu), cus, {1.0f, 1.15f, 1.5f}));
-        take(Shape::kThin, splits, rounds(splits * items<Thin>(p, swiglu), cus, {0.8f, 1.05f, 1.3f}));
-    }
-    if (best.shape == Shape::kThin && best.splits == 1 && 2 * items<Thin>(p, swiglu) < cus) best.shape = Shape::kSmall;
-    return best;
-}
+static_assert(is<Many>(Shape::kMany) && is<Some>(Shape::kSome) && is<Thin>(Shape::kThin) && is<Small>(Shape::kSmall), "moe_plan.hpp");
 
 template <bool SWIGLU>
 clove_status_t run_shape(Shape s, const Params& p, hipStream_t stream) {
@@ -1072,12 +1010,12 @@ clove_status_t run_shape(Shape s, const Params& p, hipStream_t stream) {
     return run_tile<Small, SWIGLU>(p, stream);
 }
 
-// The call's scratch, taken for the first of its parts, whose pairs are the most
+// The call's kernels and scratch, settled by the first of its parts, whose pairs are the most
 struct Held {
+    bool begun = false;
+    Choice by;
     void* p = nullptr;
     size_t bytes = 0;
-    int pairs = 0;
-    Plan plan;
 };
 
 template <bool SWIGLU>
@@ -1091,53 +1029,21 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     p.splits = 1;
     p.split_groups = p.G;
     p.x_bytes = (int64_t)(SWIGLU ? a.T : p.P) * a.K * 2;
-    const int64_t expert_bytes = (int64_t)(SWIGLU ? 2 : 1) * a.O * (a.K / 2);
     const bool aligned = a.K > 0 && a.K % 32 == 0 && aligned16(a.X) && aligned16(a.W);
-    // Below three pairs an expert on average: no lists, no tiles (64 experts of 2 x 1408 rows of
-    // 2048, 6 a token: 20 tokens 45 us against 47 with tiles, 40 60 and 55, 80 89 and 59); below
-    // eight where there are fewer tiles than half of the CUs and K is too short to be split (8
-    // experts: 28 pairs down to 768 from 768 7.9 us and 11.0, 50 from 14336 to 1408 59 and 40)
-    p.on = a.O;
-    const bool few = aligned && (p.P < 3 * a.experts || (p.P < 8 * a.experts && p.G <= 16 && 2 * items<Thin>(p, SWIGLU) < cus));
-    if (few && !SWIGLU && 4 * p.P <= 3 * a.experts && !too_many((int64_t)a.T * cdiv(a.O, 16), 256)) {
-        // Most experts hit have one pair: a workgroup for each token and 16 outputs (32 where that leaves
-        // one a CU, or the waves with little: 41 tokens on 1 of 128, 2752 rows of 256 7.3 and 9.4 us)
-        // takes one launch and no memory between.  It reads the weights of an expert hit twice twice, and
-        // all of a token's places through one CU: by expert where that takes more than the second launch's
-        // 4 us, at the 19 GB/s of a CU and 4.2 TB/s of all that both kernels reach (us, by token and by
-        // expert: 1 token on 8 of 16 experts, 704 rows of 8192 31.6 and 15.2, 6 of 16, 1472 of 2048 8.6
-        // and 10.0; 10 on 6 of 128, 2048 of 8192 128 and 107; 8 on 1 of 128, 1024 of 4096 7.3 and 10.6)
-        const float mb = (float)a.O * a.K * 0.53e-6f, places = min(a.top_k, a.experts), units = cdiv(p.G, NG);
-        const float hit = a.experts * (1.0f - powf(1.0f - places / a.experts, a.T));
-        if (max(units * a.top_k * 0.215f, p.P * mb / 4.2f) <= max(units * 0.43f, hit * mb / 4.2f) + 4.0f) {
-            const int64_t grid = (int64_t)a.T * cdiv(a.O, 16);
-            if (grid <= cus) return run_few_down<1>(p, 16, stream);
-            if (grid <= 2 * cus) return run_few_down<2>(p, 16, stream);
-            return units * a.top_k <= 2 ? run_few_down<2>(p, 4, stream) : run_few_down<1>(p, 4, stream);
-        }
-    }
-    const bool tiles = aligned && expert_bytes < ((int64_t)1 << 31);  // (launch_moe_w4a16 bounds X)
-    // As many outputs at a time as workgroups of 256 threads for 16 of them and 32 pairs make a
-    // launch; scratch: the lists of the pairs by expert, and for down the products with as many
-    // outputs at a time as 512 MB hold, the products of parts of K up to 64 MB.  The first part of
-    // the tokens settles it for all
-    const bool lists = !few && (!tiles || p.P > SCAN * 128);
+    if (!held.begun) held.by = choose({SWIGLU, aligned, a.T, a.top_k, a.experts, a.O, a.K, cus});
+    held.begun = true;
+    const Choice& by = held.by;
+    if constexpr (!SWIGLU)
+        if (by.way == Way::kToken) return by.blocks == 1 ? run_few_down<1>(p, by.waves, stream) : run_few_down<2>(p, by.waves, stream);
+    // Scratch: the lists of the pairs by expert, for down the products with `chunk` outputs at a
+    // time, the products of parts of K up to 64 MB
+    const bool lists = (by.way == Way::kTiles && p.P > SCAN * 128) || by.way == Way::kAny;
     const size_t off = lists ? round256((size_t)(a.experts + 1) * 4) : 0, order = lists ? round256((size_t)p.P * 4) : 0;
-    const bool begins = held.pairs == 0;
-    if (begins) held.pairs = p.P;
-    int64_t most = (int64_t)16 * ((1 << 24) - 8) / (held.pairs / 32 + a.experts) / 256 * 256;
-    // (moe_combine: 65535 workgroups of 512 outputs)
-    if (!SWIGLU) most = min(min(most, (int64_t)512 * 65535), max((int64_t)256, ((int64_t)512 << 20) / ((int64_t)held.pairs * 4) / 256 * 256));
-    const int chunk = most < a.O ? cdiv(cdiv(a.O, (int)cdiv64(a.O, most)), 256) * 256 : a.O;
-    if (begins && tiles && !few) {
-        p.on = chunk;
-        held.plan = plan(p, SWIGLU, cus);
-    }
-    if (tiles && !few) {
-        p.split_groups = cdiv(p.G, held.plan.splits);
+    if (by.way == Way::kTiles) {
+        p.split_groups = cdiv(p.G, by.splits);
         p.splits = cdiv(p.G, p.split_groups);
     }
-    if (!SWIGLU || p.splits > 1) p.ldp = ((SWIGLU ? 2 * a.O : min(chunk, a.O)) + 3) & ~3;
+    if (!SWIGLU || p.splits > 1) p.ldp = ((SWIGLU ? 2 * a.O : min(by.chunk, a.O)) + 3) & ~3;
     const size_t bytes = off + order + (size_t)p.splits * p.P * p.ldp * 4;
     if (bytes > held.bytes) {
         if (const clove_status_t st = acquire_buffer(stream, kBufMoe, bytes, &held.p); st != CLOVE_OK) return st;
@@ -1153,20 +1059,18 @@ clove_status_t run(const MoeArgs& a, int cus, hipStream_t stream, Held& held) {
     if (SWIGLU && p.splits > 1) {
         // (the products of gate and up rows as of any others, and SwiGLU of their sums)
         p.a.O = p.on = 2 * a.O;
-        if (const clove_status_t st = run_shape<false>(held.plan.shape, p, stream); st != CLOVE_OK) return st;
+        if (const clove_status_t st = run_shape<false>(by.shape, p, stream); st != CLOVE_OK) return st;
         CLOVE_LAUNCH(moe_swiglu, dim3((unsigned)p.P, (unsigned)cdiv(a.O, 512)), dim3(128), 0, stream, p);
         return check_launch();
     }
-    for (int64_t o = 0; o < a.O; o += chunk) {
+    for (int64_t o = 0; o < a.O; o += by.chunk) {
         p.o0 = (int)o;
-        p.on = min(chunk, a.O - p.o0);
+        p.on = min(by.chunk, a.O - p.o0);
         clove_status_t st = CLOVE_OK;
-        if (few) {
-            // (2 pairs of an expert at a time while most have one or none, else 8: 1 token on 2 of 8
-            // experts of 2 x 14336 rows of 4096 28.3 us against 32.2, 32 on 8 of 128 71 against 47)
-            st = 2 * p.P <= a.experts ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
-        } else if (tiles) {
-            st = run_shape<SWIGLU>(held.plan.shape, p, stream);
+        if (by.way == Way::kExpert) {
+            st = by.pairs == 2 ? run_few<SWIGLU, 2, true>(p, cus, stream) : run_few<SWIGLU, 8, false>(p, cus, stream);
+        } else if (by.way == Way::kTiles) {
+            st = run_shape<SWIGLU>(by.shape, p, stream);
         } else {
             p.rows_t = cdiv(p.on, SWIGLU ? AR / 2 : AR);
             const int64_t grid = ((int64_t)p.P / AC + a.experts) * p.rows_t;
