@@ -187,6 +187,23 @@ def test_norm_squares_that_leave_fp32(dtype, stream, T, D, size, eps):
         _close(h, h64, dtype, bh)
 
 
+@pytest.mark.parametrize("D", [8, 199, 2049])
+def test_norm_infinite_scale(D):
+    """Every element is infinite, with its sign, or NaN where it was 0, and no norm is a number."""
+    import torch
+    cg = _cg()
+    g = rng("norm-infinite", D)
+    x, x64 = _rounded(g, "fp16", 3, D)
+    x[1, D // 2] = 0.0
+    x[2] = 0.0
+    y, h = torch.empty(3, D, device="cuda"), torch.empty_like(x)
+    cg.block_norm(x, torch.ones_like(y), h, 3, D, y_out=y, scale=float("inf"))
+    y64, h64 = ref.block_norm(_f64(x), np.ones((3, D)), None, None, np.inf, None, 1e-6)
+    assert np.isinf(y64[0]).all() and np.isnan(y64[2]).all() and np.isnan(h64).all()
+    _close(y, y64, "fp32", 0.0)
+    _close(h, h64, "fp16", 0.0)
+
+
 # ---- moe_route ----------------------------------------------------------------
 
 def _route(cg, x, bias, k, E=None, **kw):
