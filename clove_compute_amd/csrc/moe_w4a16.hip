@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(1024) moe_few_down(const Params p) {
 // to them.  That is as many VALU operations as folding group sums into a second
 // set of accumulators, and half the registers: a wave holds 64 x 128 outputs with
 // two waves on a SIMD, so that an unpacked weight meets four blocks of pairs.  A
-// group whose scale is 0 leaves the unit as it is and its weights are made 0.
+// group whose scale is 0 leaves the unit as it is and its weights are made 0 (or
+// NaN, where the zero point is infinite or NaN, as in the other kernels).
 //
 // 4096 pairs on 8 experts of 2 x 11008 rows of 4096 take 747 us, 0.99 PFLOP/s (a library
 // product of fp16 weights reaches 1.20): the matrix pipe is busy 55 % of the cycles, and
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(CF::NT) moe_tile(const Params p) {
                         const bool none = sc == 0.0f;
                         ratio[i] = none ? 1.0f : unit[i] / sc;
                         unit[i] = none ? unit[i] : sc;
-                        const _Float16 nz = (_Float16)(none ? 0.0f : z * (-1.0f / 512.0f));
+                        const _Float16 nz = (_Float16)(z * (none ? 0.0f : -1.0f / 512.0f));
                         zz[i] = f16x2{nz, nz};
                         mul[i] = none ? f16x2{(_Float16)0.0f, (_Float16)0.0f} : f16x2{(_Float16)2048.0f, (_Float16)32768.0f};
                     }

@@ -240,6 +240,20 @@ def test_infinite_and_nan_scales_stay_in_their_row(call):
     assert _bits([c.before]) == _bits([before])
 
 
+@calls
+def test_zero_points_that_are_not_finite(call):
+    """(q - z) 0 is no number either where z is none: in every kernel the outputs of such a row, and no other."""
+    c = Call(call, "bad-zeros")
+    s, z = c.c.s.cpu().numpy(), c.c.z.cpu().numpy()
+    for row, group, zero, scale in [(3, 0, np.nan, 0.0), (6, -1, np.inf, 0.0), (8, 0, -np.inf, 0.01), (11, -1, np.nan, -0.0)]:
+        s[:, row, group], z[:, row, group] = scale, zero
+    c.c.z = _dev(z)
+    c.scales(s)
+    good = np.array([o for o in range(c.O) if o not in (3, 6, 8, 11)])
+    got = c.check(columns=good)
+    assert not np.isfinite(_f64(got)[:c.rows][:, [3, 6, 8, 11]]).any()
+
+
 @pytest.mark.parametrize("call", [next(c for c in plan.CALLS if c[:2] == k) for k in sorted({c[:2] for c in plan.CALLS})], ids=plan.named)
 def test_graphs_and_workspaces(call):
     """Replays with other ids and rows, and eager work between them; the call in a bound workspace of the
