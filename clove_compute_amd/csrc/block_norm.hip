@@ -8,6 +8,8 @@
 // left is HBM for many tokens (8192 rows of 4096, fp16 with an fp32 stream, both
 // norms and a gate, 470 MB: 79 to 83 us, 5.7 to 5.9 TB/s, where a copy reaches
 // 5.1), and for one (a row of 2048: 2.4 us) a launch and two round trips.
+#include <algorithm>
+
 #include "moe.hpp"
 
 namespace clove {
@@ -176,7 +178,7 @@ clove_status_t run(const BlockNormArgs& a, hipStream_t stream) {
     auto k = cpt == 1 ? block_norm<DT, RT, 1> : cpt == 2 ? block_norm<DT, RT, 2> : block_norm<DT, RT, 4>;
     // (a launch counts fewer than 2^32 threads)
     for (int64_t t = 0, most = ((int64_t)1 << 31) / nt; t < a.T; t += most)
-        CLOVE_LAUNCH(k, dim3((unsigned)min(most, a.T - t)), dim3((unsigned)nt), 0, stream, a, t);
+        CLOVE_LAUNCH(k, dim3((unsigned)std::min(most, a.T - t)), dim3((unsigned)nt), 0, stream, a, t);
     return check_launch();
 }
 

@@ -27,6 +27,14 @@ struct Call {
     int G() const { return (int)up(K, 128); }
 };
 
+// Tokens at a time: X below the 2^31 bytes that a buffer's offsets reach, at most 2^19 pairs, so
+// that the lists and launches are small beside the products.  (0: not even one.  In std::min's 64
+// bits: HIP's own min on the host is of 32.)
+inline int64_t tokens_at_a_time(bool swiglu, int top_k, int K) {
+    const int64_t per_token = (int64_t)(swiglu ? 1 : top_k) * K * 2, pairs = (int64_t)1 << 19;
+    return std::min(pairs, per_token ? (((int64_t)1 << 31) - 1) / per_token * top_k : pairs) / top_k;
+}
+
 enum class Way { kToken, kExpert, kTiles, kAny };  // moe_few_down, moe_few, moe_tile, moe_any
 enum class Shape { kMany, kSome, kThin, kSmall };
 struct Dims {

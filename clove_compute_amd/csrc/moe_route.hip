@@ -5,6 +5,7 @@
 //
 // s and c are 64 bits: of some hundred experts two often agree to 2^-24, and
 // which of them comes first must not depend on an exponential's last bit.
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -256,7 +257,7 @@ clove_status_t launch(const RouteArgs& a, hipStream_t stream) {
     constexpr int TOKENS = WAVES * (64 / L);  // of a workgroup
     // (a launch counts fewer than 2^32 threads)
     for (int64_t t = 0, most = (int64_t)1 << 25; t < a.T; t += most)
-        CLOVE_LAUNCH((moe_route<DT, V, L, BIAS>), dim3((unsigned)cdiv64(min(most, a.T - t), TOKENS)), dim3(64 * WAVES), 0, stream, a,
+        CLOVE_LAUNCH((moe_route<DT, V, L, BIAS>), dim3((unsigned)cdiv64(std::min(most, a.T - t), TOKENS)), dim3(64 * WAVES), 0, stream, a,
                      FastDiv(a.experts / a.groups), (int)t);
     return check_launch();
 }

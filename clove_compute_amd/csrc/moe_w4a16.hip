@@ -1093,10 +1093,7 @@ clove_status_t launch_moe_w4a16(const MoeArgs& a, bool swiglu, hipStream_t strea
     using namespace moe;
     DeviceInfo dev;
     if (const clove_status_t st = current_device_info(&dev); st != CLOVE_OK) return st;
-    // as many tokens at a time as keep X below the 2^31 bytes that a buffer's offsets reach, and
-    // the lists and launches small beside the products
-    const int64_t per_token = (int64_t)(swiglu ? 1 : a.top_k) * a.K * 2;
-    const int64_t most = min((int64_t)1 << 19, per_token ? (((int64_t)1 << 31) - 1) / per_token * a.top_k : (int64_t)1 << 19) / a.top_k;
+    const int64_t per_token = (int64_t)(swiglu ? 1 : a.top_k) * a.K * 2, most = tokens_at_a_time(swiglu, a.top_k, a.K);
     if (most < 1) return CLOVE_ERR_INVALID_DIM;
     Held held;
     for (int64_t t = 0; t < a.T;) {

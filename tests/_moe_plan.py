@@ -16,6 +16,7 @@ extern "C" void host_choose(int swiglu, int aligned, int T, int top_k, int exper
     out[0] = (int)c.way, out[1] = c.blocks, out[2] = c.waves, out[3] = c.pairs;
     out[4] = (int)c.shape, out[5] = c.splits, out[6] = c.chunk;
 }
+extern "C" long host_tokens(int swiglu, int top_k, int K) { return tokens_at_a_time(swiglu != 0, top_k, K); }
 """
 CUS = 256
 _lib = None
@@ -31,6 +32,12 @@ def _built():
             subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I", CSRC, src, "-o", so], check=True)
             _lib = ctypes.CDLL(so)
     return _lib
+
+
+def tokens_at_a_time(op, k, K):
+    lib = _built()
+    lib.host_tokens.restype = ctypes.c_long
+    return lib.host_tokens(op == "up", k, K)
 
 
 def choice(op, T, k, E, O, K, aligned=True, cus=CUS):

@@ -668,6 +668,13 @@ def test_outputs_past_one_grid():
     assert bool((y.view(-1) == want).all())
 
 
+@pytest.mark.parametrize("T,k,E,O,K", [(3, 6, 31, 469, 2), (1, 4, 4, 1, 2), (5, 64, 100, 20, 30), (2, 64, 80, 33, 8), (9, 20, 32, 40, 2), (40, 64, 3, 24, 4)])
+def test_more_places_than_columns(T, k, E, O, K):
+    cg = _cg()
+    _check_up(cg, Case("places-up", T, k, E, 2 * O, K, absent=0.1))
+    _check_down(cg, Case("places-down", T, k, E, O, K, absent=0.1))
+
+
 @pytest.mark.parametrize("O,K", [(40, 0), (5, 0)])
 def test_no_k(O, K):
     import torch

@@ -40,3 +40,13 @@ def test_outputs_at_a_time():
         chunk = plan.choice("down", T, k, 4, O, 64)[1]
         assert 0 < chunk < O and chunk % 256 == 0 and chunk <= 512 * 65535 and (chunk == 256 or T * k * chunk * 4 <= 512 << 20)
     assert 0 < plan.choice("up", 550, 2, 1024, 262400, 32)[1] < 262400
+
+
+def test_tokens_at_a_time():
+    """As many as 2^19 pairs, and an X below 2^31 bytes, allow, however few columns or many places there are."""
+    for op in ("up", "down"):
+        for k in (1, 2, 3, 6, 8, 20, 64):
+            for K in (0, 2, 8, 10, 30, 32, 64, 4096, 1 << 20, (1 << 24) - 2, 1 << 29, (1 << 30) - 2, 1 << 30, (1 << 31) - 2):
+                n, row = plan.tokens_at_a_time(op, k, K), 2 * K * (1 if op == "up" else k)
+                assert n * k <= 1 << 19 and n * row < 1 << 31
+                assert (n + 1) * k > 1 << 19 or (n + 1) * row >= 1 << 31
