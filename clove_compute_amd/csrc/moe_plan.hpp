@@ -63,10 +63,10 @@ inline int64_t tiles(Shape s, const Call& c, int on) {
 // hold, and the rest, which takes less time the fewer of them share a CU (`time`: of one beside
 // 0, 1, 2 others, 1 for a 128 x 64 tile alone on its CU, which takes 0.8 us for a group and ten
 // groups' worth to begin and end).  Where they leave CUs idle K is split: more workgroups, and
-// fp32 sums of the parts to write and add up (for SwiGLU by a launch more).  Over 276 shapes
-// of 3 to 1100 pairs an expert, 4 to 128 experts, 256 to 16384 rows of 256 to 14336 the choice
-// is 1 % off the best of the shapes and splits on average; by the pairs an expert has on
-// average, without splits, 7 %.  Some (us, weights from HBM):
+// fp32 sums of the parts to write and add up (for SwiGLU by a launch more).  Over 187 drawn
+// shapes that go to tiles the choice is 1.4 % off the best of all kernels, shapes and splits on
+// average and 1.4 times at worst; of the 108 of few pairs (choose()) 2.9 % and 2.3 times.
+// Some (us, weights from HBM):
 //                                             256 x 128  128 x 64  128 x 32
 //   up 4096 on 8 experts of 22016 rows of 4096     747       898
 //   up 20000 on 128 of 768 of 4896                 296       229

@@ -493,11 +493,15 @@ __global__ void __launch_bounds__(1024) moe_few_down(const Params p) {
 // group whose scale is 0 leaves the unit as it is and its weights are made 0 (or
 // NaN, where the zero point is infinite or NaN, as in the other kernels).
 //
-// 4096 pairs on 8 experts of 2 x 11008 rows of 4096 take 747 us, 0.99 PFLOP/s (a library
-// product of fp16 weights reaches 1.20): the matrix pipe is busy 55 % of the cycles, and
-// the VALU, mostly with unpacking.  65536 pairs on 128 experts of 2048 rows of 768: 282
-// us, as much of it the 537 MB of fp32 products as the six groups of K.  540 pairs on 64
-// experts of 2 x 1408 rows of 2048 (197 MB): 57 us, 3.4 TB/s, the VALU busy for 55 %.
+// 4096 pairs on 8 experts of 2 x 11008 rows of 4096 take 744 to 800 us by the card, 0.92
+// to 0.99 PFLOP/s (a library product of fp16 weights reaches 1.20): matrix pipe and VALU,
+// mostly unpacking, are busy for 55 % of the cycles each and do not fill each other's
+// gaps.  What a tile costs beside its groups of K is its beginning (three dependent
+// latencies: the experts' offsets, its pairs, its first stage) and its end (stores that
+// nothing else of the workgroup runs beside), together some ten groups' time.  65536
+// pairs on 128 experts of 2048 rows of 768: 282 us, 537 MB of fp32 products and six
+// groups of K.  540 pairs on 64 experts of 2 x 1408 rows of 2048 (197 MB): 58 us, 3.4
+// TB/s, sixteen groups, and nine pairs to a tile of 32.
 // ---------------------------------------------------------------------------
 template <int WR_, int WC_, int FW_, int FX_, int S_, int KS_>
 struct Cfg {

@@ -422,9 +422,10 @@ clove_status_t clove_penalize_logits(const void* logits, int64_t logits_stride, 
  * x, gate, the weights and h are `dtype` (FP16 or BF16), residual and y are
  * residual_dtype (the same, or FP32).  h comes from the fp32 y, not from the
  * rounded one; squares that leave fp32 are taken of scaled rows, so a finite row
- * of any size has its norm.  gate is one row for all tokens (gate_stride 0) or a row for
- * each, NULL: 1; pre_weight NULL: 1; x NULL: y = residual (a stack's first
- * norm; post_weight, gate and scale are not used); residual NULL: 0 (not both).
+ * of any size has its norm.  gate is one row for all tokens (gate_stride 0) or a
+ * row for each, NULL: 1; pre_weight NULL: 1; x NULL: y = residual (a stack's
+ * first norm; post_weight, gate and scale are not used); residual NULL: 0 (not
+ * both).
  * y_out or h_out may be NULL: not wanted.
  * Rows [T, D], strides in elements.  y_out may be residual, y_out or h_out may
  * be x or gate (same rows and type; of several rows the same stride); else
@@ -474,15 +475,15 @@ clove_status_t clove_moe_route(const void* logits, int64_t logits_stride, int dt
  * fp32 (no rounding before SwiGLU).  A pair whose id lies outside [0, experts)
  * (a padding token, an expert of another device) has no product and its row of
  * H is left as it is; an expert may come twice in a row.  K is even.  Which
- * kernel runs goes by the sizes and alignments alone, and a row's bits do not
- * depend on what other tokens chose.  Fastest with K % 32 == 0 and 16-byte
- * aligned X and W_q.
+ * kernel runs goes by the sizes, the alignments and the device's number of CUs
+ * alone, and a row's bits do not depend on what other tokens chose.  Fastest
+ * with K % 32 == 0 and 16-byte aligned X and W_q.
  * Zero points round to the nearest integer, as clove_gemm_w4a16's; q - z is
  * exact up to 2048 in magnitude and rounded to fp16 past that.
  * Scratch: 4 bytes a pair, at most 2 MB (more pairs than 2^19, or an X of 2^31
- * bytes, go in parts), and up to 64 MB of fp32 products where K is split.  2^31 tiles of 32 rows by 32 pairs and more, or one
- * token's X of 2^31 bytes (here a row, below top_k rows), are
- * CLOVE_ERR_INVALID_DIM.
+ * bytes, go in parts), and up to 64 MB of fp32 products where K is split.  2^31
+ * tiles of 32 rows by 32 pairs and more, or one token's X of 2^31 bytes (here a
+ * row, below top_k rows), are CLOVE_ERR_INVALID_DIM.
  */
 clove_status_t clove_moe_w4a16_swiglu(const void* X, const int32_t* expert_ids, const uint8_t* W_q,
                                       const void* W_scale, const void* W_zero, void* H, int T, int top_k,
